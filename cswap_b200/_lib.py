@@ -83,11 +83,25 @@ class ZfpField(C.Structure):
                 ("data", C.c_void_p)]
 
 
+class AttentionShape(C.Structure):
+    _fields_ = [("type", C.c_int), ("causal", C.c_int), ("batch", C.c_size_t), ("heads", C.c_size_t),
+                ("kv_heads", C.c_size_t), ("q_len", C.c_size_t), ("k_len", C.c_size_t), ("dim", C.c_size_t),
+                ("scale", C.c_float), ("kv_lens", C.c_void_p)]
+
+
+class AttentionOperand(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_ssize_t), ("head_stride", C.c_ssize_t),
+                ("token_stride", C.c_ssize_t)]
+
+
 _P = C.c_void_p
 _SZ = C.c_size_t
 _SSZ = C.c_ssize_t
 _U = C.c_uint
 _I = C.c_int
+_F = C.c_float
+_SH = C.POINTER(AttentionShape)
+_OP = C.POINTER(AttentionOperand)
 
 # name -> (restype, argtypes); every symbol the two headers declare
 SIGNATURES = {
@@ -135,6 +149,17 @@ SIGNATURES = {
                                C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "csw_host_alloc": (_I, [_SZ, C.POINTER(_P)]),
     "csw_host_free": (_I, [_P]),
+    "csw_q8_bytes": (_I, [_SZ, C.POINTER(_SZ)]),
+    "csw_q8_compress": (_I, [_P, _I, _SZ, _P, _SZ, _P]),
+    "csw_q8_decompress": (_I, [_P, _SZ, _SZ, _P, _I, _P]),
+    "csw_gelu_forward": (_I, [_P, _I, _SZ, _P, _P, _SZ, _P]),
+    "csw_gelu_backward": (_I, [_P, _I, _P, _SZ, _SZ, _P, _P, _P]),
+    "csw_layer_norm_forward": (_I, [_P, _P, _P, _P, _I, _I, _SZ, _SZ, _F, _P, _P, _P, _P, _P]),
+    "csw_layer_norm_workspace": (_I, [_SZ, _SZ, C.POINTER(_SZ)]),
+    "csw_layer_norm_backward": (_I, [_P, _P, _P, _P, _P, _I, _I, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P]),
+    "csw_attention_forward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _P]),
+    "csw_attention_workspace": (_I, [_SH, C.POINTER(_SZ)]),
+    "csw_attention_backward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _OP, _OP, _OP, _OP, _P, _SZ, _P]),
     # reference-named entry points
     "PreGPUcompression": (None, [_I, _I, _P, _P, _I, _I, _P]),
     "PreAcc": (None, [_P, _I, _P, _I, _I, _P]),

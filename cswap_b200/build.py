@@ -1,5 +1,5 @@
 """Builds libcswap_b200.so in-tree with nvcc for sm_100a (cross-compiles without a GPU) and the CPython extension
-behind codec.py."""
+behind codec.py and ops.py."""
 from __future__ import annotations
 
 import importlib.metadata
@@ -13,8 +13,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcswap_b200.so")
 ROOT = os.path.dirname(HERE)
 SOURCES = ["zfp_kernels.cu", "sparse_kernels.cu", "cswap_abi.cu", "swap_manager.cu", "cost_model.cu",
-           "sparse_static.cu"]
-HEADERS = ["pdl.cuh", "zfp_core.cuh", "zfp_field.cuh", "zfp_kernels.h", "sparse_kernels.h", "tile_counts.cuh", "internal.h",
+           "sparse_static.cu", "q8_kernels.cu", "norm_kernels.cu", "attention_kernels.cu", "ops_abi.cu"]
+HEADERS = ["values.cuh", "q8_kernels.h", "norm_kernels.h", "attention_kernels.h",
+           "pdl.cuh", "zfp_core.cuh", "zfp_field.cuh", "zfp_kernels.h", "sparse_kernels.h", "tile_counts.cuh", "internal.h",
            os.path.join("..", "..", "include", "cswap_b200.h"), os.path.join("..", "..", "include", "cswap_compat.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -65,7 +66,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-EXT_SOURCE = os.path.join(CSRC, "codec_ext.cpp")
+EXT_SOURCES = [os.path.join(CSRC, s) for s in ("codec_ext.cpp", "ops_ext.cpp")]
 EXT = os.path.join(HERE, "_codec_ext.so")
 EXT_STAMP = os.path.join(HERE, "build", "_codec_ext.built_for")
 
@@ -80,7 +81,7 @@ def _built_for() -> str:
 
 
 def _ext_up_to_date() -> bool:
-    deps = [EXT_SOURCE, os.path.join(ROOT, "include", "cswap_b200.h"), os.path.abspath(__file__)]
+    deps = EXT_SOURCES + [os.path.join(CSRC, "ext_util.h"), os.path.join(ROOT, "include", "cswap_b200.h"), os.path.abspath(__file__)]
     if not os.path.exists(EXT) or not os.path.exists(EXT_STAMP):
         return False
     if any(os.path.getmtime(EXT) < os.path.getmtime(d) for d in deps):
@@ -105,7 +106,7 @@ def build_ext(force: bool = False) -> str | None:
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(t, "include"),
            "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I", cuda_inc,
-           EXT_SOURCE, "-o", EXT, "-L", os.path.join(t, "lib"), "-L", HERE,
+           *EXT_SOURCES, "-o", EXT, "-L", os.path.join(t, "lib"), "-L", HERE,
            f"-Wl,-rpath,{os.path.join(t, 'lib')}", "-Wl,-rpath,$ORIGIN",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lcswap_b200"]
     subprocess.check_call(cmd)

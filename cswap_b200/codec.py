@@ -16,6 +16,8 @@ from ._lib import LibraryMissing, SparseLayout, check, lib
 
 # policy codes (CSWAP+/Execution.h:70,86,107,243)
 POLICY_KEEP, POLICY_DROP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP = 0, 1, 2, 3, 6
+# the framework's own: held on the device as an 8-bit checkpoint (ops.py)
+POLICY_Q8 = 8
 
 
 # The extension module behind the tensor-level calls (csrc/codec_ext.cpp), loaded on first use

@@ -41,6 +41,12 @@ __device__ __forceinline__ void pdl_wait(T* __restrict__& p) {
   asm volatile("griddepcontrol.wait;" : "+l"(p)::"memory");
 }
 
+// and for further pointers of the same kernel, behind that
+template <class... T>
+__device__ __forceinline__ void pdl_behind(T* __restrict__&... p) {
+  (..., [&] { asm volatile("" : "+l"(p)::"memory"); }());
+}
+
 // An error that a call returns is its caller's to report: left pending in the runtime as well,
 // the next cudaGetLastError of the process (torch's after a launch of its own, say) would meet it.
 inline cudaError_t taken(cudaError_t e) {

@@ -19,6 +19,8 @@
  *                                         sites CSWAP+/Execution.h:224-233,
  *                                         CSWAP+/resnet-cifar10.cpp:407-437)
  *   6. legacy entry points with the reference's own names (cswap_compat.h)
+ *   7. operators of a training step that save little for backward: 8-bit checkpoints, GELU on them, layer norm,
+ *      attention
  */
 #ifndef CSWAP_B200_H
 #define CSWAP_B200_H
@@ -346,6 +348,73 @@ csw_status csw_cost_decide(const csw_cost_model* model, const csw_tensor_desc* t
  * is (no copy in, no stall - and no memory freed). */
 csw_status csw_cost_simulate(const csw_cost_model* model, const csw_tensor_desc* tensors, size_t n, double fwd_total_s,
                              const int* policy, double* exposed, double* total_stall_s);
+
+/* ---- 7. operators of a training step that save little for backward -------- */
+/* Types of values.  All sums, norms and softmax statistics are float32; a result is rounded to its type once. */
+enum { CSW_TYPE_F32 = 0, CSW_TYPE_F16 = 1, CSW_TYPE_BF16 = 2 };
+
+/* 8-bit checkpoint of n values: [codes: n int8][from the next multiple of 16 bytes: ceil(n/128) float32 scales].
+ * Groups of 128 consecutive values share a scale.  With m the group's largest magnitude, scale = m / 127 and
+ * code = rint(x * (127 / m)), ties to even, each step one float32 operation; the value held is code * scale.  Groups
+ * with m < 2^-120 are held as zeros, groups with a NaN or an infinity as NaNs.  The buffer is 16-byte aligned. */
+csw_status csw_q8_bytes(size_t n, size_t* bytes);
+csw_status csw_q8_compress(const void* d_in, int type, size_t n, void* d_out, size_t cap, csw_stream_t stream);
+csw_status csw_q8_decompress(const void* d_in, size_t bytes, size_t n, void* d_out, int type, csw_stream_t stream);
+
+/* y = x Phi(x), Phi the normal distribution function, and the 8-bit checkpoint of x in the same pass. */
+csw_status csw_gelu_forward(const void* d_x, int type, size_t n, void* d_y, void* d_packed, size_t cap,
+                            csw_stream_t stream);
+/* With x the values that the checkpoint holds: dx = dy (Phi(x) + x phi(x)); where d_y is given it receives x Phi(x)
+ * (what the weight gradient of a product behind the GELU needs, so that nobody has to keep it).  d_dx and d_y may
+ * not overlap; d_dx may be d_dy. */
+csw_status csw_gelu_backward(const void* d_dy, int type, const void* d_packed, size_t bytes, size_t n, void* d_dx,
+                             void* d_y, csw_stream_t stream);
+
+/* Layer norm of rows x cols values over cols, of x or, where d_residual is given, of x + residual, which d_sum then
+ * receives (rounded to the type; it is what is normed).  weight and bias (cols values of param_type: type, or float32)
+ * may be NULL: 1 and 0.  d_mean and d_rstd: rows float32, for backward. */
+csw_status csw_layer_norm_forward(const void* d_x, const void* d_residual, const void* d_weight, const void* d_bias,
+                                  int type, int param_type, size_t rows, size_t cols, float eps, void* d_y, void* d_sum,
+                                  float* d_mean, float* d_rstd, csw_stream_t stream);
+/* Backward: d_x is what was normed (d_sum, with a residual; d_dx is then the gradient of both terms).  d_dweight and
+ * d_dbias (param_type) may be NULL; where one is given the workspace holds csw_layer_norm_workspace bytes (of the
+ * current device).  The same call gives the same bits every time. */
+csw_status csw_layer_norm_workspace(size_t rows, size_t cols, size_t* bytes);
+csw_status csw_layer_norm_backward(const void* d_dy, const void* d_x, const float* d_mean, const float* d_rstd,
+                                   const void* d_weight, int type, int param_type, size_t rows, size_t cols, void* d_dx,
+                                   void* d_dweight, void* d_dbias, void* d_workspace, size_t workspace_bytes,
+                                   csw_stream_t stream);
+
+/* Attention: o = softmax(scale q k^T) v for every head.  float16 or bfloat16; dim a multiple of 8 up to 128; heads a
+ * multiple of kv_heads: query heads h of one group of heads / kv_heads consecutive ones read key head
+ * h / (heads / kv_heads).  causal: query i sees the keys up to i + k_len - q_len.  kv_lens (device, `batch` int32, or
+ * NULL): batch entry b has kv_lens[b] keys (taken into 0 ... k_len); what lies behind them in k and v is not used,
+ * whatever it is.  A query that sees no key gets o = 0 and lse = -inf, and no gradient passes through it. */
+typedef struct {
+  int type, causal;
+  size_t batch, heads, kv_heads, q_len, k_len, dim;
+  float scale;
+  const int32_t* kv_lens;
+} csw_attention_shape;
+/* Where a tensor lies: data[b * batch_stride + h * head_stride + t * token_stride + 0 ... dim - 1], strides in
+ * elements, not negative and multiples of 8, data 16-byte aligned. */
+typedef struct {
+  void* data;
+  ptrdiff_t batch_stride, head_stride, token_stride;
+} csw_attention_operand;
+/* d_lse: batch x heads x q_len float32, the natural logarithm of each row's sum of exp(scale q.k). */
+csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_attention_operand* q,
+                                 const csw_attention_operand* k, const csw_attention_operand* v,
+                                 const csw_attention_operand* o, float* d_lse, csw_stream_t stream);
+/* Backward forms the probabilities again from q, k and d_lse.  Gradients of keys and values are summed over the query
+ * heads that share them, in a fixed order. */
+csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes);
+csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_attention_operand* q,
+                                  const csw_attention_operand* k, const csw_attention_operand* v,
+                                  const csw_attention_operand* o, const float* d_lse, const csw_attention_operand* dout,
+                                  const csw_attention_operand* dq, const csw_attention_operand* dk,
+                                  const csw_attention_operand* dv, void* d_workspace, size_t workspace_bytes,
+                                  csw_stream_t stream);
 
 /* ---- pinned host memory helpers (for callers without a CUDA binding) ------ */
 csw_status csw_host_alloc(size_t bytes, void** p);
