@@ -7,24 +7,48 @@
 // Only L is kept for backward, which forms the probabilities again.  A row that sees no key has o = 0, L = -inf and
 // takes part in no gradient.
 //
-// One warp a row, lanes along the head's dimension.
+// All products run on the tensor cores, 128 x 128 scores at a time: tiles of 128 tokens are copied into shared memory
+// by TMA (columns behind the head's dimension and rows behind the sequence arrive as zeros, so that any dimension up to
+// 64 or 128 runs as that), scores and accumulators lie in tensor memory, and the probabilities, rounded to the operands'
+// type, go back to tensor memory over the scores they came from, as the first operand of the second product.  The
+// second operand of that product is the tile that is in shared memory anyway, read across its rows.
+//
+// Three kernels, each with a warp that copies, a warp whose first lane issues the products, and warps for the softmax,
+// a thread a row or half a row:
+//   forward   a tile of queries, over the tiles of keys: s, p, o += p v
+//   dq        the same rows: s, dp = do v, ds, dq += ds k
+//   dkv       a tile of keys, over the tiles of queries of every head that shares them: s and dp transposed,
+//             dv += p do, dk += ds q
+// dq and dkv each form the scores for themselves: seven products where five would do, but no sums over CTAs, whose
+// order would change the result from call to call, and no float32 copy of dq in memory.
 #include <cuda_runtime.h>
 
+#include <cmath>
+#include <type_traits>
+
 #include "attention_kernels.h"
+#include "internal.h"
 #include "pdl.cuh"
+#include "tensor_core.cuh"
 #include "values.cuh"
 
 namespace csw {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kPer = 4;  // values of a head of up to 128 that a lane holds
+using namespace tc;
+
+constexpr int kTile = 128;                 // tokens of a tile
+constexpr uint32_t kChunk = kTile * 128;   // bytes of a tile's 64 columns
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Set where a wait ran out.
+__device__ int attention_gave_up;
 
 struct View {
   void* p;
   int64_t b, h, t;
   template <class T>
-  __device__ T* row(uint64_t batch, uint64_t head, uint64_t token) const {
+  __device__ T* row(uint32_t batch, uint32_t head, uint32_t token) const {
     return static_cast<T*>(p) + (int64_t)batch * b + (int64_t)head * h + (int64_t)token * t;
   }
 };
@@ -33,153 +57,837 @@ View view_of(const csw_attention_operand& o) { return {o.data, o.batch_stride, o
 struct Shape {
   uint32_t batch, heads, kv_heads, q_len, k_len, dim;
   int causal;
-  float scale;
+  bool negate;     // the scale is negative: the products are negated instead
+  float scale;     // as given
+  float exponent;  // |scale| log2(e), and not zero, so that masked scores stay -inf
   const int32_t* lens;
-  __device__ uint32_t keys(uint32_t b) const {
-    return lens ? (uint32_t)min(max(lens[b], 0), (int)k_len) : k_len;
+  __device__ int keys(uint32_t b) const { return lens ? min(max(lens[b], 0), (int)k_len) : (int)k_len; }
+  // keys that query i sees
+  __device__ int limit(int i, int keys) const {
+    return causal ? min(keys, max(i + (int)k_len - (int)q_len + 1, 0)) : keys;
   }
 };
-Shape shape_of(const csw_attention_shape& s) {
-  return {(uint32_t)s.batch, (uint32_t)s.heads, (uint32_t)s.kv_heads, (uint32_t)s.q_len, (uint32_t)s.k_len,
-          (uint32_t)s.dim,   s.causal,          s.scale,               s.kv_lens};
-}
 
-template <class T>
-__device__ __forceinline__ void load_row(const T* p, uint32_t dim, uint32_t lane, float (&f)[kPer]) {
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) f[i] = lane + 32 * i < dim ? widen(p[lane + 32 * i]) : 0.0f;
+__device__ __forceinline__ void give_up(uint32_t* flag) {
+  *reinterpret_cast<volatile uint32_t*>(flag) = 1;
+  atomicExch(&attention_gave_up, 1);
 }
-template <class T>
-__device__ __forceinline__ void store_row(T* p, uint32_t dim, uint32_t lane, const float (&f)[kPer]) {
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (lane + 32 * i < dim) p[lane + 32 * i] = narrow<T>(f[i]);
-}
-__device__ __forceinline__ float dot(const float (&a)[kPer], const float (&b)[kPer]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) s += a[i] * b[i];
-#pragma unroll
-  for (int d = 16; d; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-  return s;
-}
-
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) attention_forward_kernel(Shape s, View q, View k, View v, View o, float* lse) {
-  pdl_wait();
-  const uint64_t r = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const uint32_t lane = threadIdx.x % 32;
-  if (r >= (uint64_t)s.batch * s.heads * s.q_len) return;
-  const uint32_t i = r % s.q_len, h = r / s.q_len % s.heads, b = r / s.q_len / s.heads, g = h / (s.heads / s.kv_heads);
-  int64_t n = s.keys(b);
-  if (s.causal) n = min(n, (int64_t)i + s.k_len - s.q_len + 1);
-  float a[kPer], acc[kPer] = {}, top = -INFINITY, sum = 0.0f;
-  load_row(q.row<T>(b, h, i), s.dim, lane, a);
-  for (int64_t j = 0; j < n; ++j) {
-    float kk[kPer], vv[kPer];
-    load_row(k.row<T>(b, g, j), s.dim, lane, kk);
-    load_row(v.row<T>(b, g, j), s.dim, lane, vv);
-    const float x = dot(a, kk) * s.scale;
-    const float m = fmaxf(top, x);
-    const float f = top == m ? 1.0f : expf(top - m), p = x == m ? 1.0f : expf(x - m);
-    top = m;
-    sum = sum * f + p;
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f + p * vv[c];
+// Leaves the role it stands in; the second form for warps that go on together.
+#define CSW_WAIT(bar, parity)      \
+  if (!bar_wait(bar, parity)) {    \
+    give_up(flag);                 \
+    return;                        \
   }
-#pragma unroll
-  for (int c = 0; c < kPer; ++c) acc[c] = n > 0 ? acc[c] / sum : 0.0f;
-  store_row(o.row<T>(b, h, i), s.dim, lane, acc);
-  if (lane == 0) lse[r] = n > 0 ? top + logf(sum) : -INFINITY;
-}
-
-// dq, and D for the other kernel
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps)
-    attention_dq_kernel(Shape s, View q, View k, View v, View o, View dout, const float* lse, View dq, float* delta) {
-  pdl_wait();
-  const uint64_t r = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const uint32_t lane = threadIdx.x % 32;
-  if (r >= (uint64_t)s.batch * s.heads * s.q_len) return;
-  const uint32_t i = r % s.q_len, h = r / s.q_len % s.heads, b = r / s.q_len / s.heads, g = h / (s.heads / s.kv_heads);
-  int64_t n = s.keys(b);
-  if (s.causal) n = min(n, (int64_t)i + s.k_len - s.q_len + 1);
-  float a[kPer], out[kPer], d[kPer], acc[kPer] = {};
-  load_row(q.row<T>(b, h, i), s.dim, lane, a);
-  load_row(o.row<T>(b, h, i), s.dim, lane, out);
-  load_row(dout.row<T>(b, h, i), s.dim, lane, d);
-  const float D = dot(out, d), L = lse[r];
-  if (lane == 0) delta[r] = D;
-  for (int64_t j = 0; j < n; ++j) {
-    float kk[kPer], vv[kPer];
-    load_row(k.row<T>(b, g, j), s.dim, lane, kk);
-    load_row(v.row<T>(b, g, j), s.dim, lane, vv);
-    const float p = expf(dot(a, kk) * s.scale - L);
-    const float ds = p * (dot(d, vv) - D) * s.scale;
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] += ds * kk[c];
+#define CSW_WAIT_WARP(bar, parity)                              \
+  if (!__all_sync(0xffffffffu, bar_wait(bar, parity))) {        \
+    give_up(flag);                                              \
+    return;                                                     \
   }
-  store_row(dq.row<T>(b, h, i), s.dim, lane, acc);
-}
 
 template <class T>
-__global__ void __launch_bounds__(32 * kWarps) attention_dkv_kernel(Shape s, View q, View k, View v, View dout,
-                                                                    const float* lse, const float* delta, View dk,
-                                                                    View dv) {
-  pdl_wait();
-  const uint64_t r = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const uint32_t lane = threadIdx.x % 32;
-  if (r >= (uint64_t)s.batch * s.kv_heads * s.k_len) return;
-  const uint32_t j = r % s.k_len, g = r / s.k_len % s.kv_heads, b = r / s.k_len / s.kv_heads;
-  const uint32_t share = s.heads / s.kv_heads;
-  float kk[kPer], vv[kPer], ak[kPer] = {}, av[kPer] = {};
-  load_row(k.row<T>(b, g, j), s.dim, lane, kk);
-  load_row(v.row<T>(b, g, j), s.dim, lane, vv);
-  int64_t first = j < s.keys(b) ? 0 : s.q_len;
-  if (s.causal) first = max(first, (int64_t)j - s.k_len + s.q_len);
-  for (uint32_t h = g * share; h < (g + 1) * share; ++h) {
-    for (int64_t i = first; i < s.q_len; ++i) {
-      float a[kPer], d[kPer];
-      load_row(q.row<T>(b, h, i), s.dim, lane, a);
-      load_row(dout.row<T>(b, h, i), s.dim, lane, d);
-      const uint64_t at = ((uint64_t)b * s.heads + h) * s.q_len + i;
-      const float p = expf(dot(a, kk) * s.scale - lse[at]);
-      const float ds = p * (dot(d, vv) - delta[at]) * s.scale;
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <class T>
+constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+
+// 32 columns of an accumulator, times f, to 32 values of a row of `dim`
+template <class T>
+__device__ __forceinline__ void store_columns(T* row, uint32_t at, uint32_t dim, const uint32_t* r, float f) {
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) ak[c] += ds * a[c], av[c] += p * d[c];
+  for (int i = 0; i < 32; i += 8) {
+    if (at + i < dim) {
+      uint4 v;
+      v.x = pack2<T>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
+      v.y = pack2<T>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
+      v.z = pack2<T>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
+      v.w = pack2<T>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
+      *reinterpret_cast<uint4*>(row + at + i) = v;
     }
   }
-  store_row(dk.row<T>(b, g, j), s.dim, lane, ak);
-  store_row(dv.row<T>(b, g, j), s.dim, lane, av);
 }
 
-unsigned blocks_for(uint64_t rows) { return (unsigned)((rows + kWarps - 1) / kWarps); }
+// All columns of a tile's rows [first, 128), zeroed by 128 threads: what lies behind a sequence must not meet the
+// zeros of its probabilities as a NaN.
+template <int DP>
+__device__ __forceinline__ void zero_rows(char* tile, int first, int thread) {
+  if (thread >= first) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(tile + c * kChunk + thread * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+  async_fence();
+}
+
+template <int DP>
+__device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int head,
+                                            int batch) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) copy_tile(dst + c * kChunk, map, bar, c * 64, token, head, batch);
+}
+// acc (+)= A B^T: both read along their rows, the reduction over the head's dimension
+template <int DP>
+__device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t b, uint32_t desc) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const uint32_t at = k / 4 * kChunk + k % 4 * 32;
+    mma(acc, tile_desc(a + at, 16), tile_desc(b + at, 16), desc, k > 0);
+  }
+}
+// acc (+)= P B: P in tensor memory, B read across its rows, the reduction over 128 tokens.  P's first 64 columns lie
+// at p, the others at p + half.
+template <int DP>
+__device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
+                                               bool add) {
+#pragma unroll
+  for (int k = 0; k < kTile / 16; ++k)
+    mma_tmem(acc, p + k / 4 * half + k % 4 * 8, tile_desc(b + k * 2048, kChunk), desc, add || k > 0);
+}
+
+// Dynamic shared memory begins anywhere; the tiles lie on 1024 bytes.
+__device__ __forceinline__ char* tiles_of(char* raw) {
+  return raw + ((1024 - (smem_at(raw) & 1023)) & 1023);
+}
+
+// What every kernel ends with, also where a wait ran out: copies on their way get time to land, tensor memory is freed.
+template <int COLUMNS>
+__device__ __forceinline__ void leave(uint32_t* flag, uint32_t tmem, bool owner) {
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (*reinterpret_cast<volatile uint32_t*>(flag))
+    for (int i = 0; i < 1000; ++i) __nanosleep(10000);
+  if (owner) tmem_free<COLUMNS>(tmem);
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+struct Forward {
+  CUtensorMap q, k, v;
+  Shape s;
+  View o;
+  float* lse;
+};
+
+// NWG tiles of 128 queries a CTA; columns of tensor memory: the scores of each, then the sums of each.
+template <int DP, int NWG>
+struct ForwardPlan {
+  static constexpr int kThreads = NWG * 128 + 64;
+  static constexpr uint32_t kTileBytes = kTile * DP * 2;
+  static constexpr int kStages = 4;
+  static constexpr size_t kShared = (NWG + kStages) * kTileBytes + 1024;
+  static constexpr int kColumns = NWG * (128 + DP) > 256 ? 512 : 256;
+};
+
+template <class T, int DP, int NWG>
+__global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 : 1)
+    attention_forward_kernel(const __grid_constant__ Forward a) {
+  using Plan = ForwardPlan<DP, NWG>;
+  extern __shared__ char raw[];
+  __shared__ uint64_t bars[1 + 2 * Plan::kStages + 3 * NWG];
+  __shared__ uint32_t tmem_at, flag_word;
+  char* tiles = tiles_of(raw);
+  const uint32_t tiles_at = smem_at(tiles);
+  const uint32_t q_full = smem_at(bars), full = q_full + 8, empty = full + 8 * Plan::kStages,
+                 s_full = empty + 8 * Plan::kStages, p_ready = s_full + 8 * NWG, o_full = p_ready + 8 * NWG;
+  uint32_t* flag = &flag_word;
+  const int warp = threadIdx.x / 32;
+
+  if (threadIdx.x == 0) {
+    bar_init(q_full, 1);
+    for (int i = 0; i < Plan::kStages; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+    for (int i = 0; i < NWG; ++i) bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 128), bar_init(o_full + 8 * i, 1);
+    init_visible();
+    flag_word = 0;
+  }
+  if (warp == 4 * NWG + 1) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  fence_before();
+  __syncthreads();
+  fence_after();
+  pdl_wait();
+  const uint32_t tmem = tmem_at;
+
+  // the last tiles of a causal mask see the most keys: they go first
+  const Shape& s = a.s;
+  const uint32_t per = s.batch * s.heads, tiles_q = gridDim.x / per;
+  const uint32_t bh = blockIdx.x % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
+  const int q0 = (int)(tiles_q - 1 - blockIdx.x / per) * NWG * kTile;
+  const int keys = s.keys(b);
+  int count[NWG], most = 0;  // tiles of keys that each tile of queries sees
+#pragma unroll
+  for (int w = 0; w < NWG; ++w) {
+    const int first = q0 + w * kTile;
+    count[w] = first < (int)s.q_len ? (s.limit(min(first + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile : 0;
+    most = max(most, count[w]);
+  }
+  const uint32_t ring = tiles_at + NWG * Plan::kTileBytes;
+
+  if (warp == 4 * NWG) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || most == 0) return;
+      bar_expect(q_full, NWG * Plan::kTileBytes);
+#pragma unroll
+      for (int w = 0; w < NWG; ++w)
+        copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, q0 + w * kTile, h, b);
+      for (int i = 0; i < 2 * most; ++i) {  // k 0, v 0, k 1, v 1, ...
+        const int stage = i % Plan::kStages;
+        if (i >= Plan::kStages) CSW_WAIT(empty + 8 * stage, (i / Plan::kStages - 1) & 1);
+        bar_expect(full + 8 * stage, Plan::kTileBytes);
+        copy_tokens<DP>(ring + stage * Plan::kTileBytes, i % 2 ? &a.v : &a.k, full + 8 * stage, i / 2 * kTile, g, b);
+      }
+    }();
+  } else if (warp == 4 * NWG + 1) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || most == 0) return;
+      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
+      const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
+      CSW_WAIT(q_full, 0);
+      for (int j = 0; j <= most; ++j) {
+        const int k = 2 * j % Plan::kStages, v = (2 * j - 1 + Plan::kStages) % Plan::kStages;
+        if (j < most) CSW_WAIT(full + 8 * k, 2 * j / Plan::kStages & 1);
+        if (j > 0) CSW_WAIT(full + 8 * v, (2 * j - 1) / Plan::kStages & 1);
+#pragma unroll
+        for (int w = 0; w < NWG; ++w) {
+          const uint32_t sw = tmem + w * 128, ow = tmem + NWG * 128 + w * DP;
+          if (j > 0 && j <= count[w]) {
+            CSW_WAIT(p_ready + 8 * w, (j - 1) & 1);
+            fence_after();
+            product_tokens<DP>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
+            if (j == count[w]) commit(o_full + 8 * w);
+          }
+          if (j < count[w]) {
+            product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores);
+            commit(s_full + 8 * w);
+          }
+        }
+        if (j < most) commit(empty + 8 * k);
+        if (j > 0) commit(empty + 8 * v);
+      }
+    }();
+  } else {
+    const int w = warp / 4, t = threadIdx.x % 128;
+    const int row = q0 + w * kTile + t;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t sw = tmem + w * 128 + lanes, ow = tmem + NWG * 128 + w * DP + lanes;
+    const int n = NWG == 1 || w == 0 ? count[0] : count[NWG - 1];
+    [&] {
+      const int limit = s.limit(row, keys), least = s.limit(q0 + w * kTile, keys);
+      float top = -INFINITY, sum = 0.0f;
+      for (int j = 0; j < n; ++j) {
+        CSW_WAIT_WARP(s_full + 8 * w, j & 1);
+        fence_after();
+        uint32_t r[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load32(sw + 32 * i, r + 32 * i);
+        wait_loads();
+        if ((j + 1) * kTile > least) {
+          const int end = limit - j * kTile;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= end) r[i] = 0xff800000u;
+        }
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(r[i]);
+#pragma unroll
+        for (int i = 4; i < 128; ++i) m[i % 4] = fmaxf(m[i % 4], __uint_as_float(r[i]));
+        const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        // The maximum is followed only where it grows by more than 2^8: the sums' exponents have room for that, and
+        // so has float16, whose largest number is 2^16.
+        if (__any_sync(0xffffffffu, (now - top) * s.exponent > 8.0f)) {
+          const float next = fmaxf(top, now);
+          const float f = next == -INFINITY ? 1.0f : exp2_fast((top - next) * s.exponent);
+          top = next;
+          sum *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              load32(ow + c, o);
+              wait_loads();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              store32(ow + c, o);
+            }
+          }
+        }
+        const float shift = top == -INFINITY ? 0.0f : top * s.exponent;
+        float add[4] = {};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i]), s.exponent, -shift));
+            const float y = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i + 1]), s.exponent, -shift));
+            add[i % 2] += x, add[2 + i % 2] += y;
+            p[i] = pack2<T>(x, y);
+          }
+          store16(sw + 16 * q, p);
+        }
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        // the tile of values that the sequence ends in, once for all that read it
+        if (s.lens && (j + 1) * kTile > keys && (w == 0 || j >= count[0])) {
+          const int i = 2 * j + 1, stage = i % Plan::kStages;
+          CSW_WAIT_WARP(full + 8 * stage, i / Plan::kStages & 1);
+          zero_rows<DP>(tiles + (NWG + stage) * Plan::kTileBytes, keys - j * kTile, t);
+        }
+        wait_stores();
+        fence_before();
+        bar_arrive(p_ready + 8 * w);
+      }
+      if (n > 0) {
+        CSW_WAIT_WARP(o_full + 8 * w, 0);
+        fence_after();
+      }
+      const bool stored = row < (int)s.q_len;
+      T* out = stored ? a.o.row<T>(b, h, row) : nullptr;
+      const float f = n == 0 || sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32] = {};
+        if (n > 0) {
+          load32(ow + c, o);
+          wait_loads();
+        }
+        if (stored) store_columns(out, c, s.dim, o, f);
+      }
+      if (stored) a.lse[(uint64_t)bh * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
+    }();
+  }
+  leave<Plan::kColumns>(flag, tmem, warp == 4 * NWG + 1);
+}
+
+// ---- backward: D and the exponents' shifts --------------------------------------------------------------------------
+// rows[0]: log2(e) L, +inf for a row that sees nothing and behind the last row, so that its probabilities are zero;
+// rows[1]: D.  Both per head, padded to whole tiles.
+template <class T>
+__global__ void __launch_bounds__(256) attention_rows_kernel(Shape s, View o, View dout, const float* lse, float* rows,
+                                                             uint32_t padded, uint32_t lanes) {
+  pdl_wait();
+  const uint64_t r = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / lanes, total = (uint64_t)s.batch * s.heads * padded;
+  const uint32_t lane = threadIdx.x % lanes, i = r % padded, bh = r / padded;
+  float d = 0.0f;
+  if (r < total && i < s.q_len && lane * 8 < s.dim) {
+    float x[8], y[8];
+    load_pack(o.row<T>(bh / s.heads, bh % s.heads, i) + lane * 8, x);
+    load_pack(dout.row<T>(bh / s.heads, bh % s.heads, i) + lane * 8, y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) d += x[k] * y[k];
+  }
+  for (uint32_t k = lanes / 2; k; k /= 2) d += __shfl_xor_sync(0xffffffffu, d, k);
+  if (r < total && lane == 0) {
+    const float l = i < s.q_len ? lse[(uint64_t)bh * s.q_len + i] : -INFINITY;
+    rows[r] = l == -INFINITY ? INFINITY : l * kLog2e;
+    rows[total + r] = l == -INFINITY ? 0.0f : d;
+  }
+}
+
+struct Backward {
+  CUtensorMap q, k, v, dout;
+  Shape s;
+  View dq, dk, dv;
+  const float* rows;
+  uint32_t padded;
+};
+
+// Both kernels: 256 threads for the scores (two a row, 64 columns each), one tile of tensor memory for s, one for dp,
+// then the sums.  Two tiles stay in shared memory; the others come in pairs, two pairs in flight.
+template <int DP>
+struct BackwardPlan {
+  static constexpr int kThreads = 256 + 64;
+  static constexpr uint32_t kTileBytes = kTile * DP * 2;
+  static constexpr size_t kShared = 6 * kTileBytes + 1024;
+  static constexpr int kColumns = 512;
+};
+
+// ds = p (dp - D) for 32 columns, rounded and packed over the dp that it came from
+template <class T>
+__device__ __forceinline__ void to_gradients(const float* p, const uint32_t* dp, const float* d, uint32_t* out) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    out[i] = pack2<T>(p[2 * i] * (__uint_as_float(dp[2 * i]) - d[2 * i]),
+                      p[2 * i + 1] * (__uint_as_float(dp[2 * i + 1]) - d[2 * i + 1]));
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_kernel(const __grid_constant__ Backward a) {
+  using Plan = BackwardPlan<DP>;
+  extern __shared__ char raw[];
+  __shared__ uint64_t bars[10];
+  __shared__ uint32_t tmem_at, flag_word;
+  char* tiles = tiles_of(raw);
+  const uint32_t tiles_at = smem_at(tiles);
+  const uint32_t q_full = smem_at(bars), full = q_full + 8, empty = full + 16, s_full = empty + 16, s_free = s_full + 8,
+                 dp_full = s_free + 8, ds_ready = dp_full + 8, done = ds_ready + 8;
+  uint32_t* flag = &flag_word;
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    bar_init(q_full, 1), bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
+    bar_init(done, 1);
+    for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+    init_visible();
+    flag_word = 0;
+  }
+  if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  fence_before();
+  __syncthreads();
+  fence_after();
+  pdl_wait();
+  const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256;
+
+  const Shape& s = a.s;
+  const uint32_t per = s.batch * s.heads, tiles_q = gridDim.x / per;
+  const uint32_t bh = blockIdx.x % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
+  const int q0 = (int)(tiles_q - 1 - blockIdx.x / per) * kTile;
+  const int keys = s.keys(b);
+  const int n = (s.limit(min(q0 + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile;
+  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // q, do, then k and v, twice
+
+  if (warp == 8) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || n == 0) return;
+      bar_expect(q_full, 2 * Plan::kTileBytes);
+      copy_tokens<DP>(tiles_at, &a.q, q_full, q0, h, b);
+      copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, q0, h, b);
+      for (int j = 0; j < n; ++j) {
+        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (j % 2);
+        if (j >= 2) CSW_WAIT(empty + 8 * (j % 2), (j / 2 - 1) & 1);
+        bar_expect(bar, 2 * Plan::kTileBytes);
+        copy_tokens<DP>(at, &a.k, bar, j * kTile, g, b);
+        copy_tokens<DP>(at + Plan::kTileBytes, &a.v, bar, j * kTile, g, b);
+      }
+    }();
+  } else if (warp == 9) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || n == 0) return;
+      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
+      const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
+      CSW_WAIT(q_full, 0);
+      CSW_WAIT(full, 0);
+      product_rows<DP>(s_at, tiles_at, ring, scores);
+      commit(s_full);
+      product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, ring + Plan::kTileBytes, slopes);
+      commit(dp_full);
+      for (int j = 0; j < n; ++j) {
+        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, next = ring + (j + 1) % 2 * 2 * Plan::kTileBytes;
+        if (j + 1 < n) {
+          CSW_WAIT(full + 8 * ((j + 1) % 2), (j + 1) / 2 & 1);
+          CSW_WAIT(s_free, j & 1);
+          fence_after();
+          product_rows<DP>(s_at, tiles_at, next, scores);
+          commit(s_full);
+        }
+        CSW_WAIT(ds_ready, j & 1);
+        fence_after();
+        product_tokens<DP>(dq_at, dp_at, 64, at, sums, j > 0);
+        commit(empty + 8 * (j % 2));
+        if (j + 1 < n) {
+          product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, next + Plan::kTileBytes, slopes);
+          commit(dp_full);
+        }
+      }
+      commit(done);
+    }();
+  } else {
+    const int w = warp / 4, t = threadIdx.x % 128, row = q0 + t;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    [&] {
+      const int limit = s.limit(row, keys), least = s.limit(q0, keys);
+      // padded to whole tiles: every thread has a row
+      const float* mine = a.rows + (uint64_t)bh * a.padded + row;
+      const float shift = mine[0], d = mine[(uint64_t)per * a.padded];
+      for (int j = 0; j < n; ++j) {
+        CSW_WAIT_WARP(s_full, j & 1);
+        fence_after();
+        float p[64];
+        {
+          uint32_t r[64];
+          load32(s_at + 64 * w + lanes, r);
+          load32(s_at + 64 * w + 32 + lanes, r + 32);
+          wait_loads();
+          fence_before();
+          bar_arrive(s_free);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) p[i] = exp2_fast(fmaf(__uint_as_float(r[i]), s.exponent, -shift));
+        }
+        const bool masked = (j + 1) * kTile > least;
+        const int end = limit - j * kTile - 64 * w;
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= end) p[i] = 0.0f;
+        }
+        CSW_WAIT_WARP(dp_full, j & 1);
+        fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32], out[16];
+          float dd[32];
+          load32(dp_at + 64 * w + 32 * c + lanes, r);
+          wait_loads();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * c + i >= end) r[i] = 0;  // of a key behind the sequence: whatever its value held
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) dd[i] = d;
+          to_gradients<T>(p + 32 * c, r, dd, out);
+          store16(dp_at + 64 * w + 16 * c + lanes, out);
+        }
+        if (w == 0 && s.lens && (j + 1) * kTile > keys) {
+          CSW_WAIT_WARP(full + 8 * (j % 2), j / 2 & 1);
+          zero_rows<DP>(tiles + (2 + j % 2 * 2) * Plan::kTileBytes, keys - j * kTile, t);
+        }
+        wait_stores();
+        fence_before();
+        bar_arrive(ds_ready);
+      }
+      if (n > 0) {
+        CSW_WAIT_WARP(done, 0);
+        fence_after();
+      }
+      const bool stored = row < (int)s.q_len;
+      const bool live = n > 0 && shift != INFINITY;
+      T* out = stored ? a.dq.row<T>(b, h, row) : nullptr;
+#pragma unroll
+      for (int c = 0; c < DP / 2; c += 32) {
+        const int at = w * (DP / 2) + c;
+        uint32_t r[32] = {};
+        if (n > 0) {
+          load32(dq_at + at + lanes, r);
+          wait_loads();
+        }
+        if (!live) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        if (stored) store_columns(out, at, s.dim, r, s.scale);
+      }
+    }();
+  }
+  leave<Plan::kColumns>(flag, tmem, warp == 9);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
+  using Plan = BackwardPlan<DP>;
+  extern __shared__ char raw[];
+  __shared__ uint64_t bars[10];
+  __shared__ __align__(16) float rows[2][2][kTile];  // of each pair in flight: the exponents' shifts, D
+  __shared__ uint32_t tmem_at, flag_word;
+  char* tiles = tiles_of(raw);
+  const uint32_t tiles_at = smem_at(tiles);
+  const uint32_t kv_full = smem_at(bars), full = kv_full + 8, empty = full + 16, s_full = empty + 16,
+                 p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8, done = ds_ready + 8;
+  uint32_t* flag = &flag_word;
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    bar_init(kv_full, 1), bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
+    bar_init(done, 1);
+    for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+    init_visible();
+    flag_word = 0;
+  }
+  if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  fence_before();
+  __syncthreads();
+  fence_after();
+  pdl_wait();
+  const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = dv_at + DP;
+
+  // the first keys of a causal mask are seen by the most queries: they go first
+  const Shape& s = a.s;
+  const uint32_t per = s.batch * s.kv_heads, bg = blockIdx.x % per, b = bg / s.kv_heads, g = bg % s.kv_heads;
+  const int k0 = (int)(blockIdx.x / per) * kTile, keys = s.keys(b);
+  const uint32_t share = s.heads / s.kv_heads;
+  // query i sees key j from i = j - (k_len - q_len) on
+  const int from = s.causal ? max(k0 - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
+  const int tiles_q = ((int)s.q_len + kTile - 1) / kTile, each = k0 < keys ? max(tiles_q - from, 0) : 0;
+  const int n = each * (int)share;
+  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // k, v, then q and do, twice
+
+  if (warp == 8) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || n == 0) return;
+      bar_expect(kv_full, 2 * Plan::kTileBytes);
+      copy_tokens<DP>(tiles_at, &a.k, kv_full, k0, g, b);
+      copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, k0, g, b);
+      const uint64_t plane = (uint64_t)s.batch * s.heads * a.padded;
+      int i = from;
+      uint32_t h = g * share;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (j % 2);
+        if (j >= 2) CSW_WAIT(empty + 8 * (j % 2), (j / 2 - 1) & 1);
+        bar_expect(bar, 2 * Plan::kTileBytes + 2 * kTile * 4);
+        copy_tokens<DP>(at, &a.q, bar, i * kTile, h, b);
+        copy_tokens<DP>(at + Plan::kTileBytes, &a.dout, bar, i * kTile, h, b);
+        const float* src = a.rows + ((uint64_t)b * s.heads + h) * a.padded + (uint64_t)i * kTile;
+        copy_bytes(smem_at(rows[j % 2][0]), src, kTile * 4, bar);
+        copy_bytes(smem_at(rows[j % 2][1]), src + plane, kTile * 4, bar);
+        if (++i == tiles_q) i = from, ++h;
+      }
+    }();
+  } else if (warp == 9) {
+    [&] {
+      if (threadIdx.x % 32 != 0 || n == 0) return;
+      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
+      const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
+      CSW_WAIT(kv_full, 0);
+      CSW_WAIT(full, 0);
+      product_rows<DP>(s_at, tiles_at, ring, scores);
+      commit(s_full);
+      product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, ring + Plan::kTileBytes, slopes);
+      commit(dp_full);
+      for (int j = 0; j < n; ++j) {
+        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, next = ring + (j + 1) % 2 * 2 * Plan::kTileBytes;
+        CSW_WAIT(p_ready, j & 1);
+        fence_after();
+        product_tokens<DP>(dv_at, s_at, 64, at + Plan::kTileBytes, sums, j > 0);
+        if (j + 1 < n) {
+          CSW_WAIT(full + 8 * ((j + 1) % 2), (j + 1) / 2 & 1);
+          product_rows<DP>(s_at, tiles_at, next, scores);
+          commit(s_full);
+        }
+        CSW_WAIT(ds_ready, j & 1);
+        fence_after();
+        product_tokens<DP>(dk_at, dp_at, 64, at, sums, j > 0);
+        commit(empty + 8 * (j % 2));
+        if (j + 1 < n) {
+          product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, next + Plan::kTileBytes, slopes);
+          commit(dp_full);
+        }
+      }
+      commit(done);
+    }();
+  } else {
+    const int w = warp / 4, t = threadIdx.x % 128, row = k0 + t;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    [&] {
+      const int sees = s.causal ? row - ((int)s.k_len - (int)s.q_len) : INT32_MIN;  // the first query that sees this key
+      int i = from;
+      for (int j = 0; j < n; ++j) {
+        CSW_WAIT_WARP(full + 8 * (j % 2), j / 2 & 1);  // the rows' numbers
+        CSW_WAIT_WARP(s_full, j & 1);
+        fence_after();
+        float p[64];
+        const float4* shifts = reinterpret_cast<const float4*>(rows[j % 2][0] + 64 * w);
+        const float4* deltas = reinterpret_cast<const float4*>(rows[j % 2][1] + 64 * w);
+        {
+          uint32_t r[64];
+          load32(s_at + 64 * w + lanes, r);
+          load32(s_at + 64 * w + 32 + lanes, r + 32);
+          wait_loads();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float4 f = shifts[k];
+            p[4 * k] = exp2_fast(fmaf(__uint_as_float(r[4 * k]), s.exponent, -f.x));
+            p[4 * k + 1] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 1]), s.exponent, -f.y));
+            p[4 * k + 2] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 2]), s.exponent, -f.z));
+            p[4 * k + 3] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 3]), s.exponent, -f.w));
+          }
+        }
+        const int begin = sees - i * kTile - 64 * w;
+        if (s.causal && k0 + kTile - 1 - ((int)s.k_len - (int)s.q_len) > i * kTile) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k)
+            if (k < begin) p[k] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t out[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
+          store16(s_at + 64 * w + 16 * c + lanes, out);
+        }
+        wait_stores();
+        fence_before();
+        bar_arrive(p_ready);
+
+        CSW_WAIT_WARP(dp_full, j & 1);
+        fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32], out[16];
+          float d[32];
+          load32(dp_at + 64 * w + 32 * c + lanes, r);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 f = deltas[8 * c + k];
+            d[4 * k] = f.x, d[4 * k + 1] = f.y, d[4 * k + 2] = f.z, d[4 * k + 3] = f.w;
+          }
+          wait_loads();
+          to_gradients<T>(p + 32 * c, r, d, out);
+          store16(dp_at + 64 * w + 16 * c + lanes, out);
+        }
+        wait_stores();
+        fence_before();
+        bar_arrive(ds_ready);
+        if (++i == tiles_q) i = from;
+      }
+      if (n > 0) {
+        CSW_WAIT_WARP(done, 0);
+        fence_after();
+      }
+      // A key behind its sequence has no gradient, whatever its row of the tile held.
+      const bool stored = row < (int)s.k_len, live = n > 0 && row < keys;
+      T* out = stored ? (w == 0 ? a.dv : a.dk).template row<T>(b, g, row) : nullptr;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32] = {};
+        if (n > 0) {
+          load32((w == 0 ? dv_at : dk_at) + c + lanes, r);
+          wait_loads();
+        }
+        if (!live) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        if (stored) store_columns(out, c, s.dim, r, w == 0 ? 1.0f : s.scale);
+      }
+    }();
+  }
+  leave<Plan::kColumns>(flag, tmem, warp == 9);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+Shape shape_of(const csw_attention_shape& s) {
+  const float e = fmaxf(fabsf(s.scale) * kLog2e, 0x1p-100f);
+  return {(uint32_t)s.batch, (uint32_t)s.heads, (uint32_t)s.kv_heads, (uint32_t)s.q_len, (uint32_t)s.k_len,
+          (uint32_t)s.dim,   s.causal,          s.scale < 0.0f,       s.scale,           e, s.kv_lens};
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+  static const Encode f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (taken(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r)) != cudaSuccess) return Encode();
+    return r == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(p) : Encode();
+  }();
+  return f;
+}
+
+// Describing a tensor for tile copies is a call of the driver, which needs the device's context on this thread; a
+// thread that has made no call of the runtime yet (autograd's, say) has none.
+cudaError_t bind_context() {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  return taken(e == cudaSuccess ? cudaSetDevice(dev) : e);
+}
+
+// tiles of 128 tokens x 64 columns of an operand
+bool map_of(CUtensorMap* map, const csw_attention_operand& o, const csw_attention_shape& s, uint64_t heads, uint64_t tokens) {
+  const Encode encode = encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {s.dim, tokens, heads, s.batch};
+  // the stride of an axis of one step is not looked at, but has to be one
+  auto bytes = [](ptrdiff_t stride, uint64_t n) { return n > 1 && stride > 0 ? (cuuint64_t)stride * 2 : (cuuint64_t)16; };
+  const cuuint64_t strides[3] = {bytes(o.token_stride, tokens), bytes(o.head_stride, heads), bytes(o.batch_stride, s.batch)};
+  const cuuint32_t box[4] = {64, kTile, 1, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, s.type == CSW_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                o.data, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class A>
+cudaError_t run(void (*kernel)(const A), uint64_t grid, int threads, size_t shared, cudaStream_t stream, const A& a) {
+  const cudaError_t e = taken(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+  return e != cudaSuccess ? e : pdl_launch(kernel, (unsigned)grid, threads, shared, stream, a);
+}
+
+template <class T, int DP, int NWG>
+cudaError_t forward(const Forward& a, const csw_attention_shape& s, cudaStream_t stream) {
+  using Plan = ForwardPlan<DP, NWG>;
+  const uint64_t grid = (s.q_len + NWG * kTile - 1) / (NWG * kTile) * s.batch * s.heads;
+  return run(attention_forward_kernel<T, DP, NWG>, grid, Plan::kThreads, Plan::kShared, stream, a);
+}
+template <class T>
+cudaError_t forward_of(const Forward& a, const csw_attention_shape& s, cudaStream_t stream) {
+  return s.dim <= 64 ? forward<T, 64, 1>(a, s, stream) : forward<T, 128, 2>(a, s, stream);
+}
+
+template <class T, int DP>
+cudaError_t backward(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
+  using Plan = BackwardPlan<DP>;
+  cudaError_t e = cudaSuccess;
+  if (s.q_len)
+    e = run(attention_dq_kernel<T, DP>, (s.q_len + kTile - 1) / kTile * s.batch * s.heads, Plan::kThreads, Plan::kShared,
+            stream, a);
+  if (e == cudaSuccess && s.k_len)
+    e = run(attention_dkv_kernel<T, DP>, (s.k_len + kTile - 1) / kTile * s.batch * s.kv_heads, Plan::kThreads,
+            Plan::kShared, stream, a);
+  return e;
+}
+template <class T>
+cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
+  return s.dim <= 64 ? backward<T, 64>(a, s, stream) : backward<T, 128>(a, s, stream);
+}
+
+cudaError_t take_status(int* value) {
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(value, attention_gave_up, sizeof(int));
+  if (e == cudaSuccess && *value) e = cudaMemcpyToSymbol(attention_gave_up, &zero, sizeof(int));
+  return e;
+}
+const bool registered = (take_kernel_status = take_status, true);
 
 }  // namespace
+
+uint64_t attention_padded(uint64_t q_len) { return (q_len + kTile - 1) / kTile * kTile; }
 
 cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_attention_operand& q,
                                      const csw_attention_operand& k, const csw_attention_operand& v,
                                      const csw_attention_operand& o, float* lse, cudaStream_t stream) {
-  const uint64_t rows = (uint64_t)s.batch * s.heads * s.q_len;
-  if (rows == 0) return cudaSuccess;
-  const auto kernel = s.type == CSW_TYPE_F16 ? attention_forward_kernel<__half> : attention_forward_kernel<__nv_bfloat16>;
-  return pdl_launch(kernel, blocks_for(rows), 32 * kWarps, 0, stream, shape_of(s), view_of(q), view_of(k), view_of(v),
-                    view_of(o), lse);
+  if (s.batch == 0 || s.q_len == 0) return cudaSuccess;
+  if (const cudaError_t e = bind_context()) return e;
+  Forward a;
+  a.s = shape_of(s), a.o = view_of(o), a.lse = lse;
+  if (!map_of(&a.q, q, s, s.heads, s.q_len)) return cudaErrorInvalidValue;
+  a.k = a.v = a.q;  // without keys nothing is copied from them
+  if (s.k_len && (!map_of(&a.k, k, s, s.kv_heads, s.k_len) || !map_of(&a.v, v, s, s.kv_heads, s.k_len)))
+    return cudaErrorInvalidValue;
+  return s.type == CSW_TYPE_F16 ? forward_of<__half>(a, s, stream) : forward_of<__nv_bfloat16>(a, s, stream);
 }
 
-cudaError_t attention_backward_launch(const csw_attention_shape& s, const AttentionBackward& a, cudaStream_t stream) {
-  const uint64_t q_rows = (uint64_t)s.batch * s.heads * s.q_len, k_rows = (uint64_t)s.batch * s.kv_heads * s.k_len;
-  cudaError_t e = cudaSuccess;
+cudaError_t attention_backward_launch(const csw_attention_shape& s, const AttentionBackward& b, cudaStream_t stream) {
+  if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return cudaSuccess;
+  if (const cudaError_t e = bind_context()) return e;
+  Backward a;
+  a.s = shape_of(s), a.dq = view_of(b.dq), a.dk = view_of(b.dk), a.dv = view_of(b.dv);
+  a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
   const bool half = s.type == CSW_TYPE_F16;
-  if (q_rows)
-    e = pdl_launch(half ? attention_dq_kernel<__half> : attention_dq_kernel<__nv_bfloat16>, blocks_for(q_rows),
-                   32 * kWarps, 0, stream, shape_of(s), view_of(a.q), view_of(a.k), view_of(a.v), view_of(a.o),
-                   view_of(a.dout), a.lse, view_of(a.dq), a.delta);
-  if (e == cudaSuccess && k_rows)
-    e = pdl_launch(half ? attention_dkv_kernel<__half> : attention_dkv_kernel<__nv_bfloat16>, blocks_for(k_rows),
-                   32 * kWarps, 0, stream, shape_of(s), view_of(a.q), view_of(a.k), view_of(a.v), view_of(a.dout),
-                   a.lse, (const float*)a.delta, view_of(a.dk), view_of(a.dv));
-  return e;
+  a.q = a.k = a.v = a.dout = CUtensorMap{};  // of an empty side nothing is copied
+  if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len)))
+    return cudaErrorInvalidValue;
+  if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len)))
+    return cudaErrorInvalidValue;
+  if (s.q_len) {
+    uint32_t lanes = 1;
+    while (lanes * 8 < s.dim) lanes *= 2;
+    const uint64_t threads = (uint64_t)s.batch * s.heads * a.padded * lanes;
+    const cudaError_t e =
+        pdl_launch(half ? attention_rows_kernel<__half> : attention_rows_kernel<__nv_bfloat16>,
+                   (unsigned)((threads + 255) / 256), 256, 0, stream, a.s, view_of(b.o), view_of(b.dout), b.lse, b.rows,
+                   a.padded, lanes);
+    if (e != cudaSuccess) return e;
+  }
+  return half ? backward_of<__half>(a, s, stream) : backward_of<__nv_bfloat16>(a, s, stream);
 }
 
 }  // namespace csw

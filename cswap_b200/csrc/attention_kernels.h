@@ -15,8 +15,9 @@ cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_att
 struct AttentionBackward {
   csw_attention_operand q, k, v, o, dout, dq, dk, dv;
   const float* lse;
-  float* delta;  // workspace: batch x heads x q_len
+  float* rows;  // workspace: 2 x batch x heads x attention_padded(q_len)
 };
+uint64_t attention_padded(uint64_t q_len);
 cudaError_t attention_backward_launch(const csw_attention_shape& s, const AttentionBackward& a, cudaStream_t stream);
 
 }  // namespace csw

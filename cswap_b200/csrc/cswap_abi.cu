@@ -19,6 +19,7 @@
 namespace csw {
 
 thread_local int tl_cuda_error = 0;
+cudaError_t (*take_kernel_status)(int* value) = nullptr;
 
 csw_status cuda_fail(cudaError_t e) {
   tl_cuda_error = (int)e;
@@ -104,6 +105,9 @@ csw_status csw_device_status(csw_stream_t stream) {
   int h = 0;
   e = cudaMemcpy(&h, d_status, sizeof(int), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(e);
+  int waits = 0;
+  if (take_kernel_status && (e = take_kernel_status(&waits)) != cudaSuccess) return cuda_fail(e);
+  if (waits != 0) return CSW_ERR_TIMEOUT;
   if (h != 0) {
     e = cudaMemset(d_status, 0, sizeof(int));
     if (e != cudaSuccess) return cuda_fail(e);

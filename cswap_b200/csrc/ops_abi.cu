@@ -144,7 +144,7 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
 
 csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes) {
   if (!bytes || !attention_args(shape)) return CSW_ERR_ARG;
-  *bytes = shape->batch * shape->heads * shape->q_len * sizeof(float);
+  *bytes = 2 * shape->batch * shape->heads * attention_padded(shape->q_len) * sizeof(float);
   return CSW_OK;
 }
 
@@ -161,7 +161,7 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
     if (!operand(p, shape, s.q_len)) return CSW_ERR_ARG;
   for (const csw_attention_operand* p : {k, v, dk, dv})
     if (!operand(p, shape, s.k_len)) return CSW_ERR_ARG;
-  if (need && (!good(d_lse, CSW_TYPE_F32) || !good(d_workspace, CSW_TYPE_F32))) return CSW_ERR_ARG;
+  if (need && (!good(d_lse, CSW_TYPE_F32) || !d_workspace || !aligned(d_workspace, 16))) return CSW_ERR_ARG;
   if (workspace_bytes < need) return CSW_ERR_SIZE;
   return done(attention_backward_launch(s, {*q, *k, *v, *o, *dout, *dq, *dk, *dv, d_lse, (float*)d_workspace}, stream));
 }

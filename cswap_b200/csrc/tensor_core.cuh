@@ -1,0 +1,153 @@
+// The instructions that the attention kernels are built on: mbarriers, tile copies (TMA), and the fifth-generation
+// tensor cores with their accumulators in tensor memory (tcgen05).
+//
+// Every wait on an mbarrier is bounded: where it runs out, the kernel sets a status word that the host reads
+// (csw_device_status), its warps leave their loops, and it frees its tensor memory and returns.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace csw {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- mbarriers ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// true once the phase of this parity is over; false where it does not end within two seconds or so
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  const long long start = clock64();
+  do {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  } while (clock64() - start < (1ll << 32));
+  return false;
+}
+__device__ __forceinline__ void init_visible() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+// shared memory written by ordinary stores, before the tensor cores or a tile copy see it
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- copies into shared memory -------------------------------------------------------------------------------------
+// a tile of [dim, token, head, batch] coordinates; dim is a multiple of 8 two-byte values (16 bytes)
+__device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int dim, int token, int head,
+                                          int batch) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(dim), "r"(token), "r"(head), "r"(batch)
+      : "memory");
+}
+// bytes (a multiple of 16) from a 16-byte boundary
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// ---- tensor memory -------------------------------------------------------------------------------------------------
+// by one whole warp; the address arrives at *at in shared memory
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_alloc(uint32_t at) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "n"(COLUMNS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define CSW_R4(a, i) a(i), a(i + 1), a(i + 2), a(i + 3)
+#define CSW_R16(a, i) CSW_R4(a, i), CSW_R4(a, i + 4), CSW_R4(a, i + 8), CSW_R4(a, i + 12)
+#define CSW_R32(a, i) CSW_R16(a, i), CSW_R16(a, i + 16)
+#define CSW_OUT(i) "=r"(r[i])
+#define CSW_IN(i) "r"(r[i])
+// 32 columns of the lane that is this thread's (lane 32 (warp % 4) + thread % 32; `at` names the warp's first lane)
+__device__ __forceinline__ void load32(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : CSW_R32(CSW_OUT, 0)
+      : "r"(at));
+}
+__device__ __forceinline__ void store32(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::CSW_R32(CSW_IN, 0),
+      "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::CSW_R16(CSW_IN, 0),
+      "r"(at)
+      : "memory");
+}
+#undef CSW_R4
+#undef CSW_R16
+#undef CSW_R32
+#undef CSW_OUT
+#undef CSW_IN
+
+// ---- products ------------------------------------------------------------------------------------------------------
+// Tiles in shared memory are rows of 128 bytes, swizzled over 8 rows as the tile copies leave them.  Read along its
+// rows (the reduction runs along a row), 16 two-byte values of the reduction are 32 bytes further in the row; read
+// across them (the reduction runs over rows), they are 16 rows, 2048 bytes, further on.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lbo) {
+  return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// 128 x N products of two-byte values, sums in float32.  across: the second operand's tile is read across its rows.
+__host__ __device__ constexpr uint32_t product_desc(bool bf16, int n, bool across, bool negate) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (negate ? 1u << 13 : 0u) | (across ? 1u << 16 : 0u) |
+         (uint32_t)(n / 8) << 17 | (uint32_t)(128 / 16) << 24;
+}
+// one reduction step of 16: both operands in shared memory
+__device__ __forceinline__ void mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+// the first operand in tensor memory, two values a column
+__device__ __forceinline__ void mma_tmem(uint32_t acc, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(acc),
+      "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+// arrives at `bar` when all products issued before have ended
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace tc
+}  // namespace csw
