@@ -99,19 +99,18 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 template <class T>
 constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
 
-// 32 columns of an accumulator, times f, to 32 values of a row of `dim`
+// 32 columns of an accumulator, times f, to columns [at, at + 32) of row `row` of a tile of 64, swizzled as the tile
+// copies want it
 template <class T>
-__device__ __forceinline__ void store_columns(T* row, uint32_t at, uint32_t dim, const uint32_t* r, float f) {
+__device__ __forceinline__ void stage_columns(char* tile, int row, int at, const uint32_t* r, float f) {
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
-    if (at + i < dim) {
-      uint4 v;
-      v.x = pack2<T>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
-      v.y = pack2<T>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
-      v.z = pack2<T>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
-      v.w = pack2<T>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
-      *reinterpret_cast<uint4*>(row + at + i) = v;
-    }
+    uint4 v;
+    v.x = pack2<T>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
+    v.y = pack2<T>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
+    v.z = pack2<T>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
+    v.w = pack2<T>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((at + i) / 8) ^ (row & 7)) * 16) = v;
   }
 }
 
@@ -154,9 +153,36 @@ __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_
     mma_tmem(acc, p + k / 4 * half + k % 4 * 8, tile_desc(b + k * 2048, kChunk), desc, add || k > 0);
 }
 
-// Dynamic shared memory begins anywhere; the tiles lie on 1024 bytes.
-__device__ __forceinline__ char* tiles_of(char* raw) {
-  return raw + ((1024 - (smem_at(raw) & 1023)) & 1023);
+// ---- a CTA's work -----------------------------------------------------------------------------------------------------
+// The grid has a CTA for each piece of work (a tile of queries or keys of one head).  One that is done takes over the
+// piece of a CTA that has not started, so that copies and products of the next piece begin while the softmax warps still
+// write the last one, whatever lengths the sequences have.  The copying warp asks, and tells the others two pieces
+// ahead: the piece, -1 at the end, and its sequence's number of keys.
+struct Work {
+  uint4 answer;
+  int2 piece[2];
+  uint64_t bars[5];  // the answer's; told and read, for each of the two
+};
+struct WorkBars {
+  uint32_t answer, answered, told, read;
+  __device__ explicit WorkBars(Work& w)
+      : answer(smem_at(&w.answer)), answered(smem_at(w.bars)), told(answered + 8), read(answered + 24) {}
+  // one thread, once; `warps` of them listen
+  __device__ void init(int warps) const {
+    bar_init(answered, 1);
+    for (int i = 0; i < 2; ++i) bar_init(told + 8 * i, 1), bar_init(read + 8 * i, warps);
+  }
+};
+// What a listening warp (or one lane that stands for it) hears as its i-th piece; false where a wait ran out.
+__device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, int i, bool whole_warp, int2* piece) {
+  bool ok = bar_wait(bars.told + 8 * (i % 2), i / 2 & 1);
+  if (whole_warp) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  const volatile int* told = &w.piece[i % 2].x;
+  *piece = make_int2(told[0], told[1]);
+  if (whole_warp) __syncwarp();
+  if (!whole_warp || threadIdx.x % 32 == 0) bar_arrive(bars.read + 8 * (i % 2));
+  return true;
 }
 
 // What every kernel ends with, also where a wait ran out: copies on their way get time to land, tensor memory is freed.
@@ -171,199 +197,296 @@ __device__ __forceinline__ void leave(uint32_t* flag, uint32_t tmem, bool owner)
   if (owner) tmem_free<COLUMNS>(tmem);
 }
 
+// The copying warp's lane over all its pieces: f(piece, keys, i) copies what the i-th piece needs, and returns false
+// where a wait ran out.
+template <class F>
+__device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_t* flag, F&& f) {
+  int2 piece = make_int2(blockIdx.x, 0);
+  for (int i = 0;; ++i) {
+    if (i >= 2) CSW_WAIT(bars.read + 8 * (i % 2), (i / 2 - 1) & 1);
+    if (piece.x >= 0) piece.y = f.keys(piece.x);
+    w.piece[i % 2] = piece;
+    bar_arrive(bars.told + 8 * (i % 2));
+    if (piece.x < 0) return;
+    if (!f.copy(piece)) {
+      give_up(flag);
+      return;
+    }
+    // Not earlier: a piece that is taken waits until this one is done, however long that is.
+    bar_expect(bars.answered, 16);
+    take_next(bars.answer, bars.answered);
+    CSW_WAIT(bars.answered, i & 1);
+    piece.x = taken_index(bars.answer);
+    async_fence();  // the answer is read before the next one is written
+  }
+}
+
+// A tile of 64 columns that `threads` threads have staged goes to memory; one of them, `first`, stores.
+__device__ __forceinline__ void stage_free(bool first, int id, int threads) {
+  if (first) stores_read();
+  group_sync(id, threads);
+}
+__device__ __forceinline__ void stage_out(bool first, int id, int threads, const CUtensorMap* map, uint32_t tile, int dim,
+                                          int token, int head, int batch) {
+  async_fence();
+  group_sync(id, threads);
+  if (first) store_tile(map, tile, dim, token, head, batch);
+}
+
 // ---- forward --------------------------------------------------------------------------------------------------------
 struct Forward {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o;
   Shape s;
-  View o;
   float* lse;
 };
 
-// NWG tiles of 128 queries a CTA; columns of tensor memory: the scores of each, then the sums of each.
+// NWG tiles of 128 queries a CTA; columns of tensor memory: the scores of each, then the sums of each.  Shared memory:
+// the queries, a ring of key and value tiles, and 64 columns of results of each.
 template <int DP, int NWG>
 struct ForwardPlan {
   static constexpr int kThreads = NWG * 128 + 64;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
   static constexpr int kStages = 4;
-  static constexpr size_t kShared = (NWG + kStages) * kTileBytes + 1024;
+  static constexpr size_t kShared = (NWG + kStages) * kTileBytes + NWG * kChunk;
   static constexpr int kColumns = NWG * (128 + DP) > 256 ? 512 : 256;
+};
+
+// Piece `index` of the forward grid.  The last tiles of a causal mask see the most keys: they go first.
+template <int NWG>
+struct Queries {
+  uint32_t bh, b, h, g;
+  int q0, count[NWG], most;  // tiles of keys that each tile of queries sees
+  __device__ Queries(const Shape& s, int index, int keys) {
+    const uint32_t per = s.batch * s.heads, tiles = gridDim.x / per;
+    bh = index % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
+    q0 = (int)(tiles - 1 - index / per) * NWG * kTile;
+    most = 0;
+#pragma unroll
+    for (int w = 0; w < NWG; ++w) {
+      const int first = q0 + w * kTile;
+      count[w] = first < (int)s.q_len ? (s.limit(min(first + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile : 0;
+      most = max(most, count[w]);
+    }
+  }
 };
 
 template <class T, int DP, int NWG>
 __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 : 1)
     attention_forward_kernel(const __grid_constant__ Forward a) {
   using Plan = ForwardPlan<DP, NWG>;
-  extern __shared__ char raw[];
-  __shared__ uint64_t bars[1 + 2 * Plan::kStages + 3 * NWG];
+  extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
+  __shared__ Work work;
+  __shared__ uint64_t bars[2 + 2 * Plan::kStages + 4 * NWG];
   __shared__ uint32_t tmem_at, flag_word;
-  char* tiles = tiles_of(raw);
   const uint32_t tiles_at = smem_at(tiles);
-  const uint32_t q_full = smem_at(bars), full = q_full + 8, empty = full + 8 * Plan::kStages,
-                 s_full = empty + 8 * Plan::kStages, p_ready = s_full + 8 * NWG, o_full = p_ready + 8 * NWG;
+  const WorkBars work_bars(work);
+  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 8 * Plan::kStages,
+                 s_full = empty + 8 * Plan::kStages, p_ready = s_full + 8 * NWG, o_full = p_ready + 8 * NWG,
+                 o_free = o_full + 8 * NWG;
   uint32_t* flag = &flag_word;
   const int warp = threadIdx.x / 32;
 
   if (threadIdx.x == 0) {
-    bar_init(q_full, 1);
+    work_bars.init(1 + 4 * NWG);
+    bar_init(q_full, 1), bar_init(q_empty, 1);
     for (int i = 0; i < Plan::kStages; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
-    for (int i = 0; i < NWG; ++i) bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 128), bar_init(o_full + 8 * i, 1);
+    for (int i = 0; i < NWG; ++i) {
+      bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 128);
+      bar_init(o_full + 8 * i, 1), bar_init(o_free + 8 * i, 128);
+    }
     init_visible();
     flag_word = 0;
   }
   if (warp == 4 * NWG + 1) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  if (warp == 4 * NWG && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.k), prefetch_map(&a.v);
   fence_before();
   __syncthreads();
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at;
-
-  // the last tiles of a causal mask see the most keys: they go first
   const Shape& s = a.s;
-  const uint32_t per = s.batch * s.heads, tiles_q = gridDim.x / per;
-  const uint32_t bh = blockIdx.x % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
-  const int q0 = (int)(tiles_q - 1 - blockIdx.x / per) * NWG * kTile;
-  const int keys = s.keys(b);
-  int count[NWG], most = 0;  // tiles of keys that each tile of queries sees
-#pragma unroll
-  for (int w = 0; w < NWG; ++w) {
-    const int first = q0 + w * kTile;
-    count[w] = first < (int)s.q_len ? (s.limit(min(first + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile : 0;
-    most = max(most, count[w]);
-  }
   const uint32_t ring = tiles_at + NWG * Plan::kTileBytes;
 
   if (warp == 4 * NWG) {
-    [&] {
-      if (threadIdx.x % 32 != 0 || most == 0) return;
-      bar_expect(q_full, NWG * Plan::kTileBytes);
+    struct Copies {
+      const Forward& a;
+      uint32_t tiles_at, ring, q_full, q_empty, full, empty;
+      int i = 0, u = 0;  // tiles of the ring, pieces with any
+      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.heads) / a.s.heads); }
+      __device__ bool copy(int2 piece) {
+        const Queries<NWG> at(a.s, piece.x, piece.y);
+        if (at.most == 0) return true;
+        if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
+        bar_expect(q_full, NWG * Plan::kTileBytes);
 #pragma unroll
-      for (int w = 0; w < NWG; ++w)
-        copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, q0 + w * kTile, h, b);
-      for (int i = 0; i < 2 * most; ++i) {  // k 0, v 0, k 1, v 1, ...
-        const int stage = i % Plan::kStages;
-        if (i >= Plan::kStages) CSW_WAIT(empty + 8 * stage, (i / Plan::kStages - 1) & 1);
-        bar_expect(full + 8 * stage, Plan::kTileBytes);
-        copy_tokens<DP>(ring + stage * Plan::kTileBytes, i % 2 ? &a.v : &a.k, full + 8 * stage, i / 2 * kTile, g, b);
+        for (int w = 0; w < NWG; ++w)
+          copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, at.q0 + w * kTile, at.h, at.b);
+        for (int j = 0; j < 2 * at.most; ++j, ++i) {  // k 0, v 0, k 1, v 1, ...
+          const int stage = i % Plan::kStages;
+          if (i >= Plan::kStages && !bar_wait(empty + 8 * stage, (i / Plan::kStages - 1) & 1)) return false;
+          bar_expect(full + 8 * stage, Plan::kTileBytes);
+          copy_tokens<DP>(ring + stage * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * stage, j / 2 * kTile, at.g, at.b);
+        }
+        ++u;
+        return true;
       }
-    }();
+    };
+    if (threadIdx.x % 32 == 0)
+      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 4 * NWG + 1) {
     [&] {
-      if (threadIdx.x % 32 != 0 || most == 0) return;
+      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      CSW_WAIT(q_full, 0);
-      for (int j = 0; j <= most; ++j) {
-        const int k = 2 * j % Plan::kStages, v = (2 * j - 1 + Plan::kStages) % Plan::kStages;
-        if (j < most) CSW_WAIT(full + 8 * k, 2 * j / Plan::kStages & 1);
-        if (j > 0) CSW_WAIT(full + 8 * v, (2 * j - 1) / Plan::kStages & 1);
+      int base = 0, u = 0, tile[NWG] = {}, done[NWG] = {};  // of the ring; pieces; of each tile of queries: tiles, pieces
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const Queries<NWG> at(s, piece.x, piece.y);
+        if (at.most == 0) continue;
+        CSW_WAIT(q_full, u & 1);
+        for (int j = 0; j <= at.most; ++j) {
+          const int ki = base + 2 * j, vi = ki - 1, k = ki % Plan::kStages, v = vi % Plan::kStages;
+          if (j < at.most) CSW_WAIT(full + 8 * k, ki / Plan::kStages & 1);
+          if (j > 0) CSW_WAIT(full + 8 * v, vi / Plan::kStages & 1);
 #pragma unroll
-        for (int w = 0; w < NWG; ++w) {
-          const uint32_t sw = tmem + w * 128, ow = tmem + NWG * 128 + w * DP;
-          if (j > 0 && j <= count[w]) {
-            CSW_WAIT(p_ready + 8 * w, (j - 1) & 1);
-            fence_after();
-            product_tokens<DP>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
-            if (j == count[w]) commit(o_full + 8 * w);
+          for (int w = 0; w < NWG; ++w) {
+            const uint32_t sw = tmem + w * 128, ow = tmem + NWG * 128 + w * DP;
+            if (j > 0 && j <= at.count[w]) {
+              CSW_WAIT(p_ready + 8 * w, tile[w]++ & 1);
+              if (j == 1 && done[w] > 0) CSW_WAIT(o_free + 8 * w, (done[w] - 1) & 1);
+              fence_after();
+              product_tokens<DP>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
+              if (j == at.count[w]) commit(o_full + 8 * w), ++done[w];
+            }
+            if (j < at.count[w]) {
+              product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores);
+              commit(s_full + 8 * w);
+            }
           }
-          if (j < count[w]) {
-            product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores);
-            commit(s_full + 8 * w);
-          }
+          if (j < at.most) commit(empty + 8 * k);
+          if (j > 0) commit(empty + 8 * v);
+          if (j + 1 == at.most) commit(q_empty);
         }
-        if (j < most) commit(empty + 8 * k);
-        if (j > 0) commit(empty + 8 * v);
+        base += 2 * at.most, ++u;
       }
     }();
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
-    const int row = q0 + w * kTile + t;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t sw = tmem + w * 128 + lanes, ow = tmem + NWG * 128 + w * DP + lanes;
-    const int n = NWG == 1 || w == 0 ? count[0] : count[NWG - 1];
+    char* stage = tiles + (NWG + Plan::kStages) * Plan::kTileBytes + w * kChunk;
     [&] {
-      const int limit = s.limit(row, keys), least = s.limit(q0 + w * kTile, keys);
-      float top = -INFINITY, sum = 0.0f;
-      for (int j = 0; j < n; ++j) {
-        CSW_WAIT_WARP(s_full + 8 * w, j & 1);
-        fence_after();
-        uint32_t r[128];
+      int tile = 0, done = 0, base = 0;
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const Queries<NWG> at(s, piece.x, piece.y);
+        const int keys = piece.y, n = NWG == 1 || w == 0 ? at.count[0] : at.count[NWG - 1];
+        const int q0 = at.q0 + w * kTile, row = q0 + t;
+        const int limit = s.limit(row, keys), least = s.limit(q0, keys);
+        float top = -INFINITY, sum = 0.0f;
+        for (int j = 0; j < n; ++j) {
+          CSW_WAIT_WARP(s_full + 8 * w, tile & 1);
+          ++tile;
+          fence_after();
+          uint32_t r[128];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load32(sw + 32 * i, r + 32 * i);
-        wait_loads();
-        if ((j + 1) * kTile > least) {
-          const int end = limit - j * kTile;
+          for (int i = 0; i < 4; ++i) load32(sw + 32 * i, r + 32 * i);
+          wait_loads();
+          if ((j + 1) * kTile > least) {
+            const int end = limit - j * kTile;
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= end) r[i] = 0xff800000u;
-        }
-        float m[4];
+            for (int q = 0; q < 4; ++q) {
+              if (end < 32 * q + 32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(r[i]);
-#pragma unroll
-        for (int i = 4; i < 128; ++i) m[i % 4] = fmaxf(m[i % 4], __uint_as_float(r[i]));
-        const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        // The maximum is followed only where it grows by more than 2^8: the sums' exponents have room for that, and
-        // so has float16, whose largest number is 2^16.
-        if (__any_sync(0xffffffffu, (now - top) * s.exponent > 8.0f)) {
-          const float next = fmaxf(top, now);
-          const float f = next == -INFINITY ? 1.0f : exp2_fast((top - next) * s.exponent);
-          top = next;
-          sum *= f;
-          if (j > 0) {
-#pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t o[32];
-              load32(ow + c, o);
-              wait_loads();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              store32(ow + c, o);
+                for (int i = 32 * q; i < 32 * q + 32; ++i)
+                  if (i >= end) r[i] = 0xff800000u;
+              }
             }
           }
-        }
-        const float shift = top == -INFINITY ? 0.0f : top * s.exponent;
-        float add[4] = {};
+          float m[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t p[16];
+          for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(r[i]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float x = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i]), s.exponent, -shift));
-            const float y = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i + 1]), s.exponent, -shift));
-            add[i % 2] += x, add[2 + i % 2] += y;
-            p[i] = pack2<T>(x, y);
+          for (int i = 4; i < 128; ++i) m[i % 4] = fmaxf(m[i % 4], __uint_as_float(r[i]));
+          const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          // The maximum is followed only where it grows by more than 2^8: the sums' exponents have room for that, and
+          // so has float16, whose largest number is 2^16.
+          if (__any_sync(0xffffffffu, (now - top) * s.exponent > 8.0f)) {
+            const float next = fmaxf(top, now);
+            const float f = next == -INFINITY ? 1.0f : exp2_fast((top - next) * s.exponent);
+            top = next;
+            sum *= f;
+            if (j > 0) {
+#pragma unroll
+              for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                load32(ow + c, o);
+                wait_loads();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                store32(ow + c, o);
+              }
+            }
           }
-          store16(sw + 16 * q, p);
-        }
-        sum += (add[0] + add[1]) + (add[2] + add[3]);
-        // the tile of values that the sequence ends in, once for all that read it
-        if (s.lens && (j + 1) * kTile > keys && (w == 0 || j >= count[0])) {
-          const int i = 2 * j + 1, stage = i % Plan::kStages;
-          CSW_WAIT_WARP(full + 8 * stage, i / Plan::kStages & 1);
-          zero_rows<DP>(tiles + (NWG + stage) * Plan::kTileBytes, keys - j * kTile, t);
-        }
-        wait_stores();
-        fence_before();
-        bar_arrive(p_ready + 8 * w);
-      }
-      if (n > 0) {
-        CSW_WAIT_WARP(o_full + 8 * w, 0);
-        fence_after();
-      }
-      const bool stored = row < (int)s.q_len;
-      T* out = stored ? a.o.row<T>(b, h, row) : nullptr;
-      const float f = n == 0 || sum == 0.0f ? 0.0f : 1.0f / sum;
+          const float shift = top == -INFINITY ? 0.0f : top * s.exponent;
+          float add[4] = {};
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32] = {};
-        if (n > 0) {
-          load32(ow + c, o);
-          wait_loads();
+          for (int q = 0; q < 4; ++q) {
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i]), s.exponent, -shift));
+              const float y = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i + 1]), s.exponent, -shift));
+              add[i % 2] += x, add[2 + i % 2] += y;
+              p[i] = pack2<T>(x, y);
+            }
+            store16(sw + 16 * q, p);
+          }
+          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          // the tile of values that the sequence ends in, once for all that read it
+          if (s.lens && (j + 1) * kTile > keys && (w == 0 || j >= at.count[0])) {
+            const int i = base + 2 * j + 1, slot = i % Plan::kStages;
+            CSW_WAIT_WARP(full + 8 * slot, i / Plan::kStages & 1);
+            zero_rows<DP>(tiles + (NWG + slot) * Plan::kTileBytes, keys - j * kTile, t);
+          }
+          wait_stores();
+          fence_before();
+          bar_arrive(p_ready + 8 * w);
         }
-        if (stored) store_columns(out, c, s.dim, o, f);
+        base += 2 * at.most;
+        if (n > 0) {
+          CSW_WAIT_WARP(o_full + 8 * w, done & 1);
+          ++done;
+          fence_after();
+        }
+        const float f = n == 0 || sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (row < (int)s.q_len)
+          a.lse[(uint64_t)at.bh * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
+#pragma unroll
+        for (int c = 0; c < DP; c += 64) {
+          stage_free(t == 0, 1 + w, 128);
+#pragma unroll
+          for (int i = 0; i < 64; i += 32) {
+            uint32_t o[32] = {};
+            if (n > 0) {
+              load32(ow + c + i, o);
+              wait_loads();
+            }
+            stage_columns<T>(stage, t, i, o, f);
+          }
+          if (n > 0 && c + 64 == DP) {
+            fence_before();
+            bar_arrive(o_free + 8 * w);
+          }
+          stage_out(t == 0 && q0 < (int)s.q_len, 1 + w, 128, &a.o, smem_at(stage), c, q0, at.h, at.b);
+        }
       }
-      if (stored) a.lse[(uint64_t)bh * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
     }();
+    if (t == 0) stores_read();
   }
   leave<Plan::kColumns>(flag, tmem, warp == 4 * NWG + 1);
 }
@@ -394,371 +517,475 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(Shape s, View o, Vi
 }
 
 struct Backward {
-  CUtensorMap q, k, v, dout;
+  CUtensorMap q, k, v, dout, dq, dk, dv;
   Shape s;
-  View dq, dk, dv;
-  const float* rows;
+  float* rows;
   uint32_t padded;
 };
 
 // Both kernels: 256 threads for the scores (two a row, 64 columns each), one tile of tensor memory for s, one for dp,
-// then the sums.  Two tiles stay in shared memory; the others come in pairs, two pairs in flight.
+// then the sums.  Two tiles stay in shared memory for a piece; the others come in pairs, two pairs in flight; 64 columns
+// of results for each half of the threads.
 template <int DP>
 struct BackwardPlan {
   static constexpr int kThreads = 256 + 64;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
-  static constexpr size_t kShared = 6 * kTileBytes + 1024;
+  static constexpr size_t kShared = 6 * kTileBytes + 2 * kChunk;
   static constexpr int kColumns = 512;
 };
 
-// ds = p (dp - D) for 32 columns, rounded and packed over the dp that it came from
+// ds = p (dp - D) for 32 columns, rounded and packed over the dp that it came from; their sum
 template <class T>
-__device__ __forceinline__ void to_gradients(const float* p, const uint32_t* dp, const float* d, uint32_t* out) {
+__device__ __forceinline__ float to_gradients(const float* p, const uint32_t* dp, const float* d, uint32_t* out) {
+  float sum[2] = {};
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    out[i] = pack2<T>(p[2 * i] * (__uint_as_float(dp[2 * i]) - d[2 * i]),
-                      p[2 * i + 1] * (__uint_as_float(dp[2 * i + 1]) - d[2 * i + 1]));
+  for (int i = 0; i < 16; ++i) {
+    const float x = p[2 * i] * (__uint_as_float(dp[2 * i]) - d[2 * i]);
+    const float y = p[2 * i + 1] * (__uint_as_float(dp[2 * i + 1]) - d[2 * i + 1]);
+    sum[0] += x, sum[1] += y;
+    out[i] = pack2<T>(x, y);
+  }
+  return sum[0] + sum[1];
 }
 
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  extern __shared__ char raw[];
-  __shared__ uint64_t bars[10];
+  extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
+  __shared__ Work work;
+  __shared__ uint64_t bars[12];
+  __shared__ float halves[kTile];
   __shared__ uint32_t tmem_at, flag_word;
-  char* tiles = tiles_of(raw);
   const uint32_t tiles_at = smem_at(tiles);
-  const uint32_t q_full = smem_at(bars), full = q_full + 8, empty = full + 16, s_full = empty + 16, s_free = s_full + 8,
-                 dp_full = s_free + 8, ds_ready = dp_full + 8, done = ds_ready + 8;
+  const WorkBars work_bars(work);
+  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 16, s_full = empty + 16,
+                 s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8, dq_full = ds_ready + 8,
+                 dq_free = dq_full + 8;
   uint32_t* flag = &flag_word;
   const int warp = threadIdx.x / 32;
   if (threadIdx.x == 0) {
-    bar_init(q_full, 1), bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
-    bar_init(done, 1);
+    work_bars.init(9);
+    bar_init(q_full, 1), bar_init(q_empty, 1), bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1);
+    bar_init(ds_ready, 256), bar_init(dq_full, 1), bar_init(dq_free, 256);
     for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
   }
   if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
   fence_before();
   __syncthreads();
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256;
-
   const Shape& s = a.s;
-  const uint32_t per = s.batch * s.heads, tiles_q = gridDim.x / per;
-  const uint32_t bh = blockIdx.x % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
-  const int q0 = (int)(tiles_q - 1 - blockIdx.x / per) * kTile;
-  const int keys = s.keys(b);
-  const int n = (s.limit(min(q0 + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile;
   const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // q, do, then k and v, twice
 
   if (warp == 8) {
-    [&] {
-      if (threadIdx.x % 32 != 0 || n == 0) return;
-      bar_expect(q_full, 2 * Plan::kTileBytes);
-      copy_tokens<DP>(tiles_at, &a.q, q_full, q0, h, b);
-      copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, q0, h, b);
-      for (int j = 0; j < n; ++j) {
-        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (j % 2);
-        if (j >= 2) CSW_WAIT(empty + 8 * (j % 2), (j / 2 - 1) & 1);
-        bar_expect(bar, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(at, &a.k, bar, j * kTile, g, b);
-        copy_tokens<DP>(at + Plan::kTileBytes, &a.v, bar, j * kTile, g, b);
+    struct Copies {
+      const Backward& a;
+      uint32_t tiles_at, ring, q_full, q_empty, full, empty;
+      int i = 0, u = 0;  // pairs, pieces with any
+      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.heads) / a.s.heads); }
+      __device__ bool copy(int2 piece) {
+        const Queries<1> at(a.s, piece.x, piece.y);
+        if (at.most == 0) return true;
+        if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
+        bar_expect(q_full, 2 * Plan::kTileBytes);
+        copy_tokens<DP>(tiles_at, &a.q, q_full, at.q0, at.h, at.b);
+        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, at.q0, at.h, at.b);
+        for (int j = 0; j < at.most; ++j, ++i) {
+          const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
+          if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
+          bar_expect(bar, 2 * Plan::kTileBytes);
+          copy_tokens<DP>(to, &a.k, bar, j * kTile, at.g, at.b);
+          copy_tokens<DP>(to + Plan::kTileBytes, &a.v, bar, j * kTile, at.g, at.b);
+        }
+        ++u;
+        return true;
       }
-    }();
+    };
+    if (threadIdx.x % 32 == 0)
+      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 9) {
     [&] {
-      if (threadIdx.x % 32 != 0 || n == 0) return;
+      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      CSW_WAIT(q_full, 0);
-      CSW_WAIT(full, 0);
-      product_rows<DP>(s_at, tiles_at, ring, scores);
-      commit(s_full);
-      product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, ring + Plan::kTileBytes, slopes);
-      commit(dp_full);
-      for (int j = 0; j < n; ++j) {
-        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, next = ring + (j + 1) % 2 * 2 * Plan::kTileBytes;
-        if (j + 1 < n) {
-          CSW_WAIT(full + 8 * ((j + 1) % 2), (j + 1) / 2 & 1);
-          CSW_WAIT(s_free, j & 1);
-          fence_after();
-          product_rows<DP>(s_at, tiles_at, next, scores);
-          commit(s_full);
+      int i = 0, u = 0;
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const int n = Queries<1>(s, piece.x, piece.y).most;
+        if (n == 0) continue;
+        CSW_WAIT(q_full, u & 1);
+        // The scores' place is free once they have been read (s_free), that of dp behind the product that read it.
+        for (int j = -1; j < n; ++j, ++i) {
+          // i counts pairs from the one in front of this piece's first; its own numbers are one less
+          const int now = i - 1 - u, next = now + 1;
+          const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
+          if (j + 1 < n) {
+            CSW_WAIT(full + 8 * (next & 1), next / 2 & 1);
+            if (next > 0) CSW_WAIT(s_free, now & 1);
+            fence_after();
+            product_rows<DP>(s_at, tiles_at, then, scores);
+            commit(s_full);
+          }
+          if (j >= 0) {
+            CSW_WAIT(ds_ready, now & 1);
+            if (j == 0 && u > 0) CSW_WAIT(dq_free, (u - 1) & 1);
+            fence_after();
+            product_tokens<DP>(dq_at, dp_at, 64, at, sums, j > 0);
+            commit(empty + 8 * (now & 1));
+            if (j + 1 == n) commit(dq_full);
+          }
+          if (j + 1 < n) {
+            product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
+            commit(dp_full);
+            if (j + 2 == n) commit(q_empty);
+          }
         }
-        CSW_WAIT(ds_ready, j & 1);
-        fence_after();
-        product_tokens<DP>(dq_at, dp_at, 64, at, sums, j > 0);
-        commit(empty + 8 * (j % 2));
-        if (j + 1 < n) {
-          product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, next + Plan::kTileBytes, slopes);
-          commit(dp_full);
-        }
+        ++u;
       }
-      commit(done);
     }();
   } else {
-    const int w = warp / 4, t = threadIdx.x % 128, row = q0 + t;
+    const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    // 128 columns of results are staged as two tiles, 64 as one that all threads share
+    constexpr int kGroup = DP == 128 ? 128 : 256;
+    const int id = DP == 128 ? 1 + w : 1;
+    const bool first = DP == 128 ? t == 0 : threadIdx.x == 0;
+    char* stage = tiles + 6 * Plan::kTileBytes + (DP == 128 ? w * kChunk : 0);
     [&] {
-      const int limit = s.limit(row, keys), least = s.limit(q0, keys);
-      // padded to whole tiles: every thread has a row
-      const float* mine = a.rows + (uint64_t)bh * a.padded + row;
-      const float shift = mine[0], d = mine[(uint64_t)per * a.padded];
-      for (int j = 0; j < n; ++j) {
-        CSW_WAIT_WARP(s_full, j & 1);
-        fence_after();
-        float p[64];
-        {
-          uint32_t r[64];
-          load32(s_at + 64 * w + lanes, r);
-          load32(s_at + 64 * w + 32 + lanes, r + 32);
-          wait_loads();
-          fence_before();
-          bar_arrive(s_free);
+      int i = 0, u = 0;
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const Queries<1> at(s, piece.x, piece.y);
+        const int keys = piece.y, n = at.most, row = at.q0 + t;
+        const int limit = s.limit(row, keys), least = s.limit(at.q0, keys);
+        // padded to whole tiles: every thread has a row
+        float* mine = a.rows + (uint64_t)at.bh * a.padded + row;
+        float* d_at = mine + (uint64_t)s.batch * s.heads * a.padded;
+        const float shift = mine[0], d = *d_at;
+        float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
+        for (int j = 0; j < n; ++j, ++i) {
+          CSW_WAIT_WARP(s_full, i & 1);
+          fence_after();
+          float p[64];
+          {
+            uint32_t r[64];
+            load32(s_at + 64 * w + lanes, r);
+            load32(s_at + 64 * w + 32 + lanes, r + 32);
+            wait_loads();
+            fence_before();
+            bar_arrive(s_free);
 #pragma unroll
-          for (int i = 0; i < 64; ++i) p[i] = exp2_fast(fmaf(__uint_as_float(r[i]), s.exponent, -shift));
-        }
-        const bool masked = (j + 1) * kTile > least;
-        const int end = limit - j * kTile - 64 * w;
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= end) p[i] = 0.0f;
-        }
-        CSW_WAIT_WARP(dp_full, j & 1);
-        fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32], out[16];
-          float dd[32];
-          load32(dp_at + 64 * w + 32 * c + lanes, r);
-          wait_loads();
+            for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
+          }
+          const bool masked = (j + 1) * kTile > least;
+          const int end = limit - j * kTile - 64 * w;
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (32 * c + i >= end) r[i] = 0;  // of a key behind the sequence: whatever its value held
+            for (int k = 0; k < 64; ++k)
+              if (k >= end) p[k] = 0.0f;
           }
+          CSW_WAIT_WARP(dp_full, i & 1);
+          fence_after();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) dd[i] = d;
-          to_gradients<T>(p + 32 * c, r, dd, out);
-          store16(dp_at + 64 * w + 16 * c + lanes, out);
-        }
-        if (w == 0 && s.lens && (j + 1) * kTile > keys) {
-          CSW_WAIT_WARP(full + 8 * (j % 2), j / 2 & 1);
-          zero_rows<DP>(tiles + (2 + j % 2 * 2) * Plan::kTileBytes, keys - j * kTile, t);
-        }
-        wait_stores();
-        fence_before();
-        bar_arrive(ds_ready);
-      }
-      if (n > 0) {
-        CSW_WAIT_WARP(done, 0);
-        fence_after();
-      }
-      const bool stored = row < (int)s.q_len;
-      const bool live = n > 0 && shift != INFINITY;
-      T* out = stored ? a.dq.row<T>(b, h, row) : nullptr;
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32], out[16];
+            float dd[32];
+            load32(dp_at + 64 * w + 32 * c + lanes, r);
+            wait_loads();
+            if (masked) {
 #pragma unroll
-      for (int c = 0; c < DP / 2; c += 32) {
-        const int at = w * (DP / 2) + c;
-        uint32_t r[32] = {};
+              for (int k = 0; k < 32; ++k)
+                if (32 * c + k >= end) r[k] = 0;  // of a key behind the sequence: whatever its value held
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) dd[k] = d;
+            left += to_gradients<T>(p + 32 * c, r, dd, out);
+            store16(dp_at + 64 * w + 16 * c + lanes, out);
+          }
+          if (w == 0 && s.lens && (j + 1) * kTile > keys) {
+            CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);
+            zero_rows<DP>(tiles + (2 + (i & 1) * 2) * Plan::kTileBytes, keys - j * kTile, t);
+          }
+          wait_stores();
+          fence_before();
+          bar_arrive(ds_ready);
+        }
         if (n > 0) {
-          load32(dq_at + at + lanes, r);
-          wait_loads();
+          CSW_WAIT_WARP(dq_full, u & 1);
+          ++u;
+          fence_after();
         }
-        if (!live) {
+        const bool live = n > 0 && shift != INFINITY;
+        if (w == 1) halves[t] = left;
+        stage_free(first, id, kGroup);
+        constexpr int kMine = DP / 2;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = 0;
+        for (int c = 0; c < kMine; c += 32) {
+          uint32_t r[32] = {};
+          if (n > 0) {
+            load32(dq_at + w * kMine + c + lanes, r);
+            wait_loads();
+          }
+          if (!live) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = 0;
+          }
+          stage_columns<T>(stage, t, DP == 128 ? c : 32 * w, r, s.scale);
         }
-        if (stored) store_columns(out, at, s.dim, r, s.scale);
+        if (n > 0) {
+          fence_before();
+          bar_arrive(dq_free);
+        }
+        stage_out(first, id, kGroup, &a.dq, smem_at(stage), DP == 128 ? 64 * w : 0, at.q0, at.h, at.b);
+        if (DP == 128) group_sync(3, 256);
+        // The next kernel's D has no rounding of o in it: it is sum p dp, which this one has formed on the way.
+        if (w == 0 && live) *d_at = d + left + halves[t];
+        group_sync(3, 256);
       }
     }();
+    if (first) stores_read();
   }
   leave<Plan::kColumns>(flag, tmem, warp == 9);
 }
 
+// Piece `index` of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
+struct Keys {
+  uint32_t b, g;
+  int k0, from, tiles, n;  // the first tile of queries that sees any of them; tiles of queries; pairs in all
+  __device__ Keys(const Shape& s, int index, int keys) {
+    const uint32_t per = s.batch * s.kv_heads, bg = index % per;
+    b = bg / s.kv_heads, g = bg % s.kv_heads, k0 = (int)(index / per) * kTile;
+    // query i sees key j from i = j - (k_len - q_len) on
+    from = s.causal ? max(k0 - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
+    tiles = ((int)s.q_len + kTile - 1) / kTile;
+    n = (k0 < keys ? max(tiles - from, 0) : 0) * (int)(s.heads / s.kv_heads);
+  }
+};
+
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  extern __shared__ char raw[];
-  __shared__ uint64_t bars[10];
+  extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
+  __shared__ Work work;
+  __shared__ uint64_t bars[12];
   __shared__ __align__(16) float rows[2][2][kTile];  // of each pair in flight: the exponents' shifts, D
   __shared__ uint32_t tmem_at, flag_word;
-  char* tiles = tiles_of(raw);
-  const uint32_t tiles_at = smem_at(tiles);
-  const uint32_t kv_full = smem_at(bars), full = kv_full + 8, empty = full + 16, s_full = empty + 16,
-                 p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8, done = ds_ready + 8;
+  const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
+  const WorkBars work_bars(work);
+  const uint32_t kv_full = smem_at(bars), kv_empty = kv_full + 8, full = kv_full + 16, empty = full + 16,
+                 s_full = empty + 16, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
+                 sums_full = ds_ready + 8, sums_free = sums_full + 8;
   uint32_t* flag = &flag_word;
   const int warp = threadIdx.x / 32;
   if (threadIdx.x == 0) {
-    bar_init(kv_full, 1), bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
-    bar_init(done, 1);
+    work_bars.init(9);
+    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1);
+    bar_init(ds_ready, 256), bar_init(sums_full, 1), bar_init(sums_free, 256);
     for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
   }
   if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
   fence_before();
   __syncthreads();
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = dv_at + DP;
-
-  // the first keys of a causal mask are seen by the most queries: they go first
   const Shape& s = a.s;
-  const uint32_t per = s.batch * s.kv_heads, bg = blockIdx.x % per, b = bg / s.kv_heads, g = bg % s.kv_heads;
-  const int k0 = (int)(blockIdx.x / per) * kTile, keys = s.keys(b);
-  const uint32_t share = s.heads / s.kv_heads;
-  // query i sees key j from i = j - (k_len - q_len) on
-  const int from = s.causal ? max(k0 - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
-  const int tiles_q = ((int)s.q_len + kTile - 1) / kTile, each = k0 < keys ? max(tiles_q - from, 0) : 0;
-  const int n = each * (int)share;
   const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // k, v, then q and do, twice
 
   if (warp == 8) {
-    [&] {
-      if (threadIdx.x % 32 != 0 || n == 0) return;
-      bar_expect(kv_full, 2 * Plan::kTileBytes);
-      copy_tokens<DP>(tiles_at, &a.k, kv_full, k0, g, b);
-      copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, k0, g, b);
-      const uint64_t plane = (uint64_t)s.batch * s.heads * a.padded;
-      int i = from;
-      uint32_t h = g * share;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (j % 2);
-        if (j >= 2) CSW_WAIT(empty + 8 * (j % 2), (j / 2 - 1) & 1);
-        bar_expect(bar, 2 * Plan::kTileBytes + 2 * kTile * 4);
-        copy_tokens<DP>(at, &a.q, bar, i * kTile, h, b);
-        copy_tokens<DP>(at + Plan::kTileBytes, &a.dout, bar, i * kTile, h, b);
-        const float* src = a.rows + ((uint64_t)b * s.heads + h) * a.padded + (uint64_t)i * kTile;
-        copy_bytes(smem_at(rows[j % 2][0]), src, kTile * 4, bar);
-        copy_bytes(smem_at(rows[j % 2][1]), src + plane, kTile * 4, bar);
-        if (++i == tiles_q) i = from, ++h;
+    struct Copies {
+      const Backward& a;
+      uint32_t tiles_at, ring, rows_at, kv_full, kv_empty, full, empty;
+      int i = 0, u = 0;
+      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.kv_heads) / a.s.kv_heads); }
+      __device__ bool copy(int2 piece) {
+        const Keys at(a.s, piece.x, piece.y);
+        if (at.n == 0) return true;
+        if (u > 0 && !bar_wait(kv_empty, (u - 1) & 1)) return false;
+        bar_expect(kv_full, 2 * Plan::kTileBytes);
+        copy_tokens<DP>(tiles_at, &a.k, kv_full, at.k0, at.g, at.b);
+        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, at.k0, at.g, at.b);
+        const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
+        int q = at.from;
+        uint32_t h = at.g * (a.s.heads / a.s.kv_heads);
+        for (int j = 0; j < at.n; ++j, ++i) {
+          const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
+          if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
+          bar_expect(bar, 2 * Plan::kTileBytes + 2 * kTile * 4);
+          copy_tokens<DP>(to, &a.q, bar, q * kTile, h, at.b);
+          copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, bar, q * kTile, h, at.b);
+          const float* src = a.rows + ((uint64_t)at.b * a.s.heads + h) * a.padded + (uint64_t)q * kTile;
+          copy_bytes(rows_at + i % 2 * (8 * kTile), src, kTile * 4, bar);
+          copy_bytes(rows_at + i % 2 * (8 * kTile) + 4 * kTile, src + plane, kTile * 4, bar);
+          if (++q == at.tiles) q = at.from, ++h;
+        }
+        ++u;
+        return true;
       }
-    }();
+    };
+    if (threadIdx.x % 32 == 0)
+      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
   } else if (warp == 9) {
     [&] {
-      if (threadIdx.x % 32 != 0 || n == 0) return;
+      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      CSW_WAIT(kv_full, 0);
-      CSW_WAIT(full, 0);
-      product_rows<DP>(s_at, tiles_at, ring, scores);
-      commit(s_full);
-      product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, ring + Plan::kTileBytes, slopes);
-      commit(dp_full);
-      for (int j = 0; j < n; ++j) {
-        const uint32_t at = ring + j % 2 * 2 * Plan::kTileBytes, next = ring + (j + 1) % 2 * 2 * Plan::kTileBytes;
-        CSW_WAIT(p_ready, j & 1);
-        fence_after();
-        product_tokens<DP>(dv_at, s_at, 64, at + Plan::kTileBytes, sums, j > 0);
-        if (j + 1 < n) {
-          CSW_WAIT(full + 8 * ((j + 1) % 2), (j + 1) / 2 & 1);
-          product_rows<DP>(s_at, tiles_at, next, scores);
-          commit(s_full);
+      int i = 0, u = 0;
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const int n = Keys(s, piece.x, piece.y).n;
+        if (n == 0) continue;
+        CSW_WAIT(kv_full, u & 1);
+        // Each tile's place in tensor memory is written again behind the product that reads it.
+        for (int j = -1; j < n; ++j, ++i) {
+          const int now = i - 1 - u, next = now + 1;
+          const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
+          if (j >= 0) {
+            CSW_WAIT(p_ready, now & 1);
+            if (j == 0 && u > 0) CSW_WAIT(sums_free, (u - 1) & 1);
+            fence_after();
+            product_tokens<DP>(dv_at, s_at, 64, at + Plan::kTileBytes, sums, j > 0);
+          }
+          if (j + 1 < n) {
+            CSW_WAIT(full + 8 * (next & 1), next / 2 & 1);
+            product_rows<DP>(s_at, tiles_at, then, scores);
+            commit(s_full);
+          }
+          if (j >= 0) {
+            CSW_WAIT(ds_ready, now & 1);
+            fence_after();
+            product_tokens<DP>(dk_at, dp_at, 64, at, sums, j > 0);
+            commit(empty + 8 * (now & 1));
+            if (j + 1 == n) commit(sums_full);
+          }
+          if (j + 1 < n) {
+            product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
+            commit(dp_full);
+            if (j + 2 == n) commit(kv_empty);
+          }
         }
-        CSW_WAIT(ds_ready, j & 1);
-        fence_after();
-        product_tokens<DP>(dk_at, dp_at, 64, at, sums, j > 0);
-        commit(empty + 8 * (j % 2));
-        if (j + 1 < n) {
-          product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, next + Plan::kTileBytes, slopes);
-          commit(dp_full);
-        }
+        ++u;
       }
-      commit(done);
     }();
   } else {
-    const int w = warp / 4, t = threadIdx.x % 128, row = k0 + t;
+    const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    char* stage = tiles + 6 * Plan::kTileBytes + w * kChunk;
     [&] {
-      const int sees = s.causal ? row - ((int)s.k_len - (int)s.q_len) : INT32_MIN;  // the first query that sees this key
-      int i = from;
-      for (int j = 0; j < n; ++j) {
-        CSW_WAIT_WARP(full + 8 * (j % 2), j / 2 & 1);  // the rows' numbers
-        CSW_WAIT_WARP(s_full, j & 1);
-        fence_after();
-        float p[64];
-        const float4* shifts = reinterpret_cast<const float4*>(rows[j % 2][0] + 64 * w);
-        const float4* deltas = reinterpret_cast<const float4*>(rows[j % 2][1] + 64 * w);
-        {
-          uint32_t r[64];
-          load32(s_at + 64 * w + lanes, r);
-          load32(s_at + 64 * w + 32 + lanes, r + 32);
-          wait_loads();
+      int i = 0, u = 0;
+      for (int it = 0;; ++it) {
+        int2 piece;
+        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
+        if (piece.x < 0) return;
+        const Keys at(s, piece.x, piece.y);
+        const int n = at.n, row = at.k0 + t, off = (int)s.k_len - (int)s.q_len;
+        int q = at.from;
+        for (int j = 0; j < n; ++j, ++i) {
+          CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);  // the rows' numbers
+          CSW_WAIT_WARP(s_full, i & 1);
+          fence_after();
+          float p[64];
+          const float4* shifts = reinterpret_cast<const float4*>(rows[i & 1][0] + 64 * w);
+          const float4* deltas = reinterpret_cast<const float4*>(rows[i & 1][1] + 64 * w);
+          {
+            uint32_t r[64];
+            load32(s_at + 64 * w + lanes, r);
+            load32(s_at + 64 * w + 32 + lanes, r + 32);
+            wait_loads();
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float4 f = shifts[k];
-            p[4 * k] = exp2_fast(fmaf(__uint_as_float(r[4 * k]), s.exponent, -f.x));
-            p[4 * k + 1] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 1]), s.exponent, -f.y));
-            p[4 * k + 2] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 2]), s.exponent, -f.z));
-            p[4 * k + 3] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 3]), s.exponent, -f.w));
+            for (int k = 0; k < 16; ++k) {
+              const float4 f = shifts[k];
+              p[4 * k] = exp2_fast(fmaf(__uint_as_float(r[4 * k]), s.exponent, -f.x));
+              p[4 * k + 1] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 1]), s.exponent, -f.y));
+              p[4 * k + 2] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 2]), s.exponent, -f.z));
+              p[4 * k + 3] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 3]), s.exponent, -f.w));
+            }
           }
-        }
-        const int begin = sees - i * kTile - 64 * w;
-        if (s.causal && k0 + kTile - 1 - ((int)s.k_len - (int)s.q_len) > i * kTile) {
+          if (s.causal && at.k0 + kTile - 1 - off > q * kTile) {
+            const int begin = row - off - q * kTile - 64 * w;  // the first query that sees this key
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (k < begin) p[k] = 0.0f;
-        }
+            for (int k = 0; k < 64; ++k)
+              if (k < begin) p[k] = 0.0f;
+          }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t out[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t out[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
-          store16(s_at + 64 * w + 16 * c + lanes, out);
-        }
-        wait_stores();
-        fence_before();
-        bar_arrive(p_ready);
+            for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
+            store16(s_at + 64 * w + 16 * c + lanes, out);
+          }
+          wait_stores();
+          fence_before();
+          bar_arrive(p_ready);
 
-        CSW_WAIT_WARP(dp_full, j & 1);
-        fence_after();
+          CSW_WAIT_WARP(dp_full, i & 1);
+          fence_after();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32], out[16];
-          float d[32];
-          load32(dp_at + 64 * w + 32 * c + lanes, r);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32], out[16];
+            float d[32];
+            load32(dp_at + 64 * w + 32 * c + lanes, r);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float4 f = deltas[8 * c + k];
-            d[4 * k] = f.x, d[4 * k + 1] = f.y, d[4 * k + 2] = f.z, d[4 * k + 3] = f.w;
+            for (int k = 0; k < 8; ++k) {
+              const float4 f = deltas[8 * c + k];
+              d[4 * k] = f.x, d[4 * k + 1] = f.y, d[4 * k + 2] = f.z, d[4 * k + 3] = f.w;
+            }
+            wait_loads();
+            to_gradients<T>(p + 32 * c, r, d, out);
+            store16(dp_at + 64 * w + 16 * c + lanes, out);
           }
-          wait_loads();
-          to_gradients<T>(p + 32 * c, r, d, out);
-          store16(dp_at + 64 * w + 16 * c + lanes, out);
+          wait_stores();
+          fence_before();
+          bar_arrive(ds_ready);
+          if (++q == at.tiles) q = at.from;
         }
-        wait_stores();
-        fence_before();
-        bar_arrive(ds_ready);
-        if (++i == tiles_q) i = from;
-      }
-      if (n > 0) {
-        CSW_WAIT_WARP(done, 0);
-        fence_after();
-      }
-      // A key behind its sequence has no gradient, whatever its row of the tile held.
-      const bool stored = row < (int)s.k_len, live = n > 0 && row < keys;
-      T* out = stored ? (w == 0 ? a.dv : a.dk).template row<T>(b, g, row) : nullptr;
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t r[32] = {};
         if (n > 0) {
-          load32((w == 0 ? dv_at : dk_at) + c + lanes, r);
-          wait_loads();
+          CSW_WAIT_WARP(sums_full, u & 1);
+          ++u;
+          fence_after();
         }
-        if (!live) {
+        // A key behind its sequence has no gradient, whatever its row of the tile held.
+        const bool live = n > 0 && row < piece.y;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = 0;
+        for (int c = 0; c < DP; c += 64) {
+          stage_free(t == 0, 1 + w, 128);
+#pragma unroll
+          for (int k = 0; k < 64; k += 32) {
+            uint32_t r[32] = {};
+            if (n > 0) {
+              load32((w == 0 ? dv_at : dk_at) + c + k + lanes, r);
+              wait_loads();
+            }
+            if (!live) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x) r[x] = 0;
+            }
+            stage_columns<T>(stage, t, k, r, w == 0 ? 1.0f : s.scale);
+          }
+          if (n > 0 && c + 64 == DP) {
+            fence_before();
+            bar_arrive(sums_free);
+          }
+          stage_out(t == 0, 1 + w, 128, w == 0 ? &a.dv : &a.dk, smem_at(stage), c, at.k0, at.g, at.b);
         }
-        if (stored) store_columns(out, c, s.dim, r, w == 0 ? 1.0f : s.scale);
       }
     }();
+    if (t == 0) stores_read();
   }
   leave<Plan::kColumns>(flag, tmem, warp == 9);
 }
@@ -857,8 +1084,8 @@ cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_att
   if (s.batch == 0 || s.q_len == 0) return cudaSuccess;
   if (const cudaError_t e = bind_context()) return e;
   Forward a;
-  a.s = shape_of(s), a.o = view_of(o), a.lse = lse;
-  if (!map_of(&a.q, q, s, s.heads, s.q_len)) return cudaErrorInvalidValue;
+  a.s = shape_of(s), a.lse = lse;
+  if (!map_of(&a.q, q, s, s.heads, s.q_len) || !map_of(&a.o, o, s, s.heads, s.q_len)) return cudaErrorInvalidValue;
   a.k = a.v = a.q;  // without keys nothing is copied from them
   if (s.k_len && (!map_of(&a.k, k, s, s.kv_heads, s.k_len) || !map_of(&a.v, v, s, s.kv_heads, s.k_len)))
     return cudaErrorInvalidValue;
@@ -869,13 +1096,16 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return cudaSuccess;
   if (const cudaError_t e = bind_context()) return e;
   Backward a;
-  a.s = shape_of(s), a.dq = view_of(b.dq), a.dk = view_of(b.dk), a.dv = view_of(b.dv);
+  a.s = shape_of(s);
   a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
   const bool half = s.type == CSW_TYPE_F16;
-  a.q = a.k = a.v = a.dout = CUtensorMap{};  // of an empty side nothing is copied
-  if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len)))
+  // of an empty side nothing is copied
+  a.q = a.k = a.v = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
+  if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len) ||
+                  !map_of(&a.dq, b.dq, s, s.heads, s.q_len)))
     return cudaErrorInvalidValue;
-  if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len)))
+  if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len) ||
+                  !map_of(&a.dk, b.dk, s, s.kv_heads, s.k_len) || !map_of(&a.dv, b.dv, s, s.kv_heads, s.k_len)))
     return cudaErrorInvalidValue;
   if (s.q_len) {
     uint32_t lanes = 1;

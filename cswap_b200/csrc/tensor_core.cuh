@@ -60,6 +60,48 @@ __device__ __forceinline__ void copy_bytes(uint32_t dst, const void* src, uint32
                : "memory");
 }
 
+// ---- copies out of shared memory -----------------------------------------------------------------------------------
+// what of the tile lies behind the tensor is left out
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, uint32_t src, int dim, int token, int head, int batch) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(src), "r"(dim), "r"(token), "r"(head), "r"(batch)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// the source of this thread's stores may be written again
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// some warps of a CTA
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// ---- work ----------------------------------------------------------------------------------------------------------
+// Asks for a CTA of this grid that has not started: it will not start, and its work is the caller's.  The answer (16
+// bytes) arrives at `bar`.  Not to be asked again after a refusal.
+__device__ __forceinline__ void take_next(uint32_t answer, uint32_t bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+      "r"(bar)
+      : "memory");
+}
+// the index of the CTA that was taken, -1 for a refusal
+__device__ __forceinline__ int taken_index(uint32_t answer) {
+  int index;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "=r"(index)
+      : "r"(answer)
+      : "memory");
+  return index;
+}
+
 // ---- tensor memory -------------------------------------------------------------------------------------------------
 // by one whole warp; the address arrives at *at in shared memory
 template <int COLUMNS>
