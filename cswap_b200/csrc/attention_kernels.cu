@@ -55,7 +55,7 @@ struct View {
 View view_of(const csw_attention_operand& o) { return {o.data, o.batch_stride, o.head_stride, o.token_stride}; }
 
 struct Shape {
-  uint32_t batch, heads, kv_heads, q_len, k_len, dim;
+  uint32_t batch, heads, kv_heads, q_len, k_len, dim, share;  // share: query heads of a key head
   int causal;
   bool negate;     // the scale is negative: the products are negated instead
   float scale;     // as given
@@ -137,10 +137,13 @@ __device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map
 // acc (+)= A B^T: both read along their rows, the reduction over the head's dimension
 template <int DP>
 __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t b, uint32_t desc) {
+  const uint64_t da = tile_desc(a, 16), db = tile_desc(b, 16);
+  if (elected()) {
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const uint32_t at = k / 4 * kChunk + k % 4 * 32;
-    mma(acc, tile_desc(a + at, 16), tile_desc(b + at, 16), desc, k > 0);
+    for (int k = 0; k < DP / 16; ++k) {
+      const uint32_t at = (k / 4 * kChunk + k % 4 * 32) / 16;
+      mma(acc, da + at, db + at, desc, k > 0);
+    }
   }
 }
 // acc (+)= P B: P in tensor memory, B read across its rows, the reduction over 128 tokens.  P's first 64 columns lie
@@ -148,9 +151,15 @@ __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t 
 template <int DP>
 __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
                                                bool add) {
+  const uint64_t db = tile_desc(b, kChunk);
+  if (elected()) {
 #pragma unroll
-  for (int k = 0; k < kTile / 16; ++k)
-    mma_tmem(acc, p + k / 4 * half + k % 4 * 8, tile_desc(b + k * 2048, kChunk), desc, add || k > 0);
+    for (int k = 0; k < kTile / 16; ++k)
+      mma_tmem(acc, p + k / 4 * half + k % 4 * 8, db + k * (2048 / 16), desc, add || k > 0);
+  }
+}
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+  if (elected()) commit(bar);
 }
 
 // ---- a CTA's work -----------------------------------------------------------------------------------------------------
@@ -158,9 +167,14 @@ __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_
 // piece of a CTA that has not started, so that copies and products of the next piece begin while the softmax warps still
 // write the last one, whatever lengths the sequences have.  The copying warp asks, and tells the others two pieces
 // ahead: the piece, -1 at the end, and its sequence's number of keys.
+struct Piece {
+  int first;         // token, -1: there is no piece
+  int keys;          // of its sequence
+  int batch, head, kv_head, row;  // row: batch x heads + head, of what is held per row and head
+};
 struct Work {
   uint4 answer;
-  int2 piece[2];
+  Piece piece[2];
   uint64_t bars[5];  // the answer's; told and read, for each of the two
 };
 struct WorkBars {
@@ -173,15 +187,15 @@ struct WorkBars {
     for (int i = 0; i < 2; ++i) bar_init(told + 8 * i, 1), bar_init(read + 8 * i, warps);
   }
 };
-// What a listening warp (or one lane that stands for it) hears as its i-th piece; false where a wait ran out.
-__device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, int i, bool whole_warp, int2* piece) {
-  bool ok = bar_wait(bars.told + 8 * (i % 2), i / 2 & 1);
-  if (whole_warp) ok = __all_sync(0xffffffffu, ok);
-  if (!ok) return false;
-  const volatile int* told = &w.piece[i % 2].x;
-  *piece = make_int2(told[0], told[1]);
-  if (whole_warp) __syncwarp();
-  if (!whole_warp || threadIdx.x % 32 == 0) bar_arrive(bars.read + 8 * (i % 2));
+// What a warp hears as its i-th piece; false where a wait ran out.
+__device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, int i, Piece* piece) {
+  if (!__all_sync(0xffffffffu, bar_wait(bars.told + 8 * (i % 2), i / 2 & 1))) return false;
+  // one lane's reading: the compiler then knows that all have the same
+  const volatile Piece& told = w.piece[i % 2];
+  piece->first = __shfl_sync(0xffffffffu, told.first, 0), piece->keys = __shfl_sync(0xffffffffu, told.keys, 0);
+  piece->batch = __shfl_sync(0xffffffffu, told.batch, 0), piece->head = __shfl_sync(0xffffffffu, told.head, 0);
+  piece->kv_head = __shfl_sync(0xffffffffu, told.kv_head, 0), piece->row = __shfl_sync(0xffffffffu, told.row, 0);
+  if (threadIdx.x % 32 == 0) bar_arrive(bars.read + 8 * (i % 2));
   return true;
 }
 
@@ -197,17 +211,18 @@ __device__ __forceinline__ void leave(uint32_t* flag, uint32_t tmem, bool owner)
   if (owner) tmem_free<COLUMNS>(tmem);
 }
 
-// The copying warp's lane over all its pieces: f(piece, keys, i) copies what the i-th piece needs, and returns false
-// where a wait ran out.
+// The copying warp's lane over all its pieces: f.piece(index) says which one a CTA has, f.copy(piece) copies what it
+// needs, and returns false where a wait ran out.
 template <class F>
 __device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_t* flag, F&& f) {
-  int2 piece = make_int2(blockIdx.x, 0);
+  int index = blockIdx.x;
   for (int i = 0;; ++i) {
     if (i >= 2) CSW_WAIT(bars.read + 8 * (i % 2), (i / 2 - 1) & 1);
-    if (piece.x >= 0) piece.y = f.keys(piece.x);
+    Piece piece{-1};
+    if (index >= 0) piece = f.piece(index);
     w.piece[i % 2] = piece;
     bar_arrive(bars.told + 8 * (i % 2));
-    if (piece.x < 0) return;
+    if (index < 0) return;
     if (!f.copy(piece)) {
       give_up(flag);
       return;
@@ -216,7 +231,7 @@ __device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_
     bar_expect(bars.answered, 16);
     take_next(bars.answer, bars.answered);
     CSW_WAIT(bars.answered, i & 1);
-    piece.x = taken_index(bars.answer);
+    index = taken_index(bars.answer);
     async_fence();  // the answer is read before the next one is written
   }
 }
@@ -251,20 +266,20 @@ struct ForwardPlan {
   static constexpr int kColumns = NWG * (128 + DP) > 256 ? 512 : 256;
 };
 
-// Piece `index` of the forward grid.  The last tiles of a causal mask see the most keys: they go first.
+// Piece `index` of a grid over `tokens` queries a CTA.  The last ones of a causal mask see the most keys: they go first.
+__device__ __forceinline__ Piece piece_of_queries(const Shape& s, int index, int tokens) {
+  const int per = s.batch * s.heads, tiles = gridDim.x / per, row = index % per, b = row / s.heads, h = row % s.heads;
+  return {(tiles - 1 - index / per) * tokens, s.keys(b), b, h, h / (int)s.share, row};
+}
 template <int NWG>
 struct Queries {
-  uint32_t bh, b, h, g;
-  int q0, count[NWG], most;  // tiles of keys that each tile of queries sees
-  __device__ Queries(const Shape& s, int index, int keys) {
-    const uint32_t per = s.batch * s.heads, tiles = gridDim.x / per;
-    bh = index % per, b = bh / s.heads, h = bh % s.heads, g = h / (s.heads / s.kv_heads);
-    q0 = (int)(tiles - 1 - index / per) * NWG * kTile;
+  int count[NWG], most;  // tiles of keys that each tile of queries sees
+  __device__ Queries(const Shape& s, const Piece& p) {
     most = 0;
 #pragma unroll
     for (int w = 0; w < NWG; ++w) {
-      const int first = q0 + w * kTile;
-      count[w] = first < (int)s.q_len ? (s.limit(min(first + kTile, (int)s.q_len) - 1, keys) + kTile - 1) / kTile : 0;
+      const int first = p.first + w * kTile;
+      count[w] = first < (int)s.q_len ? (s.limit(min(first + kTile, (int)s.q_len) - 1, p.keys) + kTile - 1) / kTile : 0;
       most = max(most, count[w]);
     }
   }
@@ -284,7 +299,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
                  s_full = empty + 8 * Plan::kStages, p_ready = s_full + 8 * NWG, o_full = p_ready + 8 * NWG,
                  o_free = o_full + 8 * NWG;
   uint32_t* flag = &flag_word;
-  const int warp = threadIdx.x / 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
 
   if (threadIdx.x == 0) {
     work_bars.init(1 + 4 * NWG);
@@ -312,20 +327,20 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
       const Forward& a;
       uint32_t tiles_at, ring, q_full, q_empty, full, empty;
       int i = 0, u = 0;  // tiles of the ring, pieces with any
-      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.heads) / a.s.heads); }
-      __device__ bool copy(int2 piece) {
-        const Queries<NWG> at(a.s, piece.x, piece.y);
+      __device__ Piece piece(int index) const { return piece_of_queries(a.s, index, NWG * kTile); }
+      __device__ bool copy(const Piece& p) {
+        const Queries<NWG> at(a.s, p);
         if (at.most == 0) return true;
         if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
         bar_expect(q_full, NWG * Plan::kTileBytes);
 #pragma unroll
         for (int w = 0; w < NWG; ++w)
-          copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, at.q0 + w * kTile, at.h, at.b);
+          copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, p.first + w * kTile, p.head, p.batch);
         for (int j = 0; j < 2 * at.most; ++j, ++i) {  // k 0, v 0, k 1, v 1, ...
           const int stage = i % Plan::kStages;
           if (i >= Plan::kStages && !bar_wait(empty + 8 * stage, (i / Plan::kStages - 1) & 1)) return false;
           bar_expect(full + 8 * stage, Plan::kTileBytes);
-          copy_tokens<DP>(ring + stage * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * stage, j / 2 * kTile, at.g, at.b);
+          copy_tokens<DP>(ring + stage * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * stage, j / 2 * kTile, p.kv_head, p.batch);
         }
         ++u;
         return true;
@@ -335,39 +350,38 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 4 * NWG + 1) {
     [&] {
-      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       int base = 0, u = 0, tile[NWG] = {}, done[NWG] = {};  // of the ring; pieces; of each tile of queries: tiles, pieces
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const Queries<NWG> at(s, piece.x, piece.y);
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const Queries<NWG> at(s, piece);
         if (at.most == 0) continue;
-        CSW_WAIT(q_full, u & 1);
+        CSW_WAIT_WARP(q_full, u & 1);
         for (int j = 0; j <= at.most; ++j) {
           const int ki = base + 2 * j, vi = ki - 1, k = ki % Plan::kStages, v = vi % Plan::kStages;
-          if (j < at.most) CSW_WAIT(full + 8 * k, ki / Plan::kStages & 1);
-          if (j > 0) CSW_WAIT(full + 8 * v, vi / Plan::kStages & 1);
+          if (j < at.most) CSW_WAIT_WARP(full + 8 * k, ki / Plan::kStages & 1);
+          if (j > 0) CSW_WAIT_WARP(full + 8 * v, vi / Plan::kStages & 1);
 #pragma unroll
           for (int w = 0; w < NWG; ++w) {
             const uint32_t sw = tmem + w * 128, ow = tmem + NWG * 128 + w * DP;
             if (j > 0 && j <= at.count[w]) {
-              CSW_WAIT(p_ready + 8 * w, tile[w]++ & 1);
-              if (j == 1 && done[w] > 0) CSW_WAIT(o_free + 8 * w, (done[w] - 1) & 1);
+              CSW_WAIT_WARP(p_ready + 8 * w, tile[w]++ & 1);
+              if (j == 1 && done[w] > 0) CSW_WAIT_WARP(o_free + 8 * w, (done[w] - 1) & 1);
               fence_after();
               product_tokens<DP>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
-              if (j == at.count[w]) commit(o_full + 8 * w), ++done[w];
+              if (j == at.count[w]) commit_to(o_full + 8 * w), ++done[w];
             }
             if (j < at.count[w]) {
               product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores);
-              commit(s_full + 8 * w);
+              commit_to(s_full + 8 * w);
             }
           }
-          if (j < at.most) commit(empty + 8 * k);
-          if (j > 0) commit(empty + 8 * v);
-          if (j + 1 == at.most) commit(q_empty);
+          if (j < at.most) commit_to(empty + 8 * k);
+          if (j > 0) commit_to(empty + 8 * v);
+          if (j + 1 == at.most) commit_to(q_empty);
         }
         base += 2 * at.most, ++u;
       }
@@ -380,12 +394,12 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     [&] {
       int tile = 0, done = 0, base = 0;
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const Queries<NWG> at(s, piece.x, piece.y);
-        const int keys = piece.y, n = NWG == 1 || w == 0 ? at.count[0] : at.count[NWG - 1];
-        const int q0 = at.q0 + w * kTile, row = q0 + t;
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const Queries<NWG> at(s, piece);
+        const int keys = piece.keys, n = NWG == 1 || w == 0 ? at.count[0] : at.count[NWG - 1];
+        const int q0 = piece.first + w * kTile, row = q0 + t;
         const int limit = s.limit(row, keys), least = s.limit(q0, keys);
         float top = -INFINITY, sum = 0.0f;
         for (int j = 0; j < n; ++j) {
@@ -465,24 +479,21 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
         }
         const float f = n == 0 || sum == 0.0f ? 0.0f : 1.0f / sum;
         if (row < (int)s.q_len)
-          a.lse[(uint64_t)at.bh * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
+          a.lse[(uint64_t)piece.row * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
           stage_free(t == 0, 1 + w, 128);
-#pragma unroll
-          for (int i = 0; i < 64; i += 32) {
-            uint32_t o[32] = {};
-            if (n > 0) {
-              load32(ow + c + i, o);
-              wait_loads();
+          uint32_t o[64] = {};
+          if (n > 0) {
+            load32(ow + c, o), load32(ow + c + 32, o + 32);
+            wait_loads();
+            if (c + 64 == DP) {
+              fence_before();
+              bar_arrive(o_free + 8 * w);
             }
-            stage_columns<T>(stage, t, i, o, f);
           }
-          if (n > 0 && c + 64 == DP) {
-            fence_before();
-            bar_arrive(o_free + 8 * w);
-          }
-          stage_out(t == 0 && q0 < (int)s.q_len, 1 + w, 128, &a.o, smem_at(stage), c, q0, at.h, at.b);
+          stage_columns<T>(stage, t, 0, o, f), stage_columns<T>(stage, t, 32, o + 32, f);
+          stage_out(t == 0 && q0 < (int)s.q_len, 1 + w, 128, &a.o, smem_at(stage), c, q0, piece.head, piece.batch);
         }
       }
     }();
@@ -562,7 +573,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
                  s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8, dq_full = ds_ready + 8,
                  dq_free = dq_full + 8;
   uint32_t* flag = &flag_word;
-  const int warp = threadIdx.x / 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(9);
     bar_init(q_full, 1), bar_init(q_empty, 1), bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1);
@@ -586,20 +597,20 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       const Backward& a;
       uint32_t tiles_at, ring, q_full, q_empty, full, empty;
       int i = 0, u = 0;  // pairs, pieces with any
-      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.heads) / a.s.heads); }
-      __device__ bool copy(int2 piece) {
-        const Queries<1> at(a.s, piece.x, piece.y);
+      __device__ Piece piece(int index) const { return piece_of_queries(a.s, index, kTile); }
+      __device__ bool copy(const Piece& p) {
+        const Queries<1> at(a.s, p);
         if (at.most == 0) return true;
         if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
         bar_expect(q_full, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(tiles_at, &a.q, q_full, at.q0, at.h, at.b);
-        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, at.q0, at.h, at.b);
+        copy_tokens<DP>(tiles_at, &a.q, q_full, p.first, p.head, p.batch);
+        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, p.first, p.head, p.batch);
         for (int j = 0; j < at.most; ++j, ++i) {
           const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
           if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
           bar_expect(bar, 2 * Plan::kTileBytes);
-          copy_tokens<DP>(to, &a.k, bar, j * kTile, at.g, at.b);
-          copy_tokens<DP>(to + Plan::kTileBytes, &a.v, bar, j * kTile, at.g, at.b);
+          copy_tokens<DP>(to, &a.k, bar, j * kTile, p.kv_head, p.batch);
+          copy_tokens<DP>(to + Plan::kTileBytes, &a.v, bar, j * kTile, p.kv_head, p.batch);
         }
         ++u;
         return true;
@@ -609,42 +620,41 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 9) {
     [&] {
-      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const int n = Queries<1>(s, piece.x, piece.y).most;
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const int n = Queries<1>(s, piece).most;
         if (n == 0) continue;
-        CSW_WAIT(q_full, u & 1);
+        CSW_WAIT_WARP(q_full, u & 1);
         // The scores' place is free once they have been read (s_free), that of dp behind the product that read it.
         for (int j = -1; j < n; ++j, ++i) {
           // i counts pairs from the one in front of this piece's first; its own numbers are one less
           const int now = i - 1 - u, next = now + 1;
           const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
           if (j + 1 < n) {
-            CSW_WAIT(full + 8 * (next & 1), next / 2 & 1);
-            if (next > 0) CSW_WAIT(s_free, now & 1);
+            CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
+            if (next > 0) CSW_WAIT_WARP(s_free, now & 1);
             fence_after();
             product_rows<DP>(s_at, tiles_at, then, scores);
-            commit(s_full);
+            commit_to(s_full);
           }
           if (j >= 0) {
-            CSW_WAIT(ds_ready, now & 1);
-            if (j == 0 && u > 0) CSW_WAIT(dq_free, (u - 1) & 1);
+            CSW_WAIT_WARP(ds_ready, now & 1);
+            if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
             fence_after();
             product_tokens<DP>(dq_at, dp_at, 64, at, sums, j > 0);
-            commit(empty + 8 * (now & 1));
-            if (j + 1 == n) commit(dq_full);
+            commit_to(empty + 8 * (now & 1));
+            if (j + 1 == n) commit_to(dq_full);
           }
           if (j + 1 < n) {
             product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
-            commit(dp_full);
-            if (j + 2 == n) commit(q_empty);
+            commit_to(dp_full);
+            if (j + 2 == n) commit_to(q_empty);
           }
         }
         ++u;
@@ -661,14 +671,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const Queries<1> at(s, piece.x, piece.y);
-        const int keys = piece.y, n = at.most, row = at.q0 + t;
-        const int limit = s.limit(row, keys), least = s.limit(at.q0, keys);
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const Queries<1> at(s, piece);
+        const int keys = piece.keys, n = at.most, row = piece.first + t;
+        const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
         // padded to whole tiles: every thread has a row
-        float* mine = a.rows + (uint64_t)at.bh * a.padded + row;
+        float* mine = a.rows + (uint64_t)piece.row * a.padded + row;
         float* d_at = mine + (uint64_t)s.batch * s.heads * a.padded;
         const float shift = mine[0], d = *d_at;
         float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
@@ -745,7 +755,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           fence_before();
           bar_arrive(dq_free);
         }
-        stage_out(first, id, kGroup, &a.dq, smem_at(stage), DP == 128 ? 64 * w : 0, at.q0, at.h, at.b);
+        stage_out(first, id, kGroup, &a.dq, smem_at(stage), DP == 128 ? 64 * w : 0, piece.first, piece.head, piece.batch);
         if (DP == 128) group_sync(3, 256);
         // The next kernel's D has no rounding of o in it: it is sum p dp, which this one has formed on the way.
         if (w == 0 && live) *d_at = d + left + halves[t];
@@ -757,17 +767,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   leave<Plan::kColumns>(flag, tmem, warp == 9);
 }
 
-// Piece `index` of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
+// Pieces of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
 struct Keys {
-  uint32_t b, g;
-  int k0, from, tiles, n;  // the first tile of queries that sees any of them; tiles of queries; pairs in all
-  __device__ Keys(const Shape& s, int index, int keys) {
-    const uint32_t per = s.batch * s.kv_heads, bg = index % per;
-    b = bg / s.kv_heads, g = bg % s.kv_heads, k0 = (int)(index / per) * kTile;
+  int from, tiles, n;  // the first tile of queries that sees any of them; tiles of queries; pairs in all
+  __device__ Keys(const Shape& s, const Piece& p) {
     // query i sees key j from i = j - (k_len - q_len) on
-    from = s.causal ? max(k0 - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
+    from = s.causal ? max(p.first - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
     tiles = ((int)s.q_len + kTile - 1) / kTile;
-    n = (k0 < keys ? max(tiles - from, 0) : 0) * (int)(s.heads / s.kv_heads);
+    n = (p.first < p.keys ? max(tiles - from, 0) : 0) * (int)s.share;
   }
 };
 
@@ -785,7 +792,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
                  s_full = empty + 16, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
                  sums_full = ds_ready + 8, sums_free = sums_full + 8;
   uint32_t* flag = &flag_word;
-  const int warp = threadIdx.x / 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(9);
     bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1);
@@ -809,27 +816,31 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       const Backward& a;
       uint32_t tiles_at, ring, rows_at, kv_full, kv_empty, full, empty;
       int i = 0, u = 0;
-      __device__ int keys(int index) const { return a.s.keys(index % (a.s.batch * a.s.kv_heads) / a.s.kv_heads); }
-      __device__ bool copy(int2 piece) {
-        const Keys at(a.s, piece.x, piece.y);
+      __device__ Piece piece(int index) const {
+        const int per = a.s.batch * a.s.kv_heads, row = index % per, b = row / a.s.kv_heads, g = row % a.s.kv_heads;
+        const int head = g * (int)a.s.share;  // the first of those that share
+        return {index / per * kTile, a.s.keys(b), b, head, g, b * (int)a.s.heads + head};
+      }
+      __device__ bool copy(const Piece& p) {
+        const Keys at(a.s, p);
         if (at.n == 0) return true;
         if (u > 0 && !bar_wait(kv_empty, (u - 1) & 1)) return false;
         bar_expect(kv_full, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(tiles_at, &a.k, kv_full, at.k0, at.g, at.b);
-        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, at.k0, at.g, at.b);
+        copy_tokens<DP>(tiles_at, &a.k, kv_full, p.first, p.kv_head, p.batch);
+        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, p.first, p.kv_head, p.batch);
         const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
         int q = at.from;
-        uint32_t h = at.g * (a.s.heads / a.s.kv_heads);
+        int h = p.head, row = p.row;
         for (int j = 0; j < at.n; ++j, ++i) {
           const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
           if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
           bar_expect(bar, 2 * Plan::kTileBytes + 2 * kTile * 4);
-          copy_tokens<DP>(to, &a.q, bar, q * kTile, h, at.b);
-          copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, bar, q * kTile, h, at.b);
-          const float* src = a.rows + ((uint64_t)at.b * a.s.heads + h) * a.padded + (uint64_t)q * kTile;
+          copy_tokens<DP>(to, &a.q, bar, q * kTile, h, p.batch);
+          copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, bar, q * kTile, h, p.batch);
+          const float* src = a.rows + (uint64_t)row * a.padded + (uint64_t)q * kTile;
           copy_bytes(rows_at + i % 2 * (8 * kTile), src, kTile * 4, bar);
           copy_bytes(rows_at + i % 2 * (8 * kTile) + 4 * kTile, src + plane, kTile * 4, bar);
-          if (++q == at.tiles) q = at.from, ++h;
+          if (++q == at.tiles) q = at.from, ++h, ++row;
         }
         ++u;
         return true;
@@ -839,44 +850,43 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
   } else if (warp == 9) {
     [&] {
-      if (threadIdx.x % 32 != 0) return;
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, false, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const int n = Keys(s, piece.x, piece.y).n;
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const int n = Keys(s, piece).n;
         if (n == 0) continue;
-        CSW_WAIT(kv_full, u & 1);
+        CSW_WAIT_WARP(kv_full, u & 1);
         // Each tile's place in tensor memory is written again behind the product that reads it.
         for (int j = -1; j < n; ++j, ++i) {
           const int now = i - 1 - u, next = now + 1;
           const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
           if (j >= 0) {
-            CSW_WAIT(p_ready, now & 1);
-            if (j == 0 && u > 0) CSW_WAIT(sums_free, (u - 1) & 1);
+            CSW_WAIT_WARP(p_ready, now & 1);
+            if (j == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
             fence_after();
             product_tokens<DP>(dv_at, s_at, 64, at + Plan::kTileBytes, sums, j > 0);
           }
           if (j + 1 < n) {
-            CSW_WAIT(full + 8 * (next & 1), next / 2 & 1);
+            CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
             product_rows<DP>(s_at, tiles_at, then, scores);
-            commit(s_full);
+            commit_to(s_full);
           }
           if (j >= 0) {
-            CSW_WAIT(ds_ready, now & 1);
+            CSW_WAIT_WARP(ds_ready, now & 1);
             fence_after();
             product_tokens<DP>(dk_at, dp_at, 64, at, sums, j > 0);
-            commit(empty + 8 * (now & 1));
-            if (j + 1 == n) commit(sums_full);
+            commit_to(empty + 8 * (now & 1));
+            if (j + 1 == n) commit_to(sums_full);
           }
           if (j + 1 < n) {
             product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
-            commit(dp_full);
-            if (j + 2 == n) commit(kv_empty);
+            commit_to(dp_full);
+            if (j + 2 == n) commit_to(kv_empty);
           }
         }
         ++u;
@@ -889,11 +899,11 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
-        int2 piece;
-        if (!hear(work, work_bars, it, true, &piece)) return give_up(flag);
-        if (piece.x < 0) return;
-        const Keys at(s, piece.x, piece.y);
-        const int n = at.n, row = at.k0 + t, off = (int)s.k_len - (int)s.q_len;
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const Keys at(s, piece);
+        const int n = at.n, row = piece.first + t, off = (int)s.k_len - (int)s.q_len;
         int q = at.from;
         for (int j = 0; j < n; ++j, ++i) {
           CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);  // the rows' numbers
@@ -916,7 +926,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
               p[4 * k + 3] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 3]), s.exponent, -f.w));
             }
           }
-          if (s.causal && at.k0 + kTile - 1 - off > q * kTile) {
+          if (s.causal && piece.first + kTile - 1 - off > q * kTile) {
             const int begin = row - off - q * kTile - 64 * w;  // the first query that sees this key
 #pragma unroll
             for (int k = 0; k < 64; ++k)
@@ -960,28 +970,27 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           fence_after();
         }
         // A key behind its sequence has no gradient, whatever its row of the tile held.
-        const bool live = n > 0 && row < piece.y;
+        const bool live = n > 0 && row < piece.keys;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
           stage_free(t == 0, 1 + w, 128);
-#pragma unroll
-          for (int k = 0; k < 64; k += 32) {
-            uint32_t r[32] = {};
-            if (n > 0) {
-              load32((w == 0 ? dv_at : dk_at) + c + k + lanes, r);
-              wait_loads();
+          uint32_t r[64] = {};
+          if (n > 0) {
+            const uint32_t from = (w == 0 ? dv_at : dk_at) + c + lanes;
+            load32(from, r), load32(from + 32, r + 32);
+            wait_loads();
+            if (c + 64 == DP) {
+              fence_before();
+              bar_arrive(sums_free);
             }
-            if (!live) {
+          }
+          if (!live) {
 #pragma unroll
-              for (int x = 0; x < 32; ++x) r[x] = 0;
-            }
-            stage_columns<T>(stage, t, k, r, w == 0 ? 1.0f : s.scale);
+            for (int k = 0; k < 64; ++k) r[k] = 0;
           }
-          if (n > 0 && c + 64 == DP) {
-            fence_before();
-            bar_arrive(sums_free);
-          }
-          stage_out(t == 0, 1 + w, 128, w == 0 ? &a.dv : &a.dk, smem_at(stage), c, at.k0, at.g, at.b);
+          const float f = w == 0 ? 1.0f : s.scale;
+          stage_columns<T>(stage, t, 0, r, f), stage_columns<T>(stage, t, 32, r + 32, f);
+          stage_out(t == 0, 1 + w, 128, w == 0 ? &a.dv : &a.dk, smem_at(stage), c, piece.first, piece.kv_head, piece.batch);
         }
       }
     }();
@@ -994,7 +1003,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
 Shape shape_of(const csw_attention_shape& s) {
   const float e = fmaxf(fabsf(s.scale) * kLog2e, 0x1p-100f);
   return {(uint32_t)s.batch, (uint32_t)s.heads, (uint32_t)s.kv_heads, (uint32_t)s.q_len, (uint32_t)s.k_len,
-          (uint32_t)s.dim,   s.causal,          s.scale < 0.0f,       s.scale,           e, s.kv_lens};
+          (uint32_t)s.dim,   (uint32_t)(s.heads / s.kv_heads), s.causal, s.scale < 0.0f, s.scale, e, s.kv_lens};
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -155,6 +155,7 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
 // Tiles in shared memory are rows of 128 bytes, swizzled over 8 rows as the tile copies leave them.  Read along its
 // rows (the reduction runs along a row), 16 two-byte values of the reduction are 32 bytes further in the row; read
 // across them (the reduction runs over rows), they are 16 rows, 2048 bytes, further on.
+// (The address field holds units of 16 bytes, so that steps are added to the whole word.)
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lbo) {
   return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
          (uint64_t)2 << 61;
@@ -163,6 +164,14 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lbo) {
 __host__ __device__ constexpr uint32_t product_desc(bool bf16, int n, bool across, bool negate) {
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (negate ? 1u << 13 : 0u) | (across ? 1u << 16 : 0u) |
          (uint32_t)(n / 8) << 17 | (uint32_t)(128 / 16) << 24;
+}
+// One lane of a warp whose lanes are together, the same one every time.  What the products take lies in registers that a
+// warp shares; code that a whole warp runs, up to the instruction itself, computes there, where a lane on its own has to
+// move every operand over (a step of a product then took some 100 clocks to issue instead of its 32 to 64).
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes;
 }
 // one reduction step of 16: both operands in shared memory
 __device__ __forceinline__ void mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t desc, bool add) {
