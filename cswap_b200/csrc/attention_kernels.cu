@@ -285,6 +285,90 @@ struct Queries {
   }
 };
 
+// A thread's row of 128 scores in tensor memory, 32 columns at a time, twice: the largest score, then the exponentials,
+// which go over the scores, and their sum.  MASKED: only the first `chunks` chunks of 32 are seen by any row of the warp,
+// and this row sees `end` columns.
+__device__ __forceinline__ void top_of(float (&m)[4], const uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = max3(m[c], __uint_as_float(r[i + 2 * c]), __uint_as_float(r[i + 2 * c + 1]));
+  settle(m[0], m[1], m[2], m[3]);
+}
+template <bool MASKED>
+__device__ __forceinline__ float row_top(uint32_t at, int chunks, int end) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (MASKED) {
+#pragma unroll 1
+    for (int q = 0; q < chunks; ++q, end -= 32) {
+      uint32_t r[32];
+      load32(at + 32 * q, r);
+      wait_loads(r);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i >= end) r[i] = 0xff800000u;
+      top_of(m, r);
+    }
+  } else {
+    uint32_t r[2][32];
+    load32(at, r[0]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      wait_loads(r[q % 2]);
+      if (q < 3) load32(at + 32 * (q + 1), r[(q + 1) % 2]);
+      top_of(m, r[q % 2]);
+    }
+  }
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+template <class T>
+__device__ __forceinline__ void exp_of(Pair (&add)[2], const uint32_t* r, float exponent, float shift, int end,
+                                       uint32_t* p) {
+  const Pair by = {exponent, exponent}, less = {-shift, -shift};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    Pair x = fma2({__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])}, by, less);
+    x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
+    if (2 * i >= end) x.x = 0.0f;
+    if (2 * i + 1 >= end) x.y = 0.0f;
+    add[i % 2] = add2(add[i % 2], x);
+    p[i] = pack2<T>(x.x, x.y);
+  }
+  settle(add[0].x, add[0].y, add[1].x, add[1].y);
+}
+template <class T, bool MASKED>
+__device__ __forceinline__ float row_exp(uint32_t at, int chunks, int end, float exponent, float shift) {
+  Pair add[2] = {};
+  if (MASKED) {
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q, end -= 32) {
+      uint32_t p[16];
+      if (q < chunks) {
+        uint32_t r[32];
+        load32(at + 32 * q, r);
+        wait_loads(r);
+        exp_of<T>(add, r, exponent, shift, end, p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = 0;
+      }
+      store16(at + 16 * q, p);
+    }
+  } else {
+    uint32_t r[2][32];
+    load32(at, r[0]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t p[16];
+      wait_loads(r[q % 2]);
+      if (q < 3) load32(at + 32 * (q + 1), r[(q + 1) % 2]);
+      exp_of<T>(add, r[q % 2], exponent, shift, 32, p);
+      store16(at + 16 * q, p);
+    }
+  }
+  return (add[0].x + add[0].y) + (add[1].x + add[1].y);
+}
+
 template <class T, int DP, int NWG>
 __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 : 1)
     attention_forward_kernel(const __grid_constant__ Forward a) {
@@ -406,27 +490,11 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           CSW_WAIT_WARP(s_full + 8 * w, tile & 1);
           ++tile;
           fence_after();
-          uint32_t r[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) load32(sw + 32 * i, r + 32 * i);
-          wait_loads();
-          if ((j + 1) * kTile > least) {
-            const int end = limit - j * kTile;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (end < 32 * q + 32) {
-#pragma unroll
-                for (int i = 32 * q; i < 32 * q + 32; ++i)
-                  if (i >= end) r[i] = 0xff800000u;
-              }
-            }
-          }
-          float m[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(r[i]);
-#pragma unroll
-          for (int i = 4; i < 128; ++i) m[i % 4] = fmaxf(m[i % 4], __uint_as_float(r[i]));
-          const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          // What the mask leaves out for a whole warp is not looked at.
+          const bool masked = (j + 1) * kTile > least;
+          const int end = limit - j * kTile;
+          const int chunks = masked ? min((s.limit(q0 + warp % 4 * 32 + 31, keys) - j * kTile + 31) / 32, 4) : 4;
+          const float now = masked ? row_top<true>(sw, chunks, end) : row_top<false>(sw, 4, 0);
           // The maximum is followed only where it grows by more than 2^8: the sums' exponents have room for that, and
           // so has float16, whose largest number is 2^16.
           if (__any_sync(0xffffffffu, (now - top) * s.exponent > 8.0f)) {
@@ -439,7 +507,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               for (int c = 0; c < DP; c += 32) {
                 uint32_t o[32];
                 load32(ow + c, o);
-                wait_loads();
+                wait_loads(o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                 store32(ow + c, o);
@@ -447,20 +515,8 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
             }
           }
           const float shift = top == -INFINITY ? 0.0f : top * s.exponent;
-          float add[4] = {};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i]), s.exponent, -shift));
-              const float y = exp2_fast(fmaf(__uint_as_float(r[32 * q + 2 * i + 1]), s.exponent, -shift));
-              add[i % 2] += x, add[2 + i % 2] += y;
-              p[i] = pack2<T>(x, y);
-            }
-            store16(sw + 16 * q, p);
-          }
-          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          sum += masked ? row_exp<T, true>(sw, chunks, end, s.exponent, shift)
+                        : row_exp<T, false>(sw, 4, 0, s.exponent, shift);
           // the tile of values that the sequence ends in, once for all that read it
           if (s.lens && (j + 1) * kTile > keys && (w == 0 || j >= at.count[0])) {
             const int i = base + 2 * j + 1, slot = i % Plan::kStages;
@@ -486,7 +542,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           uint32_t o[64] = {};
           if (n > 0) {
             load32(ow + c, o), load32(ow + c + 32, o + 32);
-            wait_loads();
+            wait_loads(o), wait_loads(o + 32);
             if (c + 64 == DP) {
               fence_before();
               bar_arrive(o_free + 8 * w);
@@ -690,7 +746,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             uint32_t r[64];
             load32(s_at + 64 * w + lanes, r);
             load32(s_at + 64 * w + 32 + lanes, r + 32);
-            wait_loads();
+            wait_loads(r), wait_loads(r + 32);
             fence_before();
             bar_arrive(s_free);
 #pragma unroll
@@ -710,7 +766,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             uint32_t r[32], out[16];
             float dd[32];
             load32(dp_at + 64 * w + 32 * c + lanes, r);
-            wait_loads();
+            wait_loads(r);
             if (masked) {
 #pragma unroll
               for (int k = 0; k < 32; ++k)
@@ -743,7 +799,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           uint32_t r[32] = {};
           if (n > 0) {
             load32(dq_at + w * kMine + c + lanes, r);
-            wait_loads();
+            wait_loads(r);
           }
           if (!live) {
 #pragma unroll
@@ -916,7 +972,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
             uint32_t r[64];
             load32(s_at + 64 * w + lanes, r);
             load32(s_at + 64 * w + 32 + lanes, r + 32);
-            wait_loads();
+            wait_loads(r), wait_loads(r + 32);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float4 f = shifts[k];
@@ -955,7 +1011,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
               const float4 f = deltas[8 * c + k];
               d[4 * k] = f.x, d[4 * k + 1] = f.y, d[4 * k + 2] = f.z, d[4 * k + 3] = f.w;
             }
-            wait_loads();
+            wait_loads(r);
             to_gradients<T>(p + 32 * c, r, d, out);
             store16(dp_at + 64 * w + 16 * c + lanes, out);
           }
@@ -978,7 +1034,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           if (n > 0) {
             const uint32_t from = (w == 0 ? dv_at : dk_at) + c + lanes;
             load32(from, r), load32(from + 32, r + 32);
-            wait_loads();
+            wait_loads(r), wait_loads(r + 32);
             if (c + 64 == DP) {
               fence_before();
               bar_arrive(sums_free);

@@ -115,7 +115,6 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define CSW_R4(a, i) a(i), a(i + 1), a(i + 2), a(i + 3)
@@ -123,6 +122,7 @@ __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.s
 #define CSW_R32(a, i) CSW_R16(a, i), CSW_R16(a, i + 16)
 #define CSW_OUT(i) "=r"(r[i])
 #define CSW_IN(i) "r"(r[i])
+#define CSW_BOTH(i) "+r"(r[i])
 // 32 columns of the lane that is this thread's (lane 32 (warp % 4) + thread % 32; `at` names the warp's first lane)
 __device__ __forceinline__ void load32(uint32_t at, uint32_t* r) {
   asm volatile(
@@ -130,6 +130,14 @@ __device__ __forceinline__ void load32(uint32_t at, uint32_t* r) {
       "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : CSW_R32(CSW_OUT, 0)
       : "r"(at));
+}
+// All loads are there; the 32 values depend on it, so that nothing that uses them can stand in front.
+__device__ __forceinline__ void wait_loads(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : CSW_R32(CSW_BOTH, 0)::"memory");
+}
+// what has been computed up to here is not put off
+__device__ __forceinline__ void settle(float& a, float& b, float& c, float& d) {
+  asm volatile("" : "+f"(a), "+f"(b), "+f"(c), "+f"(d));
 }
 __device__ __forceinline__ void store32(uint32_t at, const uint32_t* r) {
   asm volatile(
@@ -150,6 +158,7 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
 #undef CSW_R32
 #undef CSW_OUT
 #undef CSW_IN
+#undef CSW_BOTH
 
 // ---- products ------------------------------------------------------------------------------------------------------
 // Tiles in shared memory are rows of 128 bytes, swizzled over 8 rows as the tile copies leave them.  Read along its
@@ -198,6 +207,57 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two float32 operations in one instruction
+struct Pair {
+  float x, y;
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// 2^x without the unit for it: the whole part n goes into the exponent, 2^f for the rest, -1/2 ... 1/2, is a polynomial
+// of degree 5 (fitted for the least relative error, 1.6 10^-7).  x from -126 up to 127; below that 2^-126 stands for it.
+__device__ __forceinline__ Pair exp2_poly(Pair x) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 2^23: a sum with it is rounded to a whole number, its low bits
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const Pair t = add2(x, {kMagic, kMagic});
+  const Pair n = add2(t, {-kMagic, -kMagic});
+  const Pair f = fma2(n, {-1.0f, -1.0f}, x);
+  Pair p = fma2(f, {0.0013276472454890609f, 0.0013276472454890609f}, {0.009675540961325169f, 0.009675540961325169f});
+  p = fma2(p, f, {0.05550713092088699f, 0.05550713092088699f});
+  p = fma2(p, f, {0.24022120237350464f, 0.24022120237350464f});
+  p = fma2(p, f, {0.6931469440460205f, 0.6931469440460205f});
+  p = fma2(p, f, {1.0000001192092896f, 1.0000001192092896f});
+  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return p;
 }
 
 }  // namespace tc
