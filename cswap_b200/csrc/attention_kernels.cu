@@ -44,16 +44,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Set where a wait ran out.
 __device__ int attention_gave_up;
 
-struct View {
-  void* p;
-  int64_t b, h, t;
-  template <class T>
-  __device__ T* row(uint32_t batch, uint32_t head, uint32_t token) const {
-    return static_cast<T*>(p) + (int64_t)batch * b + (int64_t)head * h + (int64_t)token * t;
-  }
-};
-View view_of(const csw_attention_operand& o) { return {o.data, o.batch_stride, o.head_stride, o.token_stride}; }
-
 struct Shape {
   uint32_t batch, heads, kv_heads, q_len, k_len, dim, share;  // share: query heads of a key head
   int causal;
@@ -146,15 +136,15 @@ __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t 
     }
   }
 }
-// acc (+)= P B: P in tensor memory, B read across its rows, the reduction over 128 tokens.  P's first 64 columns lie
+// acc (+)= P B: P in tensor memory, B read across its rows, the reduction over TOKENS tokens.  P's first 64 columns lie
 // at p, the others at p + half.
-template <int DP>
+template <int TOKENS>
 __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
                                                bool add) {
   const uint64_t db = tile_desc(b, kChunk);
   if (elected()) {
 #pragma unroll
-    for (int k = 0; k < kTile / 16; ++k)
+    for (int k = 0; k < TOKENS / 16; ++k)
       mma_tmem(acc, p + k / 4 * half + k % 4 * 8, db + k * (2048 / 16), desc, add || k > 0);
   }
 }
@@ -455,7 +445,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               CSW_WAIT_WARP(p_ready + 8 * w, tile[w]++ & 1);
               if (j == 1 && done[w] > 0) CSW_WAIT_WARP(o_free + 8 * w, (done[w] - 1) & 1);
               fence_after();
-              product_tokens<DP>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
+              product_tokens<kTile>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
               if (j == at.count[w]) commit_to(o_full + 8 * w), ++done[w];
             }
             if (j < at.count[w]) {
@@ -558,34 +548,13 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
   leave<Plan::kColumns>(flag, tmem, warp == 4 * NWG + 1);
 }
 
-// ---- backward: D and the exponents' shifts --------------------------------------------------------------------------
-// rows[0]: log2(e) L, +inf for a row that sees nothing and behind the last row, so that its probabilities are zero;
-// rows[1]: D.  Both per head, padded to whole tiles.
-template <class T>
-__global__ void __launch_bounds__(256) attention_rows_kernel(Shape s, View o, View dout, const float* lse, float* rows,
-                                                             uint32_t padded, uint32_t lanes) {
-  pdl_wait();
-  const uint64_t r = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / lanes, total = (uint64_t)s.batch * s.heads * padded;
-  const uint32_t lane = threadIdx.x % lanes, i = r % padded, bh = r / padded;
-  float d = 0.0f;
-  if (r < total && i < s.q_len && lane * 8 < s.dim) {
-    float x[8], y[8];
-    load_pack(o.row<T>(bh / s.heads, bh % s.heads, i) + lane * 8, x);
-    load_pack(dout.row<T>(bh / s.heads, bh % s.heads, i) + lane * 8, y);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) d += x[k] * y[k];
-  }
-  for (uint32_t k = lanes / 2; k; k /= 2) d += __shfl_xor_sync(0xffffffffu, d, k);
-  if (r < total && lane == 0) {
-    const float l = i < s.q_len ? lse[(uint64_t)bh * s.q_len + i] : -INFINITY;
-    rows[r] = l == -INFINITY ? INFINITY : l * kLog2e;
-    rows[total + r] = l == -INFINITY ? 0.0f : d;
-  }
-}
-
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// Per head and query, padded to whole tiles, dq leaves for dkv in rows[0] log2(e) L, +inf for a query that sees nothing
+// and behind the last one, so that its probabilities are zero, and in rows[1] D.
 struct Backward {
-  CUtensorMap q, k, v, dout, dq, dk, dv;
+  CUtensorMap q, k, v, o, dout, dq, dk, dv;
   Shape s;
+  const float* lse;
   float* rows;
   uint32_t padded;
 };
@@ -593,8 +562,13 @@ struct Backward {
 // Both kernels: 256 threads for the scores (two a row, 64 columns each), one tile of tensor memory for s, one for dp,
 // then the sums.  Two tiles stay in shared memory for a piece; the others come in pairs, two pairs in flight; 64 columns
 // of results for each half of the threads.
+//
+// With heads of up to 64 the products are short, and the softmax warps would wait for each: their halves then go each
+// their own way, with products of 64 columns for each.  With 128 the tensor cores are the bound, and products of 128
+// columns keep them busier (of 64 columns they would read shared memory for 48 clocks a step and compute for 32).
 template <int DP>
 struct BackwardPlan {
+  static constexpr int kHalves = DP == 64 ? 2 : 1, kColumnsEach = kTile / kHalves;
   static constexpr int kThreads = 256 + 64;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
   static constexpr size_t kShared = 6 * kTileBytes + 2 * kChunk;
@@ -620,26 +594,31 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   using Plan = BackwardPlan<DP>;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[12];
-  __shared__ float halves[kTile];
+  constexpr int H = Plan::kHalves;
+  __shared__ uint64_t bars[9 + 4 * H];
+  __shared__ float halves[3][kTile];  // D of each half of the threads; the sums of ds of the second
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
-  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 16, s_full = empty + 16,
-                 s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8, dq_full = ds_ready + 8,
-                 dq_free = dq_full + 8;
+  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 16, dq_full = empty + 16,
+                 dq_free = dq_full + 8, o_empty = dq_free + 8, s_full = o_empty + 8, s_free = s_full + 8 * H,
+                 dp_full = s_free + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(9);
-    bar_init(q_full, 1), bar_init(q_empty, 1), bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1);
-    bar_init(ds_ready, 256), bar_init(dq_full, 1), bar_init(dq_free, 256);
+    bar_init(q_full, 1), bar_init(q_empty, 2), bar_init(dq_full, 1), bar_init(dq_free, 256);
+    bar_init(o_empty, DP == 128 ? 2 : 1);
+    for (int i = 0; i < H; ++i) {
+      bar_init(s_full + 8 * i, 1), bar_init(s_free + 8 * i, 256 / H);
+      bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
+    }
     for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
   }
   if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
-  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
+  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v), prefetch_map(&a.o);
   fence_before();
   __syncthreads();
   fence_after();
@@ -651,14 +630,17 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   if (warp == 8) {
     struct Copies {
       const Backward& a;
-      uint32_t tiles_at, ring, q_full, q_empty, full, empty;
-      int i = 0, u = 0;  // pairs, pieces with any
+      uint32_t tiles_at, ring, q_full, q_empty, full, empty, o_empty;
+      int i = 0, u = 0, it = 0;  // pairs, pieces with any, pieces
       __device__ Piece piece(int index) const { return piece_of_queries(a.s, index, kTile); }
       __device__ bool copy(const Piece& p) {
         const Queries<1> at(a.s, p);
+        if (it > 0 && !bar_wait(o_empty, (it - 1) & 1)) return false;
+        ++it;
         if (at.most == 0) return true;
         if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
-        bar_expect(q_full, 2 * Plan::kTileBytes);
+        bar_expect(q_full, 3 * Plan::kTileBytes);
+        copy_tokens<DP>(tiles_at + 6 * Plan::kTileBytes + (DP == 128 ? 0 : kChunk), &a.o, q_full, p.first, p.head, p.batch);
         copy_tokens<DP>(tiles_at, &a.q, q_full, p.first, p.head, p.batch);
         copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, p.first, p.head, p.batch);
         for (int j = 0; j < at.most; ++j, ++i) {
@@ -673,11 +655,11 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       }
     };
     if (threadIdx.x % 32 == 0)
-      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
+      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty, o_empty});
   } else if (warp == 9) {
     [&] {
-      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
-      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
+      const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
@@ -694,24 +676,30 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
           if (j + 1 < n) {
             CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
-            if (next > 0) CSW_WAIT_WARP(s_free, now & 1);
-            fence_after();
-            product_rows<DP>(s_at, tiles_at, then, scores);
-            commit_to(s_full);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              if (next > 0) CSW_WAIT_WARP(s_free + 8 * h, now & 1);
+              fence_after();
+              product_rows<DP>(s_at + 64 * h, tiles_at, then + h * (kChunk / 2), scores);
+              commit_to(s_full + 8 * h);
+            }
           }
-          if (j >= 0) {
-            CSW_WAIT_WARP(ds_ready, now & 1);
-            if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
-            fence_after();
-            product_tokens<DP>(dq_at, dp_at, 64, at, sums, j > 0);
-            commit_to(empty + 8 * (now & 1));
-            if (j + 1 == n) commit_to(dq_full);
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            if (j >= 0) {
+              CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
+              if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
+              fence_after();
+              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64, at + h * (kChunk / 2), sums, j > 0 || h > 0);
+              if (h + 1 == H) commit_to(empty + 8 * (now & 1));
+            }
+            if (j + 1 < n) {
+              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes + h * (kChunk / 2), slopes);
+              commit_to(dp_full + 8 * h);
+            }
           }
-          if (j + 1 < n) {
-            product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
-            commit_to(dp_full);
-            if (j + 2 == n) commit_to(q_empty);
-          }
+          if (j + 1 == n) commit_to(dq_full);
+          if (j + 2 == n) commit_to(q_empty);
         }
         ++u;
       }
@@ -720,6 +708,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     // 128 columns of results are staged as two tiles, 64 as one that all threads share
+    const uint32_t own = 8 * (H == 2 ? w : 0);
     constexpr int kGroup = DP == 128 ? 128 : 256;
     const int id = DP == 128 ? 1 + w : 1;
     const bool first = DP == 128 ? t == 0 : threadIdx.x == 0;
@@ -733,13 +722,31 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const Queries<1> at(s, piece);
         const int keys = piece.keys, n = at.most, row = piece.first + t;
         const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
-        // padded to whole tiles: every thread has a row
-        float* mine = a.rows + (uint64_t)piece.row * a.padded + row;
-        float* d_at = mine + (uint64_t)s.batch * s.heads * a.padded;
-        const float shift = mine[0], d = *d_at;
+        const float lse = row < (int)s.q_len ? a.lse[(uint64_t)piece.row * s.q_len + row] : -INFINITY;
+        const float shift = lse == -INFINITY ? INFINITY : lse * kLog2e;
+        float d = 0.0f;
+        if (n > 0) {
+          CSW_WAIT_WARP(q_full, u & 1);
+          const char* o_row = tiles + 6 * Plan::kTileBytes + (DP == 128 ? w * kChunk : kChunk) + t * 128;
+          const char* do_row = tiles + Plan::kTileBytes + (DP == 128 ? w * kChunk : 0) + t * 128;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const int unit = ((DP == 128 ? k : 4 * w + k) ^ (t & 7)) * 16;
+            float x[8], y[8];
+            load_pack(reinterpret_cast<const T*>(o_row + unit), x);
+            load_pack(reinterpret_cast<const T*>(do_row + unit), y);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) d += x[c] * y[c];
+          }
+          halves[w][t] = d;
+          group_sync(3, 256);
+          d = halves[0][t] + halves[1][t];
+          if (threadIdx.x == 0) bar_arrive(q_empty);  // which the last product of the scores does too
+        }
+        if (DP == 64 && threadIdx.x == 0) bar_arrive(o_empty);
         float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
         for (int j = 0; j < n; ++j, ++i) {
-          CSW_WAIT_WARP(s_full, i & 1);
+          CSW_WAIT_WARP(s_full + own, i & 1);
           fence_after();
           float p[64];
           {
@@ -748,7 +755,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             load32(s_at + 64 * w + 32 + lanes, r + 32);
             wait_loads(r), wait_loads(r + 32);
             fence_before();
-            bar_arrive(s_free);
+            bar_arrive(s_free + own);
 #pragma unroll
             for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
           }
@@ -759,7 +766,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             for (int k = 0; k < 64; ++k)
               if (k >= end) p[k] = 0.0f;
           }
-          CSW_WAIT_WARP(dp_full, i & 1);
+          CSW_WAIT_WARP(dp_full + own, i & 1);
           fence_after();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -783,7 +790,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           }
           wait_stores();
           fence_before();
-          bar_arrive(ds_ready);
+          bar_arrive(ds_ready + own);
         }
         if (n > 0) {
           CSW_WAIT_WARP(dq_full, u & 1);
@@ -791,7 +798,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           fence_after();
         }
         const bool live = n > 0 && shift != INFINITY;
-        if (w == 1) halves[t] = left;
+        if (w == 1) halves[2][t] = left;
         stage_free(first, id, kGroup);
         constexpr int kMine = DP / 2;
 #pragma unroll
@@ -812,9 +819,19 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           bar_arrive(dq_free);
         }
         stage_out(first, id, kGroup, &a.dq, smem_at(stage), DP == 128 ? 64 * w : 0, piece.first, piece.head, piece.batch);
-        if (DP == 128) group_sync(3, 256);
-        // The next kernel's D has no rounding of o in it: it is sum p dp, which this one has formed on the way.
-        if (w == 0 && live) *d_at = d + left + halves[t];
+        if (DP == 128) {
+          if (first) {
+            stores_read();  // o comes where the results have been
+            bar_arrive(o_empty);
+          }
+          group_sync(3, 256);
+        }
+        if (w == 0) {
+          float* mine = a.rows + (uint64_t)piece.row * a.padded + row;
+          mine[0] = shift;
+          // dkv's D has no rounding of o in it: it is sum p dp, which this kernel has formed on the way.
+          mine[(uint64_t)s.batch * s.heads * a.padded] = live ? d + left + halves[2][t] : 0.0f;
+        }
         group_sync(3, 256);
       }
     }();
@@ -839,20 +856,24 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   using Plan = BackwardPlan<DP>;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[12];
+  constexpr int H = Plan::kHalves;
+  __shared__ uint64_t bars[8 + 4 * H];
   __shared__ __align__(16) float rows[2][2][kTile];  // of each pair in flight: the exponents' shifts, D
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
   const WorkBars work_bars(work);
   const uint32_t kv_full = smem_at(bars), kv_empty = kv_full + 8, full = kv_full + 16, empty = full + 16,
-                 s_full = empty + 16, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
-                 sums_full = ds_ready + 8, sums_free = sums_full + 8;
+                 sums_full = empty + 16, sums_free = sums_full + 8, s_full = sums_free + 8, p_ready = s_full + 8 * H,
+                 dp_full = p_ready + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(9);
-    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1);
-    bar_init(ds_ready, 256), bar_init(sums_full, 1), bar_init(sums_free, 256);
+    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(sums_full, 1), bar_init(sums_free, 256);
+    for (int i = 0; i < H; ++i) {
+      bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 256 / H);
+      bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
+    }
     for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
@@ -906,8 +927,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
   } else if (warp == 9) {
     [&] {
-      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
-      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
+      const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
@@ -921,29 +942,36 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         for (int j = -1; j < n; ++j, ++i) {
           const int now = i - 1 - u, next = now + 1;
           const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
-          if (j >= 0) {
-            CSW_WAIT_WARP(p_ready, now & 1);
-            if (j == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
-            fence_after();
-            product_tokens<DP>(dv_at, s_at, 64, at + Plan::kTileBytes, sums, j > 0);
+          if (j + 1 < n) CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            if (j >= 0) {
+              CSW_WAIT_WARP(p_ready + 8 * h, now & 1);
+              if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
+              fence_after();
+              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64, at + Plan::kTileBytes + h * (kChunk / 2), sums,
+                                                 j > 0 || h > 0);
+            }
+            if (j + 1 < n) {
+              product_rows<DP>(s_at + 64 * h, tiles_at, then + h * (kChunk / 2), scores);
+              commit_to(s_full + 8 * h);
+            }
           }
-          if (j + 1 < n) {
-            CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
-            product_rows<DP>(s_at, tiles_at, then, scores);
-            commit_to(s_full);
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            if (j >= 0) {
+              CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
+              fence_after();
+              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64, at + h * (kChunk / 2), sums, j > 0 || h > 0);
+              if (h + 1 == H) commit_to(empty + 8 * (now & 1));
+            }
+            if (j + 1 < n) {
+              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes + h * (kChunk / 2), slopes);
+              commit_to(dp_full + 8 * h);
+            }
           }
-          if (j >= 0) {
-            CSW_WAIT_WARP(ds_ready, now & 1);
-            fence_after();
-            product_tokens<DP>(dk_at, dp_at, 64, at, sums, j > 0);
-            commit_to(empty + 8 * (now & 1));
-            if (j + 1 == n) commit_to(sums_full);
-          }
-          if (j + 1 < n) {
-            product_rows<DP>(dp_at, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes, slopes);
-            commit_to(dp_full);
-            if (j + 2 == n) commit_to(kv_empty);
-          }
+          if (j + 1 == n) commit_to(sums_full);
+          if (j + 2 == n) commit_to(kv_empty);
         }
         ++u;
       }
@@ -951,6 +979,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t own = 8 * (H == 2 ? w : 0);
     char* stage = tiles + 6 * Plan::kTileBytes + w * kChunk;
     [&] {
       int i = 0, u = 0;
@@ -963,7 +992,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         int q = at.from;
         for (int j = 0; j < n; ++j, ++i) {
           CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);  // the rows' numbers
-          CSW_WAIT_WARP(s_full, i & 1);
+          CSW_WAIT_WARP(s_full + own, i & 1);
           fence_after();
           float p[64];
           const float4* shifts = reinterpret_cast<const float4*>(rows[i & 1][0] + 64 * w);
@@ -997,9 +1026,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           wait_stores();
           fence_before();
-          bar_arrive(p_ready);
+          bar_arrive(p_ready + own);
 
-          CSW_WAIT_WARP(dp_full, i & 1);
+          CSW_WAIT_WARP(dp_full + own, i & 1);
           fence_after();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -1017,7 +1046,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           wait_stores();
           fence_before();
-          bar_arrive(ds_ready);
+          bar_arrive(ds_ready + own);
           if (++q == at.tiles) q = at.from;
         }
         if (n > 0) {
@@ -1162,27 +1191,16 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   if (const cudaError_t e = bind_context()) return e;
   Backward a;
   a.s = shape_of(s);
-  a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
-  const bool half = s.type == CSW_TYPE_F16;
+  a.lse = b.lse, a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
   // of an empty side nothing is copied
-  a.q = a.k = a.v = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
+  a.q = a.k = a.v = a.o = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
   if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len) ||
-                  !map_of(&a.dq, b.dq, s, s.heads, s.q_len)))
+                  !map_of(&a.o, b.o, s, s.heads, s.q_len) || !map_of(&a.dq, b.dq, s, s.heads, s.q_len)))
     return cudaErrorInvalidValue;
   if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len) ||
                   !map_of(&a.dk, b.dk, s, s.kv_heads, s.k_len) || !map_of(&a.dv, b.dv, s, s.kv_heads, s.k_len)))
     return cudaErrorInvalidValue;
-  if (s.q_len) {
-    uint32_t lanes = 1;
-    while (lanes * 8 < s.dim) lanes *= 2;
-    const uint64_t threads = (uint64_t)s.batch * s.heads * a.padded * lanes;
-    const cudaError_t e =
-        pdl_launch(half ? attention_rows_kernel<__half> : attention_rows_kernel<__nv_bfloat16>,
-                   (unsigned)((threads + 255) / 256), 256, 0, stream, a.s, view_of(b.o), view_of(b.dout), b.lse, b.rows,
-                   a.padded, lanes);
-    if (e != cudaSuccess) return e;
-  }
-  return half ? backward_of<__half>(a, s, stream) : backward_of<__nv_bfloat16>(a, s, stream);
+  return s.type == CSW_TYPE_F16 ? backward_of<__half>(a, s, stream) : backward_of<__nv_bfloat16>(a, s, stream);
 }
 
 }  // namespace csw
