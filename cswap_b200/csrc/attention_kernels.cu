@@ -44,6 +44,17 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Set where a wait ran out.
 __device__ int attention_gave_up;
 
+// a tensor that is read by rows
+struct View {
+  const void* p;
+  int64_t b, h, t;
+  template <class T>
+  __device__ const T* row(int batch, int head, int token) const {
+    return static_cast<const T*>(p) + batch * b + head * h + token * t;
+  }
+};
+View view_of(const csw_attention_operand& o) { return {o.data, o.batch_stride, o.head_stride, o.token_stride}; }
+
 struct Shape {
   uint32_t batch, heads, kv_heads, q_len, k_len, dim, share;  // share: query heads of a key head
   int causal;
@@ -552,16 +563,18 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
 // Per head and query, padded to whole tiles, dq leaves for dkv in rows[0] log2(e) L, +inf for a query that sees nothing
 // and behind the last one, so that its probabilities are zero, and in rows[1] D.
 struct Backward {
-  CUtensorMap q, k, v, o, dout, dq, dk, dv;
+  CUtensorMap q, k, v, dout, dq, dk, dv;
   Shape s;
+  View o, grad;  // o and do once more, read by rows
   const float* lse;
   float* rows;
   uint32_t padded;
 };
 
-// Both kernels: 256 threads for the scores (two a row, 64 columns each), one tile of tensor memory for s, one for dp,
-// then the sums.  Two tiles stay in shared memory for a piece; the others come in pairs, two pairs in flight; 64 columns
-// of results for each half of the threads.
+// Both kernels: 256 threads for the scores (two a row, 64 columns each), 128 that prepare a piece's rows and take its
+// results out of tensor memory, so that the first ones go from piece to piece without a pause, a warp that copies and
+// one for the products.  Tensor memory: a tile for s, one for dp, then the sums.  Shared memory: two tiles that stay for a
+// piece, a ring of the others, each with its own barriers, and twice 64 columns of results.
 //
 // With heads of up to 64 the products are short, and the softmax warps would wait for each: their halves then go each
 // their own way, with products of 64 columns for each.  With 128 the tensor cores are the bound, and products of 128
@@ -569,9 +582,10 @@ struct Backward {
 template <int DP>
 struct BackwardPlan {
   static constexpr int kHalves = DP == 64 ? 2 : 1, kColumnsEach = kTile / kHalves;
-  static constexpr int kThreads = 256 + 64;
+  static constexpr int kThreads = 256 + 128 + 64, kListeners = 13;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
-  static constexpr size_t kShared = 6 * kTileBytes + 2 * kChunk;
+  static constexpr int kRing = DP == 64 ? 8 : 4;
+  static constexpr size_t kShared = (2 + kRing) * kTileBytes + 2 * kChunk;
   static constexpr int kColumns = 512;
 };
 
@@ -589,79 +603,91 @@ __device__ __forceinline__ float to_gradients(const float* p, const uint32_t* dp
   return sum[0] + sum[1];
 }
 
+// 64 columns of an accumulator, a thread a row, to a staged tile, or zeros; loaded(): they have left tensor memory
+template <class T, class F>
+__device__ __forceinline__ void take_columns(char* stage, int t, bool any, bool live, uint32_t at, float f, F&& loaded) {
+  uint32_t r[64] = {};
+  if (any) {
+    load32(at, r), load32(at + 32, r + 32);
+    wait_loads(r), wait_loads(r + 32);
+    loaded();
+  }
+  if (!live) {
+#pragma unroll
+    for (int k = 0; k < 64; ++k) r[k] = 0;
+  }
+  stage_columns<T>(stage, t, 0, r, f), stage_columns<T>(stage, t, 32, r + 32, f);
+}
+
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
+  constexpr int H = Plan::kHalves, kRing = Plan::kRing;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  constexpr int H = Plan::kHalves;
-  __shared__ uint64_t bars[9 + 4 * H];
-  __shared__ float halves[3][kTile];  // D of each half of the threads; the sums of ds of the second
+  __shared__ uint64_t bars[6 + 2 * kRing + 4 * H];
+  __shared__ float shifts[2][kTile], deltas[2][kTile];  // of this piece and the next
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
-  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 16, dq_full = empty + 16,
-                 dq_free = dq_full + 8, o_empty = dq_free + 8, s_full = o_empty + 8, s_free = s_full + 8 * H,
-                 dp_full = s_free + 8 * H, ds_ready = dp_full + 8 * H;
+  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, dq_full = q_full + 16, dq_free = q_full + 24,
+                 rows_ready = q_full + 32, left_ready = q_full + 40, full = q_full + 48, empty = full + 8 * kRing,
+                 s_full = empty + 8 * kRing, s_free = s_full + 8 * H, dp_full = s_free + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
-    work_bars.init(9);
-    bar_init(q_full, 1), bar_init(q_empty, 2), bar_init(dq_full, 1), bar_init(dq_free, 256);
-    bar_init(o_empty, DP == 128 ? 2 : 1);
+    work_bars.init(Plan::kListeners);
+    bar_init(q_full, 1), bar_init(q_empty, 1), bar_init(dq_full, 1), bar_init(dq_free, 128);
+    bar_init(rows_ready, 128), bar_init(left_ready, 256);
+    for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     for (int i = 0; i < H; ++i) {
       bar_init(s_full + 8 * i, 1), bar_init(s_free + 8 * i, 256 / H);
       bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
     }
-    for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
   }
-  if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
-  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v), prefetch_map(&a.o);
+  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  if (warp == 12 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
   fence_before();
   __syncthreads();
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256;
   const Shape& s = a.s;
-  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // q, do, then k and v, twice
+  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // behind q and do: k 0, v 0, k 1, v 1, ...
 
-  if (warp == 8) {
+  if (warp == 12) {
     struct Copies {
       const Backward& a;
-      uint32_t tiles_at, ring, q_full, q_empty, full, empty, o_empty;
-      int i = 0, u = 0, it = 0;  // pairs, pieces with any, pieces
+      uint32_t tiles_at, ring, q_full, q_empty, full, empty;
+      int i = 0, u = 0;  // tiles of the ring, pieces with any
       __device__ Piece piece(int index) const { return piece_of_queries(a.s, index, kTile); }
       __device__ bool copy(const Piece& p) {
         const Queries<1> at(a.s, p);
-        if (it > 0 && !bar_wait(o_empty, (it - 1) & 1)) return false;
-        ++it;
         if (at.most == 0) return true;
         if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
-        bar_expect(q_full, 3 * Plan::kTileBytes);
-        copy_tokens<DP>(tiles_at + 6 * Plan::kTileBytes + (DP == 128 ? 0 : kChunk), &a.o, q_full, p.first, p.head, p.batch);
+        bar_expect(q_full, 2 * Plan::kTileBytes);
         copy_tokens<DP>(tiles_at, &a.q, q_full, p.first, p.head, p.batch);
         copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, p.first, p.head, p.batch);
-        for (int j = 0; j < at.most; ++j, ++i) {
-          const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
-          if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
-          bar_expect(bar, 2 * Plan::kTileBytes);
-          copy_tokens<DP>(to, &a.k, bar, j * kTile, p.kv_head, p.batch);
-          copy_tokens<DP>(to + Plan::kTileBytes, &a.v, bar, j * kTile, p.kv_head, p.batch);
+        for (int j = 0; j < 2 * at.most; ++j, ++i) {
+          const int slot = i % kRing;
+          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
+          bar_expect(full + 8 * slot, Plan::kTileBytes);
+          copy_tokens<DP>(ring + slot * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * slot, j / 2 * kTile, p.kv_head, p.batch);
         }
         ++u;
         return true;
       }
     };
     if (threadIdx.x % 32 == 0)
-      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty, o_empty});
-  } else if (warp == 9) {
+      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
+  } else if (warp == 13) {
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      int i = 0, u = 0;
+      int next = 0, u = 0;  // tiles of keys; pieces with any
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
@@ -670,17 +696,16 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         if (n == 0) continue;
         CSW_WAIT_WARP(q_full, u & 1);
         // The scores' place is free once they have been read (s_free), that of dp behind the product that read it.
-        for (int j = -1; j < n; ++j, ++i) {
-          // i counts pairs from the one in front of this piece's first; its own numbers are one less
-          const int now = i - 1 - u, next = now + 1;
-          const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
+        for (int j = -1; j < n; ++j) {
+          const int now = next - 1, k = 2 * next % kRing, v = k + 1, k_now = (2 * now + kRing) % kRing;
+          const uint32_t parity = 2 * next / kRing & 1;
           if (j + 1 < n) {
-            CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
+            CSW_WAIT_WARP(full + 8 * k, parity);
 #pragma unroll
             for (int h = 0; h < H; ++h) {
               if (next > 0) CSW_WAIT_WARP(s_free + 8 * h, now & 1);
               fence_after();
-              product_rows<DP>(s_at + 64 * h, tiles_at, then + h * (kChunk / 2), scores);
+              product_rows<DP>(s_at + 64 * h, tiles_at, ring + k * Plan::kTileBytes + h * (kChunk / 2), scores);
               commit_to(s_full + 8 * h);
             }
           }
@@ -690,60 +715,131 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
               CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
               if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64, at + h * (kChunk / 2), sums, j > 0 || h > 0);
-              if (h + 1 == H) commit_to(empty + 8 * (now & 1));
+              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64,
+                                                 ring + k_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
+              if (h + 1 == H) commit_to(empty + 8 * k_now);
             }
             if (j + 1 < n) {
-              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes + h * (kChunk / 2), slopes);
+              if (h == 0) CSW_WAIT_WARP(full + 8 * v, parity);
+              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, ring + v * Plan::kTileBytes + h * (kChunk / 2),
+                               slopes);
               commit_to(dp_full + 8 * h);
+              if (h + 1 == H) commit_to(empty + 8 * v);
             }
           }
           if (j + 1 == n) commit_to(dq_full);
           if (j + 2 == n) commit_to(q_empty);
+          if (j + 1 < n) ++next;
         }
         ++u;
       }
     }();
+  } else if (warp >= 8) {
+    const int t = threadIdx.x - 256;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    char* stage = tiles + (2 + kRing) * Plan::kTileBytes;
+    // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for
+    auto prepare = [&](const Piece& p, int u) {
+      constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
+      const int lane = t % kLanes, mine = t / 32 * 32 + t % 32 / kLanes;
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; i += kAtOnce) {
+        uint4 x[kAtOnce], y[kAtOnce];  // all loads before the first use: they take some 1000 clocks each
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          // rows behind the last one stand for that, and are not used
+          const int row = min(p.first + mine + (i + k) * kRows, (int)s.q_len - 1);
+          x[k] = y[k] = make_uint4(0, 0, 0, 0);
+          if (lane * 8 < (int)s.dim) {
+            x[k] = *reinterpret_cast<const uint4*>(a.o.row<T>(p.batch, p.head, row) + lane * 8);
+            y[k] = *reinterpret_cast<const uint4*>(a.grad.row<T>(p.batch, p.head, row) + lane * 8);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          float f[8], g[8], d = 0.0f;
+          load_pack(reinterpret_cast<const T*>(&x[k]), f);
+          load_pack(reinterpret_cast<const T*>(&y[k]), g);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) d += f[c] * g[c];
+#pragma unroll
+          for (int c = kLanes / 2; c; c /= 2) d += __shfl_xor_sync(0xffffffffu, d, c);
+          if (lane == 0) deltas[u & 1][mine + (i + k) * kRows] = d;
+        }
+      }
+      const int row = p.first + t;
+      const float lse = row < (int)s.q_len ? a.lse[(uint64_t)p.row * s.q_len + row] : -INFINITY;
+      shifts[u & 1][t] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+      bar_arrive(rows_ready);
+      group_sync(2, 128);
+    };
+    // The results of a piece that sees n tiles; false where a wait ran out.
+    auto finish = [&](const Piece& p, bool any, int u) -> bool {
+      const float shift = any ? shifts[u & 1][t] : INFINITY;
+      const bool live = shift != INFINITY;
+      volatile float* mine = a.rows + (uint64_t)p.row * a.padded + p.first + t;  // padded to whole tiles
+      const uint64_t plane = (uint64_t)s.batch * s.heads * a.padded;
+      float d = 0.0f;
+      if (any) {
+        if (!__all_sync(0xffffffffu, bar_wait(left_ready, u & 1) && bar_wait(dq_full, u & 1))) return false;
+        fence_after();
+        // dkv's D has no rounding of o in it: it is sum p dp, which this kernel has formed on the way.
+        d = live ? deltas[u & 1][t] + mine[0] + mine[plane] : 0.0f;
+      }
+      stage_free(t == 0, 1, 128);
+#pragma unroll
+      for (int c = 0; c < DP; c += 64)
+        take_columns<T>(stage + c / 64 * kChunk, t, any, live, dq_at + c + lanes, s.scale, [&] {
+          if (c + 64 == DP) {
+            fence_before();
+            bar_arrive(dq_free);
+          }
+        });
+      async_fence();
+      group_sync(1, 128);
+      if (t == 0) {
+#pragma unroll
+        for (int c = 0; c < DP; c += 64)
+          if (c < (int)s.dim) store_tile(&a.dq, smem_at(stage) + c / 64 * kChunk, c, p.first, p.head, p.batch);
+      }
+      mine[0] = shift;
+      mine[plane] = d;
+      return true;
+    };
+    [&] {
+      Piece last{-1};
+      int u = 0;
+      for (int it = 0;; ++it) {
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        const bool any = piece.first >= 0 && Queries<1>(s, piece).most > 0;
+        if (any) prepare(piece, u);
+        if (last.first >= 0 && !finish(last, true, u - 1)) return give_up(flag);
+        last.first = -1;
+        if (piece.first < 0) return;
+        if (any) {
+          last = piece;
+          ++u;
+        } else if (!finish(piece, false, 0)) {
+          return give_up(flag);
+        }
+      }
+    }();
+    if (t == 0) stores_read();
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
-    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    // 128 columns of results are staged as two tiles, 64 as one that all threads share
-    const uint32_t own = 8 * (H == 2 ? w : 0);
-    constexpr int kGroup = DP == 128 ? 128 : 256;
-    const int id = DP == 128 ? 1 + w : 1;
-    const bool first = DP == 128 ? t == 0 : threadIdx.x == 0;
-    char* stage = tiles + 6 * Plan::kTileBytes + (DP == 128 ? w * kChunk : 0);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, own = 8 * (H == 2 ? w : 0);
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
-        const Queries<1> at(s, piece);
-        const int keys = piece.keys, n = at.most, row = piece.first + t;
+        const int keys = piece.keys, n = Queries<1>(s, piece).most, row = piece.first + t;
+        if (n == 0) continue;
         const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
-        const float lse = row < (int)s.q_len ? a.lse[(uint64_t)piece.row * s.q_len + row] : -INFINITY;
-        const float shift = lse == -INFINITY ? INFINITY : lse * kLog2e;
-        float d = 0.0f;
-        if (n > 0) {
-          CSW_WAIT_WARP(q_full, u & 1);
-          const char* o_row = tiles + 6 * Plan::kTileBytes + (DP == 128 ? w * kChunk : kChunk) + t * 128;
-          const char* do_row = tiles + Plan::kTileBytes + (DP == 128 ? w * kChunk : 0) + t * 128;
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const int unit = ((DP == 128 ? k : 4 * w + k) ^ (t & 7)) * 16;
-            float x[8], y[8];
-            load_pack(reinterpret_cast<const T*>(o_row + unit), x);
-            load_pack(reinterpret_cast<const T*>(do_row + unit), y);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) d += x[c] * y[c];
-          }
-          halves[w][t] = d;
-          group_sync(3, 256);
-          d = halves[0][t] + halves[1][t];
-          if (threadIdx.x == 0) bar_arrive(q_empty);  // which the last product of the scores does too
-        }
-        if (DP == 64 && threadIdx.x == 0) bar_arrive(o_empty);
+        CSW_WAIT_WARP(rows_ready, u & 1);
+        const float shift = shifts[u & 1][t], d = deltas[u & 1][t];
         float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
         for (int j = 0; j < n; ++j, ++i) {
           CSW_WAIT_WARP(s_full + own, i & 1);
@@ -760,7 +856,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
           }
           const bool masked = (j + 1) * kTile > least;
-          const int end = limit - j * kTile - 64 * w;
+          int end = limit - j * kTile - 64 * w;
           if (masked) {
 #pragma unroll
             for (int k = 0; k < 64; ++k)
@@ -775,6 +871,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             load32(dp_at + 64 * w + 32 * c + lanes, r);
             wait_loads(r);
             if (masked) {
+              asm volatile("" : "+r"(end));  // compared anew, not held from above
 #pragma unroll
               for (int k = 0; k < 32; ++k)
                 if (32 * c + k >= end) r[k] = 0;  // of a key behind the sequence: whatever its value held
@@ -785,59 +882,22 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             store16(dp_at + 64 * w + 16 * c + lanes, out);
           }
           if (w == 0 && s.lens && (j + 1) * kTile > keys) {
-            CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);
-            zero_rows<DP>(tiles + (2 + (i & 1) * 2) * Plan::kTileBytes, keys - j * kTile, t);
+            const int slot = 2 * i % kRing;
+            CSW_WAIT_WARP(full + 8 * slot, 2 * i / kRing & 1);
+            zero_rows<DP>(tiles + (2 + slot) * Plan::kTileBytes, keys - j * kTile, t);
           }
           wait_stores();
           fence_before();
           bar_arrive(ds_ready + own);
         }
-        if (n > 0) {
-          CSW_WAIT_WARP(dq_full, u & 1);
-          ++u;
-          fence_after();
-        }
-        const bool live = n > 0 && shift != INFINITY;
-        if (w == 1) halves[2][t] = left;
-        stage_free(first, id, kGroup);
-        constexpr int kMine = DP / 2;
-#pragma unroll
-        for (int c = 0; c < kMine; c += 32) {
-          uint32_t r[32] = {};
-          if (n > 0) {
-            load32(dq_at + w * kMine + c + lanes, r);
-            wait_loads(r);
-          }
-          if (!live) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = 0;
-          }
-          stage_columns<T>(stage, t, DP == 128 ? c : 32 * w, r, s.scale);
-        }
-        if (n > 0) {
-          fence_before();
-          bar_arrive(dq_free);
-        }
-        stage_out(first, id, kGroup, &a.dq, smem_at(stage), DP == 128 ? 64 * w : 0, piece.first, piece.head, piece.batch);
-        if (DP == 128) {
-          if (first) {
-            stores_read();  // o comes where the results have been
-            bar_arrive(o_empty);
-          }
-          group_sync(3, 256);
-        }
-        if (w == 0) {
-          float* mine = a.rows + (uint64_t)piece.row * a.padded + row;
-          mine[0] = shift;
-          // dkv's D has no rounding of o in it: it is sum p dp, which this kernel has formed on the way.
-          mine[(uint64_t)s.batch * s.heads * a.padded] = live ? d + left + halves[2][t] : 0.0f;
-        }
-        group_sync(3, 256);
+        // by way of the place that the row's numbers will have: shared memory is full
+        a.rows[(w == 0 ? 0 : (uint64_t)s.batch * s.heads * a.padded) + (uint64_t)piece.row * a.padded + row] = left;
+        bar_arrive(left_ready);
+        ++u;
       }
     }();
-    if (first) stores_read();
   }
-  leave<Plan::kColumns>(flag, tmem, warp == 9);
+  leave<Plan::kColumns>(flag, tmem, warp == 13);
 }
 
 // Pieces of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
@@ -854,41 +914,41 @@ struct Keys {
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
+  constexpr int H = Plan::kHalves, kRing = Plan::kRing;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  constexpr int H = Plan::kHalves;
-  __shared__ uint64_t bars[8 + 4 * H];
-  __shared__ __align__(16) float rows[2][2][kTile];  // of each pair in flight: the exponents' shifts, D
+  __shared__ uint64_t bars[4 + 2 * kRing + 4 * H];
+  __shared__ __align__(16) float rows[kRing][kTile];  // with a tile of q the exponents' shifts, with one of do D
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
   const WorkBars work_bars(work);
-  const uint32_t kv_full = smem_at(bars), kv_empty = kv_full + 8, full = kv_full + 16, empty = full + 16,
-                 sums_full = empty + 16, sums_free = sums_full + 8, s_full = sums_free + 8, p_ready = s_full + 8 * H,
+  const uint32_t kv_full = smem_at(bars), kv_empty = kv_full + 8, sums_full = kv_full + 16, sums_free = kv_full + 24,
+                 full = kv_full + 32, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8 * H,
                  dp_full = p_ready + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
-    work_bars.init(9);
-    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(sums_full, 1), bar_init(sums_free, 256);
+    work_bars.init(Plan::kListeners);
+    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(sums_full, 1), bar_init(sums_free, 128);
+    for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     for (int i = 0; i < H; ++i) {
       bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 256 / H);
       bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
     }
-    for (int i = 0; i < 2; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     init_visible();
     flag_word = 0;
   }
-  if (warp == 9) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
-  if (warp == 8 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
+  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
+  if (warp == 12 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
   fence_before();
   __syncthreads();
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = dv_at + DP;
   const Shape& s = a.s;
-  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // k, v, then q and do, twice
+  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // behind k and v: q 0, do 0, q 1, do 1, ...
 
-  if (warp == 8) {
+  if (warp == 12) {
     struct Copies {
       const Backward& a;
       uint32_t tiles_at, ring, rows_at, kv_full, kv_empty, full, empty;
@@ -906,18 +966,16 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         copy_tokens<DP>(tiles_at, &a.k, kv_full, p.first, p.kv_head, p.batch);
         copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, p.first, p.kv_head, p.batch);
         const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
-        int q = at.from;
-        int h = p.head, row = p.row;
-        for (int j = 0; j < at.n; ++j, ++i) {
-          const uint32_t to = ring + i % 2 * 2 * Plan::kTileBytes, bar = full + 8 * (i % 2);
-          if (i >= 2 && !bar_wait(empty + 8 * (i % 2), (i / 2 - 1) & 1)) return false;
-          bar_expect(bar, 2 * Plan::kTileBytes + 2 * kTile * 4);
-          copy_tokens<DP>(to, &a.q, bar, q * kTile, h, p.batch);
-          copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, bar, q * kTile, h, p.batch);
-          const float* src = a.rows + (uint64_t)row * a.padded + (uint64_t)q * kTile;
-          copy_bytes(rows_at + i % 2 * (8 * kTile), src, kTile * 4, bar);
-          copy_bytes(rows_at + i % 2 * (8 * kTile) + 4 * kTile, src + plane, kTile * 4, bar);
-          if (++q == at.tiles) q = at.from, ++h, ++row;
+        int q = at.from, h = 0;
+        for (int j = 0; j < 2 * at.n; ++j, ++i) {
+          const int slot = i % kRing;
+          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
+          const uint32_t bar = full + 8 * slot;
+          bar_expect(bar, Plan::kTileBytes + kTile * 4);
+          copy_tokens<DP>(ring + slot * Plan::kTileBytes, j % 2 ? &a.dout : &a.q, bar, q * kTile, p.head + h, p.batch);
+          copy_bytes(rows_at + slot * (4 * kTile),
+                     a.rows + (j % 2 ? plane : 0) + (uint64_t)(p.row + h) * a.padded + (uint64_t)q * kTile, kTile * 4, bar);
+          if (j % 2 && ++q == at.tiles) q = at.from, ++h;
         }
         ++u;
         return true;
@@ -925,12 +983,12 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     };
     if (threadIdx.x % 32 == 0)
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
-  } else if (warp == 9) {
+  } else if (warp == 13) {
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      int i = 0, u = 0;
+      int next = 0, u = 0;  // tiles of queries; pieces with any
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
@@ -939,21 +997,22 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         if (n == 0) continue;
         CSW_WAIT_WARP(kv_full, u & 1);
         // Each tile's place in tensor memory is written again behind the product that reads it.
-        for (int j = -1; j < n; ++j, ++i) {
-          const int now = i - 1 - u, next = now + 1;
-          const uint32_t at = ring + (now & 1) * 2 * Plan::kTileBytes, then = ring + (next & 1) * 2 * Plan::kTileBytes;
-          if (j + 1 < n) CSW_WAIT_WARP(full + 8 * (next & 1), next / 2 & 1);
+        for (int j = -1; j < n; ++j) {
+          const int now = next - 1, q = 2 * next % kRing, d = q + 1, q_now = (2 * now + kRing) % kRing, d_now = q_now + 1;
+          const uint32_t parity = 2 * next / kRing & 1;
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             if (j >= 0) {
               CSW_WAIT_WARP(p_ready + 8 * h, now & 1);
               if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64, at + Plan::kTileBytes + h * (kChunk / 2), sums,
-                                                 j > 0 || h > 0);
+              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64,
+                                                 ring + d_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
+              if (h + 1 == H) commit_to(empty + 8 * d_now);
             }
             if (j + 1 < n) {
-              product_rows<DP>(s_at + 64 * h, tiles_at, then + h * (kChunk / 2), scores);
+              if (h == 0) CSW_WAIT_WARP(full + 8 * q, parity);
+              product_rows<DP>(s_at + 64 * h, tiles_at, ring + q * Plan::kTileBytes + h * (kChunk / 2), scores);
               commit_to(s_full + 8 * h);
             }
           }
@@ -962,27 +1021,71 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
             if (j >= 0) {
               CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64, at + h * (kChunk / 2), sums, j > 0 || h > 0);
-              if (h + 1 == H) commit_to(empty + 8 * (now & 1));
+              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64,
+                                                 ring + q_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
+              if (h + 1 == H) commit_to(empty + 8 * q_now);
             }
             if (j + 1 < n) {
-              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, then + Plan::kTileBytes + h * (kChunk / 2), slopes);
+              if (h == 0) CSW_WAIT_WARP(full + 8 * d, parity);
+              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, ring + d * Plan::kTileBytes + h * (kChunk / 2),
+                               slopes);
               commit_to(dp_full + 8 * h);
             }
           }
           if (j + 1 == n) commit_to(sums_full);
           if (j + 2 == n) commit_to(kv_empty);
+          if (j + 1 < n) ++next;
         }
         ++u;
       }
     }();
+  } else if (warp >= 8) {
+    const int t = threadIdx.x - 256;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    char* stage = tiles + (2 + kRing) * Plan::kTileBytes;
+    [&] {
+      int u = 0;
+      for (int it = 0;; ++it) {
+        Piece piece;
+        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (piece.first < 0) return;
+        const bool any = Keys(s, piece).n > 0;
+        if (any) {
+          CSW_WAIT_WARP(sums_full, u & 1);
+          ++u;
+          fence_after();
+        }
+        // A key behind its sequence has no gradient, whatever its row of the tile held.
+        const bool live = any && piece.first + t < piece.keys;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // dv, dk
+          const uint32_t from = (x == 0 ? dv_at : dk_at) + lanes;
+          stage_free(t == 0, 1, 128);
+#pragma unroll
+          for (int c = 0; c < DP; c += 64)
+            take_columns<T>(stage + c / 64 * kChunk, t, any, live, from + c, x == 0 ? 1.0f : s.scale, [&] {
+              if (x == 1 && c + 64 == DP) {
+                fence_before();
+                bar_arrive(sums_free);
+              }
+            });
+          async_fence();
+          group_sync(1, 128);
+          if (t == 0) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 64)
+              if (c < (int)s.dim)
+                store_tile(x == 0 ? &a.dv : &a.dk, smem_at(stage) + c / 64 * kChunk, c, piece.first, piece.kv_head, piece.batch);
+          }
+        }
+      }
+    }();
+    if (t == 0) stores_read();
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
-    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t own = 8 * (H == 2 ? w : 0);
-    char* stage = tiles + 6 * Plan::kTileBytes + w * kChunk;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, own = 8 * (H == 2 ? w : 0);
     [&] {
-      int i = 0, u = 0;
+      int i = 0;
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
@@ -991,13 +1094,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         const int n = at.n, row = piece.first + t, off = (int)s.k_len - (int)s.q_len;
         int q = at.from;
         for (int j = 0; j < n; ++j, ++i) {
-          CSW_WAIT_WARP(full + 8 * (i & 1), i / 2 & 1);  // the rows' numbers
+          const int slot = 2 * i % kRing;
+          const uint32_t parity = 2 * i / kRing & 1;
+          CSW_WAIT_WARP(full + 8 * slot, parity);  // the rows' numbers
           CSW_WAIT_WARP(s_full + own, i & 1);
           fence_after();
           float p[64];
-          const float4* shifts = reinterpret_cast<const float4*>(rows[i & 1][0] + 64 * w);
-          const float4* deltas = reinterpret_cast<const float4*>(rows[i & 1][1] + 64 * w);
           {
+            const float4* shifts = reinterpret_cast<const float4*>(rows[slot] + 64 * w);
             uint32_t r[64];
             load32(s_at + 64 * w + lanes, r);
             load32(s_at + 64 * w + 32 + lanes, r + 32);
@@ -1028,8 +1132,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           fence_before();
           bar_arrive(p_ready + own);
 
+          CSW_WAIT_WARP(full + 8 * slot + 8, parity);
           CSW_WAIT_WARP(dp_full + own, i & 1);
           fence_after();
+          const float4* deltas = reinterpret_cast<const float4*>(rows[slot + 1] + 64 * w);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t r[32], out[16];
@@ -1049,39 +1155,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           bar_arrive(ds_ready + own);
           if (++q == at.tiles) q = at.from;
         }
-        if (n > 0) {
-          CSW_WAIT_WARP(sums_full, u & 1);
-          ++u;
-          fence_after();
-        }
-        // A key behind its sequence has no gradient, whatever its row of the tile held.
-        const bool live = n > 0 && row < piece.keys;
-#pragma unroll
-        for (int c = 0; c < DP; c += 64) {
-          stage_free(t == 0, 1 + w, 128);
-          uint32_t r[64] = {};
-          if (n > 0) {
-            const uint32_t from = (w == 0 ? dv_at : dk_at) + c + lanes;
-            load32(from, r), load32(from + 32, r + 32);
-            wait_loads(r), wait_loads(r + 32);
-            if (c + 64 == DP) {
-              fence_before();
-              bar_arrive(sums_free);
-            }
-          }
-          if (!live) {
-#pragma unroll
-            for (int k = 0; k < 64; ++k) r[k] = 0;
-          }
-          const float f = w == 0 ? 1.0f : s.scale;
-          stage_columns<T>(stage, t, 0, r, f), stage_columns<T>(stage, t, 32, r + 32, f);
-          stage_out(t == 0, 1 + w, 128, w == 0 ? &a.dv : &a.dk, smem_at(stage), c, piece.first, piece.kv_head, piece.batch);
-        }
       }
     }();
-    if (t == 0) stores_read();
   }
-  leave<Plan::kColumns>(flag, tmem, warp == 9);
+  leave<Plan::kColumns>(flag, tmem, warp == 13);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
@@ -1191,11 +1268,12 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   if (const cudaError_t e = bind_context()) return e;
   Backward a;
   a.s = shape_of(s);
+  a.o = view_of(b.o), a.grad = view_of(b.dout);
   a.lse = b.lse, a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
   // of an empty side nothing is copied
-  a.q = a.k = a.v = a.o = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
+  a.q = a.k = a.v = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
   if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len) ||
-                  !map_of(&a.o, b.o, s, s.heads, s.q_len) || !map_of(&a.dq, b.dq, s, s.heads, s.q_len)))
+                  !map_of(&a.dq, b.dq, s, s.heads, s.q_len)))
     return cudaErrorInvalidValue;
   if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len) ||
                   !map_of(&a.dk, b.dk, s, s.kv_heads, s.k_len) || !map_of(&a.dv, b.dv, s, s.kv_heads, s.k_len)))
