@@ -115,18 +115,16 @@ __device__ __forceinline__ void stage_columns(char* tile, int row, int at, const
   }
 }
 
-// All columns of a tile's rows [first, 128), zeroed by 128 threads: what lies behind a sequence must not meet the
-// zeros of its probabilities as a NaN.
+// All columns of a tile's rows [first, 128), zeroed by the warp that issues the products: what lies behind a sequence
+// must not meet the zeros of its probabilities as a NaN.
 template <int DP>
-__device__ __forceinline__ void zero_rows(char* tile, int first, int thread) {
-  if (thread >= first) {
+__device__ __forceinline__ void zero_rows(char* tile, int first) {
+  for (int i = threadIdx.x % 32; i < (kTile - first) * 8; i += 32)
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<uint4*>(tile + c * kChunk + thread * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-  }
+      *reinterpret_cast<uint4*>(tile + c * kChunk + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   async_fence();
+  __syncwarp();
 }
 
 template <int DP>
@@ -135,9 +133,11 @@ __device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map
 #pragma unroll
   for (int c = 0; c < DP / 64; ++c) copy_tile(dst + c * kChunk, map, bar, c * 64, token, head, batch);
 }
-// acc (+)= A B^T: both read along their rows, the reduction over the head's dimension
+// acc (+)= A B^T: both read along their rows, the reduction over the head's dimension.  Behind the products of a call
+// the barriers that are not 0 are arrived at: once these, and all in front, have ended.
 template <int DP>
-__device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t b, uint32_t desc) {
+__device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t b, uint32_t desc, uint32_t bar0 = 0,
+                                             uint32_t bar1 = 0) {
   const uint64_t da = tile_desc(a, 16), db = tile_desc(b, 16);
   if (elected()) {
 #pragma unroll
@@ -145,18 +145,22 @@ __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t 
       const uint32_t at = (k / 4 * kChunk + k % 4 * 32) / 16;
       mma(acc, da + at, db + at, desc, k > 0);
     }
+    if (bar0) commit(bar0);
+    if (bar1) commit(bar1);
   }
 }
 // acc (+)= P B: P in tensor memory, B read across its rows, the reduction over TOKENS tokens.  P's first 64 columns lie
 // at p, the others at p + half.
 template <int TOKENS>
 __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
-                                               bool add) {
+                                               bool add, uint32_t bar0 = 0, uint32_t bar1 = 0) {
   const uint64_t db = tile_desc(b, kChunk);
   if (elected()) {
 #pragma unroll
     for (int k = 0; k < TOKENS / 16; ++k)
       mma_tmem(acc, p + k / 4 * half + k % 4 * 8, db + k * (2048 / 16), desc, add || k > 0);
+    if (bar0) commit(bar0);
+    if (bar1) commit(bar1);
   }
 }
 __device__ __forceinline__ void commit_to(uint32_t bar) {
@@ -448,7 +452,11 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
         for (int j = 0; j <= at.most; ++j) {
           const int ki = base + 2 * j, vi = ki - 1, k = ki % Plan::kStages, v = vi % Plan::kStages;
           if (j < at.most) CSW_WAIT_WARP(full + 8 * k, ki / Plan::kStages & 1);
-          if (j > 0) CSW_WAIT_WARP(full + 8 * v, vi / Plan::kStages & 1);
+          if (j > 0) {
+            CSW_WAIT_WARP(full + 8 * v, vi / Plan::kStages & 1);
+            if (s.lens && j * kTile > piece.keys)
+              zero_rows<DP>(tiles + (NWG + v) * Plan::kTileBytes, piece.keys - (j - 1) * kTile);
+          }
 #pragma unroll
           for (int w = 0; w < NWG; ++w) {
             const uint32_t sw = tmem + w * 128, ow = tmem + NWG * 128 + w * DP;
@@ -456,12 +464,12 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               CSW_WAIT_WARP(p_ready + 8 * w, tile[w]++ & 1);
               if (j == 1 && done[w] > 0) CSW_WAIT_WARP(o_free + 8 * w, (done[w] - 1) & 1);
               fence_after();
-              product_tokens<kTile>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1);
-              if (j == at.count[w]) commit_to(o_full + 8 * w), ++done[w];
+              const bool last = j == at.count[w];
+              product_tokens<kTile>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1, last ? o_full + 8 * w : 0);
+              done[w] += last;
             }
             if (j < at.count[w]) {
-              product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores);
-              commit_to(s_full + 8 * w);
+              product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores, s_full + 8 * w);
             }
           }
           if (j < at.most) commit_to(empty + 8 * k);
@@ -477,7 +485,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     const uint32_t sw = tmem + w * 128 + lanes, ow = tmem + NWG * 128 + w * DP + lanes;
     char* stage = tiles + (NWG + Plan::kStages) * Plan::kTileBytes + w * kChunk;
     [&] {
-      int tile = 0, done = 0, base = 0;
+      int tile = 0, done = 0;
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
@@ -518,17 +526,10 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           const float shift = top == -INFINITY ? 0.0f : top * s.exponent;
           sum += masked ? row_exp<T, true>(sw, chunks, end, s.exponent, shift)
                         : row_exp<T, false>(sw, 4, 0, s.exponent, shift);
-          // the tile of values that the sequence ends in, once for all that read it
-          if (s.lens && (j + 1) * kTile > keys && (w == 0 || j >= at.count[0])) {
-            const int i = base + 2 * j + 1, slot = i % Plan::kStages;
-            CSW_WAIT_WARP(full + 8 * slot, i / Plan::kStages & 1);
-            zero_rows<DP>(tiles + (NWG + slot) * Plan::kTileBytes, keys - j * kTile, t);
-          }
           wait_stores();
           fence_before();
           bar_arrive(p_ready + 8 * w);
         }
-        base += 2 * at.most;
         if (n > 0) {
           CSW_WAIT_WARP(o_full + 8 * w, done & 1);
           ++done;
@@ -584,8 +585,8 @@ struct BackwardPlan {
   static constexpr int kHalves = DP == 64 ? 2 : 1, kColumnsEach = kTile / kHalves;
   static constexpr int kThreads = 256 + 128 + 64, kListeners = 13;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
-  static constexpr int kRing = DP == 64 ? 8 : 4;
-  static constexpr size_t kShared = (2 + kRing) * kTileBytes + 2 * kChunk;
+  static constexpr int kRing = DP == 64 ? 6 : 4, kStay = DP == 64 ? 2 : 1;  // tiles; pieces whose own tiles have a place
+  static constexpr size_t kShared = (2 * kStay + kRing) * kTileBytes + 2 * kChunk;
   static constexpr int kColumns = 512;
 };
 
@@ -622,22 +623,23 @@ __device__ __forceinline__ void take_columns(char* stage, int t, bool any, bool 
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  constexpr int H = Plan::kHalves, kRing = Plan::kRing;
+  constexpr int H = Plan::kHalves, kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[6 + 2 * kRing + 4 * H];
+  __shared__ uint64_t bars[4 + 2 * kStay + 2 * kRing + 4 * H];
   __shared__ float shifts[2][kTile], deltas[2][kTile];  // of this piece and the next
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
-  const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, dq_full = q_full + 16, dq_free = q_full + 24,
-                 rows_ready = q_full + 32, left_ready = q_full + 40, full = q_full + 48, empty = full + 8 * kRing,
+  const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, rows_ready = dq_full + 16, left_ready = dq_full + 24,
+                 q_full = dq_full + 32, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
                  s_full = empty + 8 * kRing, s_free = s_full + 8 * H, dp_full = s_free + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(Plan::kListeners);
-    bar_init(q_full, 1), bar_init(q_empty, 1), bar_init(dq_full, 1), bar_init(dq_free, 128);
+    bar_init(dq_full, 1), bar_init(dq_free, 128);
+    for (int i = 0; i < kStay; ++i) bar_init(q_full + 8 * i, 1), bar_init(q_empty + 8 * i, 1);
     bar_init(rows_ready, 128), bar_init(left_ready, 256);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     for (int i = 0; i < H; ++i) {
@@ -653,9 +655,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   __syncthreads();
   fence_after();
   pdl_wait();
-  const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256;
+  const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256,
+                 left_at = dq_at + DP;  // two columns for each of two pieces: the halves' sums of ds
   const Shape& s = a.s;
-  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // behind q and do: k 0, v 0, k 1, v 1, ...
+  const uint32_t ring = tiles_at + 2 * kStay * Plan::kTileBytes;  // behind q and do: k 0, v 0, k 1, v 1, ...
 
   if (warp == 12) {
     struct Copies {
@@ -666,10 +669,11 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       __device__ bool copy(const Piece& p) {
         const Queries<1> at(a.s, p);
         if (at.most == 0) return true;
-        if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
-        bar_expect(q_full, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(tiles_at, &a.q, q_full, p.first, p.head, p.batch);
-        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.dout, q_full, p.first, p.head, p.batch);
+        const uint32_t to = tiles_at + u % kStay * 2 * Plan::kTileBytes, here = q_full + 8 * (u % kStay);
+        if (u >= kStay && !bar_wait(q_empty + 8 * (u % kStay), (u / kStay - 1) & 1)) return false;
+        bar_expect(here, 2 * Plan::kTileBytes);
+        copy_tokens<DP>(to, &a.q, here, p.first, p.head, p.batch);
+        copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, here, p.first, p.head, p.batch);
         for (int j = 0; j < 2 * at.most; ++j, ++i) {
           const int slot = i % kRing;
           if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
@@ -687,49 +691,59 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      int next = 0, u = 0;  // tiles of keys; pieces with any
+      // The scores of the next tile come in front of what follows of this one: their place is free once they have been
+      // read, that of dp behind the product that reads it.
+      uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of keys, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const int n = Queries<1>(s, piece).most;
         if (n == 0) continue;
-        CSW_WAIT_WARP(q_full, u & 1);
-        // The scores' place is free once they have been read (s_free), that of dp behind the product that read it.
+        const uint32_t stay = u % kStay, q_at = tiles_at + stay * 2 * Plan::kTileBytes;
+        CSW_WAIT_WARP(q_full + 8 * stay, u / kStay & 1);
+        uint32_t before = 0;  // the slot of this turn's tile, whose scores came the turn before
         for (int j = -1; j < n; ++j) {
-          const int now = next - 1, k = 2 * next % kRing, v = k + 1, k_now = (2 * now + kRing) % kRing;
-          const uint32_t parity = 2 * next / kRing & 1;
-          if (j + 1 < n) {
-            CSW_WAIT_WARP(full + 8 * k, parity);
+          const bool now = j >= 0, next = j + 1 < n;
+          const uint32_t k_at = ring + slot * Plan::kTileBytes, v_at = k_at + Plan::kTileBytes;
+          if (next) {
+            CSW_WAIT_WARP(full + 8 * slot, round & 1);
+            if (s.lens && (j + 2) * kTile > piece.keys) {
+              const int keys = piece.keys - (j + 1) * kTile;
+              zero_rows<DP>(tiles + (2 * kStay + slot) * Plan::kTileBytes, keys);
+              CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+              zero_rows<DP>(tiles + (2 * kStay + slot + 1) * Plan::kTileBytes, keys);
+            }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-              if (next > 0) CSW_WAIT_WARP(s_free + 8 * h, now & 1);
+              if (i > 0) CSW_WAIT_WARP(s_free + 8 * h, (i - 1) & 1);
               fence_after();
-              product_rows<DP>(s_at + 64 * h, tiles_at, ring + k * Plan::kTileBytes + h * (kChunk / 2), scores);
-              commit_to(s_full + 8 * h);
+              product_rows<DP>(s_at + 64 * h, q_at, k_at + h * (kChunk / 2), scores, s_full + 8 * h);
             }
           }
 #pragma unroll
           for (int h = 0; h < H; ++h) {
-            if (j >= 0) {
-              CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
+            if (now) {
+              CSW_WAIT_WARP(ds_ready + 8 * h, (i - 1) & 1);
               if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64,
-                                                 ring + k_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
-              if (h + 1 == H) commit_to(empty + 8 * k_now);
+              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64, ring + before * Plan::kTileBytes + h * (kChunk / 2),
+                                                 sums, j > 0 || h > 0, h + 1 == H ? empty + 8 * before : 0,
+                                                 h + 1 == H && !next ? dq_full : 0);
             }
-            if (j + 1 < n) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * v, parity);
-              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, ring + v * Plan::kTileBytes + h * (kChunk / 2),
-                               slopes);
-              commit_to(dp_full + 8 * h);
-              if (h + 1 == H) commit_to(empty + 8 * v);
+            if (next) {
+              if (h == 0) CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+              product_rows<DP>(dp_at + 64 * h, q_at + Plan::kTileBytes, v_at + h * (kChunk / 2), slopes, dp_full + 8 * h,
+                               h + 1 == H ? empty + 8 * slot + 8 : 0);
             }
           }
-          if (j + 1 == n) commit_to(dq_full);
-          if (j + 2 == n) commit_to(q_empty);
-          if (j + 1 < n) ++next;
+          if (j + 2 == n) commit_to(q_empty + 8 * stay);
+          before = slot;
+          if (next) {
+            ++i;
+            slot += 2;
+            if (slot == kRing) slot = 0, ++round;
+          }
         }
         ++u;
       }
@@ -737,7 +751,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   } else if (warp >= 8) {
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    char* stage = tiles + (2 + kRing) * Plan::kTileBytes;
+    char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
     // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for
     auto prepare = [&](const Piece& p, int u) {
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
@@ -777,14 +791,15 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     auto finish = [&](const Piece& p, bool any, int u) -> bool {
       const float shift = any ? shifts[u & 1][t] : INFINITY;
       const bool live = shift != INFINITY;
-      volatile float* mine = a.rows + (uint64_t)p.row * a.padded + p.first + t;  // padded to whole tiles
+      float* mine = a.rows + (uint64_t)p.row * a.padded + p.first + t;  // padded to whole tiles
       const uint64_t plane = (uint64_t)s.batch * s.heads * a.padded;
       float d = 0.0f;
       if (any) {
         if (!__all_sync(0xffffffffu, bar_wait(left_ready, u & 1) && bar_wait(dq_full, u & 1))) return false;
         fence_after();
         // dkv's D has no rounding of o in it: it is sum p dp, which this kernel has formed on the way.
-        d = live ? deltas[u & 1][t] + mine[0] + mine[plane] : 0.0f;
+        const float2 left = load2(left_at + 2 * (u & 1) + lanes);
+        d = live ? deltas[u & 1][t] + left.x + left.y : 0.0f;
       }
       stage_free(t == 0, 1, 128);
 #pragma unroll
@@ -856,7 +871,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
           }
           const bool masked = (j + 1) * kTile > least;
-          int end = limit - j * kTile - 64 * w;
+          const int end = limit - j * kTile - 64 * w;
           if (masked) {
 #pragma unroll
             for (int k = 0; k < 64; ++k)
@@ -870,28 +885,18 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             float dd[32];
             load32(dp_at + 64 * w + 32 * c + lanes, r);
             wait_loads(r);
-            if (masked) {
-              asm volatile("" : "+r"(end));  // compared anew, not held from above
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (32 * c + k >= end) r[k] = 0;  // of a key behind the sequence: whatever its value held
-            }
 #pragma unroll
             for (int k = 0; k < 32; ++k) dd[k] = d;
             left += to_gradients<T>(p + 32 * c, r, dd, out);
             store16(dp_at + 64 * w + 16 * c + lanes, out);
           }
-          if (w == 0 && s.lens && (j + 1) * kTile > keys) {
-            const int slot = 2 * i % kRing;
-            CSW_WAIT_WARP(full + 8 * slot, 2 * i / kRing & 1);
-            zero_rows<DP>(tiles + (2 + slot) * Plan::kTileBytes, keys - j * kTile, t);
-          }
           wait_stores();
           fence_before();
           bar_arrive(ds_ready + own);
         }
-        // by way of the place that the row's numbers will have: shared memory is full
-        a.rows[(w == 0 ? 0 : (uint64_t)s.batch * s.heads * a.padded) + (uint64_t)piece.row * a.padded + row] = left;
+        store1(left_at + 2 * (u & 1) + w + lanes, left);
+        wait_stores();
+        fence_before();
         bar_arrive(left_ready);
         ++u;
       }
@@ -914,22 +919,23 @@ struct Keys {
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  constexpr int H = Plan::kHalves, kRing = Plan::kRing;
+  constexpr int H = Plan::kHalves, kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[4 + 2 * kRing + 4 * H];
+  __shared__ uint64_t bars[2 + 2 * kStay + 2 * kRing + 4 * H];
   __shared__ __align__(16) float rows[kRing][kTile];  // with a tile of q the exponents' shifts, with one of do D
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
   const WorkBars work_bars(work);
-  const uint32_t kv_full = smem_at(bars), kv_empty = kv_full + 8, sums_full = kv_full + 16, sums_free = kv_full + 24,
-                 full = kv_full + 32, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8 * H,
+  const uint32_t sums_full = smem_at(bars), sums_free = sums_full + 8, kv_full = sums_full + 16,
+                 kv_empty = kv_full + 8 * kStay, full = kv_empty + 8 * kStay, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8 * H,
                  dp_full = p_ready + 8 * H, ds_ready = dp_full + 8 * H;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(Plan::kListeners);
-    bar_init(kv_full, 1), bar_init(kv_empty, 1), bar_init(sums_full, 1), bar_init(sums_free, 128);
+    bar_init(sums_full, 1), bar_init(sums_free, 128);
+    for (int i = 0; i < kStay; ++i) bar_init(kv_full + 8 * i, 1), bar_init(kv_empty + 8 * i, 1);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     for (int i = 0; i < H; ++i) {
       bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 256 / H);
@@ -946,7 +952,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = dv_at + DP;
   const Shape& s = a.s;
-  const uint32_t ring = tiles_at + 2 * Plan::kTileBytes;  // behind k and v: q 0, do 0, q 1, do 1, ...
+  const uint32_t ring = tiles_at + 2 * kStay * Plan::kTileBytes;  // behind k and v: q 0, do 0, q 1, do 1, ...
 
   if (warp == 12) {
     struct Copies {
@@ -961,10 +967,11 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       __device__ bool copy(const Piece& p) {
         const Keys at(a.s, p);
         if (at.n == 0) return true;
-        if (u > 0 && !bar_wait(kv_empty, (u - 1) & 1)) return false;
-        bar_expect(kv_full, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(tiles_at, &a.k, kv_full, p.first, p.kv_head, p.batch);
-        copy_tokens<DP>(tiles_at + Plan::kTileBytes, &a.v, kv_full, p.first, p.kv_head, p.batch);
+        const uint32_t to = tiles_at + u % kStay * 2 * Plan::kTileBytes, here = kv_full + 8 * (u % kStay);
+        if (u >= kStay && !bar_wait(kv_empty + 8 * (u % kStay), (u / kStay - 1) & 1)) return false;
+        bar_expect(here, 2 * Plan::kTileBytes);
+        copy_tokens<DP>(to, &a.k, here, p.first, p.kv_head, p.batch);
+        copy_tokens<DP>(to + Plan::kTileBytes, &a.v, here, p.first, p.kv_head, p.batch);
         const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
         int q = at.from, h = 0;
         for (int j = 0; j < 2 * at.n; ++j, ++i) {
@@ -988,53 +995,55 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
       const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
-      int next = 0, u = 0;  // tiles of queries; pieces with any
+      // Each place in tensor memory is written again behind the product that reads it.
+      uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of queries, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const int n = Keys(s, piece).n;
         if (n == 0) continue;
-        CSW_WAIT_WARP(kv_full, u & 1);
-        // Each tile's place in tensor memory is written again behind the product that reads it.
+        const uint32_t stay = u % kStay, k_at = tiles_at + stay * 2 * Plan::kTileBytes;
+        CSW_WAIT_WARP(kv_full + 8 * stay, u / kStay & 1);
+        uint32_t before = 0;  // the slot of this turn's tile, whose scores came the turn before
         for (int j = -1; j < n; ++j) {
-          const int now = next - 1, q = 2 * next % kRing, d = q + 1, q_now = (2 * now + kRing) % kRing, d_now = q_now + 1;
-          const uint32_t parity = 2 * next / kRing & 1;
+          const bool now = j >= 0, next = j + 1 < n;
+          const uint32_t q_at = ring + slot * Plan::kTileBytes, do_at = q_at + Plan::kTileBytes;
+          const uint32_t q_now = ring + before * Plan::kTileBytes, do_now = q_now + Plan::kTileBytes;
 #pragma unroll
           for (int h = 0; h < H; ++h) {
-            if (j >= 0) {
-              CSW_WAIT_WARP(p_ready + 8 * h, now & 1);
+            if (now) {
+              CSW_WAIT_WARP(p_ready + 8 * h, (i - 1) & 1);
               if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64,
-                                                 ring + d_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
-              if (h + 1 == H) commit_to(empty + 8 * d_now);
+              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64, do_now + h * (kChunk / 2), sums, j > 0 || h > 0,
+                                                 h + 1 == H ? empty + 8 * before + 8 : 0);
             }
-            if (j + 1 < n) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * q, parity);
-              product_rows<DP>(s_at + 64 * h, tiles_at, ring + q * Plan::kTileBytes + h * (kChunk / 2), scores);
-              commit_to(s_full + 8 * h);
+            if (next) {
+              if (h == 0) CSW_WAIT_WARP(full + 8 * slot, round & 1);
+              product_rows<DP>(s_at + 64 * h, k_at, q_at + h * (kChunk / 2), scores, s_full + 8 * h);
             }
           }
 #pragma unroll
           for (int h = 0; h < H; ++h) {
-            if (j >= 0) {
-              CSW_WAIT_WARP(ds_ready + 8 * h, now & 1);
+            if (now) {
+              CSW_WAIT_WARP(ds_ready + 8 * h, (i - 1) & 1);
               fence_after();
-              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64,
-                                                 ring + q_now * Plan::kTileBytes + h * (kChunk / 2), sums, j > 0 || h > 0);
-              if (h + 1 == H) commit_to(empty + 8 * q_now);
+              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64, q_now + h * (kChunk / 2), sums, j > 0 || h > 0,
+                                                 h + 1 == H ? empty + 8 * before : 0, h + 1 == H && !next ? sums_full : 0);
             }
-            if (j + 1 < n) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * d, parity);
-              product_rows<DP>(dp_at + 64 * h, tiles_at + Plan::kTileBytes, ring + d * Plan::kTileBytes + h * (kChunk / 2),
-                               slopes);
-              commit_to(dp_full + 8 * h);
+            if (next) {
+              if (h == 0) CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+              product_rows<DP>(dp_at + 64 * h, k_at + Plan::kTileBytes, do_at + h * (kChunk / 2), slopes, dp_full + 8 * h);
             }
           }
-          if (j + 1 == n) commit_to(sums_full);
-          if (j + 2 == n) commit_to(kv_empty);
-          if (j + 1 < n) ++next;
+          if (j + 2 == n) commit_to(kv_empty + 8 * stay);
+          before = slot;
+          if (next) {
+            ++i;
+            slot += 2;
+            if (slot == kRing) slot = 0, ++round;
+          }
         }
         ++u;
       }
@@ -1042,7 +1051,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   } else if (warp >= 8) {
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    char* stage = tiles + (2 + kRing) * Plan::kTileBytes;
+    char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
     [&] {
       int u = 0;
       for (int it = 0;; ++it) {

@@ -24,21 +24,27 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// true once the phase of this parity is over; false where it does not end within two seconds or so
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity) {
   const long long start = clock64();
   do {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
+    if (bar_try(bar, parity)) return true;
   } while (clock64() - start < (1ll << 32));
   return false;
+}
+// true once the phase of this parity is over; false where it does not end within two seconds or so
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  return bar_try(bar, parity) || bar_wait_on(bar, parity);
 }
 __device__ __forceinline__ void init_visible() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 // shared memory written by ordinary stores, before the tensor cores or a tile copy see it
@@ -152,6 +158,16 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
       "%15};" ::CSW_R16(CSW_IN, 0),
       "r"(at)
       : "memory");
+}
+__device__ __forceinline__ void store1(uint32_t at, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at), "f"(v) : "memory");
+}
+// two columns, waited for
+__device__ __forceinline__ float2 load2(uint32_t at) {
+  float2 v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v.x), "+f"(v.y)::"memory");
+  return v;
 }
 #undef CSW_R4
 #undef CSW_R16

@@ -438,6 +438,19 @@ def test_attention_padded_batch(cs, kind, causal, dim):
 
 
 @halves
+@pytest.mark.parametrize("dim,causal", [(64, False), (64, True), (128, True)])
+def test_attention_many_pieces(cs, kind, dim, causal):
+    """More tiles of heads than a device runs at once, some without any key, others with one tile or two: a CTA goes
+    through a dozen, and none of them waits for another."""
+    lens = torch.randint(0, 261, (70,), generator=torch.Generator().manual_seed(dim), dtype=torch.int32)
+    lens[::3] = 0
+    lens[1::5] = 128
+    q, k, v, do = operands(kind, 70, 16, 4, 130, 260, dim, seed=30)
+    check_attention(cs, q, k, v, do, causal=causal, lens=lens.cuda())
+    assert cs.lib().csw_device_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+@halves
 def test_attention_rows_that_see_nothing(cs, kind):
     """Causal with more queries than keys: the first rows see no key."""
     q, k, v, do = operands(kind, 1, 2, 2, 300, 20, 64, seed=2)
