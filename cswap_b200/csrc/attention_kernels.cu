@@ -149,15 +149,14 @@ __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t 
     if (bar1) commit(bar1);
   }
 }
-// acc (+)= P B: P in tensor memory, B read across its rows, the reduction over TOKENS tokens.  P's first 64 columns lie
+// acc (+)= P B: P in tensor memory, B read across its rows, the reduction over 128 tokens.  P's first 64 columns lie
 // at p, the others at p + half.
-template <int TOKENS>
 __device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
                                                bool add, uint32_t bar0 = 0, uint32_t bar1 = 0) {
   const uint64_t db = tile_desc(b, kChunk);
   if (elected()) {
 #pragma unroll
-    for (int k = 0; k < TOKENS / 16; ++k)
+    for (int k = 0; k < kTile / 16; ++k)
       mma_tmem(acc, p + k / 4 * half + k % 4 * 8, db + k * (2048 / 16), desc, add || k > 0);
     if (bar0) commit(bar0);
     if (bar1) commit(bar1);
@@ -465,7 +464,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               if (j == 1 && done[w] > 0) CSW_WAIT_WARP(o_free + 8 * w, (done[w] - 1) & 1);
               fence_after();
               const bool last = j == at.count[w];
-              product_tokens<kTile>(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1, last ? o_full + 8 * w : 0);
+              product_tokens(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1, last ? o_full + 8 * w : 0);
               done[w] += last;
             }
             if (j < at.count[w]) {
@@ -576,13 +575,8 @@ struct Backward {
 // results out of tensor memory, so that the first ones go from piece to piece without a pause, a warp that copies and
 // one for the products.  Tensor memory: a tile for s, one for dp, then the sums.  Shared memory: two tiles that stay for a
 // piece, a ring of the others, each with its own barriers, and twice 64 columns of results.
-//
-// With heads of up to 64 the products are short, and the softmax warps would wait for each: their halves then go each
-// their own way, with products of 64 columns for each.  With 128 the tensor cores are the bound, and products of 128
-// columns keep them busier (of 64 columns they would read shared memory for 48 clocks a step and compute for 32).
 template <int DP>
 struct BackwardPlan {
-  static constexpr int kHalves = DP == 64 ? 2 : 1, kColumnsEach = kTile / kHalves;
   static constexpr int kThreads = 256 + 128 + 64, kListeners = 13;
   static constexpr uint32_t kTileBytes = kTile * DP * 2;
   static constexpr int kRing = DP == 64 ? 6 : 4, kStay = DP == 64 ? 2 : 1;  // tiles; pieces whose own tiles have a place
@@ -623,17 +617,17 @@ __device__ __forceinline__ void take_columns(char* stage, int t, bool any, bool 
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  constexpr int H = Plan::kHalves, kRing = Plan::kRing, kStay = Plan::kStay;
+  constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[4 + 2 * kStay + 2 * kRing + 4 * H];
+  __shared__ uint64_t bars[4 + 2 * kStay + 2 * kRing + 4];
   __shared__ float shifts[2][kTile], deltas[2][kTile];  // of this piece and the next
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
   const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, rows_ready = dq_full + 16, left_ready = dq_full + 24,
                  q_full = dq_full + 32, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
-                 s_full = empty + 8 * kRing, s_free = s_full + 8 * H, dp_full = s_free + 8 * H, ds_ready = dp_full + 8 * H;
+                 s_full = empty + 8 * kRing, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
@@ -642,10 +636,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     for (int i = 0; i < kStay; ++i) bar_init(q_full + 8 * i, 1), bar_init(q_empty + 8 * i, 1);
     bar_init(rows_ready, 128), bar_init(left_ready, 256);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
-    for (int i = 0; i < H; ++i) {
-      bar_init(s_full + 8 * i, 1), bar_init(s_free + 8 * i, 256 / H);
-      bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
-    }
+    bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
     init_visible();
     flag_word = 0;
   }
@@ -688,8 +679,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 13) {
     [&] {
-      const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
-      const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
+      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       // The scores of the next tile come in front of what follows of this one: their place is free once they have been
       // read, that of dp behind the product that reads it.
@@ -714,28 +705,19 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
               CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
               zero_rows<DP>(tiles + (2 * kStay + slot + 1) * Plan::kTileBytes, keys);
             }
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-              if (i > 0) CSW_WAIT_WARP(s_free + 8 * h, (i - 1) & 1);
-              fence_after();
-              product_rows<DP>(s_at + 64 * h, q_at, k_at + h * (kChunk / 2), scores, s_full + 8 * h);
-            }
+            if (i > 0) CSW_WAIT_WARP(s_free, (i - 1) & 1);
+            fence_after();
+            product_rows<DP>(s_at, q_at, k_at, scores, s_full);
           }
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            if (now) {
-              CSW_WAIT_WARP(ds_ready + 8 * h, (i - 1) & 1);
-              if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
-              fence_after();
-              product_tokens<Plan::kColumnsEach>(dq_at, dp_at + 64 * h, 64, ring + before * Plan::kTileBytes + h * (kChunk / 2),
-                                                 sums, j > 0 || h > 0, h + 1 == H ? empty + 8 * before : 0,
-                                                 h + 1 == H && !next ? dq_full : 0);
-            }
-            if (next) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
-              product_rows<DP>(dp_at + 64 * h, q_at + Plan::kTileBytes, v_at + h * (kChunk / 2), slopes, dp_full + 8 * h,
-                               h + 1 == H ? empty + 8 * slot + 8 : 0);
-            }
+          if (now) {
+            CSW_WAIT_WARP(ds_ready, (i - 1) & 1);
+            if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
+            fence_after();
+            product_tokens(dq_at, dp_at, 64, ring + before * Plan::kTileBytes, sums, j > 0, empty + 8 * before, !next ? dq_full : 0);
+          }
+          if (next) {
+            CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+            product_rows<DP>(dp_at, q_at + Plan::kTileBytes, v_at, slopes, dp_full, empty + 8 * slot + 8);
           }
           if (j + 2 == n) commit_to(q_empty + 8 * stay);
           before = slot;
@@ -843,7 +825,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     if (t == 0) stores_read();
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
-    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, own = 8 * (H == 2 ? w : 0);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
@@ -857,7 +839,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const float shift = shifts[u & 1][t], d = deltas[u & 1][t];
         float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
         for (int j = 0; j < n; ++j, ++i) {
-          CSW_WAIT_WARP(s_full + own, i & 1);
+          CSW_WAIT_WARP(s_full, i & 1);
           fence_after();
           float p[64];
           {
@@ -866,7 +848,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             load32(s_at + 64 * w + 32 + lanes, r + 32);
             wait_loads(r), wait_loads(r + 32);
             fence_before();
-            bar_arrive(s_free + own);
+            bar_arrive(s_free);
 #pragma unroll
             for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
           }
@@ -877,7 +859,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             for (int k = 0; k < 64; ++k)
               if (k >= end) p[k] = 0.0f;
           }
-          CSW_WAIT_WARP(dp_full + own, i & 1);
+          CSW_WAIT_WARP(dp_full, i & 1);
           fence_after();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -892,7 +874,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           }
           wait_stores();
           fence_before();
-          bar_arrive(ds_ready + own);
+          bar_arrive(ds_ready);
         }
         store1(left_at + 2 * (u & 1) + w + lanes, left);
         wait_stores();
@@ -919,17 +901,17 @@ struct Keys {
 template <class T, int DP>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
-  constexpr int H = Plan::kHalves, kRing = Plan::kRing, kStay = Plan::kStay;
+  constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[2 + 2 * kStay + 2 * kRing + 4 * H];
+  __shared__ uint64_t bars[2 + 2 * kStay + 2 * kRing + 4];
   __shared__ __align__(16) float rows[kRing][kTile];  // with a tile of q the exponents' shifts, with one of do D
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
   const WorkBars work_bars(work);
   const uint32_t sums_full = smem_at(bars), sums_free = sums_full + 8, kv_full = sums_full + 16,
-                 kv_empty = kv_full + 8 * kStay, full = kv_empty + 8 * kStay, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8 * H,
-                 dp_full = p_ready + 8 * H, ds_ready = dp_full + 8 * H;
+                 kv_empty = kv_full + 8 * kStay, full = kv_empty + 8 * kStay, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8,
+                 dp_full = p_ready + 8, ds_ready = dp_full + 8;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
@@ -937,10 +919,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     bar_init(sums_full, 1), bar_init(sums_free, 128);
     for (int i = 0; i < kStay; ++i) bar_init(kv_full + 8 * i, 1), bar_init(kv_empty + 8 * i, 1);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
-    for (int i = 0; i < H; ++i) {
-      bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 256 / H);
-      bar_init(dp_full + 8 * i, 1), bar_init(ds_ready + 8 * i, 256 / H);
-    }
+    bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
     init_visible();
     flag_word = 0;
   }
@@ -992,8 +971,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
   } else if (warp == 13) {
     [&] {
-      const uint32_t scores = product_desc(kBf16<T>, Plan::kColumnsEach, false, s.negate);
-      const uint32_t slopes = product_desc(kBf16<T>, Plan::kColumnsEach, false, false);
+      const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
+      const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       // Each place in tensor memory is written again behind the product that reads it.
       uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of queries, pieces with any; of the ring
@@ -1010,32 +989,24 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           const bool now = j >= 0, next = j + 1 < n;
           const uint32_t q_at = ring + slot * Plan::kTileBytes, do_at = q_at + Plan::kTileBytes;
           const uint32_t q_now = ring + before * Plan::kTileBytes, do_now = q_now + Plan::kTileBytes;
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            if (now) {
-              CSW_WAIT_WARP(p_ready + 8 * h, (i - 1) & 1);
-              if (j == 0 && h == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
-              fence_after();
-              product_tokens<Plan::kColumnsEach>(dv_at, s_at + 64 * h, 64, do_now + h * (kChunk / 2), sums, j > 0 || h > 0,
-                                                 h + 1 == H ? empty + 8 * before + 8 : 0);
-            }
-            if (next) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * slot, round & 1);
-              product_rows<DP>(s_at + 64 * h, k_at, q_at + h * (kChunk / 2), scores, s_full + 8 * h);
-            }
+          if (now) {
+            CSW_WAIT_WARP(p_ready, (i - 1) & 1);
+            if (j == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
+            fence_after();
+            product_tokens(dv_at, s_at, 64, do_now, sums, j > 0, empty + 8 * before + 8);
           }
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            if (now) {
-              CSW_WAIT_WARP(ds_ready + 8 * h, (i - 1) & 1);
-              fence_after();
-              product_tokens<Plan::kColumnsEach>(dk_at, dp_at + 64 * h, 64, q_now + h * (kChunk / 2), sums, j > 0 || h > 0,
-                                                 h + 1 == H ? empty + 8 * before : 0, h + 1 == H && !next ? sums_full : 0);
-            }
-            if (next) {
-              if (h == 0) CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
-              product_rows<DP>(dp_at + 64 * h, k_at + Plan::kTileBytes, do_at + h * (kChunk / 2), slopes, dp_full + 8 * h);
-            }
+          if (next) {
+            CSW_WAIT_WARP(full + 8 * slot, round & 1);
+            product_rows<DP>(s_at, k_at, q_at, scores, s_full);
+          }
+          if (now) {
+            CSW_WAIT_WARP(ds_ready, (i - 1) & 1);
+            fence_after();
+            product_tokens(dk_at, dp_at, 64, q_now, sums, j > 0, empty + 8 * before, !next ? sums_full : 0);
+          }
+          if (next) {
+            CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+            product_rows<DP>(dp_at, k_at + Plan::kTileBytes, do_at, slopes, dp_full);
           }
           if (j + 2 == n) commit_to(kv_empty + 8 * stay);
           before = slot;
@@ -1092,7 +1063,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     if (t == 0) stores_read();
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
-    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, own = 8 * (H == 2 ? w : 0);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     [&] {
       int i = 0;
       for (int it = 0;; ++it) {
@@ -1106,7 +1077,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           const int slot = 2 * i % kRing;
           const uint32_t parity = 2 * i / kRing & 1;
           CSW_WAIT_WARP(full + 8 * slot, parity);  // the rows' numbers
-          CSW_WAIT_WARP(s_full + own, i & 1);
+          CSW_WAIT_WARP(s_full, i & 1);
           fence_after();
           float p[64];
           {
@@ -1139,10 +1110,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           wait_stores();
           fence_before();
-          bar_arrive(p_ready + own);
+          bar_arrive(p_ready);
 
           CSW_WAIT_WARP(full + 8 * slot + 8, parity);
-          CSW_WAIT_WARP(dp_full + own, i & 1);
+          CSW_WAIT_WARP(dp_full, i & 1);
           fence_after();
           const float4* deltas = reinterpret_cast<const float4*>(rows[slot + 1] + 64 * w);
 #pragma unroll
@@ -1161,7 +1132,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           wait_stores();
           fence_before();
-          bar_arrive(ds_ready + own);
+          bar_arrive(ds_ready);
           if (++q == at.tiles) q = at.from;
         }
       }

@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/cswap_b200.h"
 #include "internal.h"
@@ -34,146 +35,207 @@ __device__ __forceinline__ void param_to(void* p, int type, uint64_t i, float v)
   else if (type == CSW_TYPE_F16) static_cast<__half*>(p)[i] = narrow<__half>(v);
   else static_cast<__nv_bfloat16*>(p)[i] = narrow<__nv_bfloat16>(v);
 }
-template <int N>
-__device__ __forceinline__ void params_at(const void* p, int type, uint64_t i, float (&f)[N]) {
-  if (N == 1) {
-    f[0] = param_at(p, type, i);
-  } else if (type == CSW_TYPE_F32) {
-    const float* q = static_cast<const float*>(p) + i;
-#pragma unroll
-    for (int j = 0; j < N; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(q + j);
-      f[j] = k.x, f[j + 1] = k.y, f[j + 2] = k.z, f[j + 3] = k.w;
-    }
-  } else if (type == CSW_TYPE_F16) {
-    load_pack(static_cast<const __half*>(p) + i, f);
-  } else {
-    load_pack(static_cast<const __nv_bfloat16*>(p) + i, f);
-  }
-}
-
-// Sum over the THREADS threads that share a row (a warp, or the whole CTA); all of them get it.
+// Sums over the THREADS threads that share a row (a warp, or the whole CTA); all of them get them.  A CTA's rows take
+// turns with two places in shared memory (`turn`), so that one barrier a sum is enough: a place is written again two sums
+// later, behind a barrier that all who read it have passed.
 template <int THREADS>
-__device__ __forceinline__ float row_sum(float v, float* shared) {
-#pragma unroll
-  for (int d = 16; d; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (THREADS > 32) {
-    __syncthreads();  // the last use of `shared` is over
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) v += shared[i];
-  }
-  return v;
-}
-template <int THREADS>
-__device__ __forceinline__ float2 row_sum2(float a, float b, float2* shared) {
+__device__ __forceinline__ float2 row_sums(float a, float b, float2 (*shared)[THREADS / 32], int turn) {
 #pragma unroll
   for (int d = 16; d; d /= 2) {
     a += __shfl_xor_sync(0xffffffffu, a, d);
     b += __shfl_xor_sync(0xffffffffu, b, d);
   }
   if (THREADS > 32) {
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = make_float2(a, b);
+    float2* place = shared[turn & 1];
+    if (threadIdx.x % 32 == 0) place[threadIdx.x / 32] = make_float2(a, b);
     __syncthreads();
     a = b = 0.0f;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) a += shared[i].x, b += shared[i].y;
+    for (int i = 0; i < THREADS / 32; ++i) a += place[i].x, b += place[i].y;
   }
   return make_float2(a, b);
 }
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float v, float2 (*shared)[THREADS / 32], int turn) {
+  return row_sums<THREADS>(v, 0.0f, shared, turn).x;
+}
 
-template <class T, int VEC, int ITER, int THREADS>
-struct Shape {
-  static constexpr int kRowThreads = THREADS;
-  static constexpr int kBlock = THREADS < 128 ? 128 : THREADS;
-  static constexpr int kRowsPerBlock = kBlock / THREADS;
+// VEC values as they lie in memory, in words: held so, they take half the registers that single two-byte values would.
+template <class T, int VEC>
+struct Raw {
+  static constexpr int kWords = VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4;
+  uint32_t w[kWords];
+  __device__ float operator[](int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    const uint32_t bits = w[j / 2];
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(j % 2 ? bits & 0xffff0000u : bits << 16);
+    return __half2float(__ushort_as_half((unsigned short)(j % 2 ? bits >> 16 : bits & 0xffff)));
+  }
+  // one value into its place, which holds zeros
+  __device__ void put(int j, T v) {
+    if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v);
+    else w[j / 2] |= (uint32_t) * reinterpret_cast<const unsigned short*>(&v) << (16 * (j % 2));
+  }
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // all of them from p, aligned to 16 bytes where there are as many or more
+  __device__ void read(const T* p) {
+    if constexpr (VEC == 1) {
+      w[0] = 0;
+      put(0, *p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    }
+  }
 };
 
-// A row in the registers of THREADS threads: thread t holds VEC values from column (k THREADS + t) VEC on, for each k.
-template <class T, int VEC, int ITER, int THREADS>
-__global__ void __launch_bounds__(Shape<T, VEC, ITER, THREADS>::kBlock) norm_forward_kernel(const NormForward a) {
-  using S = Shape<T, VEC, ITER, THREADS>;
-  __shared__ float shared[THREADS > 32 ? THREADS / 32 : 1];
+// How the threads lie on the rows.  THREADS threads share a row: thread t holds VEC values from the column
+// (k THREADS + t) VEC - shift on, for each k < ITER.  Where the number of columns is no multiple of VEC, rows begin at
+// any place among the packs of VEC values (16 bytes) that memory is read in; `shift` is that place, and the packs that
+// reach over a row's ends are masked (SHIFTED).  The shift repeats every `period` rows, and a CTA takes only rows of one
+// shift: then the columns of a thread stay the same, with their weights and their sums in registers.
+template <class T, int VEC, int ITER, int THREADS, bool SHIFTED>
+struct Rows {
+  static constexpr int kBlock = THREADS == 32 ? 128 : THREADS, kTogether = kBlock / THREADS;
+  // CTAs an SM should have room for: 64 registers a thread forward, 80 backward
+  static constexpr int kForward = 1024 / kBlock, kBackward = kBlock > 768 ? 1 : 768 / kBlock;
+  uint64_t rows, total;  // total: values
+  uint32_t cols, period;
+  uint64_t row, step;    // the thread's first row, and how far on the next one is
+  int first;             // column of its first value, less than 0 for some that are masked
+  __device__ Rows(uint64_t rows_, uint64_t cols_, uint32_t period_)
+      : rows(rows_), total(rows_ * cols_), cols((uint32_t)cols_), period(period_) {
+    const uint32_t kind = blockIdx.x % period;
+    row = ((uint64_t)blockIdx.x / period * kTogether + threadIdx.x / THREADS) * period + kind;
+    step = (uint64_t)(gridDim.x / period) * kTogether * period;
+    first = (int)(threadIdx.x % THREADS) * VEC - (SHIFTED ? (int)(kind * (uint64_t)cols % VEC) : 0);
+  }
+  __device__ int column(int k) const { return first + k * THREADS * VEC; }
+  __device__ bool any(int c) const { return (!SHIFTED || c > -VEC) && c < (int)cols; }
+  __device__ bool has(int c) const { return !SHIFTED || (c >= 0 && c < (int)cols); }
+  // the values from column c on of the row that begins at `base`; what is masked is whatever lies there
+  __device__ void load(const T* p, uint64_t base, int c, Raw<T, VEC>& v) const {
+    if (!SHIFTED || base + c + VEC <= total) {
+      v.read(p + base + c);
+    } else {
+      v.clear();
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (base + c + j < total) v.put(j, p[base + c + j]);
+    }
+  }
+  __device__ void store(T* p, uint64_t base, int c, const float (&f)[VEC]) const {
+    if (!SHIFTED || (c >= 0 && c + VEC <= (int)cols)) {
+      store_pack(p + base + c, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (has(c + j)) p[base + c + j] = narrow<T>(f[j]);
+    }
+  }
+  // the thread's weights or biases, for all its rows
+  template <class P>
+  __device__ void params(const void* p, float missing, Raw<P, VEC> (&f)[ITER]) const {
+    const P* q = static_cast<const P*>(p);
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int c = column(k);
+      f[k].clear();
+      if (!any(c)) continue;
+      if (q && !SHIFTED) {
+        f[k].read(q + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (!q || has(c + j)) f[k].put(j, q ? q[c + j] : narrow<P>(missing));
+      }
+    }
+  }
+};
+
+template <class T, class P, int VEC, int ITER, int THREADS, bool SHIFTED>
+__global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
+                                  Rows<T, VEC, ITER, THREADS, SHIFTED>::kForward)
+    norm_forward_kernel(const NormForward a, uint32_t period) {
+  __shared__ float2 shared[2][THREADS / 32];
   const T* x = static_cast<const T*>(a.x);
   const T* residual = static_cast<const T*>(a.residual);
   pdl_wait(x);
   pdl_behind(residual);
-  const uint32_t t = threadIdx.x % THREADS;
-  const uint32_t cols = (uint32_t)a.cols;
-  const uint64_t row = (uint64_t)blockIdx.x * S::kRowsPerBlock + threadIdx.x / THREADS;
-  if (row >= a.rows) return;  // a whole warp, or no thread of the CTA
-  const uint64_t base = row * a.cols;
-  float v[ITER][VEC];
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const uint32_t c = (k * THREADS + t) * VEC;
-    if (c < cols) {
-      load_pack(x + base + c, v[k]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
-    }
-  }
-  if (residual) {
-    T* sum = static_cast<T*>(a.sum);
+  const Rows<T, VEC, ITER, THREADS, SHIFTED> at(a.rows, a.cols, period);
+  T* sum = static_cast<T*>(a.sum);
+  T* y = static_cast<T*>(a.y);
+  const float inv = 1.0f / (float)at.cols;
+  Raw<P, VEC> w[ITER], b[ITER];
+  at.params(a.weight, 1.0f, w);
+  at.params(a.bias, 0.0f, b);
+  int turn = 0;
+#pragma unroll 1
+  for (uint64_t row = at.row; row < at.rows; row += at.step) {
+    const uint64_t base = row * at.cols;
+    Raw<T, VEC> px[ITER], pr[ITER];
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
-      const uint32_t c = (k * THREADS + t) * VEC;
-      if (c < cols) {
-        float r[VEC];
-        load_pack(residual + base + c, r);
+      const int c = at.column(k);
+      if (at.any(c)) {
+        at.load(x, base, c, px[k]);
+        if (residual) at.load(residual, base, c, pr[k]);
+      }
+    }
+    float v[ITER][VEC], s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int c = at.column(k);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
+      if (at.any(c)) {
         // what is normed, and what backward reads, is the sum as it is held
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k][j] = widen(narrow<T>(v[k][j] + r[j]));
-        store_pack(sum + base + c, v[k]);
+        for (int j = 0; j < VEC; ++j)
+          if (at.has(c + j)) v[k][j] = residual ? widen(narrow<T>(px[k][j] + pr[k][j])) : px[k][j];
+        if (residual) at.store(sum, base, c, v[k]);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += v[k][j];
+    }
+    const float mean = row_sum<THREADS>(s, shared, turn++) * inv;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int c = at.column(k);
+      if (at.any(c)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (at.has(c + j)) v[k][j] -= mean;
+          s += v[k][j] * v[k][j];
+        }
       }
     }
-  }
-  float s = 0.0f;
+    const float rstd = 1.0f / sqrtf(row_sum<THREADS>(s, shared, turn++) * inv + a.eps);
+    if (threadIdx.x % THREADS == 0) a.mean[row] = mean, a.rstd[row] = rstd;
 #pragma unroll
-  for (int k = 0; k < ITER; ++k)
+    for (int k = 0; k < ITER; ++k) {
+      const int c = at.column(k);
+      if (at.any(c)) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s += v[k][j];
-  const float mean = row_sum<THREADS>(s, shared) / (float)cols;
-  s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const uint32_t c = (k * THREADS + t) * VEC;
-    if (c < cols) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[k][j] -= mean;
-        s += v[k][j] * v[k][j];
+        for (int j = 0; j < VEC; ++j) v[k][j] = v[k][j] * rstd * w[k][j] + b[k][j];
+        at.store(y, base, c, v[k]);
       }
-    }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<THREADS>(s, shared) / (float)cols + a.eps);
-  if (t == 0) a.mean[row] = mean, a.rstd[row] = rstd;
-  T* y = static_cast<T*>(a.y);
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const uint32_t c = (k * THREADS + t) * VEC;
-    if (c < cols) {
-      float w[VEC], b[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) w[j] = 1.0f, b[j] = 0.0f;
-      if (a.weight) params_at(a.weight, a.param_type, c, w);
-      if (a.bias) params_at(a.bias, a.param_type, c, b);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] = v[k][j] * rstd * w[j] + b[j];
-      store_pack(y + base + c, v[k]);
     }
   }
 }
 
-// Rows beyond 16384 values: read three times, one value a thread and step.
+// Long rows: read three times, one value a thread and step.
 constexpr int kLongThreads = 512;
 template <class T>
 __global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const NormForward a) {
-  __shared__ float shared[kLongThreads / 32];
+  __shared__ float2 shared[2][kLongThreads / 32];
   pdl_wait();
   const uint64_t base = (uint64_t)blockIdx.x * a.cols;
   const T* x = static_cast<const T*>(a.x) + base;
@@ -190,13 +252,13 @@ __global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const N
     s += v;
   }
   const T* src = residual ? sum : x;  // a thread reads back what it wrote itself
-  const float mean = row_sum<kLongThreads>(s, shared) / (float)a.cols;
+  const float mean = row_sum<kLongThreads>(s, shared, 0) / (float)a.cols;
   s = 0.0f;
   for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
     const float v = widen(src[c]) - mean;
     s += v * v;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<kLongThreads>(s, shared) / (float)a.cols + a.eps);
+  const float rstd = 1.0f / sqrtf(row_sum<kLongThreads>(s, shared, 1) / (float)a.cols + a.eps);
   if (threadIdx.x == 0) a.mean[blockIdx.x] = mean, a.rstd[blockIdx.x] = rstd;
   T* y = static_cast<T*>(a.y) + base;
   for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
@@ -207,88 +269,103 @@ __global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const N
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// One CTA takes rows r, r + gridDim kRowsPerBlock, ...; workspace row blockIdx.x receives its sums: dw, then db.
-template <class T, int VEC, int ITER, int THREADS>
-__global__ void __launch_bounds__(Shape<T, VEC, ITER, THREADS>::kBlock) norm_backward_kernel(const NormBackward a) {
-  using S = Shape<T, VEC, ITER, THREADS>;
-  __shared__ float2 shared[THREADS > 32 ? THREADS / 32 : 1];
+// Workspace row blockIdx.x receives the CTA's sums: dw, then db.  A row's values are held as they came, and widened anew
+// for each of the two passes over them; the next row's are on their way meanwhile.
+template <class T, class P, int VEC, int ITER, int THREADS, bool SHIFTED>
+__global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
+                                  Rows<T, VEC, ITER, THREADS, SHIFTED>::kBackward)
+    norm_backward_kernel(const NormBackward a, uint32_t period) {
+  using R = Rows<T, VEC, ITER, THREADS, SHIFTED>;
+  __shared__ float2 shared[2][THREADS / 32];
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   pdl_wait(x);
   pdl_behind(dy);
-  const uint32_t t = threadIdx.x % THREADS;
-  const uint32_t cols = (uint32_t)a.cols;
-  const float inv = 1.0f / (float)cols;
+  const R at(a.rows, a.cols, period);
+  T* dx = static_cast<T*>(a.dx);
+  const float inv = 1.0f / (float)at.cols;
   float dw[ITER][VEC], db[ITER][VEC];
 #pragma unroll
   for (int k = 0; k < ITER; ++k)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) dw[k][j] = db[k][j] = 0.0f;
-  for (uint64_t row = (uint64_t)blockIdx.x * S::kRowsPerBlock + threadIdx.x / THREADS; row < a.rows;
-       row += (uint64_t)gridDim.x * S::kRowsPerBlock) {
-    const uint64_t base = row * a.cols;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float h[ITER][VEC], g[ITER][VEC];
+  struct Held {
+    Raw<T, VEC> x[ITER], dy[ITER];
+    float mean, rstd;
+  };
+  auto load = [&](uint64_t row, Held& h) {
+    const uint64_t base = row * at.cols;
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int c = at.column(k);
+      if (at.any(c)) at.load(x, base, c, h.x[k]), at.load(dy, base, c, h.dy[k]);
+    }
+    h.mean = a.mean[row], h.rstd = a.rstd[row];
+  };
+  Held now, next;
+  if (at.row < at.rows) load(at.row, next);
+  Raw<P, VEC> w[ITER];
+  at.params(a.weight, 1.0f, w);
+  int turn = 0;
+#pragma unroll 1
+  for (uint64_t row = at.row; row < at.rows; row += at.step) {
+    now = next;
+    if (row + at.step < at.rows) load(row + at.step, next);
+    // normed value and dy of a column; a masked value is another row's, 0 in its place adds nothing
+    auto values = [&](int k, int j, float& h, float& g) {
+      const bool has = at.has(at.column(k) + j);
+      h = has ? (now.x[k][j] - now.mean) * now.rstd : 0.0f;
+      g = has ? now.dy[k][j] : 0.0f;
+    };
     float sg = 0.0f, sgh = 0.0f;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
-      const uint32_t c = (k * THREADS + t) * VEC;
-      if (c < cols) {
-        load_pack(x + base + c, h[k]);
-        load_pack(dy + base + c, g[k]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < ITER; ++k) {
-      const uint32_t c = (k * THREADS + t) * VEC;
-      if (c < cols) {
-        float w[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
-        if (a.weight) params_at(a.weight, a.param_type, c, w);
+      if (at.any(at.column(k))) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          h[k][j] = (h[k][j] - mean) * rstd;
-          dw[k][j] += g[k][j] * h[k][j];
-          db[k][j] += g[k][j];
-          g[k][j] *= w[j];
-          sg += g[k][j];
-          sgh += g[k][j] * h[k][j];
+          float h, g;
+          values(k, j, h, g);
+          dw[k][j] += g * h;
+          db[k][j] += g;
+          sg += g * w[k][j];
+          sgh += g * w[k][j] * h;
         }
       }
     }
-    const float2 s = row_sum2<THREADS>(sg, sgh, shared);
+    const float2 s = row_sums<THREADS>(sg, sgh, shared, turn++);
     const float m0 = s.x * inv, m1 = s.y * inv;
-    T* dx = static_cast<T*>(a.dx) + base;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
-      const uint32_t c = (k * THREADS + t) * VEC;
-      if (c < cols) {
+      if (at.any(at.column(k))) {
+        float f[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) g[k][j] = (g[k][j] - m0 - h[k][j] * m1) * rstd;
-        store_pack(dx + c, g[k]);
+        for (int j = 0; j < VEC; ++j) {
+          float h, g;
+          values(k, j, h, g);
+          f[j] = (g * w[k][j] - m0 - h * m1) * now.rstd;
+        }
+        at.store(dx, row * at.cols, at.column(k), f);
       }
     }
   }
   if (!a.dweight && !a.dbias) return;
   float* part = a.workspace + (uint64_t)blockIdx.x * 2 * a.cols;
-  if (S::kRowsPerBlock > 1) {
+  if (R::kTogether > 1) {
     // the warps' sums, added in the order of the warps
-    __shared__ float sums[S::kRowsPerBlock > 1 ? 2 * 32 * ITER * VEC : 1];
-    for (int w = 0; w < S::kRowsPerBlock; ++w) {
+    constexpr int kMany = R::kTogether > 1 ? 32 * ITER * VEC : 1;
+    __shared__ float sums[2][kMany];
+    for (int w = 0; w < R::kTogether; ++w) {
       if (threadIdx.x / THREADS == w) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const int i = (k * VEC + j) * 32 + t;
-            const float pw = dw[k][j] + (w ? sums[i] : 0.0f);
-            const float pb = db[k][j] + (w ? sums[i + 32 * ITER * VEC] : 0.0f);
-            if (w < S::kRowsPerBlock - 1) {
-              sums[i] = pw, sums[i + 32 * ITER * VEC] = pb;
-            } else {
-              const uint32_t c = (k * THREADS + t) * VEC + j;
-              if (c < cols) part[c] = pw, part[a.cols + c] = pb;
+            const int i = ((k * VEC + j) * 32 + threadIdx.x % 32) % kMany, c = at.column(k) + j;
+            const float pw = dw[k][j] + (w ? sums[0][i] : 0.0f), pb = db[k][j] + (w ? sums[1][i] : 0.0f);
+            if (w < R::kTogether - 1) {
+              sums[0][i] = pw, sums[1][i] = pb;
+            } else if (c >= 0 && c < (int)at.cols) {
+              part[c] = pw, part[a.cols + c] = pb;
             }
           }
       }
@@ -299,8 +376,8 @@ __global__ void __launch_bounds__(Shape<T, VEC, ITER, THREADS>::kBlock) norm_bac
     for (int k = 0; k < ITER; ++k)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const uint32_t c = (k * THREADS + t) * VEC + j;
-        if (c < cols) part[c] = dw[k][j], part[a.cols + c] = db[k][j];
+        const int c = at.column(k) + j;
+        if (c >= 0 && c < (int)at.cols) part[c] = dw[k][j], part[a.cols + c] = db[k][j];
       }
   }
 }
@@ -308,7 +385,7 @@ __global__ void __launch_bounds__(Shape<T, VEC, ITER, THREADS>::kBlock) norm_bac
 // Long rows: dx of one row a CTA, read twice ...
 template <class T>
 __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const NormBackward a) {
-  __shared__ float2 shared[kLongThreads / 32];
+  __shared__ float2 shared[2][kLongThreads / 32];
   pdl_wait();
   const uint64_t base = (uint64_t)blockIdx.x * a.cols;
   const T* x = static_cast<const T*>(a.x) + base;
@@ -320,7 +397,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const 
     sg += g;
     sgh += g * ((widen(x[c]) - mean) * rstd);
   }
-  const float2 s = row_sum2<kLongThreads>(sg, sgh, shared);
+  const float2 s = row_sums<kLongThreads>(sg, sgh, shared, 0);
   T* dx = static_cast<T*>(a.dx) + base;
   for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
     const float g = widen(dy[c]) * (a.weight ? param_at(a.weight, a.param_type, c) : 1.0f);
@@ -344,66 +421,103 @@ __global__ void __launch_bounds__(128) norm_backward_columns_kernel(const NormBa
   out[c] = dw, out[a.cols + c] = db;
 }
 
-// The partial sums of all CTAs, 32 columns a block, each thread every 8th row; then the 8 rows of threads in order.
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restrict__ parts, uint64_t n, uint64_t cols,
-                                                          void* dweight, void* dbias, int type) {
-  __shared__ float shared[2][8][32];
+// The partial sums of all CTAs, 8 columns (a sector of memory) a block, each thread every 128th row; then the rows of
+// threads, a warp for each result.
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restrict__ parts, uint64_t n, uint64_t cols,
+                                                           void* dweight, void* dbias, int type) {
+  constexpr int kCols = 8, kRows = 1024 / kCols;
+  __shared__ float shared[2][kCols][kRows + 1];
   pdl_wait(parts);
-  const uint32_t lane = threadIdx.x % 32, r = threadIdx.x / 32;
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
+  const uint32_t lane = threadIdx.x % kCols, r = threadIdx.x / kCols;
+  const uint64_t c = (uint64_t)blockIdx.x * kCols + lane;
   float w = 0.0f, b = 0.0f;
   if (c < cols) {
-    for (uint64_t i = r; i < n; i += 8) {
+#pragma unroll 4
+    for (uint64_t i = r; i < n; i += kRows) {
       w += parts[i * 2 * cols + c];
       b += parts[i * 2 * cols + cols + c];
     }
   }
-  shared[0][r][lane] = w, shared[1][r][lane] = b;
+  shared[0][lane][r] = w, shared[1][lane][r] = b;
   __syncthreads();
-  if (r < 2 && c < cols) {
-    float s = 0.0f;
+  const uint32_t warp = threadIdx.x / 32, which = warp / kCols;
+  const uint64_t mine = (uint64_t)blockIdx.x * kCols + warp % kCols;
+  if (which < 2 && mine < cols) {
+    float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += shared[r][i][lane];
-    void* out = r == 0 ? dweight : dbias;
-    if (out) param_to(out, type, c, s);
+    for (int i = 0; i < kRows / 32; ++i) v += shared[which][warp % kCols][i * 32 + threadIdx.x % 32];
+#pragma unroll
+    for (int d = 16; d; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+    void* out = which == 0 ? dweight : dbias;
+    if (out && threadIdx.x % 32 == 0) param_to(out, type, mine, v);
   }
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------------
-constexpr uint64_t kLongest = 16384;
+constexpr uint64_t kLongest = 8192;
+constexpr int kHeld = 8;  // values of a row that a thread holds
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-template <class T>
-bool whole_packs(uint64_t cols) {
-  return cols * sizeof(T) % 16 == 0;
+
+// How a row's packs lie: of 16 bytes where all rows begin on them, shifted where only the first one does.  Else, and in
+// rows of a pack or two that have nothing but ends, single values: up to 256 of them by a warp, more as a long row.
+enum class Packs { kWhole, kShifted, kSingle, kLong };
+Packs packs_of(int type, uint64_t cols, bool aligned) {
+  const uint64_t size = type == CSW_TYPE_F32 ? 4 : 2, spare = 16 / size - 1;
+  if (cols > kLongest) return Packs::kLong;
+  if (aligned && cols * size % 16 == 0) return Packs::kWhole;
+  if (aligned && cols * size >= 64 && cols + spare <= kLongest) return Packs::kShifted;
+  return cols <= 32 * kHeld ? Packs::kSingle : Packs::kLong;
+}
+uint32_t period_of(int type, uint64_t cols, Packs packs) {
+  if (packs != Packs::kShifted) return 1;
+  uint32_t p = type == CSW_TYPE_F32 ? 4 : 8;
+  for (uint64_t c = cols; p > 1 && c % 2 == 0; c /= 2) p /= 2;
+  return p;
+}
+// threads of a row, the fewest that hold it with the masked values that a shifted one has more
+int threads_of(int type, uint64_t cols, Packs packs) {
+  const uint64_t held = cols + (packs == Packs::kShifted ? 16 / (type == CSW_TYPE_F32 ? 4 : 2) - 1 : 0);
+  for (int t : {32, 64, 96, 128, 256, 512})
+    if (held <= (uint64_t)t * kHeld) return t;
+  return 1024;
 }
 
-// f<values a thread holds, threads of a row> for rows of up to kLongest values
-template <class F>
-cudaError_t with_shape(uint64_t cols, F&& f) {
-  using std::integral_constant;
-#define CSW_SHAPE(n, threads) \
-  if (cols <= (uint64_t)n * threads) return f(integral_constant<int, n>(), integral_constant<int, threads>())
-  CSW_SHAPE(8, 32);
-  CSW_SHAPE(16, 32);
-  CSW_SHAPE(24, 32);
-  CSW_SHAPE(32, 32);
-  CSW_SHAPE(16, 128);
-  CSW_SHAPE(32, 128);
-  CSW_SHAPE(16, 512);
-  CSW_SHAPE(32, 512);
-#undef CSW_SHAPE
-  return cudaErrorInvalidValue;
-}
-unsigned rows_per_block(uint64_t cols) { return cols <= 1024 ? 4 : 1; }
-
-// CTAs of a backward pass: they stay for all their rows, so that the sums leave them once.
-unsigned backward_blocks(uint64_t rows, uint64_t cols) {
-  const uint64_t want = (rows + rows_per_block(cols) - 1) / rows_per_block(cols);
-  const uint64_t resident = (uint64_t)sm_count() * (cols <= 1024 ? 3 : cols <= 4096 ? 3 : 1);
-  return (unsigned)std::min(want, resident);
+// CTAs that stay for all their rows, so that weights are read and sums written once each: as many as run at once.
+unsigned blocks_of(uint64_t rows, int threads, uint32_t period, uint64_t on_sm) {
+  const uint64_t together = threads == 32 ? 4 : 1, block = threads == 32 ? 128 : threads;
+  const uint64_t want = (rows + together * period - 1) / (together * period);  // CTAs of each shift
+  const uint64_t most = std::max<uint64_t>((uint64_t)sm_count() * std::max<uint64_t>(std::min<uint64_t>(on_sm / block, 8), 1) / period, 1);
+  return (unsigned)(std::min(want, most) * period);
 }
 constexpr uint64_t kLongParts = 64;
+
+// f(pack's values, packs a thread, threads, shifted) for rows that are not long
+template <class T, class F>
+cudaError_t with_kernel(int threads, Packs packs, F&& f) {
+  using std::integral_constant;
+  constexpr int V = 16 / sizeof(T);
+  using Yes = integral_constant<bool, true>;
+  using No = integral_constant<bool, false>;
+  using Pack16 = integral_constant<int, V>;
+  using Iter16 = integral_constant<int, kHeld / V>;
+  if (packs == Packs::kSingle)
+    return f(integral_constant<int, 1>(), integral_constant<int, kHeld>(), integral_constant<int, 32>(), No());
+  switch (threads) {
+#define CSW_THREADS(n) \
+  case n: return packs == Packs::kWhole ? f(Pack16(), Iter16(), integral_constant<int, n>(), No()) \
+                                        : f(Pack16(), Iter16(), integral_constant<int, n>(), Yes());
+    CSW_THREADS(32)
+    CSW_THREADS(64)
+    CSW_THREADS(96)
+    CSW_THREADS(128)
+    CSW_THREADS(256)
+    CSW_THREADS(512)
+    CSW_THREADS(1024)
+#undef CSW_THREADS
+    default: return cudaErrorInvalidValue;
+  }
+}
 
 }  // namespace
 
@@ -412,54 +526,71 @@ cudaError_t norm_forward_launch(const NormForward& a, cudaStream_t stream) {
   cudaError_t e = cudaErrorInvalidValue;
   with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    if (a.cols > kLongest) {
+    const Packs packs = packs_of(a.type, a.cols, aligned16(a.x) && aligned16(a.y) && aligned16(a.residual) &&
+                                                     aligned16(a.sum) && aligned16(a.weight) && aligned16(a.bias));
+    if (packs == Packs::kLong) {
       e = pdl_launch(norm_forward_long_kernel<T>, (unsigned)a.rows, kLongThreads, 0, stream, a);
       return;
     }
-    const bool vec = whole_packs<T>(a.cols) && aligned16(a.x) && aligned16(a.y) && aligned16(a.residual) &&
-                     aligned16(a.sum) && aligned16(a.weight) && aligned16(a.bias);
-    const unsigned grid = (unsigned)((a.rows + rows_per_block(a.cols) - 1) / rows_per_block(a.cols));
-    e = with_shape(a.cols, [&](auto held, auto threads) {
-      constexpr int V = 16 / sizeof(T), H = held.value, R = threads.value;
-      constexpr int B = Shape<T, V, 1, R>::kBlock;
-      return vec ? pdl_launch(norm_forward_kernel<T, V, H / V, R>, grid, B, 0, stream, a)
-                 : pdl_launch(norm_forward_kernel<T, 1, H, R>, grid, B, 0, stream, a);
+    const uint32_t period = period_of(a.type, a.cols, packs);
+    const int wide = threads_of(a.type, a.cols, packs);
+    const unsigned grid = blocks_of(a.rows, wide, period, 1024);
+    e = with_kernel<T>(wide, packs, [&](auto vec, auto iter, auto threads, auto shifted) {
+      using R = Rows<T, vec.value, iter.value, threads.value, shifted.value>;
+      return a.param_type == a.type
+                 ? pdl_launch(norm_forward_kernel<T, T, vec.value, iter.value, threads.value, shifted.value>, grid,
+                              R::kBlock, 0, stream, a, period)
+                 : pdl_launch(norm_forward_kernel<T, float, vec.value, iter.value, threads.value, shifted.value>, grid,
+                              R::kBlock, 0, stream, a, period);
     });
   });
   return e;
 }
 
+namespace {
+uint64_t parts_of(int type, uint64_t rows, uint64_t cols, bool aligned) {
+  const Packs packs = packs_of(type, cols, aligned);
+  if (packs == Packs::kLong) return std::min(rows, kLongParts);
+  return blocks_of(rows, threads_of(type, cols, packs), period_of(type, cols, packs), 768);
+}
+}  // namespace
+
 uint64_t norm_backward_partials(uint64_t rows, uint64_t cols) {
-  if (cols > kLongest) return std::min(rows, kLongParts);
-  return backward_blocks(rows, cols);
+  uint64_t most = 0;  // whichever type and alignment the call has
+  for (int type : {CSW_TYPE_F32, CSW_TYPE_BF16})
+    for (bool aligned : {false, true}) most = std::max(most, parts_of(type, rows, cols, aligned));
+  return most;
 }
 
 cudaError_t norm_backward_launch(const NormBackward& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  const uint64_t parts = norm_backward_partials(a.rows, a.cols);
+  const bool aligned = aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) && aligned16(a.weight);
+  const uint64_t parts = parts_of(a.type, a.rows, a.cols, aligned);
   const bool sums = a.dweight || a.dbias;
   if (a.rows != 0) {
     e = cudaErrorInvalidValue;
     with_type(a.type, [&](auto t) {
       using T = decltype(t);
-      if (a.cols > kLongest) {
+      const Packs packs = packs_of(a.type, a.cols, aligned);
+      if (packs == Packs::kLong) {
         e = pdl_launch(norm_backward_long_kernel<T>, (unsigned)a.rows, kLongThreads, 0, stream, a);
         if (e == cudaSuccess && sums)
           e = pdl_launch(norm_backward_columns_kernel<T>, (unsigned)((a.cols + 127) / 128 * parts), 128, 0, stream, a);
         return;
       }
-      const bool vec = whole_packs<T>(a.cols) && aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) &&
-                       aligned16(a.weight);
-      e = with_shape(a.cols, [&](auto held, auto threads) {
-        constexpr int V = 16 / sizeof(T), H = held.value, R = threads.value;
-        constexpr int B = Shape<T, V, 1, R>::kBlock;
-        return vec ? pdl_launch(norm_backward_kernel<T, V, H / V, R>, (unsigned)parts, B, 0, stream, a)
-                   : pdl_launch(norm_backward_kernel<T, 1, H, R>, (unsigned)parts, B, 0, stream, a);
+      const uint32_t period = period_of(a.type, a.cols, packs);
+      e = with_kernel<T>(threads_of(a.type, a.cols, packs), packs, [&](auto vec, auto iter, auto threads, auto shifted) {
+        using R = Rows<T, vec.value, iter.value, threads.value, shifted.value>;
+        return a.param_type == a.type
+                   ? pdl_launch(norm_backward_kernel<T, T, vec.value, iter.value, threads.value, shifted.value>,
+                                (unsigned)parts, R::kBlock, 0, stream, a, period)
+                   : pdl_launch(norm_backward_kernel<T, float, vec.value, iter.value, threads.value, shifted.value>,
+                                (unsigned)parts, R::kBlock, 0, stream, a, period);
       });
     });
   }
   if (e == cudaSuccess && sums)
-    e = pdl_launch(norm_reduce_kernel, (unsigned)((a.cols + 31) / 32), 256, 0, stream, a.workspace, parts, a.cols,
+    e = pdl_launch(norm_reduce_kernel, (unsigned)((a.cols + 7) / 8), 1024, 0, stream, a.workspace, parts, a.cols,
                    a.dweight, a.dbias, a.param_type);
   return e;
 }

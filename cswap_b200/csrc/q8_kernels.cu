@@ -88,9 +88,29 @@ __device__ __forceinline__ char4 load_codes(const char4* codes, uint64_t i, uint
   return make_char4(i < n ? p[i] : 0, i + 1 < n ? p[i + 1] : 0, i + 2 < n ? p[i + 2] : 0, 0);
 }
 
-// Phi, the distribution function of the normal distribution, and its density
-__device__ __forceinline__ float normal_sum(float x) { return normcdff(x); }
-__device__ __forceinline__ float normal_density(float x) { return 0.3989422804014327f * expf(-0.5f * x * x); }
+// Phi, the distribution function of the normal distribution, and exp(-x^2 / 2), which its density is 1 / sqrt(2 pi) of.
+// Phi(-z) = exp(-z^2 / 2) (c1 t + ... + c7 t^7) with t = 1 / (1 + 0.32 z), z >= 0: the form of Abramowitz and Stegun's
+// 7.1.26, with two terms more and coefficients fitted for the least absolute error (6 10^-9; 2 10^-7 at most as float32
+// rounds it).  The one exponential serves Phi and the density: some 20 instructions a value, where the library's
+// function made a pass over 50331648 float32 values 133 us there and 165 back, bound by instructions.
+struct Normal {
+  float sum, bell;
+};
+__device__ __forceinline__ Normal normal(float x) {
+  const float z = fabsf(x);
+  float t, bell;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(z, 0.32f, 1.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(bell) : "f"(z * z * -0.72134752044f));
+  float p = fmaf(0.04195379838347435f, t, -0.22253216803073883f);
+  p = fmaf(p, t, 0.372079998254776f);
+  p = fmaf(p, t, -0.12819476425647736f);
+  p = fmaf(p, t, 0.19610773026943207f);
+  p = fmaf(p, t, 0.11168046295642853f);
+  p = fmaf(p, t, 0.12890493869781494f);
+  const float below = p * t * bell;
+  return {x > 0.0f ? 1.0f - below : below, bell};
+}
+constexpr float kDensity = 0.3989422804014327f;  // 1 / sqrt(2 pi)
 
 // U groups a warp.  kGelu: y = x Phi(x) is written as well.
 template <class T, int U, bool kGelu>
@@ -113,7 +133,7 @@ __global__ void __launch_bounds__(32 * kWarps) q8_encode_kernel(const T* __restr
     if (kGelu) {
       float o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = v[u][j] * normal_sum(v[u][j]);
+      for (int j = 0; j < 4; ++j) o[j] = v[u][j] * normal(v[u][j]).sum;
       store4(y, i, n, vec, o);
     }
   }
@@ -150,9 +170,9 @@ __global__ void __launch_bounds__(32 * kWarps)
       float o[4], a[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = normal_sum(x[j]);
-        a[j] = x[j] * p;
-        o[j] = d[u][j] * (p + x[j] * normal_density(x[j]));
+        const Normal f = normal(x[j]);
+        a[j] = x[j] * f.sum;
+        o[j] = d[u][j] * fmaf(x[j] * kDensity, f.bell, f.sum);
       }
       store4(out, i, n, vec, o);
       if (again) store4(again, i, n, vec, a);
