@@ -35,29 +35,37 @@ __device__ __forceinline__ void param_to(void* p, int type, uint64_t i, float v)
   else if (type == CSW_TYPE_F16) static_cast<__half*>(p)[i] = narrow<__half>(v);
   else static_cast<__nv_bfloat16*>(p)[i] = narrow<__nv_bfloat16>(v);
 }
-// Sums over the THREADS threads that share a row (a warp, or the whole CTA); all of them get them.  A CTA's rows take
-// turns with two places in shared memory (`turn`), so that one barrier a sum is enough: a place is written again two sums
-// later, behind a barrier that all who read it have passed.
-template <int THREADS>
-__device__ __forceinline__ float2 row_sums(float a, float b, float2 (*shared)[THREADS / 32], int turn) {
+// Sums over the THREADS threads that share a row (a warp, or the whole CTA) of N pairs of values; all of them get them.  A
+// CTA's sums take turns with two places in shared memory (`turn`), so that one barrier a sum is enough: a place is written
+// again two sums later, behind a barrier that all who read it have passed.
+template <int THREADS, int N>
+__device__ __forceinline__ void row_sums(float2 (&v)[N], float2 (*shared)[THREADS / 32], int turn) {
 #pragma unroll
-  for (int d = 16; d; d /= 2) {
-    a += __shfl_xor_sync(0xffffffffu, a, d);
-    b += __shfl_xor_sync(0xffffffffu, b, d);
-  }
+  for (int d = 16; d; d /= 2)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n].x += __shfl_xor_sync(0xffffffffu, v[n].x, d);
+      v[n].y += __shfl_xor_sync(0xffffffffu, v[n].y, d);
+    }
   if (THREADS > 32) {
-    float2* place = shared[turn & 1];
-    if (threadIdx.x % 32 == 0) place[threadIdx.x / 32] = make_float2(a, b);
-    __syncthreads();
-    a = b = 0.0f;
+    float2(*place)[THREADS / 32] = shared + (turn & 1) * N;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) a += place[i].x, b += place[i].y;
+    for (int n = 0; n < N; ++n)
+      if (threadIdx.x % 32 == 0) place[n][threadIdx.x / 32] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) v[n].x += place[n][i].x, v[n].y += place[n][i].y;
+    }
   }
-  return make_float2(a, b);
 }
 template <int THREADS>
 __device__ __forceinline__ float row_sum(float v, float2 (*shared)[THREADS / 32], int turn) {
-  return row_sums<THREADS>(v, 0.0f, shared, turn).x;
+  float2 s[1] = {make_float2(v, 0.0f)};
+  row_sums<THREADS>(s, shared, turn);
+  return s[0].x;
 }
 
 // VEC values as they lie in memory, in words: held so, they take half the registers that single two-byte values would.
@@ -103,8 +111,11 @@ struct Raw {
 template <class T, int VEC, int ITER, int THREADS, bool SHIFTED>
 struct Rows {
   static constexpr int kBlock = THREADS == 32 ? 128 : THREADS, kTogether = kBlock / THREADS;
-  // CTAs an SM should have room for: 64 registers a thread forward, 80 backward
+  // CTAs an SM should have room for: 64 registers a thread forward, 80 or more backward
   static constexpr int kForward = 1024 / kBlock, kBackward = kBlock > 768 ? 1 : 768 / kBlock;
+  // Rows at once, backward, where a CTA has an SM to itself: a row waits for its sums' way through shuffles and shared
+  // memory, which then serves two (16384 x 4096 bfloat16 93 us, 106 one at a time).
+  static constexpr int kAtOnce = sizeof(T) == 2 && THREADS == 512 ? 2 : 1;
   uint64_t rows, total;  // total: values
   uint32_t cols, period;
   uint64_t row, step;    // the thread's first row, and how far on the next one is
@@ -276,7 +287,8 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
                                   Rows<T, VEC, ITER, THREADS, SHIFTED>::kBackward)
     norm_backward_kernel(const NormBackward a, uint32_t period) {
   using R = Rows<T, VEC, ITER, THREADS, SHIFTED>;
-  __shared__ float2 shared[2][THREADS / 32];
+  constexpr int N = R::kAtOnce;
+  __shared__ float2 shared[2 * N][THREADS / 32];
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   pdl_wait(x);
@@ -284,11 +296,13 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
   const R at(a.rows, a.cols, period);
   T* dx = static_cast<T*>(a.dx);
   const float inv = 1.0f / (float)at.cols;
-  float dw[ITER][VEC], db[ITER][VEC];
+  // values go two at a time, in instructions for both
+  constexpr int kPairs = (VEC + 1) / 2;
+  Pair dw[ITER][kPairs], db[ITER][kPairs];
 #pragma unroll
   for (int k = 0; k < ITER; ++k)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) dw[k][j] = db[k][j] = 0.0f;
+    for (int j = 0; j < kPairs; ++j) dw[k][j] = db[k][j] = both(0.0f);
   struct Held {
     Raw<T, VEC> x[ITER], dy[ITER];
     float mean, rstd;
@@ -302,58 +316,83 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
     }
     h.mean = a.mean[row], h.rstd = a.rstd[row];
   };
-  Held now, next;
-  if (at.row < at.rows) load(at.row, next);
+  Held now[N], next[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (at.row + n * at.step < at.rows) load(at.row + n * at.step, next[n]);
   Raw<P, VEC> w[ITER];
   at.params(a.weight, 1.0f, w);
   int turn = 0;
 #pragma unroll 1
-  for (uint64_t row = at.row; row < at.rows; row += at.step) {
-    now = next;
-    if (row + at.step < at.rows) load(row + at.step, next);
-    // normed value and dy of a column; a masked value is another row's, 0 in its place adds nothing
-    auto values = [&](int k, int j, float& h, float& g) {
-      const bool has = at.has(at.column(k) + j);
-      h = has ? (now.x[k][j] - now.mean) * now.rstd : 0.0f;
-      g = has ? now.dy[k][j] : 0.0f;
+  for (uint64_t row = at.row; row < at.rows; row += N * at.step) {
+    float2 sums[N];
+    // normed values and dy of a pair of columns; a masked value is another row's, 0 in its place adds nothing
+    auto pair = [&](const auto& raw, int j) { return Pair{raw[j], VEC > 1 ? raw[j + 1] : 0.0f}; };
+    auto values = [&](int n, int k, int j, Pair& h, Pair& g) {
+      h = mul2(add2(pair(now[n].x[k], j), both(-now[n].mean)), both(now[n].rstd));
+      g = pair(now[n].dy[k], j);
+      if (SHIFTED) {
+        const int c = at.column(k) + j;
+        if (!at.has(c)) h.x = g.x = 0.0f;
+        if (!at.has(c + 1)) h.y = g.y = 0.0f;
+      }
     };
-    float sg = 0.0f, sgh = 0.0f;
 #pragma unroll
-    for (int k = 0; k < ITER; ++k) {
-      if (at.any(at.column(k))) {
+    for (int n = 0; n < N; ++n) {
+      now[n] = next[n];
+      const uint64_t then = row + (N + n) * at.step;
+      if (then < at.rows) load(then, next[n]);
+      Pair sg = both(0.0f), sgh = both(0.0f);
+      if (n == 0 || row + n * at.step < at.rows) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float h, g;
-          values(k, j, h, g);
-          dw[k][j] += g * h;
-          db[k][j] += g;
-          sg += g * w[k][j];
-          sgh += g * w[k][j] * h;
+        for (int k = 0; k < ITER; ++k) {
+          if (at.any(at.column(k))) {
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+              Pair h, g;
+              values(n, k, 2 * j, h, g);
+              dw[k][j] = fma2(g, h, dw[k][j]);
+              db[k][j] = add2(db[k][j], g);
+              g = mul2(g, pair(w[k], 2 * j));
+              sg = add2(sg, g);
+              sgh = fma2(g, h, sgh);
+            }
+          }
         }
       }
+      sums[n] = make_float2(sg.x + sg.y, sgh.x + sgh.y);
     }
-    const float2 s = row_sums<THREADS>(sg, sgh, shared, turn++);
-    const float m0 = s.x * inv, m1 = s.y * inv;
+    row_sums<THREADS>(sums, shared, turn++);
 #pragma unroll
-    for (int k = 0; k < ITER; ++k) {
-      if (at.any(at.column(k))) {
-        float f[VEC];
+    for (int n = 0; n < N; ++n) {
+      if (n > 0 && row + n * at.step >= at.rows) break;
+      // (g w - m0 - h m1) rstd
+      const float d = now[n].rstd;
+      const Pair m0 = both(-sums[n].x * inv * d), m1 = both(-sums[n].y * inv * d);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float h, g;
-          values(k, j, h, g);
-          f[j] = (g * w[k][j] - m0 - h * m1) * now.rstd;
+      for (int k = 0; k < ITER; ++k) {
+        if (at.any(at.column(k))) {
+          float f[VEC];
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            Pair h, g;
+            values(n, k, 2 * j, h, g);
+            const Pair v = fma2(h, m1, fma2(mul2(g, pair(w[k], 2 * j)), both(d), m0));
+            f[2 * j] = v.x;
+            if (VEC > 1) f[2 * j + (VEC > 1)] = v.y;
+          }
+          at.store(dx, (row + n * at.step) * at.cols, at.column(k), f);
         }
-        at.store(dx, row * at.cols, at.column(k), f);
       }
     }
   }
+  auto one = [](const Pair& p, int j) { return j % 2 ? p.y : p.x; };
   if (!a.dweight && !a.dbias) return;
   float* part = a.workspace + (uint64_t)blockIdx.x * 2 * a.cols;
   if (R::kTogether > 1) {
     // the warps' sums, added in the order of the warps
     constexpr int kMany = R::kTogether > 1 ? 32 * ITER * VEC : 1;
-    __shared__ float sums[2][kMany];
+    __shared__ float together[2][kMany];
     for (int w = 0; w < R::kTogether; ++w) {
       if (threadIdx.x / THREADS == w) {
 #pragma unroll
@@ -361,9 +400,9 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             const int i = ((k * VEC + j) * 32 + threadIdx.x % 32) % kMany, c = at.column(k) + j;
-            const float pw = dw[k][j] + (w ? sums[0][i] : 0.0f), pb = db[k][j] + (w ? sums[1][i] : 0.0f);
+            const float pw = one(dw[k][j / 2], j) + (w ? together[0][i] : 0.0f), pb = one(db[k][j / 2], j) + (w ? together[1][i] : 0.0f);
             if (w < R::kTogether - 1) {
-              sums[0][i] = pw, sums[1][i] = pb;
+              together[0][i] = pw, together[1][i] = pb;
             } else if (c >= 0 && c < (int)at.cols) {
               part[c] = pw, part[a.cols + c] = pb;
             }
@@ -377,7 +416,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const int c = at.column(k) + j;
-        if (c >= 0 && c < (int)at.cols) part[c] = dw[k][j], part[a.cols + c] = db[k][j];
+        if (c >= 0 && c < (int)at.cols) part[c] = one(dw[k][j / 2], j), part[a.cols + c] = one(db[k][j / 2], j);
       }
   }
 }
@@ -397,7 +436,9 @@ __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const 
     sg += g;
     sgh += g * ((widen(x[c]) - mean) * rstd);
   }
-  const float2 s = row_sums<kLongThreads>(sg, sgh, shared, 0);
+  float2 sums[1] = {make_float2(sg, sgh)};
+  row_sums<kLongThreads>(sums, shared, 0);
+  const float2 s = sums[0];
   T* dx = static_cast<T*>(a.dx) + base;
   for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
     const float g = widen(dy[c]) * (a.weight ? param_at(a.weight, a.param_type, c) : 1.0f);

@@ -9,6 +9,8 @@
 
 #include <cstdint>
 
+#include "values.cuh"
+
 namespace csw {
 namespace tc {
 
@@ -228,26 +230,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-// two float32 operations in one instruction
-struct Pair {
-  float x, y;
-};
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair r;
-  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 
