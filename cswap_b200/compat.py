@@ -7,7 +7,8 @@ the top of every forward pass, `torch.cswapsetratio(r)`, and wrap each layer as
     torch.cswappre(pre, type); out = layer(pre); torch.cswappost(pre, out, type)
 
 (CIFAR10/cifar10.py:86,106, CIFAR10/models/vgg.py:23-46), where `type` is the
-policy for the layer's input: 0 keep, 2 raw swap, 3 sparse, 6 ZFP.  Here the
+policy for the layer's input: 0 keep, 2 raw swap, 3 sparse, 6 ZFP (and 8, the
+framework's own: kept on the device in 8 bits).  Here the
 same five names are module functions over one process-wide `Execution`:
 
     import cswap_b200.compat as cswap
@@ -24,7 +25,7 @@ from typing import Optional
 
 import torch
 
-from .codec import POLICY_DROP, POLICY_KEEP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP
+from .codec import POLICY_DROP, POLICY_KEEP, POLICY_Q8, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP
 from .execution import Execution, LayerType
 from .swap import SwapManager
 
@@ -65,7 +66,7 @@ def cswappre(pre: torch.Tensor, type: int = 0) -> None:  # noqa: A002 - the refe
     exe = execution()
     tid = getattr(pre, "tensor_id", -1)
     if 0 <= tid < _MAX_IDS:
-        exe.policy[tid] = int(type) if int(type) in (POLICY_DROP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP) \
+        exe.policy[tid] = int(type) if int(type) in (POLICY_DROP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP, POLICY_Q8) \
             else POLICY_KEEP
         exe.begin_stage[tid] = exe.index + 1
     exe.pre(pre, LayerType.ACT)

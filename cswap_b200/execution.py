@@ -20,7 +20,10 @@ dropped tensor is rebuilt in backward by running its producer again on the
 producer's own input, which is in turn swapped in or rebuilt as needed.  Only
 stateless callables may be passed (a BatchNorm module would update its running
 statistics a second time; pass a closure over F.batch_norm without them).  A
-tensor whose producer was not given stays on the device.  `policy_` 3 and 4
+tensor whose producer was not given stays on the device.  Policy 8, the
+framework's own, keeps the tensor on the device as an 8-bit checkpoint
+(`ops.q8_compress`, 1.03 bytes a value) and takes the values it holds for
+backward: no link time, a quarter of the memory.  `policy_` 3 and 4
 select the vDNN and SuperNeurons baselines as in Execution.h:70,243,248.
 
 The reference swaps the storage's DataPtr under the autograd graph and relies
@@ -40,8 +43,9 @@ from typing import Dict, List, Optional, Sequence, Union
 
 import torch
 
-from .codec import POLICY_DROP, POLICY_KEEP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP
+from .codec import POLICY_DROP, POLICY_KEEP, POLICY_Q8, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP
 from ._lib import CswapError
+from .ops import q8_compress, q8_decompress
 from .swap import CostModel, SwapManager, TensorDesc, Ticket
 
 
@@ -56,15 +60,16 @@ class LayerType(enum.IntEnum):
 
 
 class _Record:
-    """Residency of one activation storage: on the device (`tensor`) or
-    swapped out (`ticket`)."""
+    """Residency of one activation storage: on the device (`tensor`),
+    swapped out (`ticket`) or held in 8 bits (`packed`)."""
 
-    __slots__ = ("tensor", "ticket", "numel", "order", "exe", "producer", "dropped", "saved", "ahead",
+    __slots__ = ("tensor", "ticket", "packed", "numel", "order", "exe", "producer", "dropped", "saved", "ahead",
                  "__weakref__")
 
     def __init__(self, tensor: torch.Tensor, exe: "Execution"):
         self.tensor: Optional[torch.Tensor] = tensor
         self.ticket: Optional[Ticket] = None
+        self.packed: Optional[torch.Tensor] = None  # policy 8: the 8-bit checkpoint
         self.numel = tensor.numel()
         self.order = -1
         self.exe = weakref.ref(exe)
@@ -89,6 +94,8 @@ class _Record:
                 else:
                     self.tensor = exe.mgr.swap_in(self.ticket).view(-1)
                 exe._after_swap_in(self)
+            elif self.packed is not None:
+                self.tensor, self.packed = q8_decompress(self.packed, self.numel), None
             else:
                 fn, packed = self.producer
                 with torch.no_grad():
@@ -145,6 +152,7 @@ class Execution:
         self._prof_saved: Dict[int, bool] = {}
         self._prof_start = None
         self.swapped_tensors = 0
+        self.held_tensors = 0
         self.dropped_tensors = 0
         self.recomputed_tensors = 0
         self.skipped_for_memory = 0
@@ -253,13 +261,13 @@ class Execution:
             if tid < 0 or tid >= len(self.begin_stage) or self.index != self.begin_stage[tid] or t.grad_fn is None:
                 continue
             pol = self._effective_policy(tid, layer_type)
-            if pol not in (POLICY_DROP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP):
+            if pol not in (POLICY_DROP, POLICY_RAW, POLICY_SPARSE, POLICY_ZFP, POLICY_Q8):
                 continue
             key = self._key(t)
             if key is None:
                 continue
             rec = self._record_for(t, key)
-            if rec.ticket is not None or rec.dropped:
+            if rec.ticket is not None or rec.packed is not None or rec.dropped:
                 continue
             if pol == POLICY_DROP:
                 if rec.producer is not None:  # without its producer the tensor simply stays
@@ -280,6 +288,11 @@ class Execution:
             self._prof_start = ev
 
     def _start_swap(self, rec: _Record, pol: int) -> None:
+        if pol == POLICY_Q8:
+            rec.packed = q8_compress(rec.tensor)
+            self._pending.append(rec)
+            self.held_tensors += 1
+            return
         try:
             rec.ticket = self.mgr.swap_out(rec.tensor, pol)
         except CswapError as err:
@@ -329,7 +342,7 @@ class Execution:
                     rec = self._records.get(t.untyped_storage().data_ptr())
                     self._prof_saved[tid] = bool(rec is not None and rec.saved)
         for rec, pol in self._deferred:
-            if rec.saved and rec.ticket is None and rec.tensor is not None:
+            if rec.saved and rec.ticket is None and rec.packed is None and rec.tensor is not None:
                 self._start_swap(rec, pol)
             elif not rec.saved:
                 self.skipped_unsaved += 1

@@ -6,7 +6,9 @@ by layer in Execution.pre/post exactly the way the reference's drivers do.
   next layer consumes it) of CSWAP+/vgg16-cifar10.cpp:77-245,381-397.
 * A BERT-style encoder with every linear / matmul / softmax / dropout /
   layer-norm / activation wrapped, as CSWAP+/bert.cpp:370-801 does, with the
-  dimensions left to the caller (the benchmark uses the BERT-base shape).
+  dimensions left to the caller (the benchmark uses the BERT-base shape).  With
+  `lean` its attention, feed-forward part and norms are the operators of ops.py,
+  which save little for backward in the first place.
 
 Inputs are synthetic (the datasets are not part of this repository) and
 weights are randomly initialised.
@@ -21,6 +23,7 @@ import torch.nn.functional as F
 
 from .codec import POLICY_KEEP, POLICY_RAW, POLICY_ZFP
 from .execution import Execution, LayerType
+from .ops import attention, gelu_linear, layer_norm
 
 
 # ---------------------------------------------------------------------------
@@ -114,9 +117,14 @@ def vgg16_reference_policy(exe: Execution, compressed: int = POLICY_ZFP) -> None
 # BERT-style encoder (bert.cpp:370-801)
 # ---------------------------------------------------------------------------
 class BertEncoder(nn.Module):
+    """`lean`: attention that keeps one number a row (in bfloat16, its probabilities without dropout), a feed-forward
+    part that keeps its activation in 8 bits, norms that take the residual's sum with them.  The parameters are the
+    same, so that a state of one kind loads into the other."""
+
     def __init__(self, vocab: int = 30522, hidden: int = 768, layers: int = 12, heads: int = 12, ffn: int = 3072,
-                 max_seq: int = 512, dropout: float = 0.1):
+                 max_seq: int = 512, dropout: float = 0.1, lean: bool = False):
         super().__init__()
+        self.lean = lean
         self.hidden, self.heads, self.nlayers, self.p = hidden, heads, layers, dropout
         self.tok = nn.Embedding(vocab, hidden)
         self.pos = nn.Embedding(max_seq, hidden)
@@ -147,10 +155,28 @@ class BertEncoder(nn.Module):
         x = step(lambda i: self.tok(i) + self.pos(pos), ids, LayerType.ACT, True)
         x = step(self.emb_ln, x, LayerType.BN)
         x = step(lambda t: F.dropout(t, self.p, self.training), x)
+
+        def heads(t):
+            return t.view(B, S, nh, dh).transpose(1, 2).to(torch.bfloat16)
+
+        def norm(ln, a, b):
+            return layer_norm(a, ln.weight, ln.bias, ln.eps, residual=b)
+
         for l in range(self.nlayers):
             q = step(self.q[l], x, LayerType.FC)
             k = step(self.k[l], x, LayerType.FC)
             v = step(self.v[l], x, LayerType.FC)
+            if self.lean:
+                ctx = step(lambda a, b, c: attention(heads(a), heads(b), heads(c)).transpose(1, 2).reshape(B, S, H)
+                           .to(x.dtype), [q, k, v], LayerType.FC)
+                ao = step(self.o[l], ctx, LayerType.FC)
+                ao = step(lambda t: F.dropout(t, self.p, self.training), ao)
+                x = step(lambda a, b: norm(self.ln1[l], a, b), [ao, x], LayerType.BN)
+                h = step(self.f1[l], x, LayerType.FC)
+                h = step(lambda t: gelu_linear(t, self.f2[l].weight, self.f2[l].bias), h, LayerType.FC)
+                h = step(lambda t: F.dropout(t, self.p, self.training), h)
+                x = step(lambda a, b: norm(self.ln2[l], a, b), [h, x], LayerType.BN)
+                continue
             qh = step(lambda t: t.view(B, S, nh, dh).transpose(1, 2).contiguous(), q)
             kh = step(lambda t: t.view(B, S, nh, dh).permute(0, 2, 3, 1).contiguous(), k)
             vh = step(lambda t: t.view(B, S, nh, dh).transpose(1, 2).contiguous(), v)
