@@ -584,6 +584,13 @@ struct BackwardPlan {
   static constexpr int kColumns = 512;
 };
 
+// D = do.o carries the rounding of o, 2^-9 or 2^-12 of it.  sum ds, which would be zero, is what D is off by (r), and is
+// put right in dkv's D.  dq would have to lose r sum p k: where a tile of queries sees no more than this many tiles of
+// keys that sum is formed too, by a product of its own.  In rows that see more keys o is smaller, by the square root of
+// their number, and with it r: of dq's error, 0.0024 of its norm in bfloat16 (ds and dq are rounded), r made up a
+// thirtieth at 2048 causal keys, but more than half of 0.0038 at 40.
+constexpr int kFewTiles = 2;
+
 // ds = p (dp - D) for 32 columns, rounded and packed over the dp that it came from; their sum
 template <class T>
 __device__ __forceinline__ float to_gradients(const float* p, const uint32_t* dp, const float* d, uint32_t* out) {
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   fence_after();
   pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256,
-                 left_at = dq_at + DP;  // two columns for each of two pieces: the halves' sums of ds
+                 pk_at = dq_at + DP;  // sum p k
   const Shape& s = a.s;
   const uint32_t ring = tiles_at + 2 * kStay * Plan::kTileBytes;  // behind q and do: k 0, v 0, k 1, v 1, ...
 
@@ -691,12 +698,20 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         if (piece.first < 0) return;
         const int n = Queries<1>(s, piece).most;
         if (n == 0) continue;
+        const bool few = n <= kFewTiles;
         const uint32_t stay = u % kStay, q_at = tiles_at + stay * 2 * Plan::kTileBytes;
         CSW_WAIT_WARP(q_full + 8 * stay, u / kStay & 1);
         uint32_t before = 0;  // the slot of this turn's tile, whose scores came the turn before
         for (int j = -1; j < n; ++j) {
           const bool now = j >= 0, next = j + 1 < n;
           const uint32_t k_at = ring + slot * Plan::kTileBytes, v_at = k_at + Plan::kTileBytes;
+          const uint32_t k_now = ring + before * Plan::kTileBytes;
+          if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
+          if (now && few) {
+            CSW_WAIT_WARP(s_free, (i - 1) & 1);  // the probabilities are there
+            fence_after();
+            product_tokens(pk_at, s_at, 64, k_now, sums, j > 0);
+          }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot, round & 1);
             if (s.lens && (j + 2) * kTile > piece.keys) {
@@ -711,9 +726,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           }
           if (now) {
             CSW_WAIT_WARP(ds_ready, (i - 1) & 1);
-            if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
             fence_after();
-            product_tokens(dq_at, dp_at, 64, ring + before * Plan::kTileBytes, sums, j > 0, empty + 8 * before, !next ? dq_full : 0);
+            product_tokens(dq_at, dp_at, 64, k_now, sums, j > 0, empty + 8 * before, !next ? dq_full : 0);
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
@@ -735,6 +749,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
     // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for
+    float shift = INFINITY, delta = 0.0f;  // of this thread's row of the piece that was prepared last
     auto prepare = [&](const Piece& p, int u) {
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
       const int lane = t % kLanes, mine = t / 32 * 32 + t % 32 / kLanes;
@@ -765,33 +780,46 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       }
       const int row = p.first + t;
       const float lse = row < (int)s.q_len ? a.lse[(uint64_t)p.row * s.q_len + row] : -INFINITY;
-      shifts[u & 1][t] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-      bar_arrive(rows_ready);
+      shift = lse == -INFINITY ? INFINITY : lse * kLog2e;
+      shifts[u & 1][t] = shift;
       group_sync(2, 128);
+      delta = deltas[u & 1][t];
+      bar_arrive(rows_ready);
     };
-    // The results of a piece that sees n tiles; false where a wait ran out.
-    auto finish = [&](const Piece& p, bool any, int u) -> bool {
-      const float shift = any ? shifts[u & 1][t] : INFINITY;
+    // The results of a piece that sees n tiles, and its row's exponent shift and D; false where a wait ran out.
+    auto finish = [&](const Piece& p, int n, int u, float shift, float d) -> bool {
       const bool live = shift != INFINITY;
-      float* mine = a.rows + (uint64_t)p.row * a.padded + p.first + t;  // padded to whole tiles
-      const uint64_t plane = (uint64_t)s.batch * s.heads * a.padded;
-      float d = 0.0f;
-      if (any) {
+      float off = 0.0f;
+      if (n > 0) {
         if (!__all_sync(0xffffffffu, bar_wait(left_ready, u & 1) && bar_wait(dq_full, u & 1))) return false;
         fence_after();
-        // dkv's D has no rounding of o in it: it is sum p dp, which this kernel has formed on the way.
-        const float2 left = load2(left_at + 2 * (u & 1) + lanes);
-        d = live ? deltas[u & 1][t] + left.x + left.y : 0.0f;
+        off = live ? shifts[u & 1][t] + deltas[u & 1][t] : 0.0f;
       }
       stage_free(t == 0, 1, 128);
 #pragma unroll
-      for (int c = 0; c < DP; c += 64)
-        take_columns<T>(stage + c / 64 * kChunk, t, any, live, dq_at + c + lanes, s.scale, [&] {
-          if (c + 64 == DP) {
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32] = {};
+        if (n > 0) {
+          load32(dq_at + c + lanes, r);
+          wait_loads(r);
+          if (n <= kFewTiles) {
+            uint32_t m[32];
+            load32(pk_at + c + lanes, m);
+            wait_loads(m);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(fmaf(-off, __uint_as_float(m[k]), __uint_as_float(r[k])));
+          }
+          if (c + 32 == DP) {
             fence_before();
             bar_arrive(dq_free);
           }
-        });
+        }
+        if (!live) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        stage_columns<T>(stage + c / 64 * kChunk, t, c % 64, r, s.scale);
+      }
       async_fence();
       group_sync(1, 128);
       if (t == 0) {
@@ -799,25 +827,27 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         for (int c = 0; c < DP; c += 64)
           if (c < (int)s.dim) store_tile(&a.dq, smem_at(stage) + c / 64 * kChunk, c, p.first, p.head, p.batch);
       }
+      float* mine = a.rows + (uint64_t)p.row * a.padded + p.first + t;  // padded to whole tiles
       mine[0] = shift;
-      mine[plane] = d;
+      mine[(uint64_t)s.batch * s.heads * a.padded] = live ? d + off : 0.0f;
       return true;
     };
     [&] {
       Piece last{-1};
-      int u = 0;
+      int last_n = 0, u = 0;
       for (int it = 0;; ++it) {
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
-        const bool any = piece.first >= 0 && Queries<1>(s, piece).most > 0;
-        if (any) prepare(piece, u);
-        if (last.first >= 0 && !finish(last, true, u - 1)) return give_up(flag);
+        const int n = piece.first >= 0 ? Queries<1>(s, piece).most : 0;
+        const float last_shift = shift, last_delta = delta;
+        if (n > 0) prepare(piece, u);
+        if (last.first >= 0 && !finish(last, last_n, u - 1, last_shift, last_delta)) return give_up(flag);
         last.first = -1;
         if (piece.first < 0) return;
-        if (any) {
-          last = piece;
+        if (n > 0) {
+          last = piece, last_n = n;
           ++u;
-        } else if (!finish(piece, false, 0)) {
+        } else if (!finish(piece, 0, 0, INFINITY, 0.0f)) {
           return give_up(flag);
         }
       }
@@ -837,7 +867,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
         CSW_WAIT_WARP(rows_ready, u & 1);
         const float shift = shifts[u & 1][t], d = deltas[u & 1][t];
-        float left = 0.0f;  // sum of ds: zero, had D been taken with o before it was rounded
+        group_sync(3, 256);  // both halves have read: the places are written below
+        const bool few = n <= kFewTiles;
+        float left = 0.0f;  // sum of ds
         for (int j = 0; j < n; ++j, ++i) {
           CSW_WAIT_WARP(s_full, i & 1);
           fence_after();
@@ -847,8 +879,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             load32(s_at + 64 * w + lanes, r);
             load32(s_at + 64 * w + 32 + lanes, r + 32);
             wait_loads(r), wait_loads(r + 32);
-            fence_before();
-            bar_arrive(s_free);
+            if (!few) {
+              fence_before();
+              bar_arrive(s_free);
+            }
 #pragma unroll
             for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
           }
@@ -858,6 +892,18 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
 #pragma unroll
             for (int k = 0; k < 64; ++k)
               if (k >= end) p[k] = 0.0f;
+          }
+          if (few) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t out[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
+              store16(s_at + 64 * w + 16 * c + lanes, out);
+            }
+            wait_stores();
+            fence_before();
+            bar_arrive(s_free);
           }
           CSW_WAIT_WARP(dp_full, i & 1);
           fence_after();
@@ -876,9 +922,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           fence_before();
           bar_arrive(ds_ready);
         }
-        store1(left_at + 2 * (u & 1) + w + lanes, left);
-        wait_stores();
-        fence_before();
+        (w == 0 ? shifts : deltas)[u & 1][t] = left;
         bar_arrive(left_ready);
         ++u;
       }

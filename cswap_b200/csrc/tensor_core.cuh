@@ -161,16 +161,6 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
       "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void store1(uint32_t at, float v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at), "f"(v) : "memory");
-}
-// two columns, waited for
-__device__ __forceinline__ float2 load2(uint32_t at) {
-  float2 v;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v.x), "+f"(v.y)::"memory");
-  return v;
-}
 #undef CSW_R4
 #undef CSW_R16
 #undef CSW_R32
