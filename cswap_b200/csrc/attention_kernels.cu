@@ -133,12 +133,14 @@ __device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map
 #pragma unroll
   for (int c = 0; c < DP / 64; ++c) copy_tile(dst + c * kChunk, map, bar, c * 64, token, head, batch);
 }
+// Tiles are named by their descriptors, read along or across their rows; those of a ring are a step apart.
+__device__ __forceinline__ uint64_t along(uint32_t tile) { return tile_desc(tile, 16); }
+__device__ __forceinline__ uint64_t across(uint32_t tile) { return tile_desc(tile, kChunk); }
 // acc (+)= A B^T: both read along their rows, the reduction over the head's dimension.  Behind the products of a call
 // the barriers that are not 0 are arrived at: once these, and all in front, have ended.
 template <int DP>
-__device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t b, uint32_t desc, uint32_t bar0 = 0,
+__device__ __forceinline__ void product_rows(uint32_t acc, uint64_t da, uint64_t db, uint32_t desc, uint32_t bar0 = 0,
                                              uint32_t bar1 = 0) {
-  const uint64_t da = tile_desc(a, 16), db = tile_desc(b, 16);
   if (elected()) {
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
@@ -151,9 +153,8 @@ __device__ __forceinline__ void product_rows(uint32_t acc, uint32_t a, uint32_t 
 }
 // acc (+)= P B: P in tensor memory, B read across its rows, the reduction over 128 tokens.  P's first 64 columns lie
 // at p, the others at p + half.
-__device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint32_t b, uint32_t desc,
+__device__ __forceinline__ void product_tokens(uint32_t acc, uint32_t p, uint32_t half, uint64_t db, uint32_t desc,
                                                bool add, uint32_t bar0 = 0, uint32_t bar1 = 0) {
-  const uint64_t db = tile_desc(b, kChunk);
   if (elected()) {
 #pragma unroll
     for (int k = 0; k < kTile / 16; ++k)
@@ -440,6 +441,8 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
+      constexpr uint32_t kStep = Plan::kTileBytes / 16;
+      const uint64_t q_rows = along(tiles_at), ring_rows = along(ring), ring_tokens = across(ring);
       int base = 0, u = 0, tile[NWG] = {}, done[NWG] = {};  // of the ring; pieces; of each tile of queries: tiles, pieces
       for (int it = 0;; ++it) {
         Piece piece;
@@ -464,11 +467,11 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               if (j == 1 && done[w] > 0) CSW_WAIT_WARP(o_free + 8 * w, (done[w] - 1) & 1);
               fence_after();
               const bool last = j == at.count[w];
-              product_tokens(ow, sw, 32, ring + v * Plan::kTileBytes, sums, j > 1, last ? o_full + 8 * w : 0);
+              product_tokens(ow, sw, 32, ring_tokens + v * kStep, sums, j > 1, last ? o_full + 8 * w : 0);
               done[w] += last;
             }
             if (j < at.count[w]) {
-              product_rows<DP>(sw, tiles_at + w * Plan::kTileBytes, ring + k * Plan::kTileBytes, scores, s_full + 8 * w);
+              product_rows<DP>(sw, q_rows + w * kStep, ring_rows + k * kStep, scores, s_full + 8 * w);
             }
           }
           if (j < at.most) commit_to(empty + 8 * k);
@@ -591,6 +594,18 @@ struct BackwardPlan {
 // thirtieth at 2048 causal keys, but more than half of 0.0038 at 40.
 constexpr int kFewTiles = 2;
 
+// The probabilities of columns k and k + 1.  One pair in four by polynomial: the unit for exponentials takes 8 clocks for
+// a warp's, a thousand for a tile's, and the softmax warps have little else to do meanwhile.
+__device__ __forceinline__ void exp_pair(int k, const uint32_t* r, Pair by, Pair less, float* p) {
+  Pair x = fma2({__uint_as_float(r[k]), __uint_as_float(r[k + 1])}, by, less);
+  if (k % 8 == 6) {
+    x = exp2_poly(x);
+  } else {
+    x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
+  }
+  p[k] = x.x, p[k + 1] = x.y;
+}
+
 // ds = p (dp - D) for 32 columns, rounded and packed over the dp that it came from; their sum
 template <class T>
 __device__ __forceinline__ float to_gradients(const float* p, const uint32_t* dp, const float* d, uint32_t* out) {
@@ -691,6 +706,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       // The scores of the next tile come in front of what follows of this one: their place is free once they have been
       // read, that of dp behind the product that reads it.
+      constexpr uint32_t kStep = Plan::kTileBytes / 16;
+      const uint64_t stay_rows = along(tiles_at), ring_rows = along(ring), ring_tokens = across(ring);
       uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of keys, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
@@ -699,13 +716,13 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const int n = Queries<1>(s, piece).most;
         if (n == 0) continue;
         const bool few = n <= kFewTiles;
-        const uint32_t stay = u % kStay, q_at = tiles_at + stay * 2 * Plan::kTileBytes;
+        const uint32_t stay = u % kStay;
+        const uint64_t q_rows = stay_rows + stay * 2 * kStep;  // do behind it
         CSW_WAIT_WARP(q_full + 8 * stay, u / kStay & 1);
         uint32_t before = 0;  // the slot of this turn's tile, whose scores came the turn before
         for (int j = -1; j < n; ++j) {
           const bool now = j >= 0, next = j + 1 < n;
-          const uint32_t k_at = ring + slot * Plan::kTileBytes, v_at = k_at + Plan::kTileBytes;
-          const uint32_t k_now = ring + before * Plan::kTileBytes;
+          const uint64_t k_rows = ring_rows + slot * kStep, k_now = ring_tokens + before * kStep;
           if (j == 0 && u > 0) CSW_WAIT_WARP(dq_free, (u - 1) & 1);
           if (now && few) {
             CSW_WAIT_WARP(s_free, (i - 1) & 1);  // the probabilities are there
@@ -722,7 +739,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             }
             if (i > 0) CSW_WAIT_WARP(s_free, (i - 1) & 1);
             fence_after();
-            product_rows<DP>(s_at, q_at, k_at, scores, s_full);
+            product_rows<DP>(s_at, q_rows, k_rows, scores, s_full);
           }
           if (now) {
             CSW_WAIT_WARP(ds_ready, (i - 1) & 1);
@@ -731,7 +748,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
-            product_rows<DP>(dp_at, q_at + Plan::kTileBytes, v_at, slopes, dp_full, empty + 8 * slot + 8);
+            product_rows<DP>(dp_at, q_rows + kStep, k_rows + kStep, slopes, dp_full, empty + 8 * slot + 8);
           }
           if (j + 2 == n) commit_to(q_empty + 8 * stay);
           before = slot;
@@ -884,7 +901,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
               bar_arrive(s_free);
             }
 #pragma unroll
-            for (int k = 0; k < 64; ++k) p[k] = exp2_fast(fmaf(__uint_as_float(r[k]), s.exponent, -shift));
+            for (int k = 0; k < 64; k += 2)
+              exp_pair(k, r, both(s.exponent), both(-shift), p);
           }
           const bool masked = (j + 1) * kTile > least;
           const int end = limit - j * kTile - 64 * w;
@@ -1019,6 +1037,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       const uint32_t slopes = product_desc(kBf16<T>, kTile, false, false);
       const uint32_t sums = product_desc(kBf16<T>, DP, true, false);
       // Each place in tensor memory is written again behind the product that reads it.
+      constexpr uint32_t kStep = Plan::kTileBytes / 16;
+      const uint64_t stay_rows = along(tiles_at), ring_rows = along(ring), ring_tokens = across(ring);
       uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of queries, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
@@ -1026,22 +1046,22 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         if (piece.first < 0) return;
         const int n = Keys(s, piece).n;
         if (n == 0) continue;
-        const uint32_t stay = u % kStay, k_at = tiles_at + stay * 2 * Plan::kTileBytes;
+        const uint32_t stay = u % kStay;
+        const uint64_t k_rows = stay_rows + stay * 2 * kStep;  // v behind it
         CSW_WAIT_WARP(kv_full + 8 * stay, u / kStay & 1);
         uint32_t before = 0;  // the slot of this turn's tile, whose scores came the turn before
         for (int j = -1; j < n; ++j) {
           const bool now = j >= 0, next = j + 1 < n;
-          const uint32_t q_at = ring + slot * Plan::kTileBytes, do_at = q_at + Plan::kTileBytes;
-          const uint32_t q_now = ring + before * Plan::kTileBytes, do_now = q_now + Plan::kTileBytes;
+          const uint64_t q_rows = ring_rows + slot * kStep, q_now = ring_tokens + before * kStep;  // do behind them
           if (now) {
             CSW_WAIT_WARP(p_ready, (i - 1) & 1);
             if (j == 0 && u > 0) CSW_WAIT_WARP(sums_free, (u - 1) & 1);
             fence_after();
-            product_tokens(dv_at, s_at, 64, do_now, sums, j > 0, empty + 8 * before + 8);
+            product_tokens(dv_at, s_at, 64, q_now + kStep, sums, j > 0, empty + 8 * before + 8);
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot, round & 1);
-            product_rows<DP>(s_at, k_at, q_at, scores, s_full);
+            product_rows<DP>(s_at, k_rows, q_rows, scores, s_full);
           }
           if (now) {
             CSW_WAIT_WARP(ds_ready, (i - 1) & 1);
@@ -1050,7 +1070,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
-            product_rows<DP>(dp_at, k_at + Plan::kTileBytes, do_at, slopes, dp_full);
+            product_rows<DP>(dp_at, k_rows + kStep, q_rows + kStep, slopes, dp_full);
           }
           if (j + 2 == n) commit_to(kv_empty + 8 * stay);
           before = slot;
@@ -1133,10 +1153,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float4 f = shifts[k];
-              p[4 * k] = exp2_fast(fmaf(__uint_as_float(r[4 * k]), s.exponent, -f.x));
-              p[4 * k + 1] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 1]), s.exponent, -f.y));
-              p[4 * k + 2] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 2]), s.exponent, -f.z));
-              p[4 * k + 3] = exp2_fast(fmaf(__uint_as_float(r[4 * k + 3]), s.exponent, -f.w));
+              exp_pair(4 * k, r, both(s.exponent), {-f.x, -f.y}, p);
+              exp_pair(4 * k + 2, r, both(s.exponent), {-f.z, -f.w}, p);
             }
           }
           if (s.causal && piece.first + kTile - 1 - off > q * kTile) {

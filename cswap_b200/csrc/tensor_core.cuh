@@ -223,5 +223,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// 2^x without the unit for it: the whole part n goes into the exponent, 2^f for the rest, -1/2 ... 1/2, is a polynomial
+// of degree 5 (fitted for the least relative error, 1.6 10^-7).  x from -126 up to 127; below that 2^-126 stands for it.
+__device__ __forceinline__ Pair exp2_poly(Pair x) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 2^23: a sum with it is rounded to a whole number, its low bits
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const Pair t = add2(x, {kMagic, kMagic});
+  const Pair n = add2(t, {-kMagic, -kMagic});
+  const Pair f = fma2(n, {-1.0f, -1.0f}, x);
+  Pair p = fma2(f, {0.0013276472454890609f, 0.0013276472454890609f}, {0.009675540961325169f, 0.009675540961325169f});
+  p = fma2(p, f, {0.05550713092088699f, 0.05550713092088699f});
+  p = fma2(p, f, {0.24022120237350464f, 0.24022120237350464f});
+  p = fma2(p, f, {0.6931469440460205f, 0.6931469440460205f});
+  p = fma2(p, f, {1.0000001192092896f, 1.0000001192092896f});
+  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return p;
+}
+
 }  // namespace tc
 }  // namespace csw
