@@ -333,7 +333,12 @@ __device__ __forceinline__ void exp_of(Pair (&add)[2], const uint32_t* r, float 
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     Pair x = fma2({__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])}, by, less);
-    x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
+    // One pair in four by polynomial: the unit for exponentials takes 8 clocks for a warp's, more than all else of a value.
+    if (i % 4 == 3) {
+      x = exp2_poly(x);
+    } else {
+      x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
+    }
     if (2 * i >= end) x.x = 0.0f;
     if (2 * i + 1 >= end) x.y = 0.0f;
     add[i % 2] = add2(add[i % 2], x);
@@ -401,12 +406,13 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     init_visible();
     flag_word = 0;
   }
-  if (warp == 4 * NWG + 1) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   if (warp == 4 * NWG && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.k), prefetch_map(&a.v);
+  // In front of the allocation: what runs before in the stream may want this SM's tensor memory yet.
+  pdl_wait();
+  if (warp == 4 * NWG + 1) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   fence_before();
   __syncthreads();
   fence_after();
-  pdl_wait();
   const uint32_t tmem = tmem_at;
   const Shape& s = a.s;
   const uint32_t ring = tiles_at + NWG * Plan::kTileBytes;
@@ -662,12 +668,13 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     init_visible();
     flag_word = 0;
   }
-  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   if (warp == 12 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
+  // In front of the allocation: what runs before in the stream may want this SM's tensor memory yet.
+  pdl_wait();
+  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   fence_before();
   __syncthreads();
   fence_after();
-  pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dq_at = tmem + 256,
                  pk_at = dq_at + DP;  // sum p k
   const Shape& s = a.s;
@@ -985,12 +992,13 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     init_visible();
     flag_word = 0;
   }
-  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   if (warp == 12 && threadIdx.x % 32 == 0) prefetch_map(&a.q), prefetch_map(&a.dout), prefetch_map(&a.k), prefetch_map(&a.v);
+  // In front of the allocation: what runs before in the stream may want this SM's tensor memory yet.
+  pdl_wait();
+  if (warp == 13) tmem_alloc<Plan::kColumns>(smem_at(&tmem_at));
   fence_before();
   __syncthreads();
   fence_after();
-  pdl_wait();
   const uint32_t tmem = tmem_at, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = dv_at + DP;
   const Shape& s = a.s;
   const uint32_t ring = tiles_at + 2 * kStay * Plan::kTileBytes;  // behind k and v: q 0, do 0, q 1, do 1, ...

@@ -35,15 +35,17 @@ bool norm_args(int type, int param_type, size_t rows, size_t cols) {
 }
 
 // whether the operand can be addressed and, if its rows are copied as tiles, lies as a tile copy needs it
-bool operand(const csw_attention_operand* o, const csw_attention_shape* s, size_t tokens) {
+bool operand(const csw_attention_operand* o, const csw_attention_shape* s, size_t heads, size_t tokens) {
   if (!o) return false;
-  if (s->batch == 0 || s->heads == 0 || tokens == 0) return true;
-  return o->data && aligned(o->data, 16) && o->batch_stride % 8 == 0 && o->head_stride % 8 == 0 &&
-         o->token_stride % 8 == 0 && o->batch_stride >= 0 && o->head_stride >= 0 && o->token_stride >= 0;
+  if (s->batch == 0 || tokens == 0) return true;
+  // the stride of an axis of one step is not used
+  auto strides = [](ptrdiff_t stride, size_t n) { return n < 2 || (stride > 0 && stride % 8 == 0); };
+  return o->data && aligned(o->data, 16) && strides(o->batch_stride, s->batch) && strides(o->head_stride, heads) &&
+         strides(o->token_stride, tokens);
 }
 bool attention_args(const csw_attention_shape* s) {
   if (!s || (s->type != CSW_TYPE_F16 && s->type != CSW_TYPE_BF16)) return false;
-  constexpr size_t kMost = (size_t)1 << 30;
+  constexpr size_t kMost = (size_t)1 << 29;  // sums of positions stay below 2^31
   if (s->batch > 65535 || s->heads > 65535 || s->q_len > kMost || s->k_len > kMost) return false;
   if (s->dim == 0 || s->dim > 128 || s->dim % 8) return false;
   if (s->kv_heads == 0 || s->heads % s->kv_heads) return false;
@@ -135,8 +137,8 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
                                  const csw_attention_operand* o, float* d_lse, csw_stream_t stream) {
   if (!attention_args(shape)) return CSW_ERR_ARG;
   const csw_attention_shape& s = *shape;
-  if (!operand(q, shape, s.q_len) || !operand(k, shape, s.k_len) || !operand(v, shape, s.k_len) ||
-      !operand(o, shape, s.q_len))
+  if (!operand(q, shape, s.heads, s.q_len) || !operand(k, shape, s.kv_heads, s.k_len) ||
+      !operand(v, shape, s.kv_heads, s.k_len) || !operand(o, shape, s.heads, s.q_len))
     return CSW_ERR_ARG;
   if (s.batch * s.q_len != 0 && !good(d_lse, CSW_TYPE_F32)) return CSW_ERR_ARG;
   return done(attention_forward_launch(s, *q, *k, *v, *o, d_lse, stream));
@@ -158,9 +160,9 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
   if (csw_attention_workspace(shape, &need) != CSW_OK) return CSW_ERR_ARG;
   const csw_attention_shape& s = *shape;
   for (const csw_attention_operand* p : {q, o, dout, dq})
-    if (!operand(p, shape, s.q_len)) return CSW_ERR_ARG;
+    if (!operand(p, shape, s.heads, s.q_len)) return CSW_ERR_ARG;
   for (const csw_attention_operand* p : {k, v, dk, dv})
-    if (!operand(p, shape, s.k_len)) return CSW_ERR_ARG;
+    if (!operand(p, shape, s.kv_heads, s.k_len)) return CSW_ERR_ARG;
   if (need && (!good(d_lse, CSW_TYPE_F32) || !d_workspace || !aligned(d_workspace, 16))) return CSW_ERR_ARG;
   if (workspace_bytes < need) return CSW_ERR_SIZE;
   return done(attention_backward_launch(s, {*q, *k, *v, *o, *dout, *dq, *dk, *dv, d_lse, (float*)d_workspace}, stream));

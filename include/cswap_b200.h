@@ -363,8 +363,8 @@ csw_status csw_q8_decompress(const void* d_in, size_t bytes, size_t n, void* d_o
 csw_status csw_gelu_forward(const void* d_x, int type, size_t n, void* d_y, void* d_packed, size_t cap,
                             csw_stream_t stream);
 /* With x the values that the checkpoint holds: dx = dy (Phi(x) + x phi(x)); where d_y is given it receives x Phi(x)
- * (what the weight gradient of a product behind the GELU needs, so that nobody has to keep it).  d_dx and d_y may
- * not overlap; d_dx may be d_dy. */
+ * (what the weight gradient of a product behind the GELU needs, so that nobody has to keep it).  No two buffers
+ * overlap. */
 csw_status csw_gelu_backward(const void* d_dy, int type, const void* d_packed, size_t bytes, size_t n, void* d_dx,
                              void* d_y, csw_stream_t stream);
 
@@ -395,7 +395,8 @@ typedef struct {
   const int32_t* kv_lens;
 } csw_attention_shape;
 /* Where a tensor lies: data[b * batch_stride + h * head_stride + t * token_stride + 0 ... dim - 1], strides in
- * elements, not negative and multiples of 8, data 16-byte aligned. */
+ * elements, positive multiples of 8 below 2^39 where their axis has more than one step, data 16-byte aligned.  Lengths
+ * are at most 2^29, batch and heads 65535. */
 typedef struct {
   void* data;
   ptrdiff_t batch_stride, head_stride, token_stride;
@@ -405,7 +406,7 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
                                  const csw_attention_operand* k, const csw_attention_operand* v,
                                  const csw_attention_operand* o, float* d_lse, csw_stream_t stream);
 /* Backward forms the probabilities again from q, k and d_lse.  Gradients of keys and values are summed over the query
- * heads that share them, in a fixed order. */
+ * heads that share them, in a fixed order.  The workspace (csw_attention_workspace bytes) is 16-byte aligned. */
 csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes);
 csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_attention_operand* q,
                                   const csw_attention_operand* k, const csw_attention_operand* v,

@@ -561,3 +561,42 @@ def test_attention_refusals(cs):
                  lambda: cs.attention_backward(do, q, k, v, o[:, :2], lse)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- offsets beyond 32 bits ------------------------------------------------------------------------------------------------
+
+def test_offsets_beyond_32_bits(cs):
+    """More than 2^31 values, or as many bytes between two entries: the last ones are as right as the first."""
+    n = (1 << 31) + 1000
+    x = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    for at in (0, n - 5000):
+        x[at:at + 5000] = normal(5000, seed=at % 7, kind=torch.bfloat16)
+    y, packed = cs.gelu_forward(x)
+    assert torch.equal(packed[:n], cs.q8_compress(x)[:n])
+    dx, again = cs.gelu_backward(y, packed, recompute=True)
+    start = (n - 5000 + 127) // 128 * 128  # a tail that begins with a group stands for itself
+    tail = x[start:].clone()
+    y1, p1 = cs.gelu_forward(tail)
+    d1, a1 = cs.gelu_backward(y1, p1, recompute=True)
+    assert torch.equal(y[start:], y1) and torch.equal(packed[start:n], p1[:n - start])
+    assert torch.equal(dx[start:], d1) and torch.equal(again[start:], a1)
+    assert torch.equal(cs.q8_decompress(packed, n, dtype=torch.bfloat16)[start:],
+                       cs.q8_decompress(p1, n - start, dtype=torch.bfloat16))
+    del packed, dx, again
+    rows = n // 1000
+    x2 = x[:rows * 1000].view(rows, 1000)
+    x2[-7:] = normal(7, 1000, seed=5, kind=torch.bfloat16)
+    z, _, mean, rstd = cs.layer_norm_forward(x2)
+    z1, _, m1, r1 = cs.layer_norm_forward(x2[-7:].clone())
+    assert torch.equal(z[-7:], z1) and torch.equal(mean[-7:], m1) and torch.equal(rstd[-7:], r1)
+    g, _, _ = cs.layer_norm_backward(x2, x2, mean, rstd)
+    assert torch.equal(g[-7:], cs.layer_norm_backward(x2[-7:].clone(), x2[-7:].clone(), m1, r1)[0])
+    del z, g, y
+    far = (1 << 31) - 8192  # between two batch entries: more than 2^32 bytes
+    t = normal(2, 2, 100, 32, seed=3, kind=torch.bfloat16)
+    apart = torch.as_strided(x, (2, 2, 100, 32), (far, 3200, 32, 1))
+    apart.copy_(t)
+    want, got = cs.attention_forward(t, t, t), cs.attention_forward(apart, apart, apart)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in zip(cs.attention_backward(apart, apart, apart, apart, *got), cs.attention_backward(t, t, t, t, *want)):
+        assert torch.equal(a, b)

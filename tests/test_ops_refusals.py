@@ -102,10 +102,14 @@ def test_attention_arguments(L, mem):
                 dict(batch=65535, heads=65534, q_len=1 << 30)):
         assert forward(shape(**bad)) == ARG, bad
     assert forward(None) == ARG
-    for bad in (operand(data=None), operand(data=mem + 8), operand(b=4), operand(h=9), operand(t=-16), None):
+    for bad in (operand(data=None), operand(data=mem + 8), operand(b=4), operand(h=9), operand(t=-16), operand(h=0), operand(t=0),
+                None):
         for place in ("q", "k", "v", "out"):
-            assert forward(shape(), **{place: bad}) == ARG
+            assert forward(shape(batch=2), **{place: bad}) == ARG
     assert forward(shape(), lse=None) == ARG
+    # the stride of an axis of one step is not looked at: one token of one head, refused for its missing lse
+    assert forward(shape(heads=1, kv_heads=1, q_len=1, k_len=1), *[operand(b=0, h=0, t=0)] * 4, lse=None) == ARG
+    assert forward(shape(q_len=(1 << 29) + 1)) == ARG
     empty = operand(data=None, b=0, h=0, t=0)
     assert forward(shape(q_len=0), q=empty, out=empty, lse=None) == 0
     size = C.c_size_t()
