@@ -7,7 +7,10 @@
 // or an infinity has a NaN for its scale and stands for NaNs, so that a step that has diverged shows.
 //
 // What bounds these kernels: HBM.  A warp holds a group, four values a lane, so that the largest magnitude is one
-// redux.sync over the bit patterns (whose order is that of the magnitudes, infinities and NaN above all numbers).
+// redux.sync over the bit patterns (whose order is that of the magnitudes, infinities and NaN above all numbers), and a
+// warp's codes are one 128-byte line.  50331648 float32 values, cold: compressed in 47 us (5.3 TB/s of the 253 MB read and
+// written), back in 39 (6.5); GELU with the checkpoint 76 us (6.0), its backward pass with the activation again 113 (5.8);
+// 6.5 TB/s is what a plain copy reaches.
 #include <cuda_runtime.h>
 
 #include "../../include/cswap_b200.h"
@@ -189,7 +192,8 @@ unsigned blocks_for(uint64_t n, int per_warp) {
 }
 float* scales_of(void* packed, uint64_t n) { return reinterpret_cast<float*>((char*)packed + q8_scales_at(n)); }
 
-// Four groups a warp keep four loads in flight; below that many values a warp takes one, to spread over the SMs.
+// Four groups a warp keep four loads in flight; below that many values a warp takes one, to spread over the SMs
+// (59136 bfloat16 values: 462 warps, where four groups a warp would leave 33 of 148 SMs with any).
 constexpr uint64_t kSpread = 1 << 20;
 
 template <class T, bool kGelu>
