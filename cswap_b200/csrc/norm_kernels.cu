@@ -5,10 +5,11 @@
 //   dx = rstd (g - sum g / c - h sum(g h) / c) with g = dy w;  dw = sum over rows of dy h,  db = sum over rows of dy
 //
 // What bounds it: HBM, and for rows of thousands of values the latency of their sums.  A row is read once and held in
-// registers by the threads that share it, eight values each (a warp up to 256 values, 1024 threads up to 8192), so that
-// the variance is summed from the centred values, a second time over registers and not over memory.  With few values a
-// thread many CTAs share an SM, and one's loads run under another's sums (4099 x 1001 bfloat16, both ways: 35 us with
-// eight values a thread, 75 with a warp for a whole row).  Longer rows are read again, from L1 or L2.
+// registers by the threads that share it, eight values each (2 of a warp's threads up to 16 values, 1024 up to 8192), so
+// that the variance is summed from the centred values, a second time over registers and not over memory.  With few values
+// a thread many rows share an SM, and one's loads run under another's sums (4099 x 1001 bfloat16, both ways: 33 us with
+// eight values a thread, 75 with a warp for a whole row; 8 float16 columns 130 us for 67 million values, 2150 with a warp
+// a row).  Longer rows are read again, from L1 or L2.
 //
 // Backward, each thread keeps the sums of dw and db of its own columns over all rows that its CTA takes; they go to
 // memory once per CTA, in a fixed order, and a second launch adds them up.  No atomics: the same call gives the same bits.
@@ -41,20 +42,22 @@ __device__ __forceinline__ void param_to(void* p, int type, uint64_t i, float v)
   else if (type == CSW_TYPE_F16) static_cast<__half*>(p)[i] = narrow<__half>(v);
   else static_cast<__nv_bfloat16*>(p)[i] = narrow<__nv_bfloat16>(v);
 }
-// Sums over the THREADS threads that share a row (a warp, or the whole CTA) of N pairs of values; all of them get them.  A
+template <int THREADS>
+constexpr int kPlaces = THREADS < 32 ? 1 : THREADS / 32;
+// Sums over the THREADS threads that share a row (a part of a warp, a warp, or the whole CTA) of N pairs of values; all of them get them.  A
 // CTA's sums take turns with two places in shared memory (`turn`), so that one barrier a sum is enough: a place is written
 // again two sums later, behind a barrier that all who read it have passed.
 template <int THREADS, int N>
-__device__ __forceinline__ void row_sums(float2 (&v)[N], float2 (*shared)[THREADS / 32], int turn) {
+__device__ __forceinline__ void row_sums(float2 (&v)[N], float2 (*shared)[kPlaces<THREADS>], int turn) {
 #pragma unroll
-  for (int d = 16; d; d /= 2)
+  for (int d = THREADS < 32 ? THREADS / 2 : 16; d; d /= 2)
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       v[n].x += __shfl_xor_sync(0xffffffffu, v[n].x, d);
       v[n].y += __shfl_xor_sync(0xffffffffu, v[n].y, d);
     }
   if (THREADS > 32) {
-    float2(*place)[THREADS / 32] = shared + (turn & 1) * N;
+    float2(*place)[kPlaces<THREADS>] = shared + (turn & 1) * N;
 #pragma unroll
     for (int n = 0; n < N; ++n)
       if (threadIdx.x % 32 == 0) place[n][threadIdx.x / 32] = v[n];
@@ -68,7 +71,7 @@ __device__ __forceinline__ void row_sums(float2 (&v)[N], float2 (*shared)[THREAD
   }
 }
 template <int THREADS>
-__device__ __forceinline__ float row_sum(float v, float2 (*shared)[THREADS / 32], int turn) {
+__device__ __forceinline__ float row_sum(float v, float2 (*shared)[kPlaces<THREADS>], int turn) {
   float2 s[1] = {make_float2(v, 0.0f)};
   row_sums<THREADS>(s, shared, turn);
   return s[0].x;
@@ -116,7 +119,7 @@ struct Raw {
 // shift: then the columns of a thread stay the same, with their weights and their sums in registers.
 template <class T, int VEC, int ITER, int THREADS, bool SHIFTED>
 struct Rows {
-  static constexpr int kBlock = THREADS == 32 ? 128 : THREADS, kTogether = kBlock / THREADS;
+  static constexpr int kBlock = THREADS <= 32 ? 128 : THREADS, kTogether = kBlock / THREADS;
   // CTAs an SM should have room for: 64 registers a thread forward, 80 or more backward
   static constexpr int kForward = 1024 / kBlock, kBackward = kBlock > 768 ? 1 : 768 / kBlock;
   // Rows at once, backward, where a CTA has an SM to itself: a row waits for its sums' way through shuffles and shared
@@ -132,6 +135,11 @@ struct Rows {
     row = ((uint64_t)blockIdx.x / period * kTogether + threadIdx.x / THREADS) * period + kind;
     step = (uint64_t)(gridDim.x / period) * kTogether * period;
     first = (int)(threadIdx.x % THREADS) * VEC - (SHIFTED ? (int)(kind * (uint64_t)cols % VEC) : 0);
+  }
+  // steps of the warp's first row's thread, which has the most
+  __device__ uint64_t rounds() const {
+    const uint64_t lead = __shfl_sync(0xffffffffu, row, 0);
+    return lead < rows ? (rows - lead + step - 1) / step : 0;
   }
   __device__ int column(int k) const { return first + k * THREADS * VEC; }
   __device__ bool any(int c) const { return (!SHIFTED || c > -VEC) && c < (int)cols; }
@@ -180,7 +188,7 @@ template <class T, class P, int VEC, int ITER, int THREADS, bool SHIFTED>
 __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
                                   Rows<T, VEC, ITER, THREADS, SHIFTED>::kForward)
     norm_forward_kernel(const NormForward a, uint32_t period) {
-  __shared__ float2 shared[2][THREADS / 32];
+  __shared__ float2 shared[2][kPlaces<THREADS>];
   const T* x = static_cast<const T*>(a.x);
   const T* residual = static_cast<const T*>(a.residual);
   pdl_wait(x);
@@ -189,33 +197,50 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
   T* sum = static_cast<T*>(a.sum);
   T* y = static_cast<T*>(a.y);
   const float inv = 1.0f / (float)at.cols;
-  Raw<P, VEC> w[ITER], b[ITER];
-  at.params(a.weight, 1.0f, w);
-  at.params(a.bias, 0.0f, b);
-  int turn = 0;
-#pragma unroll 1
-  for (uint64_t row = at.row; row < at.rows; row += at.step) {
+  struct Held {
+    Raw<T, VEC> x[ITER], r[ITER];
+  };
+  auto load = [&](uint64_t row, Held& h) {
     const uint64_t base = row * at.cols;
-    Raw<T, VEC> px[ITER], pr[ITER];
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int c = at.column(k);
       if (at.any(c)) {
-        at.load(x, base, c, px[k]);
-        if (residual) at.load(residual, base, c, pr[k]);
+        at.load(x, base, c, h.x[k]);
+        if (residual) at.load(residual, base, c, h.r[k]);
       }
     }
+  };
+  // The next row's values are on their way while a row is worked on, where registers allow it (768 columns: 77 us for
+  // 67 million float16 values, 99 otherwise; but 88 us for half as many of float32, 59 otherwise).
+  constexpr bool kAhead = sizeof(T) == 2;
+  Held now, next;
+  if (kAhead && at.row < at.rows) load(at.row, next);
+  Raw<P, VEC> w[ITER], b[ITER];
+  at.params(a.weight, 1.0f, w);
+  at.params(a.bias, 0.0f, b);
+  int turn = 0;
+  // Where parts of a warp have rows of their own, all of them go on until the last is done: its sums need every lane.
+  const uint64_t rounds = THREADS < 32 ? at.rounds() : 0;
+  uint64_t row = at.row;
+#pragma unroll 1
+  for (uint64_t i = 0; THREADS < 32 ? i < rounds : row < at.rows; ++i, row += at.step) {
+    const bool mine = THREADS >= 32 || row < at.rows;
+    const uint64_t base = row * at.cols;
+    if (kAhead) now = next;
+    else if (mine) load(row, now);
+    if (kAhead && row + at.step < at.rows) load(row + at.step, next);
     float v[ITER][VEC], s = 0.0f;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int c = at.column(k);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
-      if (at.any(c)) {
+      if (mine && at.any(c)) {
         // what is normed, and what backward reads, is the sum as it is held
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          if (at.has(c + j)) v[k][j] = residual ? widen(narrow<T>(px[k][j] + pr[k][j])) : px[k][j];
+          if (at.has(c + j)) v[k][j] = residual ? widen(narrow<T>(now.x[k][j] + now.r[k][j])) : now.x[k][j];
         if (residual) at.store(sum, base, c, v[k]);
       }
 #pragma unroll
@@ -226,7 +251,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int c = at.column(k);
-      if (at.any(c)) {
+      if (mine && at.any(c)) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           if (at.has(c + j)) v[k][j] -= mean;
@@ -235,11 +260,11 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
       }
     }
     const float rstd = 1.0f / sqrtf(row_sum<THREADS>(s, shared, turn++) * inv + a.eps);
-    if (threadIdx.x % THREADS == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+    if (mine && threadIdx.x % THREADS == 0) a.mean[row] = mean, a.rstd[row] = rstd;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int c = at.column(k);
-      if (at.any(c)) {
+      if (mine && at.any(c)) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[k][j] = v[k][j] * rstd * w[k][j] + b[k][j];
         at.store(y, base, c, v[k]);
@@ -248,9 +273,9 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
   }
 }
 
-// Long rows: read three times, one value a thread and step.
+// Long rows: read three times, a pack of VEC values a thread and step.
 constexpr int kLongThreads = 512;
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const NormForward a) {
   __shared__ float2 shared[2][kLongThreads / 32];
   pdl_wait();
@@ -259,29 +284,41 @@ __global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const N
   const T* residual = a.residual ? static_cast<const T*>(a.residual) + base : nullptr;
   T* sum = residual ? static_cast<T*>(a.sum) + base : nullptr;
   float s = 0.0f;
-  for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
-    float v = widen(x[c]);
+  for (uint64_t c = threadIdx.x * VEC; c < a.cols; c += kLongThreads * VEC) {
+    float v[VEC];
+    load_pack(x + c, v);
     if (residual) {
-      const T held = narrow<T>(v + widen(residual[c]));
-      sum[c] = held;
-      v = widen(held);
+      float r[VEC];
+      load_pack(residual + c, r);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = widen(narrow<T>(v[j] + r[j]));
+      store_pack(sum + c, v);
     }
-    s += v;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += v[j];
   }
   const T* src = residual ? sum : x;  // a thread reads back what it wrote itself
   const float mean = row_sum<kLongThreads>(s, shared, 0) / (float)a.cols;
   s = 0.0f;
-  for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
-    const float v = widen(src[c]) - mean;
-    s += v * v;
+  for (uint64_t c = threadIdx.x * VEC; c < a.cols; c += kLongThreads * VEC) {
+    float v[VEC];
+    load_pack(src + c, v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += (v[j] - mean) * (v[j] - mean);
   }
   const float rstd = 1.0f / sqrtf(row_sum<kLongThreads>(s, shared, 1) / (float)a.cols + a.eps);
   if (threadIdx.x == 0) a.mean[blockIdx.x] = mean, a.rstd[blockIdx.x] = rstd;
   T* y = static_cast<T*>(a.y) + base;
-  for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
-    const float w = a.weight ? param_at(a.weight, a.param_type, c) : 1.0f;
-    const float b = a.bias ? param_at(a.bias, a.param_type, c) : 0.0f;
-    y[c] = narrow<T>((widen(src[c]) - mean) * rstd * w + b);
+  for (uint64_t c = threadIdx.x * VEC; c < a.cols; c += kLongThreads * VEC) {
+    float v[VEC];
+    load_pack(src + c, v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float w = a.weight ? param_at(a.weight, a.param_type, c + j) : 1.0f;
+      const float b = a.bias ? param_at(a.bias, a.param_type, c + j) : 0.0f;
+      v[j] = (v[j] - mean) * rstd * w + b;
+    }
+    store_pack(y + c, v);
   }
 }
 
@@ -294,7 +331,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
     norm_backward_kernel(const NormBackward a, uint32_t period) {
   using R = Rows<T, VEC, ITER, THREADS, SHIFTED>;
   constexpr int N = R::kAtOnce;
-  __shared__ float2 shared[2 * N][THREADS / 32];
+  __shared__ float2 shared[2 * N][kPlaces<THREADS>];
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   pdl_wait(x);
@@ -329,8 +366,10 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
   Raw<P, VEC> w[ITER];
   at.params(a.weight, 1.0f, w);
   int turn = 0;
+  const uint64_t rounds = THREADS < 32 ? at.rounds() : 0;  // as forward
+  uint64_t row = at.row;
 #pragma unroll 1
-  for (uint64_t row = at.row; row < at.rows; row += N * at.step) {
+  for (uint64_t i = 0; THREADS < 32 ? i < rounds : row < at.rows; i += N, row += N * at.step) {
     float2 sums[N];
     // normed values and dy of a pair of columns; a masked value is another row's, 0 in its place adds nothing
     auto pair = [&](const auto& raw, int j) { return Pair{raw[j], VEC > 1 ? raw[j + 1] : 0.0f}; };
@@ -349,7 +388,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
       const uint64_t then = row + (N + n) * at.step;
       if (then < at.rows) load(then, next[n]);
       Pair sg = both(0.0f), sgh = both(0.0f);
-      if (n == 0 || row + n * at.step < at.rows) {
+      if ((THREADS >= 32 && n == 0) || row + n * at.step < at.rows) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
           if (at.any(at.column(k))) {
@@ -371,7 +410,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
     row_sums<THREADS>(sums, shared, turn++);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      if (n > 0 && row + n * at.step >= at.rows) break;
+      if ((THREADS < 32 || n > 0) && row + n * at.step >= at.rows) break;
       // (g w - m0 - h m1) rstd
       const float d = now[n].rstd;
       const Pair m0 = both(-sums[n].x * inv * d), m1 = both(-sums[n].y * inv * d);
@@ -396,18 +435,29 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
   if (!a.dweight && !a.dbias) return;
   float* part = a.workspace + (uint64_t)blockIdx.x * 2 * a.cols;
   if (R::kTogether > 1) {
-    // the warps' sums, added in the order of the warps
-    constexpr int kMany = R::kTogether > 1 ? 32 * ITER * VEC : 1;
-    __shared__ float together[2][kMany];
-    for (int w = 0; w < R::kTogether; ++w) {
-      if (threadIdx.x / THREADS == w) {
+    // the sums of a warp's rows, then those of the four warps, in their order
+#pragma unroll
+    for (int d = THREADS < 32 ? THREADS : 32; d < 32; d *= 2)
+#pragma unroll
+      for (int k = 0; k < ITER; ++k)
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          auto other = [&](const Pair& p) { return Pair{__shfl_xor_sync(~0u, p.x, d), __shfl_xor_sync(~0u, p.y, d)}; };
+          dw[k][j] = add2(dw[k][j], other(dw[k][j]));
+          db[k][j] = add2(db[k][j], other(db[k][j]));
+        }
+    constexpr int kLanes = THREADS < 32 ? THREADS : 32, kMany = kLanes * ITER * VEC, kWarps = R::kBlock / 32;
+    __shared__ float together[2][R::kTogether > 1 ? kMany : 1];
+    for (int w = 0; w < kWarps; ++w) {
+      if (threadIdx.x / 32 == w && threadIdx.x % 32 < kLanes) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const int i = ((k * VEC + j) * 32 + threadIdx.x % 32) % kMany, c = at.column(k) + j;
-            const float pw = one(dw[k][j / 2], j) + (w ? together[0][i] : 0.0f), pb = one(db[k][j / 2], j) + (w ? together[1][i] : 0.0f);
-            if (w < R::kTogether - 1) {
+            const int i = ((k * VEC + j) * kLanes + threadIdx.x % kLanes) % kMany, c = at.column(k) + j;
+            const float pw = one(dw[k][j / 2], j) + (w ? together[0][i] : 0.0f);
+            const float pb = one(db[k][j / 2], j) + (w ? together[1][i] : 0.0f);
+            if (w < kWarps - 1) {
               together[0][i] = pw, together[1][i] = pb;
             } else if (c >= 0 && c < (int)at.cols) {
               part[c] = pw, part[a.cols + c] = pb;
@@ -428,7 +478,7 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
 }
 
 // Long rows: dx of one row a CTA, read twice ...
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const NormBackward a) {
   __shared__ float2 shared[2][kLongThreads / 32];
   pdl_wait();
@@ -436,36 +486,53 @@ __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const 
   const T* x = static_cast<const T*>(a.x) + base;
   const T* dy = static_cast<const T*>(a.dy) + base;
   const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x], inv = 1.0f / (float)a.cols;
+  auto values = [&](uint64_t c, float (&h)[VEC], float (&g)[VEC]) {
+    load_pack(x + c, h);
+    load_pack(dy + c, g);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      h[j] = (h[j] - mean) * rstd;
+      if (a.weight) g[j] *= param_at(a.weight, a.param_type, c + j);
+    }
+  };
   float sg = 0.0f, sgh = 0.0f;
-  for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
-    const float g = widen(dy[c]) * (a.weight ? param_at(a.weight, a.param_type, c) : 1.0f);
-    sg += g;
-    sgh += g * ((widen(x[c]) - mean) * rstd);
+  for (uint64_t c = threadIdx.x * VEC; c < a.cols; c += kLongThreads * VEC) {
+    float h[VEC], g[VEC];
+    values(c, h, g);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sg += g[j], sgh += g[j] * h[j];
   }
   float2 sums[1] = {make_float2(sg, sgh)};
   row_sums<kLongThreads>(sums, shared, 0);
-  const float2 s = sums[0];
   T* dx = static_cast<T*>(a.dx) + base;
-  for (uint64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
-    const float g = widen(dy[c]) * (a.weight ? param_at(a.weight, a.param_type, c) : 1.0f);
-    dx[c] = narrow<T>((g - s.x * inv - (widen(x[c]) - mean) * rstd * (s.y * inv)) * rstd);
+  for (uint64_t c = threadIdx.x * VEC; c < a.cols; c += kLongThreads * VEC) {
+    float h[VEC], g[VEC];
+    values(c, h, g);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g[j] = (g[j] - sums[0].x * inv - h[j] * (sums[0].y * inv)) * rstd;
+    store_pack(dx + c, g);
   }
 }
-// ... and the sums of a thread's column over every gridDim.y-th row
-template <class T>
+// ... and the sums of a thread's columns over every parts-th row
+template <class T, int VEC>
 __global__ void __launch_bounds__(128) norm_backward_columns_kernel(const NormBackward a) {
   pdl_wait();
-  const uint64_t parts = gridDim.x / ((a.cols + 127) / 128), part = blockIdx.x % parts;
-  const uint64_t c = blockIdx.x / parts * 128 + threadIdx.x;
+  const uint64_t parts = gridDim.x / ((a.cols + 128 * VEC - 1) / (128 * VEC)), part = blockIdx.x % parts;
+  const uint64_t c = (blockIdx.x / parts * 128 + threadIdx.x) * VEC;
   if (c >= a.cols) return;
-  float dw = 0.0f, db = 0.0f;
+  float dw[VEC] = {}, db[VEC] = {};
+#pragma unroll 4
   for (uint64_t row = part; row < a.rows; row += parts) {
-    const float g = widen(static_cast<const T*>(a.dy)[row * a.cols + c]);
-    dw += g * ((widen(static_cast<const T*>(a.x)[row * a.cols + c]) - a.mean[row]) * a.rstd[row]);
-    db += g;
+    float h[VEC], g[VEC];
+    load_pack(static_cast<const T*>(a.x) + row * a.cols + c, h);
+    load_pack(static_cast<const T*>(a.dy) + row * a.cols + c, g);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[j] += g[j] * ((h[j] - mean) * rstd), db[j] += g[j];
   }
   float* out = a.workspace + part * 2 * a.cols;
-  out[c] = dw, out[a.cols + c] = db;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) out[c + j] = dw[j], out[a.cols + c + j] = db[j];
 }
 
 // The partial sums of all CTAs, 8 columns (a sector of memory) a block, each thread every 128th row; then the rows of
@@ -504,6 +571,10 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restri
 constexpr uint64_t kLongest = 8192;
 constexpr int kHeld = 8;  // values of a row that a thread holds
 
+template <class T>
+bool whole_packs(uint64_t cols) {
+  return cols * sizeof(T) % 16 == 0;
+}
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How a row's packs lie: of 16 bytes where all rows begin on them, shifted where only the first one does.  Else, and in
@@ -525,14 +596,14 @@ uint32_t period_of(int type, uint64_t cols, Packs packs) {
 // threads of a row, the fewest that hold it with the masked values that a shifted one has more
 int threads_of(int type, uint64_t cols, Packs packs) {
   const uint64_t held = cols + (packs == Packs::kShifted ? 16 / (type == CSW_TYPE_F32 ? 4 : 2) - 1 : 0);
-  for (int t : {32, 64, 96, 128, 256, 512})
+  for (int t : {2, 8, 32, 64, 96, 128, 192, 256, 384, 512, 768})
     if (held <= (uint64_t)t * kHeld) return t;
   return 1024;
 }
 
 // CTAs that stay for all their rows, so that weights are read and sums written once each: as many as run at once.
 unsigned blocks_of(uint64_t rows, int threads, uint32_t period, uint64_t on_sm) {
-  const uint64_t together = threads == 32 ? 4 : 1, block = threads == 32 ? 128 : threads;
+  const uint64_t block = threads <= 32 ? 128 : threads, together = block / threads;
   const uint64_t want = (rows + together * period - 1) / (together * period);  // CTAs of each shift
   const uint64_t most = std::max<uint64_t>((uint64_t)sm_count() * std::max<uint64_t>(std::min<uint64_t>(on_sm / block, 8), 1) / period, 1);
   return (unsigned)(std::min(want, most) * period);
@@ -548,18 +619,28 @@ cudaError_t with_kernel(int threads, Packs packs, F&& f) {
   using No = integral_constant<bool, false>;
   using Pack16 = integral_constant<int, V>;
   using Iter16 = integral_constant<int, kHeld / V>;
-  if (packs == Packs::kSingle)
-    return f(integral_constant<int, 1>(), integral_constant<int, kHeld>(), integral_constant<int, 32>(), No());
+  if (packs == Packs::kSingle) {
+    using One = integral_constant<int, 1>;
+    using All = integral_constant<int, kHeld>;
+    return threads == 2   ? f(One(), All(), integral_constant<int, 2>(), No())
+           : threads == 8 ? f(One(), All(), integral_constant<int, 8>(), No())
+                          : f(One(), All(), integral_constant<int, 32>(), No());
+  }
   switch (threads) {
 #define CSW_THREADS(n) \
   case n: return packs == Packs::kWhole ? f(Pack16(), Iter16(), integral_constant<int, n>(), No()) \
                                         : f(Pack16(), Iter16(), integral_constant<int, n>(), Yes());
+    CSW_THREADS(2)
+    CSW_THREADS(8)
     CSW_THREADS(32)
     CSW_THREADS(64)
     CSW_THREADS(96)
     CSW_THREADS(128)
+    CSW_THREADS(192)
     CSW_THREADS(256)
+    CSW_THREADS(384)
     CSW_THREADS(512)
+    CSW_THREADS(768)
     CSW_THREADS(1024)
 #undef CSW_THREADS
     default: return cudaErrorInvalidValue;
@@ -576,7 +657,9 @@ cudaError_t norm_forward_launch(const NormForward& a, cudaStream_t stream) {
     const Packs packs = packs_of(a.type, a.cols, aligned16(a.x) && aligned16(a.y) && aligned16(a.residual) &&
                                                      aligned16(a.sum) && aligned16(a.weight) && aligned16(a.bias));
     if (packs == Packs::kLong) {
-      e = pdl_launch(norm_forward_long_kernel<T>, (unsigned)a.rows, kLongThreads, 0, stream, a);
+      const bool whole = aligned16(a.x) && aligned16(a.y) && aligned16(a.residual) && aligned16(a.sum) && whole_packs<T>(a.cols);
+      e = pdl_launch(whole ? norm_forward_long_kernel<T, 16 / sizeof(T)> : norm_forward_long_kernel<T, 1>, (unsigned)a.rows,
+                     kLongThreads, 0, stream, a);
       return;
     }
     const uint32_t period = period_of(a.type, a.cols, packs);
@@ -620,9 +703,14 @@ cudaError_t norm_backward_launch(const NormBackward& a, cudaStream_t stream) {
       using T = decltype(t);
       const Packs packs = packs_of(a.type, a.cols, aligned);
       if (packs == Packs::kLong) {
-        e = pdl_launch(norm_backward_long_kernel<T>, (unsigned)a.rows, kLongThreads, 0, stream, a);
+        constexpr int V = 16 / sizeof(T);
+        const bool whole = aligned && whole_packs<T>(a.cols);
+        const uint64_t across = 128 * (whole ? V : 1);  // columns of a CTA
+        e = pdl_launch(whole ? norm_backward_long_kernel<T, V> : norm_backward_long_kernel<T, 1>, (unsigned)a.rows,
+                       kLongThreads, 0, stream, a);
         if (e == cudaSuccess && sums)
-          e = pdl_launch(norm_backward_columns_kernel<T>, (unsigned)((a.cols + 127) / 128 * parts), 128, 0, stream, a);
+          e = pdl_launch(whole ? norm_backward_columns_kernel<T, V> : norm_backward_columns_kernel<T, 1>,
+                         (unsigned)((a.cols + across - 1) / across * parts), 128, 0, stream, a);
         return;
       }
       const uint32_t period = period_of(a.type, a.cols, packs);

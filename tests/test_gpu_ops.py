@@ -223,7 +223,7 @@ def test_gelu_linear(cs, bias):
 
 # ---- layer norm --------------------------------------------------------------------------------------------------------
 
-NORM_SHAPES = [(1, 1), (3, 2), (5, 7), (77, 768), (33, 8), (130, 255), (65, 256), (9, 257), (40, 512), (31, 769),
+NORM_SHAPES = [(1, 1), (3, 2), (5, 7), (1001, 8), (70000, 8), (999, 13), (3001, 16), (777, 40), (513, 63), (300, 64), (77, 768), (33, 8), (130, 255), (65, 256), (9, 257), (40, 512), (31, 769),
                (7, 1001), (600, 1024), (6, 1025), (5, 2048), (9, 2051), (3, 4096), (5, 4097), (4, 8192), (3, 10000),
                (3, 8191), (5, 8193), (2, 12001), (2, 16380), (3, 16383), (2, 16384), (37, 1022), (3, 16385), (70, 20000), (1300, 40)]
 
