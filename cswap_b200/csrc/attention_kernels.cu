@@ -31,6 +31,7 @@
 // exponentials, 450 on gradients, the rest on loads, stores and hand-overs).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -586,6 +587,11 @@ struct Backward {
   const float* lse;
   float* rows;
   uint32_t padded;
+  // dkv, where there are fewer tiles of keys than SMs: the tiles of queries are split into `parts`, whose sums (float32, for
+  // each part, key head, key of a whole tile: dv, then dk) a launch of its own adds up
+  int parts;
+  float* sums;
+  uint32_t k_padded;
 };
 
 // Both kernels: 256 threads for the scores (two a row, 64 columns each), 128 that prepare a piece's rows and take its
@@ -965,17 +971,28 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
 }
 
 // Pieces of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
+template <bool SPLIT>
 struct Keys {
   int from, tiles, n;  // the first tile of queries that sees any of them; tiles of queries; pairs in all
-  __device__ Keys(const Shape& s, const Piece& p) {
+  int head, q;         // the first pair's: head, counted from the first that shares, and tile of queries
+  __device__ Keys(const Shape& s, const Piece& p, int parts) {
     // query i sees key j from i = j - (k_len - q_len) on
     from = s.causal ? max(p.first - ((int)s.k_len - (int)s.q_len), 0) / kTile : 0;
     tiles = ((int)s.q_len + kTile - 1) / kTile;
-    n = (p.first < p.keys ? max(tiles - from, 0) : 0) * (int)s.share;
+    const int each = p.first < p.keys ? max(tiles - from, 0) : 0;
+    head = 0, q = from, n = each * (int)s.share;
+    if (SPLIT && n > 0) {
+      const int begin = (int)((int64_t)n * part(p) / parts);
+      n = (int)((int64_t)n * (part(p) + 1) / parts) - begin;
+      head = begin / each, q = from + begin % each;
+    }
   }
+  // Split, the part stands above the key head (which is below 65536).
+  __device__ static int part(const Piece& p) { return p.kv_head >> 16; }
+  __device__ static int kv_head(const Piece& p) { return SPLIT ? p.kv_head & 0xffff : p.kv_head; }
 };
 
-template <class T, int DP>
+template <class T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_kernel(const __grid_constant__ Backward a) {
   using Plan = BackwardPlan<DP>;
   constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
@@ -1019,18 +1036,20 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       __device__ Piece piece(int index) const {
         const int per = a.s.batch * a.s.kv_heads, row = index % per, b = row / a.s.kv_heads, g = row % a.s.kv_heads;
         const int head = g * (int)a.s.share;  // the first of those that share
-        return {index / per * kTile, a.s.keys(b), b, head, g, b * (int)a.s.heads + head};
+        const int tile = SPLIT ? index / per / a.parts : index / per, part = SPLIT ? index / per % a.parts : 0;
+        return {tile * kTile, a.s.keys(b), b, head, part << 16 | g, b * (int)a.s.heads + head};
       }
       __device__ bool copy(const Piece& p) {
-        const Keys at(a.s, p);
+        const Keys<SPLIT> at(a.s, p, a.parts);
+        const int kv_head = at.kv_head(p);
         if (at.n == 0) return true;
         const uint32_t to = tiles_at + u % kStay * 2 * Plan::kTileBytes, here = kv_full + 8 * (u % kStay);
         if (u >= kStay && !bar_wait(kv_empty + 8 * (u % kStay), (u / kStay - 1) & 1)) return false;
         bar_expect(here, 2 * Plan::kTileBytes);
-        copy_tokens<DP>(to, &a.k, here, p.first, p.kv_head, p.batch);
-        copy_tokens<DP>(to + Plan::kTileBytes, &a.v, here, p.first, p.kv_head, p.batch);
+        copy_tokens<DP>(to, &a.k, here, p.first, kv_head, p.batch);
+        copy_tokens<DP>(to + Plan::kTileBytes, &a.v, here, p.first, kv_head, p.batch);
         const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
-        int q = at.from, h = 0;
+        int q = at.q, h = at.head;
         for (int j = 0; j < 2 * at.n; ++j, ++i) {
           const int slot = i % kRing;
           if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
@@ -1060,7 +1079,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
-        const int n = Keys(s, piece).n;
+        const int n = Keys<SPLIT>(s, piece, a.parts).n;
         if (n == 0) continue;
         const uint32_t stay = u % kStay;
         const uint64_t k_rows = stay_rows + stay * 2 * kStep;  // v behind it
@@ -1109,7 +1128,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
-        const bool any = Keys(s, piece).n > 0;
+        const bool any = Keys<SPLIT>(s, piece, a.parts).n > 0;
         if (any) {
           CSW_WAIT_WARP(sums_full, u & 1);
           ++u;
@@ -1117,6 +1136,27 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         }
         // A key behind its sequence has no gradient, whatever its row of the tile held.
         const bool live = any && piece.first + t < piece.keys;
+        if constexpr (SPLIT) {
+          const uint64_t heads = (uint64_t)s.batch * s.kv_heads, head = (uint64_t)piece.batch * s.kv_heads + Keys<SPLIT>::kv_head(piece);
+          float* to = a.sums + ((Keys<SPLIT>::part(piece) * heads + head) * a.k_padded + piece.first + t) * (2 * DP);
+#pragma unroll
+          for (int c = 0; c < 2 * DP; c += 32) {  // dv, then dk, as they lie in tensor memory
+            uint32_t r[32] = {};
+            if (any) {
+              load32(dv_at + c + lanes, r);
+              wait_loads(r);
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(to + c + k) =
+                  live ? make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]) : make_uint4(0, 0, 0, 0);
+          }
+          if (any) {
+            fence_before();
+            bar_arrive(sums_free);
+          }
+          continue;
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {  // dv, dk
           const uint32_t from = (x == 0 ? dv_at : dk_at) + lanes;
@@ -1150,9 +1190,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
-        const Keys at(s, piece);
+        const Keys<SPLIT> at(s, piece, a.parts);
         const int n = at.n, row = piece.first + t, off = (int)s.k_len - (int)s.q_len;
-        int q = at.from;
+        int q = at.q;
         for (int j = 0; j < n; ++j, ++i) {
           const int slot = 2 * i % kRing;
           const uint32_t parity = 2 * i / kRing & 1;
@@ -1219,6 +1259,31 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   leave<Plan::kColumns>(flag, tmem, warp == 13);
 }
 
+// The parts' sums, in their order; a thread for 4 columns of a key's dv or dk.
+template <class T, int DP>
+__global__ void __launch_bounds__(256) attention_sums_kernel(const float* __restrict__ sums, Shape s, int parts,
+                                                             uint32_t k_padded, View dk, View dv) {
+  pdl_wait(sums);
+  constexpr int kEach = 2 * DP / 4;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, at = i / kEach, head = at / s.k_len;
+  const uint32_t key = at % s.k_len, c = i % kEach * 4;
+  if (head >= (uint64_t)s.batch * s.kv_heads || c % DP >= s.dim) return;
+  const float* from = sums + (head * k_padded + key) * (2 * DP) + c;
+  const uint64_t step = (uint64_t)s.batch * s.kv_heads * k_padded * (2 * DP);
+  float f[4] = {};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(from + p * step);
+    f[0] += v.x, f[1] += v.y, f[2] += v.z, f[3] += v.w;
+  }
+  if (c >= DP) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] *= s.scale;
+  }
+  const View& to = c < DP ? dv : dk;
+  store_pack(const_cast<T*>(to.row<T>(head / s.kv_heads, head % s.kv_heads, key)) + c % DP, f);
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------
 Shape shape_of(const csw_attention_shape& s) {
   const float e = fmaxf(fabsf(s.scale) * kLog2e, 0x1p-100f);
@@ -1279,20 +1344,26 @@ cudaError_t forward_of(const Forward& a, const csw_attention_shape& s, cudaStrea
 }
 
 template <class T, int DP>
-cudaError_t backward(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
+cudaError_t backward(const Backward& a, const csw_attention_shape& s, const View& dk, const View& dv, cudaStream_t stream) {
   using Plan = BackwardPlan<DP>;
   cudaError_t e = cudaSuccess;
   if (s.q_len)
     e = run(attention_dq_kernel<T, DP>, (s.q_len + kTile - 1) / kTile * s.batch * s.heads, Plan::kThreads, Plan::kShared,
             stream, a);
   if (e == cudaSuccess && s.k_len)
-    e = run(attention_dkv_kernel<T, DP>, (s.k_len + kTile - 1) / kTile * s.batch * s.kv_heads, Plan::kThreads,
+    e = run(a.parts > 1 ? attention_dkv_kernel<T, DP, true> : attention_dkv_kernel<T, DP, false>, (s.k_len + kTile - 1) / kTile * s.batch * s.kv_heads * a.parts, Plan::kThreads,
             Plan::kShared, stream, a);
+  if (e == cudaSuccess && a.parts > 1) {
+    const uint64_t threads = (uint64_t)s.batch * s.kv_heads * s.k_len * (2 * DP / 4);
+    e = pdl_launch(attention_sums_kernel<T, DP>, (unsigned)((threads + 255) / 256), 256, 0, stream, (const float*)a.sums,
+                   a.s, a.parts, a.k_padded, dk, dv);
+  }
   return e;
 }
 template <class T>
-cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
-  return s.dim <= 64 ? backward<T, 64>(a, s, stream) : backward<T, 128>(a, s, stream);
+cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, const View& dk, const View& dv,
+                        cudaStream_t stream) {
+  return s.dim <= 64 ? backward<T, 64>(a, s, dk, dv, stream) : backward<T, 128>(a, s, dk, dv, stream);
 }
 
 cudaError_t take_status(int* value) {
@@ -1305,7 +1376,24 @@ const bool registered = (take_kernel_status = take_status, true);
 
 }  // namespace
 
-uint64_t attention_padded(uint64_t q_len) { return (q_len + kTile - 1) / kTile * kTile; }
+namespace {
+uint64_t whole_tiles(uint64_t n) { return (n + kTile - 1) / kTile * kTile; }
+// Parts of dkv's work on a tile of keys: enough for two CTAs an SM where there are fewer tiles than SMs, of two tiles of
+// queries at least.  (1892 causal tokens, 4 heads of 80 on one: 15 tiles of keys, each with up to 60 of queries.)
+int parts_of(const csw_attention_shape& s) {
+  const uint64_t tiles = whole_tiles(s.k_len) / kTile * s.batch * s.kv_heads, sms = sm_count();
+  if (tiles == 0 || tiles >= sms) return 1;
+  const uint64_t most = whole_tiles(s.q_len) / kTile * (s.heads / s.kv_heads) / 2;
+  return (int)std::max<uint64_t>(std::min<uint64_t>({2 * sms / tiles, most, 32}), 1);
+}
+uint64_t row_values(const csw_attention_shape& s) { return 2 * (uint64_t)s.batch * s.heads * whole_tiles(s.q_len); }
+}  // namespace
+
+uint64_t attention_workspace_values(const csw_attention_shape& s) {
+  const int parts = parts_of(s);
+  const uint64_t sums = parts > 1 ? parts * (uint64_t)s.batch * s.kv_heads * whole_tiles(s.k_len) * 2 * (s.dim <= 64 ? 64 : 128) : 0;
+  return row_values(s) + sums;
+}
 
 cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_attention_operand& q,
                                      const csw_attention_operand& k, const csw_attention_operand& v,
@@ -1327,7 +1415,8 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   Backward a;
   a.s = shape_of(s);
   a.o = view_of(b.o), a.grad = view_of(b.dout);
-  a.lse = b.lse, a.rows = b.rows, a.padded = (uint32_t)attention_padded(s.q_len);
+  a.lse = b.lse, a.rows = b.workspace, a.padded = (uint32_t)whole_tiles(s.q_len);
+  a.parts = parts_of(s), a.sums = b.workspace + row_values(s), a.k_padded = (uint32_t)whole_tiles(s.k_len);
   // of an empty side nothing is copied
   a.q = a.k = a.v = a.dout = a.dq = a.dk = a.dv = CUtensorMap{};
   if (s.q_len && (!map_of(&a.q, b.q, s, s.heads, s.q_len) || !map_of(&a.dout, b.dout, s, s.heads, s.q_len) ||
@@ -1336,7 +1425,8 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len) ||
                   !map_of(&a.dk, b.dk, s, s.kv_heads, s.k_len) || !map_of(&a.dv, b.dv, s, s.kv_heads, s.k_len)))
     return cudaErrorInvalidValue;
-  return s.type == CSW_TYPE_F16 ? backward_of<__half>(a, s, stream) : backward_of<__nv_bfloat16>(a, s, stream);
+  const View dk = view_of(b.dk), dv = view_of(b.dv);
+  return s.type == CSW_TYPE_F16 ? backward_of<__half>(a, s, dk, dv, stream) : backward_of<__nv_bfloat16>(a, s, dk, dv, stream);
 }
 
 }  // namespace csw

@@ -15,9 +15,10 @@ cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_att
 struct AttentionBackward {
   csw_attention_operand q, k, v, o, dout, dq, dk, dv;
   const float* lse;
-  float* rows;  // workspace: 2 x batch x heads x attention_padded(q_len)
+  float* workspace;  // attention_workspace_values(s)
 };
-uint64_t attention_padded(uint64_t q_len);
+// float32 values that a backward pass needs on the CURRENT device
+uint64_t attention_workspace_values(const csw_attention_shape& s);
 cudaError_t attention_backward_launch(const csw_attention_shape& s, const AttentionBackward& a, cudaStream_t stream);
 
 }  // namespace csw

@@ -146,7 +146,7 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
 
 csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes) {
   if (!bytes || !attention_args(shape)) return CSW_ERR_ARG;
-  *bytes = 2 * shape->batch * shape->heads * attention_padded(shape->q_len) * sizeof(float);
+  *bytes = attention_workspace_values(*shape) * sizeof(float);
   return CSW_OK;
 }
 

@@ -406,7 +406,8 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
                                  const csw_attention_operand* k, const csw_attention_operand* v,
                                  const csw_attention_operand* o, float* d_lse, csw_stream_t stream);
 /* Backward forms the probabilities again from q, k and d_lse.  Gradients of keys and values are summed over the query
- * heads that share them, in a fixed order.  The workspace (csw_attention_workspace bytes) is 16-byte aligned. */
+ * heads that share them, in a fixed order.  The workspace (csw_attention_workspace bytes, of the
+ * current device) is 16-byte aligned. */
 csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes);
 csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_attention_operand* q,
                                   const csw_attention_operand* k, const csw_attention_operand* v,

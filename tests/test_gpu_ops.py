@@ -451,6 +451,17 @@ def test_attention_many_pieces(cs, kind, dim, causal):
 
 
 @halves
+@pytest.mark.parametrize("heads,kv_heads,ql,kl,dim,causal", [(4, 1, 700, 700, 80, True), (8, 1, 1000, 70, 64, False),
+                                                             (2, 2, 1500, 300, 40, True), (6, 1, 300, 900, 128, True)])
+def test_attention_few_keys_and_many_queries(cs, kind, heads, kv_heads, ql, kl, dim, causal):
+    """Where there are few tiles of keys their queries are split, and the parts' sums added up."""
+    lens = torch.tensor([kl - kl // 3], dtype=torch.int32, device="cuda")
+    ops = operands(kind, 1, heads, kv_heads, ql, kl, dim, seed=ql)
+    check_attention(cs, *ops, causal=causal)
+    check_attention(cs, *ops, causal=causal, lens=lens)
+
+
+@halves
 def test_attention_rows_that_see_nothing(cs, kind):
     """Causal with more queries than keys: the first rows see no key."""
     q, k, v, do = operands(kind, 1, 2, 2, 300, 20, 64, seed=2)
