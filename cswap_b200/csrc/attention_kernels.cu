@@ -13,8 +13,8 @@
 // type, go back to tensor memory over the scores they came from, as the first operand of the second product.  The
 // second operand of that product is the tile that is in shared memory anyway, read across its rows.
 //
-// Three kernels, each with a warp that copies, a warp whose first lane issues the products, and warps for the softmax,
-// a thread a row or half a row:
+// Three kernels, each with a warp that copies, a warp that issues the products, and warps for the softmax, a thread a row
+// or half a row; backward, four more that take the results out:
 //   forward   a tile of queries, over the tiles of keys: s, p, o += p v
 //   dq        the same rows: s, dp = do v, ds, dq += ds k
 //   dkv       a tile of keys, over the tiles of queries of every head that shares them: s and dp transposed,
@@ -95,18 +95,6 @@ __device__ __forceinline__ void give_up(uint32_t* flag) {
   }
 
 template <class T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <class T>
 constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
 
 // 32 columns of an accumulator, times f, to columns [at, at + 32) of row `row` of a tile of 64, swizzled as the tile
@@ -116,10 +104,10 @@ __device__ __forceinline__ void stage_columns(char* tile, int row, int at, const
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     uint4 v;
-    v.x = pack2<T>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
-    v.y = pack2<T>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
-    v.z = pack2<T>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
-    v.w = pack2<T>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
+    v.x = word_of<T>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
+    v.y = word_of<T>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
+    v.z = word_of<T>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
+    v.w = word_of<T>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
     *reinterpret_cast<uint4*>(tile + row * 128 + (((at + i) / 8) ^ (row & 7)) * 16) = v;
   }
 }
@@ -351,7 +339,7 @@ __device__ __forceinline__ void exp_of(Pair (&add)[2], const uint32_t* r, float 
     if (2 * i >= end) x.x = 0.0f;
     if (2 * i + 1 >= end) x.y = 0.0f;
     add[i % 2] = add2(add[i % 2], x);
-    p[i] = pack2<T>(x.x, x.y);
+    p[i] = word_of<T>(x.x, x.y);
   }
   settle(add[0].x, add[0].y, add[1].x, add[1].y);
 }
@@ -635,7 +623,7 @@ __device__ __forceinline__ float to_gradients(const float* p, const uint32_t* dp
     const float x = p[2 * i] * (__uint_as_float(dp[2 * i]) - d[2 * i]);
     const float y = p[2 * i + 1] * (__uint_as_float(dp[2 * i + 1]) - d[2 * i + 1]);
     sum[0] += x, sum[1] += y;
-    out[i] = pack2<T>(x, y);
+    out[i] = word_of<T>(x, y);
   }
   return sum[0] + sum[1];
 }
@@ -937,7 +925,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
             for (int c = 0; c < 2; ++c) {
               uint32_t out[16];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
+              for (int k = 0; k < 16; ++k) out[k] = word_of<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
               store16(s_at + 64 * w + 16 * c + lanes, out);
             }
             wait_stores();
@@ -1223,7 +1211,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           for (int c = 0; c < 2; ++c) {
             uint32_t out[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) out[k] = pack2<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
+            for (int k = 0; k < 16; ++k) out[k] = word_of<T>(p[32 * c + 2 * k], p[32 * c + 2 * k + 1]);
             store16(s_at + 64 * w + 16 * c + lanes, out);
           }
           wait_stores();

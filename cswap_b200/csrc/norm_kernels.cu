@@ -82,12 +82,7 @@ template <class T, int VEC>
 struct Raw {
   static constexpr int kWords = VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4;
   uint32_t w[kWords];
-  __device__ float operator[](int j) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
-    const uint32_t bits = w[j / 2];
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(j % 2 ? bits & 0xffff0000u : bits << 16);
-    return __half2float(__ushort_as_half((unsigned short)(j % 2 ? bits >> 16 : bits & 0xffff)));
-  }
+  __device__ float operator[](int j) const { return value_of<T>(w, j); }
   // one value into its place, which holds zeros
   __device__ void put(int j, T v) {
     if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v);

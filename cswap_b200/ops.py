@@ -228,7 +228,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     8 up to 128, heads a multiple of kv_heads (each key head serves heads / kv_heads consecutive query heads).  Any
     strides will do; tensors whose rows do not lie on 16-byte boundaries are copied first.  `causal`: query i sees the
     keys up to i + k_len - q_len.  `kv_lens` (int32, on the device, one for each batch entry): the number of keys of
-    that entry, taken into 0 ... k_len; keys and values behind it are not used, whatever they hold.  A query that sees
-    no key gives zeros, and no gradient passes through it."""
+    that entry, taken into 0 ... k_len; keys and values behind it are not used, whatever they hold (those that only
+    `causal` hides count with a probability of zero, and must be finite).  A query that sees no key gives zeros, and no
+    gradient passes through it."""
     _ext().check_capture(q, k, v)
     return _Attention.apply(q, k, v, causal, kv_lens, scale)
