@@ -3,6 +3,7 @@
 // 3 us on the GPU.
 #include "ext_util.h"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/function.h>
@@ -51,6 +52,13 @@ bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
 void* ptr(const at::Tensor& t) { return t.numel() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
 void* out(at::Tensor& t) { return t.numel() ? t.mutable_data_ptr() : nullptr; }
 
+// New tensors on a tensor's device, without the way through torch's dispatcher: the smallest calls are as long as their
+// allocations.
+at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+at::Tensor fresh(const at::Tensor& like) { return fresh(like, like.sizes(), like.scalar_type()); }
+
 // A new tuple of the tensors; an undefined one becomes None
 PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
   PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
@@ -73,7 +81,7 @@ bool packed_out(PyObject* o, const at::Tensor& like, size_t n, at::Tensor* packe
   size_t need;
   if (!q8_bytes(n, &need)) return false;
   if (o == Py_None) {
-    *packed = new_on(like, (int64_t)need, at::kByte);
+    *packed = fresh(like, {(int64_t)need}, at::kByte);
     return true;
   }
   const at::Tensor* t = as_tensor(o, "out");
@@ -137,7 +145,7 @@ PyObject* q8_decompress(PyObject*, PyObject* const* a, Py_ssize_t n) {
         status_ok(CSW_ERR_SIZE, "csw_q8_decompress");
         return nullptr;
       }
-      dst = new_on(*packed, (int64_t)numel, kind);
+      dst = fresh(*packed, {(int64_t)numel}, kind);
     } else {
       const at::Tensor* o = as_tensor(a[3], "out");
       if (!o || !same_device(*o, *packed, "out") || !require_flat(*o, "out")) return nullptr;
@@ -168,7 +176,7 @@ PyObject* gelu_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!x || !require_values(*x, "x", &type) || !require_flat(*x, "x") ||
         !packed_out(Py_None, *x, x->numel(), &packed))
       return nullptr;
-    at::Tensor y = at::empty(x->sizes(), x->options());
+    at::Tensor y = fresh(*x);
     const void* src = ptr(*x);
     void *dst = out(y), *codes = out(packed);
     if (!launch(*x, "csw_gelu_forward", [&](csw_stream_t s) {
@@ -191,8 +199,8 @@ PyObject* gelu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     const int recompute = PyObject_IsTrue(a[2]);
     if (recompute < 0) return nullptr;
-    at::Tensor dx = at::empty(dy->sizes(), dy->options()), y;
-    if (recompute) y = at::empty(dy->sizes(), dy->options());
+    at::Tensor dx = fresh(*dy), y;
+    if (recompute) y = fresh(*dy);
     const void *src = ptr(*dy), *codes = ptr(*packed);
     void *dst = out(dx), *again = recompute ? out(y) : nullptr;
     if (!launch(*dy, "csw_gelu_backward", [&](csw_stream_t s) {
@@ -244,9 +252,9 @@ PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       value_error("eps must not be negative");
       return nullptr;
     }
-    at::Tensor y = at::empty(x->sizes(), x->options()), sum = *x;
-    if (residual) sum = at::empty(x->sizes(), x->options());
-    at::Tensor mean = new_on(*x, rows, at::kFloat), rstd = new_on(*x, rows, at::kFloat);
+    at::Tensor y = fresh(*x), sum = *x;
+    if (residual) sum = fresh(*x);
+    at::Tensor mean = fresh(*x, {rows}, at::kFloat), rstd = fresh(*x, {rows}, at::kFloat);
     const void *src = ptr(*x), *r = residual ? ptr(*residual) : nullptr, *w = weight ? ptr(*weight) : nullptr,
                *b = bias ? ptr(*bias) : nullptr;
     void *to = out(y), *held = residual ? out(sum) : nullptr;
@@ -276,15 +284,15 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     const int wanted = PyObject_IsTrue(a[5]);
     if (wanted < 0) return nullptr;
-    at::Tensor dx = at::empty(x->sizes(), x->options()), dw, db, space;
+    at::Tensor dx = fresh(*x), dw, db, space;
     void *pw = nullptr, *pb = nullptr, *ws = nullptr;
     size_t need = 0;
     if (weight && wanted) {
       const c10::cuda::CUDAGuard on(x->device());  // the size goes by the device's SMs
       if (!status_ok(csw_layer_norm_workspace(rows, cols, &need), "csw_layer_norm_workspace")) return nullptr;
-      dw = at::empty(weight->sizes(), weight->options());
-      db = at::empty(weight->sizes(), weight->options());
-      space = new_on(*x, (int64_t)need, at::kByte);
+      dw = fresh(*weight);
+      db = fresh(*weight);
+      space = fresh(*x, {(int64_t)need}, at::kByte);
       pw = out(dw), pb = out(db), ws = out(space);
     }
     const void *g = ptr(*dy), *src = ptr(*x), *w = weight ? ptr(*weight) : nullptr;
@@ -323,8 +331,8 @@ Operand operand_of(const at::Tensor& given) {
 // A new tensor of like's shape, its tokens in front of its heads where they lie so in `like`
 Operand new_operand(const at::Tensor& like) {
   const bool tokens_first = like.size(1) > 1 && like.size(2) > 1 && like.stride(1) < like.stride(2);
-  at::Tensor t = tokens_first ? at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2)
-                              : at::empty(like.sizes(), like.options());
+  at::Tensor t = tokens_first ? fresh(like, {like.size(0), like.size(2), like.size(1), like.size(3)}, like.scalar_type()).transpose(1, 2)
+                              : fresh(like);
   return operand_of(t);
 }
 
@@ -380,7 +388,7 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arg_count(n, 6) || !attention_of(a, &f)) return nullptr;
     const c10::cuda::CUDAGuard on(f.q->device());
     const Operand q = operand_of(*f.q), k = operand_of(*f.k), v = operand_of(*f.v), o = new_operand(*f.q);
-    at::Tensor lse = at::empty({f.q->size(0), f.q->size(1), f.q->size(2)}, f.q->options().dtype(at::kFloat));
+    at::Tensor lse = fresh(*f.q, {f.q->size(0), f.q->size(1), f.q->size(2)}, at::kFloat);
     float* l = static_cast<float*>(out(lse));
     if (!launch(*f.q, "csw_attention_forward", [&](csw_stream_t s) {
           return csw_attention_forward(&f.s, &q.o, &k.o, &v.o, &o.o, l, s);
@@ -412,7 +420,7 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!status_ok(csw_attention_workspace(&f.s, &need), "csw_attention_workspace")) return nullptr;
     const Operand q = operand_of(*f.q), k = operand_of(*f.k), v = operand_of(*f.v), o = operand_of(*given),
                   d = operand_of(*dout), dq = new_operand(*f.q), dk = new_operand(*f.k), dv = new_operand(*f.v);
-    at::Tensor space = new_on(*f.q, (int64_t)need, at::kByte);
+    at::Tensor space = fresh(*f.q, {(int64_t)need}, at::kByte);
     const float* l = static_cast<const float*>(ptr(*lse));
     void* ws = out(space);
     if (!launch(*f.q, "csw_attention_backward", [&](csw_stream_t s) {
