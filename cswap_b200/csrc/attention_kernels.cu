@@ -25,10 +25,10 @@
 // What bounds it.  For 128 x 128 scores the tensor cores take 256 clocks a product with heads of 64 and 512 with heads of
 // 128, the exponentials 1024 (16 a clock and SM; a quarter of them go by polynomial instead), and the rest of the
 // softmax's instructions about as long again.  Heads of 128, 4096 causal tokens, 32 heads on 8: forward 120 us
-// (1145 TFLOP/s of the pairs that the mask leaves; a large library product reaches 1634), dq 196, dkv 216, where the
-// tensor cores are busy 65 % of the time.  Heads of 64, 32 sentences of 128 to 512 tokens, 12 heads: forward 44 us, dq 66,
-// dkv 60: some 2400 clocks a tile of backward, which the softmax warps spend one phase after the other (1250 on
-// exponentials, 450 on gradients, the rest on loads, stores and hand-overs).
+// (1145 TFLOP/s of the pairs that the mask leaves; a large library product reaches 1634), dq 196, dkv 216; the tensor
+// cores are busy 59, 53 and 70 % of the time.  Heads of 64, 32 sentences of 128 to 512 tokens, 12 heads: forward 44 us,
+// dq 66, dkv 60 (24, 24 and 33 % busy): some 2400 clocks a tile of backward, which the softmax warps spend one phase
+// after the other (1250 on exponentials, 450 on gradients, the rest on loads, stores and hand-overs).
 #include <cuda_runtime.h>
 
 #include <algorithm>
