@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "attention_kernels.h"
+#include "hand_over.cuh"
 #include "internal.h"
 #include "pdl.cuh"
 #include "tensor_core.cuh"
@@ -650,21 +651,23 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[4 + 2 * kStay + 2 * kRing + 4];
+  __shared__ uint64_t bars[6 + 2 * kStay + 2 * kRing + 4];
   __shared__ float shifts[2][kTile], deltas[2][kTile];  // of this piece and the next
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
-  const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, rows_ready = dq_full + 16, left_ready = dq_full + 24,
-                 q_full = dq_full + 32, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
+  const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, q_full = dq_full + 48, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
                  s_full = empty + 8 * kRing, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8;
+  // The next piece's rows are ready before the softmax warps have to have looked at this one's, and their sums may be
+  // ready before this one's are looked at.
+  const Turns rows_ready{dq_full + 16}, left_ready{dq_full + 32};
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
     work_bars.init(Plan::kListeners);
     bar_init(dq_full, 1), bar_init(dq_free, 128);
     for (int i = 0; i < kStay; ++i) bar_init(q_full + 8 * i, 1), bar_init(q_empty + 8 * i, 1);
-    bar_init(rows_ready, 128), bar_init(left_ready, 256);
+    for (int i = 0; i < 2; ++i) bar_init(rows_ready.bar(i), 128), bar_init(left_ready.bar(i), 256);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
     init_visible();
@@ -810,14 +813,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       shifts[u & 1][t] = shift;
       group_sync(2, 128);
       delta = deltas[u & 1][t];
-      bar_arrive(rows_ready);
+      bar_arrive(rows_ready.bar(u));
     };
     // The results of a piece that sees n tiles, and its row's exponent shift and D; false where a wait ran out.
     auto finish = [&](const Piece& p, int n, int u, float shift, float d) -> bool {
       const bool live = shift != INFINITY;
       float off = 0.0f;
       if (n > 0) {
-        if (!__all_sync(0xffffffffu, bar_wait(left_ready, u & 1) && bar_wait(dq_full, u & 1))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(left_ready.bar(u), left_ready.parity(u)) && bar_wait(dq_full, u & 1))) return false;
         fence_after();
         off = live ? shifts[u & 1][t] + deltas[u & 1][t] : 0.0f;
       }
@@ -891,7 +894,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const int keys = piece.keys, n = Queries<1>(s, piece).most, row = piece.first + t;
         if (n == 0) continue;
         const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
-        CSW_WAIT_WARP(rows_ready, u & 1);
+        CSW_WAIT_WARP(rows_ready.bar(u), rows_ready.parity(u));
         const float shift = shifts[u & 1][t], d = deltas[u & 1][t];
         group_sync(3, 256);  // both halves have read: the places are written below
         const bool few = n <= kFewTiles;
@@ -950,7 +953,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           bar_arrive(ds_ready);
         }
         (w == 0 ? shifts : deltas)[u & 1][t] = left;
-        bar_arrive(left_ready);
+        bar_arrive(left_ready.bar(u));
         ++u;
       }
     }();
