@@ -239,16 +239,15 @@ __device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_
   }
 }
 
-// A tile of 64 columns that `threads` threads have staged goes to memory; one of them, `first`, stores.
-__device__ __forceinline__ void stage_free(bool first, int id, int threads) {
+// Tiles of 64 columns are staged by a group of warps, of which one thread, `first`, stores them.  Both are false where a
+// wait ran out.
+__device__ __forceinline__ bool stage_free(bool first, Meeting& group) {
   if (first) stores_read();
-  group_sync(id, threads);
+  return group();
 }
-__device__ __forceinline__ void stage_out(bool first, int id, int threads, const CUtensorMap* map, uint32_t tile, int dim,
-                                          int token, int head, int batch) {
+__device__ __forceinline__ bool stage_full(Meeting& group) {
   async_fence();
-  group_sync(id, threads);
-  if (first) store_tile(map, tile, dim, token, head, batch);
+  return group();
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -383,13 +382,13 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
   using Plan = ForwardPlan<DP, NWG>;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[2 + 2 * Plan::kStages + 4 * NWG];
+  __shared__ uint64_t bars[2 + 2 * Plan::kStages + 5 * NWG];
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
   const uint32_t q_full = smem_at(bars), q_empty = q_full + 8, full = q_full + 16, empty = full + 8 * Plan::kStages,
                  s_full = empty + 8 * Plan::kStages, p_ready = s_full + 8 * NWG, o_full = p_ready + 8 * NWG,
-                 o_free = o_full + 8 * NWG;
+                 o_free = o_full + 8 * NWG, meet = o_free + 8 * NWG;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
 
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     for (int i = 0; i < Plan::kStages; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     for (int i = 0; i < NWG; ++i) {
       bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 128);
-      bar_init(o_full + 8 * i, 1), bar_init(o_free + 8 * i, 128);
+      bar_init(o_full + 8 * i, 1), bar_init(o_free + 8 * i, 128), bar_init(meet + 8 * i, 4);
     }
     init_visible();
     flag_word = 0;
@@ -490,6 +489,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t sw = tmem + w * 128 + lanes, ow = tmem + NWG * 128 + w * DP + lanes;
     char* stage = tiles + (NWG + Plan::kStages) * Plan::kTileBytes + w * kChunk;
+    Meeting group{meet + 8 * w};
     [&] {
       int tile = 0, done = 0;
       for (int it = 0;; ++it) {
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           a.lse[(uint64_t)piece.row * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
-          stage_free(t == 0, 1 + w, 128);
+          if (!stage_free(t == 0, group)) return give_up(flag);
           uint32_t o[64] = {};
           if (n > 0) {
             load32(ow + c, o), load32(ow + c + 32, o + 32);
@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
             }
           }
           stage_columns<T>(stage, t, 0, o, f), stage_columns<T>(stage, t, 32, o + 32, f);
-          stage_out(t == 0 && q0 < (int)s.q_len, 1 + w, 128, &a.o, smem_at(stage), c, q0, piece.head, piece.batch);
+          if (!stage_full(group)) return give_up(flag);
+          if (t == 0 && q0 < (int)s.q_len) store_tile(&a.o, smem_at(stage), c, q0, piece.head, piece.batch);
         }
       }
     }();
@@ -651,16 +652,17 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[6 + 2 * kStay + 2 * kRing + 4];
+  __shared__ uint64_t bars[8 + 2 * kStay + 2 * kRing + 4];
   __shared__ float shifts[2][kTile], deltas[2][kTile];  // of this piece and the next
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles);
   const WorkBars work_bars(work);
-  const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, q_full = dq_full + 48, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
+  const uint32_t dq_full = smem_at(bars), dq_free = dq_full + 8, q_full = dq_full + 64, q_empty = q_full + 8 * kStay, full = q_empty + 8 * kStay, empty = full + 8 * kRing,
                  s_full = empty + 8 * kRing, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8;
   // The next piece's rows are ready before the softmax warps have to have looked at this one's, and their sums may be
   // ready before this one's are looked at.
   const Turns rows_ready{dq_full + 16}, left_ready{dq_full + 32};
+  const uint32_t meet_results = dq_full + 48, meet_softmax = dq_full + 56;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
@@ -668,6 +670,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     bar_init(dq_full, 1), bar_init(dq_free, 128);
     for (int i = 0; i < kStay; ++i) bar_init(q_full + 8 * i, 1), bar_init(q_empty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) bar_init(rows_ready.bar(i), 128), bar_init(left_ready.bar(i), 256);
+    bar_init(meet_results, 4), bar_init(meet_softmax, 8);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     bar_init(s_full, 1), bar_init(s_free, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
     init_visible();
@@ -777,9 +780,11 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
-    // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for
+    Meeting group{meet_results};
+    // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for.  False
+    // where a wait ran out, as below.
     float shift = INFINITY, delta = 0.0f;  // of this thread's row of the piece that was prepared last
-    auto prepare = [&](const Piece& p, int u) {
+    auto prepare = [&](const Piece& p, int u) -> bool {
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
       const int lane = t % kLanes, mine = t / 32 * 32 + t % 32 / kLanes;
 #pragma unroll
@@ -811,9 +816,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       const float lse = row < (int)s.q_len ? a.lse[(uint64_t)p.row * s.q_len + row] : -INFINITY;
       shift = lse == -INFINITY ? INFINITY : lse * kLog2e;
       shifts[u & 1][t] = shift;
-      group_sync(2, 128);
+      if (!group()) return false;
       delta = deltas[u & 1][t];
       bar_arrive(rows_ready.bar(u));
+      return true;
     };
     // The results of a piece that sees n tiles, and its row's exponent shift and D; false where a wait ran out.
     auto finish = [&](const Piece& p, int n, int u, float shift, float d) -> bool {
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         fence_after();
         off = live ? shifts[u & 1][t] + deltas[u & 1][t] : 0.0f;
       }
-      stage_free(t == 0, 1, 128);
+      if (!stage_free(t == 0, group)) return false;
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
         uint32_t r[32] = {};
@@ -849,8 +855,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         }
         stage_columns<T>(stage + c / 64 * kChunk, t, c % 64, r, s.scale);
       }
-      async_fence();
-      group_sync(1, 128);
+      if (!stage_full(group)) return false;
       if (t == 0) {
 #pragma unroll
         for (int c = 0; c < DP; c += 64)
@@ -869,7 +874,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         const int n = piece.first >= 0 ? Queries<1>(s, piece).most : 0;
         const float last_shift = shift, last_delta = delta;
-        if (n > 0) prepare(piece, u);
+        if (n > 0 && !prepare(piece, u)) return give_up(flag);
         if (last.first >= 0 && !finish(last, last_n, u - 1, last_shift, last_delta)) return give_up(flag);
         last.first = -1;
         if (piece.first < 0) return;
@@ -885,6 +890,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    Meeting group{meet_softmax};
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
@@ -896,7 +902,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const int limit = s.limit(row, keys), least = s.limit(piece.first, keys);
         CSW_WAIT_WARP(rows_ready.bar(u), rows_ready.parity(u));
         const float shift = shifts[u & 1][t], d = deltas[u & 1][t];
-        group_sync(3, 256);  // both halves have read: the places are written below
+        if (!group()) return give_up(flag);  // both halves have read: the places are written below
         const bool few = n <= kFewTiles;
         float left = 0.0f;  // sum of ds
         for (int j = 0; j < n; ++j, ++i) {
@@ -989,14 +995,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
   constexpr int kRing = Plan::kRing, kStay = Plan::kStay;
   extern __shared__ __align__(1024) char tiles[];  // the swizzle goes by addresses
   __shared__ Work work;
-  __shared__ uint64_t bars[2 + 2 * kStay + 2 * kRing + 4];
+  __shared__ uint64_t bars[3 + 2 * kStay + 2 * kRing + 4];
   __shared__ __align__(16) float rows[kRing][kTile];  // with a tile of q the exponents' shifts, with one of do D
   __shared__ uint32_t tmem_at, flag_word;
   const uint32_t tiles_at = smem_at(tiles), rows_at = smem_at(rows);
   const WorkBars work_bars(work);
   const uint32_t sums_full = smem_at(bars), sums_free = sums_full + 8, kv_full = sums_full + 16,
                  kv_empty = kv_full + 8 * kStay, full = kv_empty + 8 * kStay, empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_ready = s_full + 8,
-                 dp_full = p_ready + 8, ds_ready = dp_full + 8;
+                 dp_full = p_ready + 8, ds_ready = dp_full + 8, meet = ds_ready + 8;
   uint32_t* flag = &flag_word;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   if (threadIdx.x == 0) {
@@ -1005,6 +1011,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     for (int i = 0; i < kStay; ++i) bar_init(kv_full + 8 * i, 1), bar_init(kv_empty + 8 * i, 1);
     for (int i = 0; i < kRing; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
     bar_init(s_full, 1), bar_init(p_ready, 256), bar_init(dp_full, 1), bar_init(ds_ready, 256);
+    bar_init(meet, 4);
     init_visible();
     flag_word = 0;
   }
@@ -1113,6 +1120,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
+    Meeting group{meet};
     [&] {
       int u = 0;
       for (int it = 0;; ++it) {
@@ -1151,7 +1159,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
 #pragma unroll
         for (int x = 0; x < 2; ++x) {  // dv, dk
           const uint32_t from = (x == 0 ? dv_at : dk_at) + lanes;
-          stage_free(t == 0, 1, 128);
+          if (!stage_free(t == 0, group)) return give_up(flag);
 #pragma unroll
           for (int c = 0; c < DP; c += 64)
             take_columns<T>(stage + c / 64 * kChunk, t, any, live, from + c, x == 0 ? 1.0f : s.scale, [&] {
@@ -1160,8 +1168,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
                 bar_arrive(sums_free);
               }
             });
-          async_fence();
-          group_sync(1, 128);
+          if (!stage_full(group)) return give_up(flag);
           if (t == 0) {
 #pragma unroll
             for (int c = 0; c < DP; c += 64)

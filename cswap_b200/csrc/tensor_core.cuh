@@ -81,10 +81,18 @@ __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// some warps of a CTA
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
+// Some warps of a CTA that meet again and again, on an mbarrier with an arrival for each of them.  Its wait is bounded,
+// where a bar.sync with a warp that has given up would never end.  A meeting cannot end before all have come to it, so
+// that nobody is two ahead and the parity tells.
+struct Meeting {
+  uint32_t bar, met = 0;
+  // false where the others have not come
+  __device__ __forceinline__ bool operator()() {
+    __syncwarp();  // what all lanes have written is in front of the arrival
+    if (threadIdx.x % 32 == 0) bar_arrive(bar);
+    return __all_sync(0xffffffffu, bar_wait(bar, met++ & 1));
+  }
+};
 
 // ---- work ----------------------------------------------------------------------------------------------------------
 // Asks for a CTA of this grid that has not started: it will not start, and its work is the caller's.  The answer (16
