@@ -321,7 +321,7 @@ __device__ __forceinline__ float row_top(uint32_t at, int chunks, int end) {
       top_of(m, r[q % 2]);
     }
   }
-  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+  return max2(max3(m[0], m[1], m[2]), m[3]);
 }
 template <class T>
 __device__ __forceinline__ void exp_of(Pair (&add)[2], const uint32_t* r, float exponent, float shift, int end,
@@ -511,9 +511,9 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           const int chunks = masked ? min((s.limit(q0 + warp % 4 * 32 + 31, keys) - j * kTile + 31) / 32, 4) : 4;
           const float now = masked ? row_top<true>(sw, chunks, end) : row_top<false>(sw, 4, 0);
           // The maximum is followed only where it grows by more than 2^8: the sums' exponents have room for that, and
-          // so has float16, whose largest number is 2^16.
-          if (__any_sync(0xffffffffu, (now - top) * s.exponent > 8.0f)) {
-            const float next = fmaxf(top, now);
+          // so has float16, whose largest number is 2^16.  A NaN is followed as well.
+          if (__any_sync(0xffffffffu, !((now - top) * s.exponent <= 8.0f))) {
+            const float next = max2(top, now);
             const float f = next == -INFINITY ? 1.0f : exp2_fast((top - next) * s.exponent);
             top = next;
             sum *= f;
@@ -541,9 +541,12 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
           ++done;
           fence_after();
         }
-        const float f = n == 0 || sum == 0.0f ? 0.0f : 1.0f / sum;
+        // Whether a row sees any key is told by the mask, not by its sum: scores may be infinite or NaN, and show.
+        const bool live = limit > 0;
+        const float f = live ? 1.0f / sum : 0.0f;
         if (row < (int)s.q_len)
-          a.lse[(uint64_t)piece.row * s.q_len + row] = sum == 0.0f ? -INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
+          a.lse[(uint64_t)piece.row * s.q_len + row] =
+              !live ? -INFINITY : top == INFINITY ? INFINITY : (top * s.exponent + log2f(sum)) * kLn2;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
           if (!stage_free(t == 0, group)) return give_up(flag);
@@ -555,6 +558,10 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
               fence_before();
               bar_arrive(o_free + 8 * w);
             }
+          }
+          if (!live) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0;
           }
           stage_columns<T>(stage, t, 0, o, f), stage_columns<T>(stage, t, 32, o + 32, f);
           if (!stage_full(group)) return give_up(flag);
@@ -569,7 +576,8 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // Per head and query, padded to whole tiles, dq leaves for dkv in rows[0] log2(e) L, +inf for a query that sees nothing
-// and behind the last one, so that its probabilities are zero, and in rows[1] D.
+// and behind the last one, so that its probabilities are zero, and in rows[1] D.  L itself may be infinite where a row
+// sees infinite scores; its probabilities are NaN, as its o is.
 struct Backward {
   CUtensorMap q, k, v, dout, dq, dk, dv;
   Shape s;
@@ -784,6 +792,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for.  False
     // where a wait ran out, as below.
     float shift = INFINITY, delta = 0.0f;  // of this thread's row of the piece that was prepared last
+    bool live = false;                     // whether it sees any key
     auto prepare = [&](const Piece& p, int u) -> bool {
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
       const int lane = t % kLanes, mine = t / 32 * 32 + t % 32 / kLanes;
@@ -813,8 +822,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         }
       }
       const int row = p.first + t;
-      const float lse = row < (int)s.q_len ? a.lse[(uint64_t)p.row * s.q_len + row] : -INFINITY;
-      shift = lse == -INFINITY ? INFINITY : lse * kLog2e;
+      live = row < (int)s.q_len && s.limit(row, p.keys) > 0;
+      const float lse = live ? a.lse[(uint64_t)p.row * s.q_len + row] : 0.0f;
+      shift = !live ? INFINITY : fabsf(lse) == INFINITY ? NAN : lse * kLog2e;
       shifts[u & 1][t] = shift;
       if (!group()) return false;
       delta = deltas[u & 1][t];
@@ -822,13 +832,13 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       return true;
     };
     // The results of a piece that sees n tiles, and its row's exponent shift and D; false where a wait ran out.
-    auto finish = [&](const Piece& p, int n, int u, float shift, float d) -> bool {
-      const bool live = shift != INFINITY;
+    auto finish = [&](const Piece& p, int n, int u, bool live, float shift, float d) -> bool {
       float off = 0.0f;
       if (n > 0) {
         if (!__all_sync(0xffffffffu, bar_wait(left_ready.bar(u), left_ready.parity(u)) && bar_wait(dq_full, u & 1))) return false;
         fence_after();
         off = live ? shifts[u & 1][t] + deltas[u & 1][t] : 0.0f;
+        if (!(fabsf(off) < INFINITY)) off = 0.0f;  // of gradients that are not finite nothing is put right
       }
       if (!stage_free(t == 0, group)) return false;
 #pragma unroll
@@ -873,15 +883,16 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         const int n = piece.first >= 0 ? Queries<1>(s, piece).most : 0;
+        const bool last_live = live;
         const float last_shift = shift, last_delta = delta;
         if (n > 0 && !prepare(piece, u)) return give_up(flag);
-        if (last.first >= 0 && !finish(last, last_n, u - 1, last_shift, last_delta)) return give_up(flag);
+        if (last.first >= 0 && !finish(last, last_n, u - 1, last_live, last_shift, last_delta)) return give_up(flag);
         last.first = -1;
         if (piece.first < 0) return;
         if (n > 0) {
           last = piece, last_n = n;
           ++u;
-        } else if (!finish(piece, 0, 0, INFINITY, 0.0f)) {
+        } else if (!finish(piece, 0, 0, false, INFINITY, 0.0f)) {
           return give_up(flag);
         }
       }

@@ -225,17 +225,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Maxima that a NaN among their operands makes NaN.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-// 2^x without the unit for it: the whole part n goes into the exponent, 2^f for the rest, -1/2 ... 1/2, is a polynomial
-// of degree 5 (fitted for the least relative error, 1.6 10^-7).  x from -126 up to 127; below that 2^-126 stands for it.
+// 2^x without the unit for it: 2^n for the whole part n is put together as a number, 2^f for the rest, -1/2 ... 1/2, is a
+// polynomial of degree 5 (fitted for the least relative error, 1.6 10^-7).  x up to 127; from -126.5 down it gives 0, and
+// NaN for a NaN: the exponent is multiplied in, since added to the bits of a NaN it would make a number of them.
 __device__ __forceinline__ Pair exp2_poly(Pair x) {
   constexpr float kMagic = 12582912.0f;  // 1.5 2^23: a sum with it is rounded to a whole number, its low bits
-  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  x.x = max2(x.x, -127.0f), x.y = max2(x.y, -127.0f);
   const Pair t = add2(x, {kMagic, kMagic});
   const Pair n = add2(t, {-kMagic, -kMagic});
   const Pair f = fma2(n, {-1.0f, -1.0f}, x);
@@ -244,9 +251,9 @@ __device__ __forceinline__ Pair exp2_poly(Pair x) {
   p = fma2(p, f, {0.24022120237350464f, 0.24022120237350464f});
   p = fma2(p, f, {0.6931469440460205f, 0.6931469440460205f});
   p = fma2(p, f, {1.0000001192092896f, 1.0000001192092896f});
-  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-  return p;
+  const Pair power = {__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                      __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)};
+  return mul2(p, power);
 }
 
 }  // namespace tc
