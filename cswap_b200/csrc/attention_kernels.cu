@@ -113,11 +113,11 @@ __device__ __forceinline__ void stage_columns(char* tile, int row, int at, const
   }
 }
 
-// All columns of a tile's rows [first, 128), zeroed by the warp that issues the products: what lies behind a sequence
-// must not meet the zeros of its probabilities as a NaN.
+// All columns of a tile's rows [first, end), zeroed by the warp that issues the products: what lies behind a sequence, or
+// belongs to a query that sees nothing, must not meet the zeros of its probabilities as a NaN.
 template <int DP>
-__device__ __forceinline__ void zero_rows(char* tile, int first) {
-  for (int i = threadIdx.x % 32; i < (kTile - first) * 8; i += 32)
+__device__ __forceinline__ void zero_rows(char* tile, int first, int end = kTile) {
+  for (int i = threadIdx.x % 32; i < (end - first) * 8; i += 32)
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c)
       *reinterpret_cast<uint4*>(tile + c * kChunk + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
@@ -1088,8 +1088,12 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         Piece piece;
         if (!hear(work, work_bars, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
-        const int n = Keys<SPLIT>(s, piece, a.parts).n;
+        const Keys<SPLIT> at(s, piece, a.parts);
+        const int n = at.n;
         if (n == 0) continue;
+        // Queries that a causal mask leaves nothing stand in front of the others, in the first keys' first tile.
+        const int dead = s.causal && piece.first == 0 ? (int)s.q_len - (int)s.k_len - at.from * kTile : 0;
+        int q = at.q;
         const uint32_t stay = u % kStay;
         const uint64_t k_rows = stay_rows + stay * 2 * kStep;  // v behind it
         CSW_WAIT_WARP(kv_full + 8 * stay, u / kStay & 1);
@@ -1105,6 +1109,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot, round & 1);
+            if (dead > 0 && q == at.from) zero_rows<DP>(tiles + (2 * kStay + slot) * Plan::kTileBytes, 0, dead);
             product_rows<DP>(s_at, k_rows, q_rows, scores, s_full);
           }
           if (now) {
@@ -1114,6 +1119,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
           }
           if (next) {
             CSW_WAIT_WARP(full + 8 * slot + 8, round & 1);
+            if (dead > 0 && q == at.from) zero_rows<DP>(tiles + (2 * kStay + slot + 1) * Plan::kTileBytes, 0, dead);
             product_rows<DP>(dp_at, k_rows + kStep, q_rows + kStep, slopes, dp_full);
           }
           if (j + 2 == n) commit_to(kv_empty + 8 * stay);
@@ -1122,6 +1128,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
             ++i;
             slot += 2;
             if (slot == kRing) slot = 0, ++round;
+            if (++q == at.tiles) q = at.from;
           }
         }
         ++u;

@@ -230,6 +230,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     keys up to i + k_len - q_len.  `kv_lens` (int32, on the device, one for each batch entry): the number of keys of
     that entry, taken into 0 ... k_len; keys and values behind it are not used, whatever they hold (those that only
     `causal` hides count with a probability of zero, and must be finite).  A query that sees no key gives zeros, and no
-    gradient passes through it."""
+    gradient passes through it, whatever it and its gradient hold."""
     _ext().check_capture(q, k, v)
     return _Attention.apply(q, k, v, causal, kv_lens, scale)

@@ -387,7 +387,8 @@ csw_status csw_layer_norm_backward(const void* d_dy, const void* d_x, const floa
  * multiple of kv_heads: query heads h of one group of heads / kv_heads consecutive ones read key head
  * h / (heads / kv_heads).  causal: query i sees the keys up to i + k_len - q_len.  kv_lens (device, `batch` int32, or
  * NULL): batch entry b has kv_lens[b] keys (taken into 0 ... k_len); what lies behind them in k and v is not used,
- * whatever it is (what only `causal` hides counts with a probability of zero, and has to be finite).  A query that sees no key gets o = 0 and lse = -inf, and no gradient passes through it. */
+ * whatever it is (what only `causal` hides counts with a probability of zero, and has to be finite).  A query that sees no
+ * key gets o = 0 and lse = -inf, and no gradient passes through it, whatever q and the gradient of o hold there. */
 typedef struct {
   int type, causal;
   size_t batch, heads, kv_heads, q_len, k_len, dim;

@@ -124,6 +124,24 @@ def test_a_bad_key_under_a_causal_mask(cs, kind, dim):
 
 
 @halves
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ql,kl", [(200, 70), (130, 128), (400, 9), (129, 1)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_queries_that_see_nothing_may_hold_anything(cs, kind, dim, ql, kl, bad):
+    """No gradient passes through them: the same bits as with zeros in their place, of q and of the gradient of o."""
+    t = {n: normal(2, 4, ql, dim, seed=i, kind=kind) for i, n in enumerate(("q", "do"))}
+    t.update({n: normal(2, 2, kl, dim, seed=5 + i, kind=kind) for i, n in enumerate("kv")})
+    dead = ql - kl
+    zero = {n: x.clone() for n, x in t.items()}
+    for n in ("q", "do"):
+        zero[n][:, :, :dead], t[n][:, :, :dead] = 0.0, bad
+    got, want = passes(cs, **t, causal=True), passes(cs, **zero, causal=True)
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+    assert not got[0][:, :, :dead].any() and not got[2][:, :, :dead].any() and (got[1][:, :, :dead] == -math.inf).all()
+
+
+@halves
 def test_gradients_of_an_overflow_are_seen(cs, kind):
     """Through autograd: a step that has diverged shows in the gradient of every operand that it went through."""
     q, k, v = (normal(1, 2, 40, 64, seed=i, kind=kind).requires_grad_(True) for i in range(3))
