@@ -16,6 +16,7 @@ from .swap import SwapManager, Ticket, CostModel, TensorDesc, blob_info  # noqa:
 from .ops import (  # noqa: F401
     q8_bytes, q8_compress, q8_decompress, gelu_forward, gelu_backward, gelu, gelu_linear,
     layer_norm_forward, layer_norm_backward, layer_norm, attention_forward, attention_backward, attention,
+    device_status,
 )
 from .execution import Execution, LayerType  # noqa: F401
 

@@ -158,6 +158,7 @@ SIGNATURES = {
     "csw_layer_norm_workspace": (_I, [_SZ, _SZ, C.POINTER(_SZ)]),
     "csw_layer_norm_backward": (_I, [_P, _P, _P, _P, _P, _I, _I, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P]),
     "csw_attention_forward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _P]),
+    "csw_attention_wait_limit": (_I, [C.c_int64]),
     "csw_attention_workspace": (_I, [_SH, C.POINTER(_SZ)]),
     "csw_attention_backward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _OP, _OP, _OP, _OP, _P, _SZ, _P]),
     # reference-named entry points

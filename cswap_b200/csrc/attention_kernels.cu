@@ -32,7 +32,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 #include "attention_kernels.h"
@@ -50,9 +52,6 @@ using namespace tc;
 constexpr int kTile = 128;                 // tokens of a tile
 constexpr uint32_t kChunk = kTile * 128;   // bytes of a tile's 64 columns
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-// Set where a wait ran out.
-__device__ int attention_gave_up;
 
 // a tensor that is read by rows
 struct View {
@@ -72,6 +71,9 @@ struct Shape {
   float scale;     // as given
   float exponent;  // |scale| log2(e), and not zero, so that masked scores stay -inf
   const int32_t* lens;
+  long long patience;  // clocks that a wait may last
+  bool idle;           // nothing is copied, so that the waits for it run out
+  uint32_t* status;    // in host memory; set where a wait ran out
   __device__ int keys(uint32_t b) const { return lens ? min(max(lens[b], 0), (int)k_len) : (int)k_len; }
   // keys that query i sees
   __device__ int limit(int i, int keys) const {
@@ -79,20 +81,17 @@ struct Shape {
   }
 };
 
-__device__ __forceinline__ void give_up(uint32_t* flag) {
-  *reinterpret_cast<volatile uint32_t*>(flag) = 1;
-  atomicExch(&attention_gave_up, 1);
-}
+__device__ __forceinline__ void give_up(uint32_t* flag) { *reinterpret_cast<volatile uint32_t*>(flag) = 1; }
 // Leaves the role it stands in; the second form for warps that go on together.
-#define CSW_WAIT(bar, parity)      \
-  if (!bar_wait(bar, parity)) {    \
-    give_up(flag);                 \
-    return;                        \
+#define CSW_WAIT(bar, parity)                \
+  if (!bar_wait(bar, parity, s.patience)) {  \
+    give_up(flag);                           \
+    return;                                  \
   }
-#define CSW_WAIT_WARP(bar, parity)                              \
-  if (!__all_sync(0xffffffffu, bar_wait(bar, parity))) {        \
-    give_up(flag);                                              \
-    return;                                                     \
+#define CSW_WAIT_WARP(bar, parity)                                         \
+  if (!__all_sync(0xffffffffu, bar_wait(bar, parity, s.patience))) {       \
+    give_up(flag);                                                         \
+    return;                                                                \
   }
 
 template <class T>
@@ -191,8 +190,8 @@ struct WorkBars {
   }
 };
 // What a warp hears as its i-th piece; false where a wait ran out.
-__device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, int i, Piece* piece) {
-  if (!__all_sync(0xffffffffu, bar_wait(bars.told + 8 * (i % 2), i / 2 & 1))) return false;
+__device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, const Shape& s, int i, Piece* piece) {
+  if (!__all_sync(0xffffffffu, bar_wait(bars.told + 8 * (i % 2), i / 2 & 1, s.patience))) return false;
   // one lane's reading: the compiler then knows that all have the same
   const volatile Piece& told = w.piece[i % 2];
   piece->first = __shfl_sync(0xffffffffu, told.first, 0), piece->keys = __shfl_sync(0xffffffffu, told.keys, 0);
@@ -202,22 +201,43 @@ __device__ __forceinline__ bool hear(Work& w, const WorkBars& bars, int i, Piece
   return true;
 }
 
-// What every kernel ends with, also where a wait ran out: copies on their way get time to land, tensor memory is freed.
-template <int COLUMNS>
-__device__ __forceinline__ void leave(uint32_t* flag, uint32_t tmem, bool owner) {
+// NaN for all rows of a tensor; a row is a whole number of 16 bytes, and 0x7fff a NaN of either type.
+__device__ __noinline__ void spoil(const View& v, uint32_t batch, uint32_t heads, uint32_t tokens, uint32_t dim) {
+  const uint32_t packs = dim / 8;
+  const uint64_t n = (uint64_t)batch * heads * tokens * packs;
+  for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint64_t row = i / packs, head = row / tokens;
+    uint4* to = const_cast<uint4*>(reinterpret_cast<const uint4*>(v.row<uint16_t>(head / heads, head % heads, row % tokens)));
+    to[i % packs] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  }
+}
+__device__ __noinline__ void spoil(float* p, uint64_t n) {
+  for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) p[i] = NAN;
+}
+// What every kernel ends with, also where a wait ran out: copies on their way get time to land, then spoil() makes all
+// results NaN, those of other CTAs that are done as well (which pieces this one still owed no single warp knows); tensor
+// memory is freed.
+template <int COLUMNS, class F>
+__device__ __forceinline__ void leave(const Shape& s, uint32_t* flag, uint32_t tmem, bool owner, F&& spoil) {
   __syncwarp();
   fence_before();
   __syncthreads();
   fence_after();
-  if (*reinterpret_cast<volatile uint32_t*>(flag))
+  if (*reinterpret_cast<volatile uint32_t*>(flag)) {
     for (int i = 0; i < 1000; ++i) __nanosleep(10000);
+    spoil();
+    if (threadIdx.x == 0) {
+      *reinterpret_cast<volatile uint32_t*>(s.status) = 1;
+      __threadfence_system();
+    }
+  }
   if (owner) tmem_free<COLUMNS>(tmem);
 }
 
 // The copying warp's lane over all its pieces: f.piece(index) says which one a CTA has, f.copy(piece) copies what it
 // needs, and returns false where a wait ran out.
 template <class F>
-__device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_t* flag, F&& f) {
+__device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, const Shape& s, uint32_t* flag, F&& f) {
   int index = blockIdx.x;
   for (int i = 0;; ++i) {
     if (i >= 2) CSW_WAIT(bars.read + 8 * (i % 2), (i / 2 - 1) & 1);
@@ -226,7 +246,7 @@ __device__ __forceinline__ void give_work(Work& w, const WorkBars& bars, uint32_
     w.piece[i % 2] = piece;
     bar_arrive(bars.told + 8 * (i % 2));
     if (index < 0) return;
-    if (!f.copy(piece)) {
+    if (s.idle || !f.copy(piece)) {
       give_up(flag);
       return;
     }
@@ -255,6 +275,7 @@ struct Forward {
   CUtensorMap q, k, v, o;
   Shape s;
   float* lse;
+  View out;  // o once more
 };
 
 // NWG tiles of 128 queries a CTA; columns of tensor memory: the scores of each, then the sums of each.  Shared memory:
@@ -423,14 +444,14 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
       __device__ bool copy(const Piece& p) {
         const Queries<NWG> at(a.s, p);
         if (at.most == 0) return true;
-        if (u > 0 && !bar_wait(q_empty, (u - 1) & 1)) return false;
+        if (u > 0 && !bar_wait(q_empty, (u - 1) & 1, a.s.patience)) return false;
         bar_expect(q_full, NWG * Plan::kTileBytes);
 #pragma unroll
         for (int w = 0; w < NWG; ++w)
           copy_tokens<DP>(tiles_at + w * Plan::kTileBytes, &a.q, q_full, p.first + w * kTile, p.head, p.batch);
         for (int j = 0; j < 2 * at.most; ++j, ++i) {  // k 0, v 0, k 1, v 1, ...
           const int stage = i % Plan::kStages;
-          if (i >= Plan::kStages && !bar_wait(empty + 8 * stage, (i / Plan::kStages - 1) & 1)) return false;
+          if (i >= Plan::kStages && !bar_wait(empty + 8 * stage, (i / Plan::kStages - 1) & 1, a.s.patience)) return false;
           bar_expect(full + 8 * stage, Plan::kTileBytes);
           copy_tokens<DP>(ring + stage * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * stage, j / 2 * kTile, p.kv_head, p.batch);
         }
@@ -439,7 +460,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
       }
     };
     if (threadIdx.x % 32 == 0)
-      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
+      give_work(work, work_bars, s, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 4 * NWG + 1) {
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
@@ -449,7 +470,7 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
       int base = 0, u = 0, tile[NWG] = {}, done[NWG] = {};  // of the ring; pieces; of each tile of queries: tiles, pieces
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const Queries<NWG> at(s, piece);
         if (at.most == 0) continue;
@@ -489,12 +510,12 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t sw = tmem + w * 128 + lanes, ow = tmem + NWG * 128 + w * DP + lanes;
     char* stage = tiles + (NWG + Plan::kStages) * Plan::kTileBytes + w * kChunk;
-    Meeting group{meet + 8 * w};
+    Meeting group{meet + 8 * w, s.patience};
     [&] {
       int tile = 0, done = 0;
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const Queries<NWG> at(s, piece);
         const int keys = piece.keys, n = NWG == 1 || w == 0 ? at.count[0] : at.count[NWG - 1];
@@ -571,7 +592,10 @@ __global__ void __launch_bounds__(ForwardPlan<DP, NWG>::kThreads, NWG == 1 ? 2 :
     }();
     if (t == 0) stores_read();
   }
-  leave<Plan::kColumns>(flag, tmem, warp == 4 * NWG + 1);
+  leave<Plan::kColumns>(s, flag, tmem, warp == 4 * NWG + 1, [&] {
+    spoil(a.out, s.batch, s.heads, s.q_len, s.dim);
+    spoil(a.lse, (uint64_t)s.batch * s.heads * s.q_len);
+  });
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
@@ -590,6 +614,7 @@ struct Backward {
   int parts;
   float* sums;
   uint32_t k_padded;
+  View dq_out, dk_out, dv_out;  // the results once more
 };
 
 // Both kernels: 256 threads for the scores (two a row, 64 columns each), 128 that prepare a piece's rows and take its
@@ -706,13 +731,13 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         const Queries<1> at(a.s, p);
         if (at.most == 0) return true;
         const uint32_t to = tiles_at + u % kStay * 2 * Plan::kTileBytes, here = q_full + 8 * (u % kStay);
-        if (u >= kStay && !bar_wait(q_empty + 8 * (u % kStay), (u / kStay - 1) & 1)) return false;
+        if (u >= kStay && !bar_wait(q_empty + 8 * (u % kStay), (u / kStay - 1) & 1, a.s.patience)) return false;
         bar_expect(here, 2 * Plan::kTileBytes);
         copy_tokens<DP>(to, &a.q, here, p.first, p.head, p.batch);
         copy_tokens<DP>(to + Plan::kTileBytes, &a.dout, here, p.first, p.head, p.batch);
         for (int j = 0; j < 2 * at.most; ++j, ++i) {
           const int slot = i % kRing;
-          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
+          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1, a.s.patience)) return false;
           bar_expect(full + 8 * slot, Plan::kTileBytes);
           copy_tokens<DP>(ring + slot * Plan::kTileBytes, j % 2 ? &a.v : &a.k, full + 8 * slot, j / 2 * kTile, p.kv_head, p.batch);
         }
@@ -721,7 +746,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       }
     };
     if (threadIdx.x % 32 == 0)
-      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
+      give_work(work, work_bars, s, flag, Copies{a, tiles_at, ring, q_full, q_empty, full, empty});
   } else if (warp == 13) {
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
@@ -734,7 +759,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of keys, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const int n = Queries<1>(s, piece).most;
         if (n == 0) continue;
@@ -788,7 +813,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
-    Meeting group{meet_results};
+    Meeting group{meet_results, s.patience};
     // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for.  False
     // where a wait ran out, as below.
     float shift = INFINITY, delta = 0.0f;  // of this thread's row of the piece that was prepared last
@@ -835,7 +860,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     auto finish = [&](const Piece& p, int n, int u, bool live, float shift, float d) -> bool {
       float off = 0.0f;
       if (n > 0) {
-        if (!__all_sync(0xffffffffu, bar_wait(left_ready.bar(u), left_ready.parity(u)) && bar_wait(dq_full, u & 1))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(left_ready.bar(u), left_ready.parity(u), s.patience) && bar_wait(dq_full, u & 1, s.patience))) return false;
         fence_after();
         off = live ? shifts[u & 1][t] + deltas[u & 1][t] : 0.0f;
         if (!(fabsf(off) < INFINITY)) off = 0.0f;  // of gradients that are not finite nothing is put right
@@ -881,7 +906,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       int last_n = 0, u = 0;
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         const int n = piece.first >= 0 ? Queries<1>(s, piece).most : 0;
         const bool last_live = live;
         const float last_shift = shift, last_delta = delta;
@@ -901,12 +926,12 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
   } else {
     const int w = warp / 4, t = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    Meeting group{meet_softmax};
+    Meeting group{meet_softmax, s.patience};
     [&] {
       int i = 0, u = 0;
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const int keys = piece.keys, n = Queries<1>(s, piece).most, row = piece.first + t;
         if (n == 0) continue;
@@ -975,7 +1000,10 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       }
     }();
   }
-  leave<Plan::kColumns>(flag, tmem, warp == 13);
+  leave<Plan::kColumns>(s, flag, tmem, warp == 13, [&] {
+    spoil(a.dq_out, s.batch, s.heads, s.q_len, s.dim);
+    spoil(a.rows, 2 * (uint64_t)s.batch * s.heads * a.padded);  // and with them what dkv makes of them
+  });
 }
 
 // Pieces of the grid over keys.  The first keys of a causal mask are seen by the most queries: they go first.
@@ -1053,7 +1081,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         const int kv_head = at.kv_head(p);
         if (at.n == 0) return true;
         const uint32_t to = tiles_at + u % kStay * 2 * Plan::kTileBytes, here = kv_full + 8 * (u % kStay);
-        if (u >= kStay && !bar_wait(kv_empty + 8 * (u % kStay), (u / kStay - 1) & 1)) return false;
+        if (u >= kStay && !bar_wait(kv_empty + 8 * (u % kStay), (u / kStay - 1) & 1, a.s.patience)) return false;
         bar_expect(here, 2 * Plan::kTileBytes);
         copy_tokens<DP>(to, &a.k, here, p.first, kv_head, p.batch);
         copy_tokens<DP>(to + Plan::kTileBytes, &a.v, here, p.first, kv_head, p.batch);
@@ -1061,7 +1089,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         int q = at.q, h = at.head;
         for (int j = 0; j < 2 * at.n; ++j, ++i) {
           const int slot = i % kRing;
-          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1)) return false;
+          if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1, a.s.patience)) return false;
           const uint32_t bar = full + 8 * slot;
           bar_expect(bar, Plan::kTileBytes + kTile * 4);
           copy_tokens<DP>(ring + slot * Plan::kTileBytes, j % 2 ? &a.dout : &a.q, bar, q * kTile, p.head + h, p.batch);
@@ -1074,7 +1102,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       }
     };
     if (threadIdx.x % 32 == 0)
-      give_work(work, work_bars, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
+      give_work(work, work_bars, s, flag, Copies{a, tiles_at, ring, rows_at, kv_full, kv_empty, full, empty});
   } else if (warp == 13) {
     [&] {
       const uint32_t scores = product_desc(kBf16<T>, kTile, false, s.negate);
@@ -1086,7 +1114,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       uint32_t i = 0, u = 0, slot = 0, round = 0;  // tiles of queries, pieces with any; of the ring
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const Keys<SPLIT> at(s, piece, a.parts);
         const int n = at.n;
@@ -1138,12 +1166,12 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
     const int t = threadIdx.x - 256;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     char* stage = tiles + (2 * kStay + kRing) * Plan::kTileBytes;
-    Meeting group{meet};
+    Meeting group{meet, s.patience};
     [&] {
       int u = 0;
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const bool any = Keys<SPLIT>(s, piece, a.parts).n > 0;
         if (any) {
@@ -1204,7 +1232,7 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       int i = 0;
       for (int it = 0;; ++it) {
         Piece piece;
-        if (!hear(work, work_bars, it, &piece)) return give_up(flag);
+        if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         if (piece.first < 0) return;
         const Keys<SPLIT> at(s, piece, a.parts);
         const int n = at.n, row = piece.first + t, off = (int)s.k_len - (int)s.q_len;
@@ -1272,7 +1300,14 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
       }
     }();
   }
-  leave<Plan::kColumns>(flag, tmem, warp == 13);
+  leave<Plan::kColumns>(s, flag, tmem, warp == 13, [&] {
+    if constexpr (SPLIT) {
+      spoil(a.sums, (uint64_t)a.parts * s.batch * s.kv_heads * a.k_padded * (2 * DP));
+    } else {
+      spoil(a.dk_out, s.batch, s.kv_heads, s.k_len, s.dim);
+      spoil(a.dv_out, s.batch, s.kv_heads, s.k_len, s.dim);
+    }
+  });
 }
 
 // The parts' sums, in their order; a thread for 4 columns of a key's dv or dk.
@@ -1301,10 +1336,38 @@ __global__ void __launch_bounds__(256) attention_sums_kernel(const float* __rest
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-Shape shape_of(const csw_attention_shape& s) {
+// A word of host memory for each device, which kernels write and the host reads without waiting for anything.
+constexpr int kMaxDevices = 64;
+uint32_t* status_words() {
+  static uint32_t* const words = [] {
+    // also while a stream is captured: the allocation has nothing to do with it
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    void* p = nullptr;
+    if (taken(cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return (uint32_t*)nullptr;
+    const size_t bytes = kMaxDevices * sizeof(uint32_t);
+    const cudaError_t e = taken(cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped));
+    taken(cudaThreadExchangeStreamCaptureMode(&mode));
+    if (e != cudaSuccess) return (uint32_t*)nullptr;
+    return (uint32_t*)std::memset(p, 0, bytes);
+  }();
+  return words;
+}
+cudaError_t status_word(uint32_t** word) {
+  int dev = 0;
+  if (const cudaError_t e = taken(cudaGetDevice(&dev))) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  uint32_t* words = status_words();
+  *word = words + dev;
+  return words ? cudaSuccess : cudaErrorMemoryAllocation;
+}
+std::atomic<long long> wait_limit{1ll << 32};  // some two seconds
+
+Shape shape_of(const csw_attention_shape& s, uint32_t* status) {
   const float e = fmaxf(fabsf(s.scale) * kLog2e, 0x1p-100f);
+  const long long wait = wait_limit.load(std::memory_order_relaxed);
   return {(uint32_t)s.batch, (uint32_t)s.heads, (uint32_t)s.kv_heads, (uint32_t)s.q_len, (uint32_t)s.k_len,
-          (uint32_t)s.dim,   (uint32_t)(s.heads / s.kv_heads), s.causal, s.scale < 0.0f, s.scale, e, s.kv_lens};
+          (uint32_t)s.dim,   (uint32_t)(s.heads / s.kv_heads), s.causal, s.scale < 0.0f, s.scale, e, s.kv_lens,
+          wait < 0 ? -wait : wait, wait < 0, status};
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -1360,7 +1423,7 @@ cudaError_t forward_of(const Forward& a, const csw_attention_shape& s, cudaStrea
 }
 
 template <class T, int DP>
-cudaError_t backward(const Backward& a, const csw_attention_shape& s, const View& dk, const View& dv, cudaStream_t stream) {
+cudaError_t backward(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
   using Plan = BackwardPlan<DP>;
   cudaError_t e = cudaSuccess;
   if (s.q_len)
@@ -1372,23 +1435,16 @@ cudaError_t backward(const Backward& a, const csw_attention_shape& s, const View
   if (e == cudaSuccess && a.parts > 1) {
     const uint64_t threads = (uint64_t)s.batch * s.kv_heads * s.k_len * (2 * DP / 4);
     e = pdl_launch(attention_sums_kernel<T, DP>, (unsigned)((threads + 255) / 256), 256, 0, stream, (const float*)a.sums,
-                   a.s, a.parts, a.k_padded, dk, dv);
+                   a.s, a.parts, a.k_padded, a.dk_out, a.dv_out);
   }
   return e;
 }
 template <class T>
-cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, const View& dk, const View& dv,
-                        cudaStream_t stream) {
-  return s.dim <= 64 ? backward<T, 64>(a, s, dk, dv, stream) : backward<T, 128>(a, s, dk, dv, stream);
+cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, cudaStream_t stream) {
+  return s.dim <= 64 ? backward<T, 64>(a, s, stream) : backward<T, 128>(a, s, stream);
 }
 
-cudaError_t take_status(int* value) {
-  const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(value, attention_gave_up, sizeof(int));
-  if (e == cudaSuccess && *value) e = cudaMemcpyToSymbol(attention_gave_up, &zero, sizeof(int));
-  return e;
-}
-const bool registered = (take_kernel_status = take_status, true);
+const bool registered = (take_kernel_status = attention_take_status, true);
 
 }  // namespace
 
@@ -1405,6 +1461,14 @@ int parts_of(const csw_attention_shape& s) {
 uint64_t row_values(const csw_attention_shape& s) { return 2 * (uint64_t)s.batch * s.heads * whole_tiles(s.q_len); }
 }  // namespace
 
+cudaError_t attention_take_status(int* gave_up) {
+  uint32_t* word;
+  const cudaError_t e = status_word(&word);
+  if (e == cudaSuccess) *gave_up = (int)__atomic_exchange_n(word, 0u, __ATOMIC_RELAXED);
+  return e;
+}
+void attention_wait_limit(long long clocks) { wait_limit.store(clocks, std::memory_order_relaxed); }
+
 uint64_t attention_workspace_values(const csw_attention_shape& s) {
   const int parts = parts_of(s);
   const uint64_t sums = parts > 1 ? parts * (uint64_t)s.batch * s.kv_heads * whole_tiles(s.k_len) * 2 * (s.dim <= 64 ? 64 : 128) : 0;
@@ -1416,8 +1480,10 @@ cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_att
                                      const csw_attention_operand& o, float* lse, cudaStream_t stream) {
   if (s.batch == 0 || s.q_len == 0) return cudaSuccess;
   if (const cudaError_t e = bind_context()) return e;
+  uint32_t* status;
+  if (const cudaError_t e = status_word(&status)) return e;
   Forward a;
-  a.s = shape_of(s), a.lse = lse;
+  a.s = shape_of(s, status), a.lse = lse, a.out = view_of(o);
   if (!map_of(&a.q, q, s, s.heads, s.q_len) || !map_of(&a.o, o, s, s.heads, s.q_len)) return cudaErrorInvalidValue;
   a.k = a.v = a.q;  // without keys nothing is copied from them
   if (s.k_len && (!map_of(&a.k, k, s, s.kv_heads, s.k_len) || !map_of(&a.v, v, s, s.kv_heads, s.k_len)))
@@ -1428,8 +1494,10 @@ cudaError_t attention_forward_launch(const csw_attention_shape& s, const csw_att
 cudaError_t attention_backward_launch(const csw_attention_shape& s, const AttentionBackward& b, cudaStream_t stream) {
   if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return cudaSuccess;
   if (const cudaError_t e = bind_context()) return e;
+  uint32_t* status;
+  if (const cudaError_t e = status_word(&status)) return e;
   Backward a;
-  a.s = shape_of(s);
+  a.s = shape_of(s, status);
   a.o = view_of(b.o), a.grad = view_of(b.dout);
   a.lse = b.lse, a.rows = b.workspace, a.padded = (uint32_t)whole_tiles(s.q_len);
   a.parts = parts_of(s), a.sums = b.workspace + row_values(s), a.k_padded = (uint32_t)whole_tiles(s.k_len);
@@ -1441,8 +1509,8 @@ cudaError_t attention_backward_launch(const csw_attention_shape& s, const Attent
   if (s.k_len && (!map_of(&a.k, b.k, s, s.kv_heads, s.k_len) || !map_of(&a.v, b.v, s, s.kv_heads, s.k_len) ||
                   !map_of(&a.dk, b.dk, s, s.kv_heads, s.k_len) || !map_of(&a.dv, b.dv, s, s.kv_heads, s.k_len)))
     return cudaErrorInvalidValue;
-  const View dk = view_of(b.dk), dv = view_of(b.dv);
-  return s.type == CSW_TYPE_F16 ? backward_of<__half>(a, s, dk, dv, stream) : backward_of<__nv_bfloat16>(a, s, dk, dv, stream);
+  a.dq_out = view_of(b.dq), a.dk_out = view_of(b.dk), a.dv_out = view_of(b.dv);
+  return s.type == CSW_TYPE_F16 ? backward_of<__half>(a, s, stream) : backward_of<__nv_bfloat16>(a, s, stream);
 }
 
 }  // namespace csw

@@ -17,8 +17,8 @@ csw_status device_state(int** d_status);
 // device and synchronises nothing.
 int sm_count();
 
-// Reads (and clears) the status word of the kernels that wait on their own copies, on the CURRENT device; set by the
-// translation unit that has them, null in a program linked without it.
+// Reads (and clears) the status word of the kernels that wait on their own copies, of the CURRENT device, without waiting for
+// them; set by the translation unit that has them, null in a program linked without it.
 extern cudaError_t (*take_kernel_status)(int* value);
 
 }  // namespace csw

@@ -54,6 +54,12 @@ bool attention_args(const csw_attention_shape* s) {
   if (rows && ((s->q_len + 127) / 128 > kMostRows / rows || (s->k_len + 127) / 128 > kMostRows / rows)) return false;
   return s->kv_lens == nullptr || aligned(s->kv_lens, 4);
 }
+// An earlier call's kernel that gave up on a wait is told here, to a call that has something to launch.
+csw_status before_attention() {
+  int gave_up = 0;
+  const csw_status st = done(attention_take_status(&gave_up));
+  return st != CSW_OK ? st : gave_up ? CSW_ERR_TIMEOUT : CSW_OK;
+}
 
 }  // namespace
 
@@ -141,7 +147,14 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
       !operand(v, shape, s.kv_heads, s.k_len) || !operand(o, shape, s.heads, s.q_len))
     return CSW_ERR_ARG;
   if (s.batch * s.q_len != 0 && !good(d_lse, CSW_TYPE_F32)) return CSW_ERR_ARG;
-  return done(attention_forward_launch(s, *q, *k, *v, *o, d_lse, stream));
+  const csw_status st = s.batch && s.q_len ? before_attention() : CSW_OK;
+  return st != CSW_OK ? st : done(attention_forward_launch(s, *q, *k, *v, *o, d_lse, stream));
+}
+
+csw_status csw_attention_wait_limit(int64_t clocks) {
+  if (clocks == INT64_MIN) return CSW_ERR_ARG;
+  attention_wait_limit(clocks);
+  return CSW_OK;
 }
 
 csw_status csw_attention_workspace(const csw_attention_shape* shape, size_t* bytes) {
@@ -165,6 +178,8 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
     if (!operand(p, shape, s.kv_heads, s.k_len)) return CSW_ERR_ARG;
   if (need && (!good(d_lse, CSW_TYPE_F32) || !d_workspace || !aligned(d_workspace, 16))) return CSW_ERR_ARG;
   if (workspace_bytes < need) return CSW_ERR_SIZE;
+  const csw_status st = s.batch && (s.q_len || s.k_len) ? before_attention() : CSW_OK;
+  if (st != CSW_OK) return st;
   return done(attention_backward_launch(s, {*q, *k, *v, *o, *dout, *dq, *dk, *dv, d_lse, (float*)d_workspace}, stream));
 }
 

@@ -1,8 +1,9 @@
 // The instructions that the attention kernels are built on: mbarriers, tile copies (TMA), and the fifth-generation
 // tensor cores with their accumulators in tensor memory (tcgen05).
 //
-// Every wait on an mbarrier is bounded: where it runs out, the kernel sets a status word that the host reads
-// (csw_device_status), its warps leave their loops, and it frees its tensor memory and returns.
+// Every wait on an mbarrier is bounded: where it runs out, the kernel sets a status word in host memory (the next call and
+// csw_device_status look at it), its warps leave their loops, and it fills its results with NaN, frees its tensor memory
+// and returns.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -37,16 +38,16 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok;
 }
-__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, long long patience) {
   const long long start = clock64();
   do {
     if (bar_try(bar, parity)) return true;
-  } while (clock64() - start < (1ll << 32));
+  } while (clock64() - start < patience);
   return false;
 }
-// true once the phase of this parity is over; false where it does not end within two seconds or so
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  return bar_try(bar, parity) || bar_wait_on(bar, parity);
+// true once the phase of this parity is over; false where it does not end within `patience` clocks or so
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long long patience) {
+  return bar_try(bar, parity) || bar_wait_on(bar, parity, patience);
 }
 __device__ __forceinline__ void init_visible() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 // shared memory written by ordinary stores, before the tensor cores or a tile copy see it
@@ -85,12 +86,14 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 // where a bar.sync with a warp that has given up would never end.  A meeting cannot end before all have come to it, so
 // that nobody is two ahead and the parity tells.
 struct Meeting {
-  uint32_t bar, met = 0;
+  uint32_t bar;
+  long long patience;
+  uint32_t met = 0;
   // false where the others have not come
   __device__ __forceinline__ bool operator()() {
     __syncwarp();  // what all lanes have written is in front of the arrival
     if (threadIdx.x % 32 == 0) bar_arrive(bar);
-    return __all_sync(0xffffffffu, bar_wait(bar, met++ & 1));
+    return __all_sync(0xffffffffu, bar_wait(bar, met++ & 1, patience));
   }
 };
 

@@ -204,6 +204,14 @@ def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     return _ext().attention_backward(do, q, k, v, causal, kv_lens, scale, o, lse)
 
 
+def device_status(device=None) -> None:
+    """Waits for the current stream of `device` (the current one unless given) and raises CswapError where a kernel there
+    gave up on a wait for its own copies or products; it is told once.  The results of such a call are NaN, and the next
+    call of an attention pass on the device raises the same, so that a program need not ask."""
+    with torch.cuda.device(device):
+        check(lib().csw_device_status(torch.cuda.current_stream().cuda_stream), "csw_device_status")
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, kv_lens, scale):

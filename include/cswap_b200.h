@@ -56,7 +56,8 @@ const char* csw_version(void);
 /* Reads (and clears) the device-side status word of the current device:
  * CSW_OK, or CSW_ERR_TIMEOUT if a kernel gave up on a bounded wait.
  * Synchronises `stream` first.  No kernel waits on another CTA or on a flag; those
- * of attention wait, for a bounded time, on their own copies and products. */
+ * of attention wait, for a bounded time, on their own copies and products (section 7
+ * says what becomes of their results). */
 csw_status csw_device_status(csw_stream_t stream);
 
 /* ---- 2. ZFP fixed-rate float32 ------------------------------------------- */
@@ -402,6 +403,13 @@ typedef struct {
   void* data;
   ptrdiff_t batch_stride, head_stride, token_stride;
 } csw_attention_operand;
+/* The kernels' warps wait for one another's copies and products, each time for two seconds or so at the most.  Where that
+ * runs out, which takes a fault of the device, what the CTA in question had to compute is NaN, in the results and in the
+ * gradients that follow from them, and the next call of csw_attention_forward or csw_attention_backward on that device,
+ * or csw_device_status, returns CSW_ERR_TIMEOUT, once; that call launches nothing.  csw_attention_wait_limit sets the time
+ * for the calls of this process from now on, in clocks of an SM (2^32 to begin with).  A negative one lets the waits run
+ * out after -clocks, since the copies they are for are not begun: what a program does then can be tried out with it. */
+csw_status csw_attention_wait_limit(int64_t clocks);
 /* d_lse: batch x heads x q_len float32, the natural logarithm of each row's sum of exp(scale q.k). */
 csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_attention_operand* q,
                                  const csw_attention_operand* k, const csw_attention_operand* v,
