@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
@@ -431,21 +432,36 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// check_capture(tensors): while a graph is captured, refuses leaves whose gradient accumulator a graph of another
-// stream keeps.  Backward would hand the gradient over to that stream in the middle of the capture, an error that
-// autograd's threads do not survive.
+// The gradient accumulator of the leaf that a tensor is, or is a view, a copy or another function of alone; null where there
+// is none, or where the tensor depends on more than one.
+std::shared_ptr<torch::autograd::Node> accumulator_of(const at::Tensor& t) {
+  if (t.is_leaf()) return torch::autograd::impl::try_get_grad_accumulator(t);
+  std::shared_ptr<torch::autograd::Node> node = t.grad_fn();
+  while (node && !node->next_edges().empty()) {
+    std::shared_ptr<torch::autograd::Node> next;
+    for (const torch::autograd::Edge& e : node->next_edges()) {
+      if (!e.is_valid()) continue;
+      if (next) return nullptr;
+      next = e.function;
+    }
+    node = std::move(next);
+  }
+  return node && dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()) ? node : nullptr;
+}
+
+// check_capture(tensors): while a graph is captured, refuses leaves, also behind views and copies, whose gradient
+// accumulator a graph of another stream keeps.  Backward would hand the gradient over to that stream in the middle of the
+// capture, an error that autograd's threads do not survive.
 PyObject* check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    bool capturing = false, asked = false;
     for (Py_ssize_t i = 0; i < n; ++i) {
       if (!THPVariable_Check(a[i])) continue;
       const at::Tensor& t = THPVariable_Unpack(a[i]);
-      if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
-      const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+      if (!t.is_cuda() || !t.requires_grad()) continue;
+      const c10::cuda::CUDAGuard on(t.device());  // the operands of a call are on one device, and refused otherwise
+      if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) break;
+      const auto node = accumulator_of(t);
       if (!node) continue;
-      if (!asked) capturing = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
-      asked = true;
-      if (!capturing) break;
       const auto stream = node->stream();
       if (stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap()) {
         PyErr_SetString(PyExc_RuntimeError,

@@ -18,7 +18,8 @@ device, take float32, float16 or bfloat16 (attention: the last two), compute in 
 once.  The same call gives the same bits every time.  There is no CPU implementation.
 
 A step that is captured into a CUDA graph must not share a leaf with a live graph of another stream (autograd would
-hand that leaf's gradient over to the other stream inside the capture); such a call raises.
+hand that leaf's gradient over to the other stream inside the capture); a call on such a leaf, or on a view or a copy of
+one, raises.  A leaf that lies further back (a weight of a projection, say) is the step's own to look after.
 """
 from __future__ import annotations
 
