@@ -159,8 +159,8 @@ class BertEncoder(nn.Module):
         def heads(t):
             return t.view(B, S, nh, dh).transpose(1, 2).to(torch.bfloat16)
 
-        def norm(ln, a, b):
-            return layer_norm(a, ln.weight, ln.bias, ln.eps, residual=b)
+        def norm(ln, a, b):  # under autocast a product's type is not that of the sum it goes into
+            return layer_norm(a.to(b.dtype), ln.weight, ln.bias, ln.eps, residual=b)
 
         for l in range(self.nlayers):
             q = step(self.q[l], x, LayerType.FC)
