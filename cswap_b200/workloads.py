@@ -15,6 +15,8 @@ weights are randomly initialised.
 """
 from __future__ import annotations
 
+import warnings
+
 from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
@@ -117,13 +119,16 @@ def vgg16_reference_policy(exe: Execution, compressed: int = POLICY_ZFP) -> None
 # BERT-style encoder (bert.cpp:370-801)
 # ---------------------------------------------------------------------------
 class BertEncoder(nn.Module):
-    """`lean`: attention that keeps one number a row (in bfloat16, its probabilities without dropout), a feed-forward
-    part that keeps its activation in 8 bits, norms that take the residual's sum with them.  The parameters are the
-    same, so that a state of one kind loads into the other."""
+    """`lean`: attention that keeps its output and one number a row besides its operands (in bfloat16, its probabilities
+    without dropout, of which a warning tells where `dropout` is not 0), a feed-forward part that keeps its activation in 8
+    bits, norms that take the residual's sum with them.  The parameters are the same, so that a state of one kind loads
+    into the other."""
 
     def __init__(self, vocab: int = 30522, hidden: int = 768, layers: int = 12, heads: int = 12, ffn: int = 3072,
                  max_seq: int = 512, dropout: float = 0.1, lean: bool = False):
         super().__init__()
+        if lean and dropout > 0:
+            warnings.warn("BertEncoder(lean=True) drops out activations alone: its attention has no dropout on probabilities")
         self.lean = lean
         self.hidden, self.heads, self.nlayers, self.p = hidden, heads, layers, dropout
         self.tok = nn.Embedding(vocab, hidden)
