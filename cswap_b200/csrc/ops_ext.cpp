@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <algorithm>
 #include <cmath>
 
 using namespace cswext;
@@ -45,6 +46,12 @@ bool require_f32(const at::Tensor& t, const at::Tensor& as, int64_t n, const cha
   if (t.scalar_type() != at::kFloat) return value_error("%s must be float32", name);
   if (t.numel() != n) return value_error("%s has the wrong number of values", name);
   return require_flat(t, name);
+}
+// an output that the caller gives, of which `written` bytes are written while others of `read` may not have been read
+bool require_apart(const at::Tensor& out, size_t written, const at::Tensor& in, size_t read) {
+  const char *a = static_cast<const char*>(out.const_data_ptr()), *b = static_cast<const char*>(in.const_data_ptr());
+  const bool apart = written == 0 || read == 0 || a + written <= b || b + read <= a;
+  return apart || value_error("%s overlaps the input", "out");
 }
 bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
   *t = nullptr;
@@ -88,7 +95,8 @@ bool packed_out(PyObject* o, const at::Tensor& like, size_t n, at::Tensor* packe
   const at::Tensor* t = as_tensor(o, "out");
   if (!t) return false;
   if (t->scalar_type() != at::kByte) return value_error("%s must be uint8", "out");
-  if (!same_device(*t, like, "out") || !require_flat(*t, "out")) return false;
+  if (!same_device(*t, like, "out") || !require_flat(*t, "out") || !require_apart(*t, need, like, like.nbytes()))
+    return false;
   *packed = *t;
   return true;
 }
@@ -120,7 +128,7 @@ PyObject* q8_compress(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // q8_decompress(packed, numel, dtype, out) -> tensor
 PyObject* q8_decompress(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    size_t numel;
+    size_t numel, need;
     int type;
     if (!arg_count(n, 4)) return nullptr;
     const at::Tensor* packed = as_tensor(a[0], "packed");
@@ -136,7 +144,6 @@ PyObject* q8_decompress(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return nullptr;
       }
       const at::ScalarType kind = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
-      size_t need;
       if (type_code(kind) < 0) {
         value_error("%s must be float32, float16 or bfloat16", "dtype");
         return nullptr;
@@ -149,7 +156,9 @@ PyObject* q8_decompress(PyObject*, PyObject* const* a, Py_ssize_t n) {
       dst = fresh(*packed, {(int64_t)numel}, kind);
     } else {
       const at::Tensor* o = as_tensor(a[3], "out");
-      if (!o || !same_device(*o, *packed, "out") || !require_flat(*o, "out")) return nullptr;
+      if (!o || !same_device(*o, *packed, "out") || !require_flat(*o, "out") || !q8_bytes(numel, &need) ||
+          !require_apart(*o, o->nbytes(), *packed, std::min<size_t>(need, packed->nbytes())))
+        return nullptr;
       if ((size_t)o->numel() != numel) {
         value_error("%s has the wrong number of values", "out");
         return nullptr;

@@ -60,13 +60,13 @@ def q8_compress(t: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
 
     With m the largest magnitude of a group of 128 consecutive values, its scale is m / 127 and a value's code
     rint(x * (127 / m)); a value is off by at most m / 254 and a rounding.  A group below 2**-120 is held as zeros, a
-    group with a NaN or an infinity as NaNs.  `out` (16-byte aligned) may be longer than needed."""
+    group with a NaN or an infinity as NaNs.  `out` (16-byte aligned, apart from `t`) may be longer than needed."""
     return _ext().q8_compress(t, out)
 
 
 def q8_decompress(packed: torch.Tensor, numel: int, dtype: torch.dtype = torch.float32,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The `numel` values that a checkpoint holds, flat, or in `out` (whose type then counts)."""
+    """The `numel` values that a checkpoint holds, flat, or in `out` (whose type then counts, apart from `packed`)."""
     return _ext().q8_decompress(packed, numel, dtype, out)
 
 

@@ -16,7 +16,6 @@ weights are randomly initialised.
 from __future__ import annotations
 
 import warnings
-
 from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch

@@ -355,7 +355,8 @@ enum { CSW_TYPE_F32 = 0, CSW_TYPE_F16 = 1, CSW_TYPE_BF16 = 2 };
 /* 8-bit checkpoint of n values: [codes: n int8][from the next multiple of 16 bytes: ceil(n/128) float32 scales].
  * Groups of 128 consecutive values share a scale.  With m the group's largest magnitude, scale = m / 127 and
  * code = rint(x * (127 / m)), ties to even, each step one float32 operation; the value held is code * scale.  Groups
- * with m < 2^-120 are held as zeros, groups with a NaN or an infinity as NaNs.  The buffer is 16-byte aligned. */
+ * with m < 2^-120 are held as zeros, groups with a NaN or an infinity as NaNs.  The buffer is 16-byte aligned, and
+ * apart from that of the values. */
 csw_status csw_q8_bytes(size_t n, size_t* bytes);
 csw_status csw_q8_compress(const void* d_in, int type, size_t n, void* d_out, size_t cap, csw_stream_t stream);
 csw_status csw_q8_decompress(const void* d_in, size_t bytes, size_t n, void* d_out, int type, csw_stream_t stream);
