@@ -817,8 +817,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
     // D of the piece's rows, DP / 8 lanes a row; they are read before the next piece's results are waited for.  False
     // where a wait ran out, as below.
     float shift = INFINITY, delta = 0.0f;  // of this thread's row of the piece that was prepared last
-    bool live = false;                     // whether it sees any key
     auto prepare = [&](const Piece& p, int u) -> bool {
+      const int own = p.first + t;
+      const float lse = own < (int)s.q_len ? a.lse[(uint64_t)p.row * s.q_len + own] : 0.0f;
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes, kAtOnce = 8;
       const int lane = t % kLanes, mine = t / 32 * 32 + t % 32 / kLanes;
 #pragma unroll
@@ -846,10 +847,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
           if (lane == 0) deltas[u & 1][mine + (i + k) * kRows] = d;
         }
       }
-      const int row = p.first + t;
-      live = row < (int)s.q_len && s.limit(row, p.keys) > 0;
-      const float lse = live ? a.lse[(uint64_t)p.row * s.q_len + row] : 0.0f;
-      shift = !live ? INFINITY : fabsf(lse) == INFINITY ? NAN : lse * kLog2e;
+      // +inf for rows that see nothing alone: probabilities that an infinite L stands for are NaN
+      shift = fabsf(lse) == INFINITY ? NAN : lse * kLog2e;
+      if (own >= (int)s.q_len || s.limit(own, p.keys) <= 0) shift = INFINITY;
       shifts[u & 1][t] = shift;
       if (!group()) return false;
       delta = deltas[u & 1][t];
@@ -857,7 +857,8 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
       return true;
     };
     // The results of a piece that sees n tiles, and its row's exponent shift and D; false where a wait ran out.
-    auto finish = [&](const Piece& p, int n, int u, bool live, float shift, float d) -> bool {
+    auto finish = [&](const Piece& p, int n, int u, float shift, float d) -> bool {
+      const bool live = shift != INFINITY;
       float off = 0.0f;
       if (n > 0) {
         if (!__all_sync(0xffffffffu, bar_wait(left_ready.bar(u), left_ready.parity(u), s.patience) && bar_wait(dq_full, u & 1, s.patience))) return false;
@@ -908,16 +909,15 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dq_ke
         Piece piece;
         if (!hear(work, work_bars, s, it, &piece)) return give_up(flag);
         const int n = piece.first >= 0 ? Queries<1>(s, piece).most : 0;
-        const bool last_live = live;
         const float last_shift = shift, last_delta = delta;
         if (n > 0 && !prepare(piece, u)) return give_up(flag);
-        if (last.first >= 0 && !finish(last, last_n, u - 1, last_live, last_shift, last_delta)) return give_up(flag);
+        if (last.first >= 0 && !finish(last, last_n, u - 1, last_shift, last_delta)) return give_up(flag);
         last.first = -1;
         if (piece.first < 0) return;
         if (n > 0) {
           last = piece, last_n = n;
           ++u;
-        } else if (!finish(piece, 0, 0, false, INFINITY, 0.0f)) {
+        } else if (!finish(piece, 0, 0, INFINITY, 0.0f)) {
           return give_up(flag);
         }
       }
