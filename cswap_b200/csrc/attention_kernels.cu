@@ -24,11 +24,19 @@
 //
 // What bounds it.  For 128 x 128 scores the tensor cores take 256 clocks a product with heads of 64 and 512 with heads of
 // 128, the exponentials 1024 (16 a clock and SM; a quarter of them go by polynomial instead), and the rest of the
-// softmax's instructions about as long again.  Heads of 128, 4096 causal tokens, 32 heads on 8: forward 120 us
-// (1145 TFLOP/s of the pairs that the mask leaves; a large library product reaches 1634), dq 196, dkv 216; the tensor
-// cores are busy 59, 53 and 70 % of the time.  Heads of 64, 32 sentences of 128 to 512 tokens, 12 heads: forward 44 us,
-// dq 66, dkv 60 (24, 24 and 33 % busy): some 2400 clocks a tile of backward, which the softmax warps spend one phase
-// after the other (1250 on exponentials, 450 on gradients, the rest on loads, stores and hand-overs).
+// softmax's instructions about as long again.  Each kernel by itself, its inputs cold: heads of 128, 4096 causal tokens,
+// 32 heads on 8: forward 122 us (1126 TFLOP/s of the pairs that the mask leaves; a large library product reaches 1634), dq
+// 193, dkv 221; the tensor cores are busy 59, 53 and 69 % of the time.  Twenty passes of all three in a row take 514 each at
+// 1965 MHz, thousands 600 at the 1640 that the power limit leaves.  Heads of 64, 32 sentences of 128 to 512 tokens,
+// 12 heads: forward 45 us, dq 67, dkv 61 (24, 24 and 33 % busy): some 2400 clocks a tile of backward, which the softmax
+// warps spend one phase after the other (1250 on exponentials, 450 on gradients, the rest on loads, stores and hand-overs).
+//
+// Numbers that are not: a NaN or an infinity that a query sees shows in its results as the formulas have it.  What the
+// masks hide counts for nothing where it lies behind a sequence, or belongs to a query that sees no key.
+//
+// That the running maximum is followed only where it grows much, and that a part of the exponentials goes by polynomial,
+// are published methods for attention on this generation of tensor cores; range reduction and polynomial are those of any
+// exponential (Cody and Waite), the coefficients fitted here.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -1087,6 +1095,9 @@ __global__ void __launch_bounds__(BackwardPlan<DP>::kThreads, 1) attention_dkv_k
         copy_tokens<DP>(to + Plan::kTileBytes, &a.v, here, p.first, kv_head, p.batch);
         const uint64_t plane = (uint64_t)a.s.batch * a.s.heads * a.padded;
         int q = at.q, h = at.head;
+        // A tile of do is free, for what the products need, before the softmax warps have read the D that came with it.
+        // It is not written earlier all the same: the tile of q in front of it in the ring is waited for first, and that is
+        // free behind the product that takes the gradients made with D.
         for (int j = 0; j < 2 * at.n; ++j, ++i) {
           const int slot = i % kRing;
           if (i >= kRing && !bar_wait(empty + 8 * slot, (i / kRing - 1) & 1, a.s.patience)) return false;

@@ -117,8 +117,10 @@ struct Rows {
   static constexpr int kBlock = THREADS <= 32 ? 128 : THREADS, kTogether = kBlock / THREADS;
   // CTAs an SM should have room for: 64 registers a thread forward, 80 or more backward
   static constexpr int kForward = 1024 / kBlock, kBackward = kBlock > 768 ? 1 : 768 / kBlock;
-  // Rows at once, backward, where a CTA has an SM to itself: a row waits for its sums' way through shuffles and shared
-  // memory, which then serves two (16384 x 4096 bfloat16 93 us, 106 one at a time).
+  // Rows at once, backward, where a CTA has an SM to itself and the registers for two: a row waits for its sums' way through
+  // shuffles and shared memory, which then serves both (16384 x 4096 bfloat16 93 us, 106 one at a time).  CTAs of 768 and
+  // 1024 threads have 80 and 64 registers a thread, which two rows do not fit into (67 million bfloat16 values, rows of
+  // 6144: 114 us one at a time, 177 two at once; of 8192: 124 and 146).
   static constexpr int kAtOnce = sizeof(T) == 2 && THREADS == 512 ? 2 : 1;
   uint64_t rows, total;  // total: values
   uint32_t cols, period;
@@ -206,8 +208,10 @@ __global__ void __launch_bounds__(Rows<T, VEC, ITER, THREADS, SHIFTED>::kBlock,
       }
     }
   };
-  // The next row's values are on their way while a row is worked on, where registers allow it (768 columns: 77 us for
-  // 67 million float16 values, 99 otherwise; but 88 us for half as many of float32, 59 otherwise).
+  // The next row's values are on their way while a row is worked on, for sixteen-bit values: 67 million bfloat16 ones, cold,
+  // in rows of 64, 768, 4096 and 8192 columns take 72, 82, 102 and 137 us, 78, 105, 115 and 165 without.  Of float32, half as
+  // many take 55, 94 and 82 us in rows of 64, 768 and 2048 with it, 53, 66 and 64 without; rows of 4096 and more, which
+  // it would help (70 us against 74, at 8192 82 against 107), go without as well.
   constexpr bool kAhead = sizeof(T) == 2;
   Held now, next;
   if (kAhead && at.row < at.rows) load(at.row, next);

@@ -21,7 +21,7 @@ producer's own input, which is in turn swapped in or rebuilt as needed.  Only
 stateless callables may be passed (a BatchNorm module would update its running
 statistics a second time; pass a closure over F.batch_norm without them).  A
 tensor whose producer was not given stays on the device.  Policy 8, the
-framework's own, keeps the tensor on the device as an 8-bit checkpoint
+framework's own, keeps the tensor (float32, as all that the engine tracks) on the device as an 8-bit checkpoint
 (`ops.q8_compress`, 1.03 bytes a value) and takes the values it holds for
 backward: no link time, a quarter of the memory.  `policy_` 3 and 4
 select the vDNN and SuperNeurons baselines as in Execution.h:70,243,248.

@@ -9,7 +9,7 @@ operators keep less to begin with, beside the codecs that shrink or move what is
 * ``gelu`` keeps its input as such a checkpoint, written in the pass that computes the output; ``gelu_linear`` with the
   linear layer behind it keeps nothing else: backward forms the activation again for the weight's gradient.
 * ``layer_norm``, optionally of a sum of two tensors, keeps what is normed and two numbers a row.
-* ``attention`` keeps one number a row besides its operands; backward forms the probabilities again.
+* ``attention`` keeps its output and one number a row besides its operands; backward forms the probabilities again.
 
 ``gelu``, ``gelu_linear``, ``layer_norm`` and ``attention`` are differentiable (once).  Below them lie the passes
 themselves, ``*_forward`` and ``*_backward``, for programs that drive their own backward pass; they take contiguous
