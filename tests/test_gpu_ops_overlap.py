@@ -21,6 +21,6 @@ def test_outputs_over_the_input():
         with pytest.raises(ValueError, match="overlaps"):
             cs.q8_decompress(packed, 256, out=space[at:at + 512].view(torch.float16))
     cs.q8_decompress(packed, 256, out=space[272:272 + 512].view(torch.float16))
-    cs.q8_compress(space[2048:3072].view(torch.float32), out=space[1024:])  # longer than it needs to be
+    cs.q8_compress(space[2560:3584].view(torch.float32), out=space[1024:])  # longer than it needs to be
     cs.q8_compress(x[:0], out=space[1024:1040])  # nothing is read
     torch.cuda.synchronize()
