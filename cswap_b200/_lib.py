@@ -94,6 +94,23 @@ class AttentionOperand(C.Structure):
                 ("token_stride", C.c_ssize_t)]
 
 
+class Fp8Matrix(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t),
+                ("code_stride", C.c_size_t), ("transposed", C.c_int)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("copy", C.c_void_p), ("exp_avg", C.c_void_p),
+                ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p),
+                ("numel", C.c_size_t), ("param_type", C.c_int), ("grad_type", C.c_int), ("copy_type", C.c_int)]
+
+
+class AdamwOptions(C.Structure):
+    _fields_ = [("bits", C.c_int), ("seed", C.c_uint32), ("step", C.c_int64), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("max_norm", C.c_double),
+                ("d_step", C.c_void_p), ("d_lr", C.c_void_p), ("d_norm", C.c_void_p)]
+
+
 _P = C.c_void_p
 _SZ = C.c_size_t
 _SSZ = C.c_ssize_t
@@ -102,6 +119,8 @@ _I = C.c_int
 _F = C.c_float
 _SH = C.POINTER(AttentionShape)
 _OP = C.POINTER(AttentionOperand)
+_MX = C.POINTER(Fp8Matrix)
+_AT = C.POINTER(AdamwTensor)
 
 # name -> (restype, argtypes); every symbol the two headers declare
 SIGNATURES = {
@@ -161,6 +180,15 @@ SIGNATURES = {
     "csw_attention_wait_limit": (_I, [C.c_int64]),
     "csw_attention_workspace": (_I, [_SH, C.POINTER(_SZ)]),
     "csw_attention_backward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _OP, _OP, _OP, _OP, _P, _SZ, _P]),
+    "csw_fp8_quantize_workspace": (_I, [_SZ, _SZ, C.POINTER(_SZ)]),
+    "csw_fp8_quantize": (_I, [_P, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _P, _SZ, _P]),
+    "csw_fp8_dequantize": (_I, [_P, _SZ, _P, _SZ, _SZ, _P, _I, _P]),
+    "csw_fp8_matmul": (_I, [_MX, _MX, _P, _I, _P, _I, _P]),
+    "csw_adamw_step": (_I, [_AT, _SZ, C.POINTER(AdamwOptions), _P]),
+    "csw_adamw8_pack": (_I, [_AT, _SZ, _P]),
+    "csw_adamw8_unpack": (_I, [_AT, _SZ, _P]),
+    "csw_gradient_norm_workspace": (_I, [_AT, _SZ, C.POINTER(_SZ)]),
+    "csw_gradient_norm": (_I, [_AT, _SZ, _P, _P, _SZ, _P]),
     # reference-named entry points
     "PreGPUcompression": (None, [_I, _I, _P, _P, _I, _I, _P]),
     "PreAcc": (None, [_P, _I, _P, _I, _I, _P]),

@@ -13,8 +13,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcswap_b200.so")
 ROOT = os.path.dirname(HERE)
 SOURCES = ["zfp_kernels.cu", "sparse_kernels.cu", "cswap_abi.cu", "swap_manager.cu", "cost_model.cu",
-           "sparse_static.cu", "q8_kernels.cu", "norm_kernels.cu", "attention_kernels.cu", "ops_abi.cu"]
-HEADERS = ["hand_over.cuh", "values.cuh", "tensor_core.cuh", "q8_kernels.h", "norm_kernels.h", "attention_kernels.h",
+           "sparse_static.cu", "q8_kernels.cu", "norm_kernels.cu", "attention_kernels.cu", "fp8_kernels.cu", "optim_kernels.cu",
+           "waits.cu", "ops_abi.cu"]
+HEADERS = ["hand_over.cuh", "waits.h", "values.cuh", "tensor_core.cuh", "q8_kernels.h", "norm_kernels.h", "attention_kernels.h",
+           "fp8_kernels.h", "optim_kernels.h",
            "pdl.cuh", "zfp_core.cuh", "zfp_field.cuh", "zfp_kernels.h", "sparse_kernels.h", "tile_counts.cuh", "internal.h",
            os.path.join("..", "..", "include", "cswap_b200.h"), os.path.join("..", "..", "include", "cswap_compat.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -66,7 +68,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-EXT_SOURCES = [os.path.join(CSRC, s) for s in ("codec_ext.cpp", "ops_ext.cpp")]
+EXT_SOURCES = [os.path.join(CSRC, s) for s in ("codec_ext.cpp", "ops_ext.cpp", "step_ext.cpp")]
 EXT = os.path.join(HERE, "_codec_ext.so")
 EXT_STAMP = os.path.join(HERE, "build", "_codec_ext.built_for")
 

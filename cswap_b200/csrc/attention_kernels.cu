@@ -40,9 +40,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
-#include <cstring>
 #include <type_traits>
 
 #include "attention_kernels.h"
@@ -51,6 +49,7 @@
 #include "pdl.cuh"
 #include "tensor_core.cuh"
 #include "values.cuh"
+#include "waits.h"
 
 namespace csw {
 namespace {
@@ -1347,64 +1346,17 @@ __global__ void __launch_bounds__(256) attention_sums_kernel(const float* __rest
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-// A word of host memory for each device, which kernels write and the host reads without waiting for anything.
-constexpr int kMaxDevices = 64;
-uint32_t* status_words() {
-  static uint32_t* const words = [] {
-    // also while a stream is captured: the allocation has nothing to do with it
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    void* p = nullptr;
-    if (taken(cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return (uint32_t*)nullptr;
-    const size_t bytes = kMaxDevices * sizeof(uint32_t);
-    const cudaError_t e = taken(cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped));
-    taken(cudaThreadExchangeStreamCaptureMode(&mode));
-    if (e != cudaSuccess) return (uint32_t*)nullptr;
-    return (uint32_t*)std::memset(p, 0, bytes);
-  }();
-  return words;
-}
-cudaError_t status_word(uint32_t** word) {
-  int dev = 0;
-  if (const cudaError_t e = taken(cudaGetDevice(&dev))) return e;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  uint32_t* words = status_words();
-  *word = words + dev;
-  return words ? cudaSuccess : cudaErrorMemoryAllocation;
-}
-std::atomic<long long> wait_limit{1ll << 32};  // some two seconds
-
 Shape shape_of(const csw_attention_shape& s, uint32_t* status) {
   const float e = fmaxf(fabsf(s.scale) * kLog2e, 0x1p-100f);
-  const long long wait = wait_limit.load(std::memory_order_relaxed);
+  const long long wait = wait_limit();
   return {(uint32_t)s.batch, (uint32_t)s.heads, (uint32_t)s.kv_heads, (uint32_t)s.q_len, (uint32_t)s.k_len,
           (uint32_t)s.dim,   (uint32_t)(s.heads / s.kv_heads), s.causal, s.scale < 0.0f, s.scale, e, s.kv_lens,
           wait < 0 ? -wait : wait, wait < 0, status};
 }
 
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-Encode encoder() {
-  static const Encode f = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (taken(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r)) != cudaSuccess) return Encode();
-    return r == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(p) : Encode();
-  }();
-  return f;
-}
-
-// Describing a tensor for tile copies is a call of the driver, which needs the device's context on this thread; a
-// thread that has made no call of the runtime yet (autograd's, say) has none.
-cudaError_t bind_context() {
-  int dev = 0;
-  const cudaError_t e = cudaGetDevice(&dev);
-  return taken(e == cudaSuccess ? cudaSetDevice(dev) : e);
-}
-
 // tiles of 128 tokens x 64 columns of an operand
 bool map_of(CUtensorMap* map, const csw_attention_operand& o, const csw_attention_shape& s, uint64_t heads, uint64_t tokens) {
-  const Encode encode = encoder();
+  const TileEncoder encode = tile_encoder();
   if (!encode) return false;
   const cuuint64_t dims[4] = {s.dim, tokens, heads, s.batch};
   // the stride of an axis of one step is not looked at, but has to be one
@@ -1455,8 +1407,6 @@ cudaError_t backward_of(const Backward& a, const csw_attention_shape& s, cudaStr
   return s.dim <= 64 ? backward<T, 64>(a, s, stream) : backward<T, 128>(a, s, stream);
 }
 
-const bool registered = (take_kernel_status = attention_take_status, true);
-
 }  // namespace
 
 namespace {
@@ -1471,14 +1421,6 @@ int parts_of(const csw_attention_shape& s) {
 }
 uint64_t row_values(const csw_attention_shape& s) { return 2 * (uint64_t)s.batch * s.heads * whole_tiles(s.q_len); }
 }  // namespace
-
-cudaError_t attention_take_status(int* gave_up) {
-  uint32_t* word;
-  const cudaError_t e = status_word(&word);
-  if (e == cudaSuccess) *gave_up = (int)__atomic_exchange_n(word, 0u, __ATOMIC_RELAXED);
-  return e;
-}
-void attention_wait_limit(long long clocks) { wait_limit.store(clocks, std::memory_order_relaxed); }
 
 uint64_t attention_workspace_values(const csw_attention_shape& s) {
   const int parts = parts_of(s);

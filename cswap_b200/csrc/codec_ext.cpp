@@ -206,6 +206,7 @@ PyMODINIT_FUNC PyInit__codec_ext() {
   g_check = PyObject_GetAttrString(lib, "check");
   Py_DECREF(lib);
   PyObject* m = g_check ? PyModule_Create(&module) : nullptr;
-  if (m && PyModule_AddFunctions(m, cswap_ops_methods) != 0) Py_CLEAR(m);
+  for (PyMethodDef* more : {cswap_ops_methods, cswap_step_methods})
+    if (m && PyModule_AddFunctions(m, more) != 0) Py_CLEAR(m);
   return m;
 }

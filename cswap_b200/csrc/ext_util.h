@@ -3,8 +3,10 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -76,6 +78,58 @@ PyObject* guarded(F&& body) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- tensors of the training operators -------------------------------------------------------------------------------
+// The CSW_TYPE_* code of a tensor's type, -1 for another one
+inline int type_code(at::ScalarType t) {
+  return t == at::kFloat ? CSW_TYPE_F32 : t == at::kHalf ? CSW_TYPE_F16 : t == at::kBFloat16 ? CSW_TYPE_BF16 : -1;
+}
+inline bool require_values(const at::Tensor& t, const char* name, int* type) {
+  if (!t.is_cuda()) return value_error("%s must be a CUDA tensor (this path has no CPU implementation)", name);
+  *type = type_code(t.scalar_type());
+  if (*type < 0) return value_error("%s must be float32, float16 or bfloat16", name);
+  return true;
+}
+inline bool require_flat(const at::Tensor& t, const char* name) {
+  if (!t.is_contiguous()) return value_error("%s must be contiguous", name);
+  return true;
+}
+inline bool same_device(const at::Tensor& t, const at::Tensor& as, const char* name) {
+  if (t.device() != as.device()) return value_error("%s is on another device", name);
+  return true;
+}
+inline bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
+  *t = nullptr;
+  return o == Py_None || (*t = as_tensor(o, name)) != nullptr;
+}
+inline void* ptr(const at::Tensor& t) { return t.numel() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
+inline void* out(at::Tensor& t) { return t.numel() ? t.mutable_data_ptr() : nullptr; }
+
+// New tensors on a tensor's device, without the way through torch's dispatcher: the smallest calls are as long as their
+// allocations.
+inline at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+inline at::Tensor fresh(const at::Tensor& like) { return fresh(like, like.sizes(), like.scalar_type()); }
+
+// A new tuple of the tensors; an undefined one becomes None
+inline PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    PyObject* o = nullptr;
+    if (r) o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_XDECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+#define CSW_METHOD(name, doc) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, doc}
+
 }  // namespace cswext
 
-extern PyMethodDef cswap_ops_methods[];  // ops_ext.cpp
+extern PyMethodDef cswap_ops_methods[];   // ops_ext.cpp
+extern PyMethodDef cswap_step_methods[];  // step_ext.cpp

@@ -1,12 +1,15 @@
-// C ABI of the training operators: argument checking.  Declarations: include/cswap_b200.h, section 7.
+// C ABI of the training operators: argument checking.  Declarations: include/cswap_b200.h, sections 7 to 9.
 #include <cuda_runtime.h>
 
 #include "../../include/cswap_b200.h"
 #include "attention_kernels.h"
+#include "fp8_kernels.h"
 #include "internal.h"
 #include "norm_kernels.h"
+#include "optim_kernels.h"
 #include "pdl.cuh"
 #include "q8_kernels.h"
+#include "waits.h"
 
 using namespace csw;
 
@@ -55,11 +58,47 @@ bool attention_args(const csw_attention_shape* s) {
   return s->kv_lens == nullptr || aligned(s->kv_lens, 4);
 }
 // An earlier call's kernel that gave up on a wait is told here, to a call that has something to launch.
-csw_status before_attention() {
+csw_status before_waits() {
   int gave_up = 0;
-  const csw_status st = done(attention_take_status(&gave_up));
+  const csw_status st = done(take_status(&gave_up));
   return st != CSW_OK ? st : gave_up ? CSW_ERR_TIMEOUT : CSW_OK;
 }
+
+// codes and scales of a matrix, as the kernels can address them
+bool matrix(const void* codes, const void* scales, size_t rows, size_t cols, size_t stride) {
+  if (rows > kMostRows || cols > kMostRows) return false;
+  if (rows == 0 || cols == 0) return true;
+  if (fp8_blocks(rows) > kMostRows / fp8_blocks(cols)) return false;
+  return codes && scales && aligned(codes, 16) && stride % 16 == 0 && stride >= cols && stride <= ((size_t)1 << 39) && stride <= kMostValues / rows;
+}
+
+constexpr size_t kMostOfTensor = (size_t)1 << 41, kMostTensors = (size_t)1 << 24;
+bool adamw_list(const csw_adamw_tensor* t, size_t count) {
+  if (count > kMostTensors || (count && !t)) return false;
+  for (size_t i = 0; i < count; ++i)
+    if (t[i].numel > kMostOfTensor) return false;
+  return true;
+}
+// the state of a tensor in so many bits
+bool adamw_state(const csw_adamw_tensor& t, int bits) {
+  if (bits == 8) return t.exp_avg && t.exp_avg_sq && t.exp_avg_scale && t.exp_avg_sq_scale;
+  return good(t.exp_avg, CSW_TYPE_F32) && good(t.exp_avg_sq, CSW_TYPE_F32) && !t.exp_avg_scale && !t.exp_avg_sq_scale;
+}
+csw_status adamw8_convert(const csw_adamw_tensor* t, size_t count, bool pack, csw_stream_t stream) {
+  if (!adamw_list(t, count)) return CSW_ERR_ARG;
+  for (size_t i = 0; i < count; ++i)
+    if (t[i].numel && (!adamw_state(t[i], 8) || !good(t[i].param, CSW_TYPE_F32) || !good(t[i].copy, CSW_TYPE_F32)))
+      return CSW_ERR_ARG;
+  return done(adamw8_convert_launch(t, count, pack, stream));
+}
+bool gradients(const csw_adamw_tensor* t, size_t count) {
+  if (!adamw_list(t, count)) return false;
+  for (size_t i = 0; i < count; ++i)
+    if (t[i].numel && (!known_type(t[i].grad_type) || !good(t[i].grad, t[i].grad_type))) return false;
+  return true;
+}
+// the rate, decay or epsilon of an optimizer; also not a NaN
+bool rate(double v) { return v >= 0.0 && v <= 3.4e38; }
 
 }  // namespace
 
@@ -147,13 +186,13 @@ csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_att
       !operand(v, shape, s.kv_heads, s.k_len) || !operand(o, shape, s.heads, s.q_len))
     return CSW_ERR_ARG;
   if (s.batch * s.q_len != 0 && !good(d_lse, CSW_TYPE_F32)) return CSW_ERR_ARG;
-  const csw_status st = s.batch && s.q_len ? before_attention() : CSW_OK;
+  const csw_status st = s.batch && s.q_len ? before_waits() : CSW_OK;
   return st != CSW_OK ? st : done(attention_forward_launch(s, *q, *k, *v, *o, d_lse, stream));
 }
 
 csw_status csw_attention_wait_limit(int64_t clocks) {
   if (clocks == INT64_MIN) return CSW_ERR_ARG;
-  attention_wait_limit(clocks);
+  set_wait_limit(clocks);
   return CSW_OK;
 }
 
@@ -178,9 +217,103 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
     if (!operand(p, shape, s.kv_heads, s.k_len)) return CSW_ERR_ARG;
   if (need && (!good(d_lse, CSW_TYPE_F32) || !d_workspace || !aligned(d_workspace, 16))) return CSW_ERR_ARG;
   if (workspace_bytes < need) return CSW_ERR_SIZE;
-  const csw_status st = s.batch && (s.q_len || s.k_len) ? before_attention() : CSW_OK;
+  const csw_status st = s.batch && (s.q_len || s.k_len) ? before_waits() : CSW_OK;
   if (st != CSW_OK) return st;
   return done(attention_backward_launch(s, {*q, *k, *v, *o, *dout, *dq, *dk, *dv, d_lse, (float*)d_workspace}, stream));
+}
+
+csw_status csw_fp8_quantize_workspace(size_t rows, size_t cols, size_t* bytes) {
+  if (!bytes || rows > kMostRows || cols > kMostRows || (rows && cols > kMostValues / rows)) return CSW_ERR_ARG;
+  *bytes = rows > kFp8Block ? fp8_blocks(rows) * cols * sizeof(float) : 0;
+  return CSW_OK;
+}
+
+csw_status csw_fp8_quantize(const void* d_x, int type, size_t rows, size_t cols, size_t x_stride, void* d_codes,
+                            size_t code_stride, void* d_scales, float* d_sums, void* d_workspace, size_t workspace_bytes,
+                            csw_stream_t stream) {
+  size_t need;
+  if (!known_type(type) || !matrix(d_codes, d_scales, rows, cols, code_stride) ||
+      csw_fp8_quantize_workspace(rows, cols, &need) != CSW_OK)
+    return CSW_ERR_ARG;
+  if (rows && cols && (!good(d_x, type) || x_stride < cols || x_stride > kMostValues / rows)) return CSW_ERR_ARG;
+  if (d_sums && !aligned(d_sums, 4)) return CSW_ERR_ARG;
+  if (d_sums && need && !good(d_workspace, CSW_TYPE_F32)) return CSW_ERR_ARG;
+  if (d_sums && workspace_bytes < need) return CSW_ERR_SIZE;
+  return done(fp8_quantize_launch({d_x, type, rows, cols, x_stride, d_codes, code_stride, static_cast<uint8_t*>(d_scales),
+                                   d_sums, static_cast<float*>(d_workspace)},
+                                  stream));
+}
+
+csw_status csw_fp8_dequantize(const void* d_codes, size_t code_stride, const void* d_scales, size_t rows, size_t cols,
+                              void* d_out, int type, csw_stream_t stream) {
+  if (!known_type(type) || !matrix(d_codes, d_scales, rows, cols, code_stride)) return CSW_ERR_ARG;
+  if (rows && cols && !good(d_out, type)) return CSW_ERR_ARG;
+  if (rows && (cols + 7) / 8 > (kMostRows * 256) / rows) return CSW_ERR_ARG;
+  return done(fp8_dequantize_launch(d_codes, code_stride, static_cast<const uint8_t*>(d_scales), rows, cols, d_out, type,
+                                    stream));
+}
+
+csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, const void* d_bias, int bias_type, void* d_out,
+                          int type, csw_stream_t stream) {
+  if (!a || !b || !known_type(type)) return CSW_ERR_ARG;
+  for (const csw_fp8_matrix* m : {a, b})
+    if (!matrix(m->codes, m->scales, m->rows, m->cols, m->code_stride)) return CSW_ERR_ARG;
+  const size_t m = a->transposed ? a->cols : a->rows, k = a->transposed ? a->rows : a->cols;
+  const size_t n = b->transposed ? b->rows : b->cols;
+  if (k != (b->transposed ? b->cols : b->rows)) return CSW_ERR_ARG;
+  if (m == 0 || n == 0) return CSW_OK;
+  constexpr size_t kMost = kMostRows - 128;  // a tile's last row stays below 2^31
+  if (m > kMost || n > kMost || fp8_blocks(m) > kMostRows / 32 / ((n + 31) / 32)) return CSW_ERR_ARG;
+  if (!good(d_out, type)) return CSW_ERR_ARG;
+  if (d_bias && (!known_type(bias_type) || !good(d_bias, bias_type))) return CSW_ERR_ARG;
+  const csw_status st = before_waits();
+  if (st != CSW_OK) return st;
+  auto of = [](const csw_fp8_matrix& x) {
+    return Fp8Matrix{x.codes, static_cast<const uint8_t*>(x.scales), x.rows, x.cols, x.code_stride, x.transposed != 0};
+  };
+  return done(fp8_matmul_launch(of(*a), of(*b), d_bias, bias_type, d_out, type, stream));
+}
+
+csw_status csw_adamw_step(const csw_adamw_tensor* tensors, size_t count, const csw_adamw_options* options,
+                          csw_stream_t stream) {
+  if (!options || (options->bits != 8 && options->bits != 32) || !gradients(tensors, count)) return CSW_ERR_ARG;
+  const csw_adamw_options& o = *options;
+  if (!rate(o.lr) || !rate(o.eps) || !rate(o.weight_decay) || !(o.beta1 >= 0.0 && o.beta1 < 1.0) ||
+      !(o.beta2 >= 0.0 && o.beta2 < 1.0))
+    return CSW_ERR_ARG;
+  if (!o.d_step && o.step < 1) return CSW_ERR_ARG;
+  if (!aligned(o.d_step, 8) || !aligned(o.d_lr, 4) || !aligned(o.d_norm, 4)) return CSW_ERR_ARG;
+  if (o.d_norm && !rate(o.max_norm)) return CSW_ERR_ARG;
+  for (size_t i = 0; i < count; ++i) {
+    const csw_adamw_tensor& t = tensors[i];
+    if (t.numel == 0) continue;
+    if (!known_type(t.param_type) || !good(t.param, t.param_type) || !adamw_state(t, o.bits)) return CSW_ERR_ARG;
+    if (t.copy && (!known_type(t.copy_type) || !good(t.copy, t.copy_type))) return CSW_ERR_ARG;
+  }
+  return done(adamw_launch(tensors, count, o, stream));
+}
+
+csw_status csw_adamw8_pack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream) {
+  return adamw8_convert(tensors, count, true, stream);
+}
+csw_status csw_adamw8_unpack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream) {
+  return adamw8_convert(tensors, count, false, stream);
+}
+
+csw_status csw_gradient_norm_workspace(const csw_adamw_tensor* tensors, size_t count, size_t* bytes) {
+  if (!bytes || !adamw_list(tensors, count)) return CSW_ERR_ARG;
+  *bytes = gradient_norm_partials(tensors, count) * sizeof(double);
+  return CSW_OK;
+}
+csw_status csw_gradient_norm(const csw_adamw_tensor* tensors, size_t count, float* d_norm, void* d_workspace,
+                             size_t workspace_bytes, csw_stream_t stream) {
+  size_t need;
+  if (!gradients(tensors, count) || !good(d_norm, CSW_TYPE_F32) ||
+      csw_gradient_norm_workspace(tensors, count, &need) != CSW_OK)
+    return CSW_ERR_ARG;
+  if (need && (!d_workspace || !aligned(d_workspace, 8))) return CSW_ERR_ARG;
+  if (workspace_bytes < need) return CSW_ERR_SIZE;
+  return done(gradient_norm_launch(tensors, count, d_norm, static_cast<double*>(d_workspace), stream));
 }
 
 }  // extern "C"

@@ -3,9 +3,7 @@
 // 3 us on the GPU.
 #include "ext_util.h"
 
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
@@ -17,24 +15,6 @@ using namespace cswext;
 
 namespace {
 
-// The CSW_TYPE_* code of a tensor's type, -1 for another one
-int type_code(at::ScalarType t) {
-  return t == at::kFloat ? CSW_TYPE_F32 : t == at::kHalf ? CSW_TYPE_F16 : t == at::kBFloat16 ? CSW_TYPE_BF16 : -1;
-}
-bool require_values(const at::Tensor& t, const char* name, int* type) {
-  if (!t.is_cuda()) return value_error("%s must be a CUDA tensor (this path has no CPU implementation)", name);
-  *type = type_code(t.scalar_type());
-  if (*type < 0) return value_error("%s must be float32, float16 or bfloat16", name);
-  return true;
-}
-bool require_flat(const at::Tensor& t, const char* name) {
-  if (!t.is_contiguous()) return value_error("%s must be contiguous", name);
-  return true;
-}
-bool same_device(const at::Tensor& t, const at::Tensor& as, const char* name) {
-  if (t.device() != as.device()) return value_error("%s is on another device", name);
-  return true;
-}
 bool require_like(const at::Tensor& t, const at::Tensor& as, const char* name) {
   if (!same_device(t, as, name)) return false;
   if (t.scalar_type() != as.scalar_type()) return value_error("%s has another type than the input", name);
@@ -53,36 +33,6 @@ bool require_apart(const at::Tensor& out, size_t written, const at::Tensor& in, 
   const bool apart = written == 0 || read == 0 || a + written <= b || b + read <= a;
   return apart || value_error("%s overlaps the input", "out");
 }
-bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
-  *t = nullptr;
-  return o == Py_None || (*t = as_tensor(o, name)) != nullptr;
-}
-void* ptr(const at::Tensor& t) { return t.numel() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
-void* out(at::Tensor& t) { return t.numel() ? t.mutable_data_ptr() : nullptr; }
-
-// New tensors on a tensor's device, without the way through torch's dispatcher: the smallest calls are as long as their
-// allocations.
-at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
-  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
-}
-at::Tensor fresh(const at::Tensor& like) { return fresh(like, like.sizes(), like.scalar_type()); }
-
-// A new tuple of the tensors; an undefined one becomes None
-PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
-  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
-  Py_ssize_t i = 0;
-  for (const at::Tensor& t : ts) {
-    PyObject* o = nullptr;
-    if (r) o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
-    if (!o) {
-      Py_XDECREF(r);
-      return nullptr;
-    }
-    PyTuple_SET_ITEM(r, i++, o);
-  }
-  return r;
-}
-
 // ---- 8-bit checkpoints ---------------------------------------------------------------------------------------------
 bool q8_bytes(size_t n, size_t* need) { return status_ok(csw_q8_bytes(n, need), "csw_q8_bytes"); }
 bool packed_out(PyObject* o, const at::Tensor& like, size_t n, at::Tensor* packed) {
@@ -482,8 +432,6 @@ PyObject* check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   });
 }
-
-#define CSW_METHOD(name, doc) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, doc}
 
 }  // namespace
 

@@ -1,0 +1,430 @@
+// AdamW over many tensors at once, its state in 32 bits or in 8, and the norm of all gradients.
+//
+//   g' = c g,  c = min(1, max_norm / (norm + 1e-6)) where a norm is given
+//   m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// State in 8 bits.  Groups of 128 consecutive values of a tensor share a scale 2^E, held as the byte E + 127: E is the least
+// for which the group's largest magnitude is at most 1.75 2^E, but -126 at least; 0 stands for a group of zeros, 255 for one
+// with a value that is no number or beyond 1.75 2^126.  A code of m is a sign, 4 bits of exponent and 3 of mantissa, of v 5
+// and 3, the greatest exponent that of 2^E, with gradual underflow.  So the code is a float32 number's bits from the 20th on,
+// once the number is scaled to the foot of the type's range, where underflow comes by itself.
+//
+// Rounding.  v changes by a thousandth a step, half a code's step is 3 to 6 %: rounded to the nearest, v would stay where it
+// once was.  So the 20 bits that are cut off round up as often as they say, by random bits from the seed, the step, the tensor's
+// place in the call and the value's index: the averages are right in the mean, and the same call gives the same bits.  v is
+// not rounded to zero in a group that has anything: m's smallest step is 2^-17 of its group's scale, the root of v's smallest
+// 2^-16.5, so that m / sqrt(v) stays of the size that it has for the group's largest.
+//
+// Every 32-bit operation that a code depends on is rounded by itself (no fused multiply-add), so that the codes follow from
+// the definition whatever a compiler does.
+//
+// One launch takes hundreds of tensors: where they lie travels in the kernel's parameters, so that nothing is copied to the
+// device and a captured call holds all that it needs.
+#include "optim_kernels.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "internal.h"
+#include "pdl.cuh"
+#include "values.cuh"
+
+namespace csw {
+namespace {
+
+constexpr int kThreads = 256, kEach = 8;  // values of a thread: a sixteenth of a group
+constexpr uint32_t kPiece = kThreads * kEach;
+constexpr int kGroup = 128;
+
+struct Entry {
+  const void* grad;
+  void *param, *copy, *m, *v;
+  uint8_t *m_scale, *v_scale;
+  uint64_t numel;
+  uint8_t param_type, grad_type, copy_type;  // CSW_TYPE_*
+  bool packs;                                // all of the tensors lie so that 8 values of one are whole packs
+};
+template <int N>
+struct Table {
+  static constexpr int kSize = N;
+  Entry tensor[N];
+  uint32_t first[N + 1];  // pieces before each tensor
+  int count;
+  uint32_t place;  // of the first tensor in the call
+};
+// Kernel parameters are 32764 bytes at most.  A launch with the large table costs the host 2 us more.
+constexpr int kFew = 40, kMany = 380;
+
+struct Step {
+  float b1, rest1, b2, rest2, eps;
+  float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  const float* norm;
+  float max_norm;
+  uint32_t call;  // random bits of the call
+  // in place of the above where the program keeps them on the device
+  const int64_t* step;
+  const float* lr;
+  double wide_b1, wide_b2, wide_lr, wide_decay;
+  uint32_t seed;
+  int64_t host_step;
+};
+
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x9e3779b1u;
+  x ^= x >> 15;
+  x *= 0x85ebca77u;
+  return x ^ x >> 16;
+}
+__host__ __device__ __forceinline__ uint32_t random_of(uint32_t from, uint32_t place) { return mix(from + place * 0x9e3779b9u); }
+
+// What depends on the step and the learning rate, in 64 bits.
+__host__ __device__ inline void settle(Step& s, int64_t t, double lr) {
+  const double n = (double)(t > 1 ? t : 1);
+  s.decay = (float)(1.0 - lr * s.wide_decay);
+  s.size = (float)(lr / -expm1(n * log(s.wide_b1)));
+  s.root = (float)(1.0 / sqrt(-expm1(n * log(s.wide_b2))));
+  s.call = random_of(s.seed, (uint32_t)t);
+}
+
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t piece) {
+  int lo = 0, hi = t.count;  // first[lo] <= piece < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (t.first[mid] <= piece) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// 8 values from index i on, zeros behind the last one
+template <class T>
+__device__ __forceinline__ void load_of(const void* from, uint64_t i, int live, bool packs, float (&f)[kEach]) {
+  const T* p = static_cast<const T*>(from) + i;
+  if (packs && live == kEach) {
+    constexpr int kPack = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < kEach; j += kPack) {
+      float v[kPack];
+      load_pack(p + j, v);
+#pragma unroll
+      for (int k = 0; k < kPack; ++k) f[j + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) f[j] = j < live ? widen(p[j]) : 0.0f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_of(void* to, uint64_t i, int live, bool packs, const float (&f)[kEach]) {
+  T* p = static_cast<T*>(to) + i;
+  if (packs && live == kEach) {
+    constexpr int kPack = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < kEach; j += kPack) {
+      float v[kPack];
+#pragma unroll
+      for (int k = 0; k < kPack; ++k) v[k] = f[j + k];
+      store_pack(p + j, v);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < live) p[j] = narrow<T>(f[j]);
+  }
+}
+__device__ __forceinline__ void load_any(const void* from, int type, uint64_t i, int live, bool packs, float (&f)[kEach]) {
+  if (type == CSW_TYPE_F32) load_of<float>(from, i, live, packs, f);
+  else if (type == CSW_TYPE_F16) load_of<__half>(from, i, live, packs, f);
+  else load_of<__nv_bfloat16>(from, i, live, packs, f);
+}
+__device__ __forceinline__ void store_any(void* to, int type, uint64_t i, int live, bool packs, const float (&f)[kEach]) {
+  if (type == CSW_TYPE_F32) store_of<float>(to, i, live, packs, f);
+  else if (type == CSW_TYPE_F16) store_of<__half>(to, i, live, packs, f);
+  else store_of<__nv_bfloat16>(to, i, live, packs, f);
+}
+
+// ---- 8-bit codes ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint2 load_codes(const void* from, uint64_t i, int live, bool packs) {
+  const uint8_t* p = static_cast<const uint8_t*>(from) + i;
+  if (packs && live == kEach) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (j < live) w[j / 4] |= (uint32_t)p[j] << (j % 4 * 8);
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_codes(void* to, uint64_t i, int live, bool packs, uint2 codes) {
+  uint8_t* p = static_cast<uint8_t*>(to) + i;
+  if (packs && live == kEach) {
+    *reinterpret_cast<uint2*>(p) = codes;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < live) p[j] = (uint8_t)((j < 4 ? codes.x : codes.y) >> (j % 4 * 8));
+  }
+}
+// SIGNED: m, else v
+template <bool SIGNED>
+constexpr float kFoot = SIGNED ? 0x1p-112f : 0x1p-96f;  // from a group's scale to the foot of float32's range
+
+template <bool SIGNED>
+__device__ __forceinline__ void values_of(uint2 codes, uint32_t scale, float (&f)[kEach]) {
+  const float power = __uint_as_float(scale == 255 ? 0x7fc00000u : scale << 23);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const uint32_t c = (j < 4 ? codes.x : codes.y) >> (j % 4 * 8);
+    const uint32_t bits = SIGNED ? (c & 0x80u) << 24 | (c & 0x7fu) << 20 : (c & 0xffu) << 20;
+    f[j] = __fmul_rn(__fmul_rn(__uint_as_float(bits), 1.0f / kFoot<SIGNED>), power);
+  }
+}
+// The largest magnitude of a group's 16 threads, as bits; a NaN's are above all others.
+__device__ __forceinline__ uint32_t top_of(const float (&f)[kEach]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+  return top;
+}
+// codes of a group whose largest magnitude is top, and its scale; cut[j]: what is added to the 20 bits that are cut off
+template <bool SIGNED>
+__device__ __forceinline__ uint2 codes_of(const float (&f)[kEach], uint32_t top, const uint32_t (&cut)[kEach],
+                                          uint32_t* scale) {
+  const int e = max((int)(top >> 23) - 127 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
+  *scale = top == 0 ? 0 : e > 126 ? 255 : (uint32_t)(e + 127);
+  if (*scale == 0 || *scale == 255) return make_uint2(0, 0);
+  const float power = __uint_as_float((uint32_t)(127 - e) << 23);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(fabsf(f[j]), power), kFoot<SIGNED>));
+    uint32_t code = (bits + cut[j]) >> 20;
+    if (SIGNED) code |= __float_as_uint(f[j]) >> 24 & 0x80u;
+    else code = max(code, 1u);
+    w[j / 4] |= code << (j % 4 * 8);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// ---- the step -----------------------------------------------------------------------------------------------------------
+template <int N, bool EIGHT>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> table,
+                                                         const __grid_constant__ Step given) {
+  __shared__ Step computed;
+  pdl_wait();
+  const int at = tensor_of(table, blockIdx.x);
+  const Entry& t = table.tensor[at];
+  const uint64_t i = (uint64_t)(blockIdx.x - table.first[at]) * kPiece + threadIdx.x * kEach;
+  const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
+  float decay = given.decay, size = given.size, root = given.root;
+  uint32_t call = given.call;
+  if (given.step || given.lr) {
+    if (threadIdx.x == 0) {
+      computed = given;
+      settle(computed, given.step ? *given.step : given.host_step, given.lr ? (double)*given.lr : given.wide_lr);
+    }
+    __syncthreads();
+    decay = computed.decay, size = computed.size, root = computed.root, call = computed.call;
+  }
+  float c = 1.0f;
+  if (given.norm) {
+    const float q = __fdiv_rn(given.max_norm, __fadd_rn(*given.norm, 1e-6f));
+    c = q >= 1.0f ? 1.0f : q;  // NaN of a norm that is none
+  }
+  float g[kEach], p[kEach], m[kEach], v[kEach];
+  load_any(t.grad, t.grad_type, i, live, t.packs, g);
+  load_any(t.param, t.param_type, i, live, t.packs, p);
+  if constexpr (EIGHT) {
+    const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
+    values_of<true>(mc, live ? t.m_scale[i / kGroup] : 0, m);
+    values_of<false>(vc, live ? t.v_scale[i / kGroup] : 0, v);
+  } else {
+    load_of<float>(t.m, i, live, t.packs, m);
+    load_of<float>(t.v, i, live, t.packs, v);
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const float s = __fmul_rn(g[j], c);
+    m[j] = __fadd_rn(__fmul_rn(m[j], given.b1), __fmul_rn(s, given.rest1));
+    v[j] = __fadd_rn(__fmul_rn(v[j], given.b2), __fmul_rn(__fmul_rn(s, given.rest2), s));
+    p[j] = p[j] * decay - size * (m[j] / (sqrtf(v[j]) * root + given.eps));
+  }
+  store_any(t.param, t.param_type, i, live, t.packs, p);
+  if (t.copy) store_any(t.copy, t.copy_type, i, live, t.packs, p);
+  if constexpr (EIGHT) {
+    const uint32_t key = random_of(call, table.place + at) + (uint32_t)i;
+    uint32_t up[kEach], low[kEach], scale;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const uint32_t r = mix(key + j);
+      up[j] = r >> 16 << 4 | 8, low[j] = (r & 0xffffu) << 4 | 8;
+      if (j >= live) m[j] = v[j] = 0.0f;
+    }
+    const uint2 mc = codes_of<true>(m, top_of(m), up, &scale);
+    store_codes(t.m, i, live, t.packs, mc);
+    if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)scale;
+    const uint2 vc = codes_of<false>(v, top_of(v), low, &scale);
+    store_codes(t.v, i, live, t.packs, vc);
+    if (live && threadIdx.x % 16 == 0) t.v_scale[i / kGroup] = (uint8_t)scale;
+  } else {
+    store_of<float>(t.m, i, live, t.packs, m);
+    store_of<float>(t.v, i, live, t.packs, v);
+  }
+}
+
+// The state in 8 bits from and to averages in 32, which stand in the places of param and copy; rounded to the nearest.
+template <int N, bool PACK>
+__global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table) {
+  pdl_wait();
+  const int at = tensor_of(table, blockIdx.x);
+  const Entry& t = table.tensor[at];
+  const uint64_t i = (uint64_t)(blockIdx.x - table.first[at]) * kPiece + threadIdx.x * kEach;
+  const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
+  float m[kEach], v[kEach];
+  if constexpr (PACK) {
+    load_of<float>(t.param, i, live, t.packs, m);
+    load_of<float>(t.copy, i, live, t.packs, v);
+    uint32_t half[kEach], scale;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) half[j] = 1u << 19;
+    const uint2 mc = codes_of<true>(m, top_of(m), half, &scale);
+    store_codes(t.m, i, live, t.packs, mc);
+    if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)scale;
+    const uint2 vc = codes_of<false>(v, top_of(v), half, &scale);
+    store_codes(t.v, i, live, t.packs, vc);
+    if (live && threadIdx.x % 16 == 0) t.v_scale[i / kGroup] = (uint8_t)scale;
+  } else {
+    const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
+    values_of<true>(mc, live ? t.m_scale[i / kGroup] : 0, m);
+    values_of<false>(vc, live ? t.v_scale[i / kGroup] : 0, v);
+    store_of<float>(t.param, i, live, t.packs, m);
+    store_of<float>(t.copy, i, live, t.packs, v);
+  }
+}
+
+// ---- the norm -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ double sum_of_threads(double s) {
+  __shared__ double warps[kThreads / 32];
+#pragma unroll
+  for (int d = 16; d; d /= 2) s += __shfl_down_sync(0xffffffffu, s, d);
+  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int w = 0; w < kThreads / 32; ++w) s += warps[w];
+  return s;
+}
+// Squares are summed in 64 bits: a norm that goes into every value must not depend on the order of its sum.
+template <int N>
+__global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ Table<N> table, double* parts) {
+  pdl_wait();
+  double s = 0.0;
+  for (uint32_t piece = blockIdx.x; piece < table.first[table.count]; piece += gridDim.x) {
+    const int at = tensor_of(table, piece);
+    const Entry& t = table.tensor[at];
+    const uint64_t i = (uint64_t)(piece - table.first[at]) * kPiece + threadIdx.x * kEach;
+    const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
+    float g[kEach];
+    load_any(t.grad, t.grad_type, i, live, t.packs, g);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) s = fma((double)g[j], (double)g[j], s);
+  }
+  s = sum_of_threads(s);
+  if (threadIdx.x == 0) parts[blockIdx.x] = s;
+}
+__global__ void __launch_bounds__(kThreads) norm_sum_kernel(const double* __restrict__ parts, uint32_t count, float* norm) {
+  pdl_wait(parts);
+  double s = 0.0;
+  for (uint32_t i = threadIdx.x; i < count; i += kThreads) s += parts[i];
+  s = sum_of_threads(s);
+  if (threadIdx.x == 0) *norm = (float)sqrt(s);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+bool lies_on(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Calls launch(table, pieces) for as many tensors at a time as a table holds; empty tensors keep their place.
+template <int N, class F>
+cudaError_t in_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch) {
+  static thread_local Table<N> table;
+  for (size_t at = 0; at < count;) {
+    table.place = (uint32_t)at;
+    uint64_t pieces = 0;
+    int n = 0;
+    for (; n < N && at < count; ++at, ++n) {
+      const csw_adamw_tensor& t = tensors[at];
+      const uint64_t more = t.numel / kPiece + (t.numel % kPiece != 0);
+      if (n && pieces + more > 0x7fffffffu) break;
+      Entry& e = table.tensor[n];
+      e = {t.grad,  t.param, t.copy, t.exp_avg, t.exp_avg_sq, static_cast<uint8_t*>(t.exp_avg_scale),
+           static_cast<uint8_t*>(t.exp_avg_sq_scale), t.numel, (uint8_t)t.param_type, (uint8_t)t.grad_type,
+           (uint8_t)t.copy_type, true};
+      const size_t state = t.exp_avg_scale ? 8 : 16;
+      e.packs = lies_on(t.grad, 16) && lies_on(t.param, 16) && lies_on(t.copy, 16) && lies_on(t.exp_avg, state) &&
+                lies_on(t.exp_avg_sq, state);
+      table.first[n] = (uint32_t)pieces;
+      pieces += more;
+    }
+    table.first[n] = (uint32_t)pieces;
+    table.count = n;
+    if (pieces == 0) continue;
+    if (const cudaError_t e = launch(table, (uint32_t)pieces)) return e;
+  }
+  return cudaSuccess;
+}
+template <class F>
+cudaError_t in_any_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch) {
+  return count <= kFew ? in_tables<kFew>(tensors, count, launch) : in_tables<kMany>(tensors, count, launch);
+}
+uint32_t norm_grid(uint64_t pieces) { return (uint32_t)std::min<uint64_t>(pieces, (uint64_t)sm_count() * 8); }
+
+}  // namespace
+
+cudaError_t adamw_launch(const csw_adamw_tensor* tensors, size_t count, const csw_adamw_options& o, cudaStream_t stream) {
+  Step s{};
+  s.b1 = (float)o.beta1, s.rest1 = (float)(1.0 - o.beta1), s.b2 = (float)o.beta2, s.rest2 = (float)(1.0 - o.beta2);
+  s.eps = (float)o.eps, s.norm = o.d_norm, s.max_norm = (float)o.max_norm, s.step = o.d_step, s.lr = o.d_lr;
+  s.wide_b1 = o.beta1, s.wide_b2 = o.beta2, s.wide_lr = o.lr, s.wide_decay = o.weight_decay;
+  s.seed = o.seed, s.host_step = o.step;
+  settle(s, o.step, o.lr);
+  return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
+    constexpr int N = std::decay_t<decltype(table)>::kSize;
+    return pdl_launch(o.bits == 8 ? adamw_kernel<N, true> : adamw_kernel<N, false>, pieces, kThreads, 0, stream, table, s);
+  });
+}
+
+cudaError_t adamw8_convert_launch(const csw_adamw_tensor* tensors, size_t count, bool pack, cudaStream_t stream) {
+  return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
+    constexpr int N = std::decay_t<decltype(table)>::kSize;
+    return pdl_launch(pack ? adamw8_convert_kernel<N, true> : adamw8_convert_kernel<N, false>, pieces, kThreads, 0, stream,
+                      table);
+  });
+}
+
+uint64_t gradient_norm_partials(const csw_adamw_tensor* tensors, size_t count) {
+  uint64_t parts = 0;
+  in_any_tables(tensors, count, [&](const auto&, uint32_t pieces) {
+    parts += norm_grid(pieces);
+    return cudaSuccess;
+  });
+  return parts;
+}
+
+cudaError_t gradient_norm_launch(const csw_adamw_tensor* tensors, size_t count, float* norm, double* partials,
+                                 cudaStream_t stream) {
+  uint32_t parts = 0;
+  const cudaError_t e = in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
+    constexpr int N = std::decay_t<decltype(table)>::kSize;
+    const uint32_t grid = norm_grid(pieces);
+    const cudaError_t e = pdl_launch(norm_parts_kernel<N>, grid, kThreads, 0, stream, table, partials + parts);
+    parts += grid;
+    return e;
+  });
+  if (e != cudaSuccess) return e;
+  return pdl_launch(norm_sum_kernel, 1, kThreads, 0, stream, (const double*)partials, parts, norm);
+}
+
+}  // namespace csw

@@ -54,20 +54,28 @@ inline cudaError_t taken(cudaError_t e) {
   return e;
 }
 
+// in clusters of `cluster` CTAs
 template <class... P, class... A>
-inline cudaError_t pdl_launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
-                              A&&... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+inline cudaError_t pdl_launch_clusters(void (*kernel)(P...), unsigned grid, unsigned cluster, unsigned block, size_t smem,
+                                       cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return taken(cudaLaunchKernelEx(&cfg, kernel, P(std::forward<A>(args))...));
+}
+template <class... P, class... A>
+inline cudaError_t pdl_launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                              A&&... args) {
+  return pdl_launch_clusters(kernel, grid, 1, block, smem, stream, std::forward<A>(args)...);
 }
 
 }  // namespace csw

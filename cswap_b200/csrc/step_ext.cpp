@@ -1,0 +1,479 @@
+// Tensor-level front end of the 8-bit floating-point matrices and the optimizer's step (the wrappers in fp8.py and optim.py
+// keep the documented signatures; these functions take every argument by position).
+#include "ext_util.h"
+
+#include <algorithm>
+#include <cmath>
+#include <utility>
+#include <vector>
+
+using namespace cswext;
+
+namespace {
+
+int64_t blocks_of(int64_t n) { return n / 128 + (n % 128 != 0); }
+int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
+
+// ---- matrices in 8-bit floating point ------------------------------------------------------------------------------
+// codes and scales as fp8_quantize gives them
+bool matrix_of(PyObject* codes, PyObject* scales, const char* name, const char* scales_name, const at::Tensor** t,
+               csw_fp8_matrix* m) {
+  const at::Tensor* c = as_tensor(codes, name);
+  const at::Tensor* s = c ? as_tensor(scales, scales_name) : nullptr;
+  if (!s) return false;
+  if (!c->is_cuda()) return value_error("%s must be a CUDA tensor (this path has no CPU implementation)", name);
+  if (c->scalar_type() != at::kFloat8_e4m3fn || c->dim() != 2)
+    return value_error("%s must be a matrix of float8_e4m3fn codes", name);
+  const int64_t rows = c->size(0), cols = c->size(1);
+  int64_t stride = rows > 1 ? c->stride(0) : padded(cols);
+  if (rows > 0 && cols > 0) {
+    const size_t held = c->storage().nbytes() - (size_t)c->storage_offset();
+    if ((cols > 1 && c->stride(1) != 1) || stride % 16 || stride < cols || held < (size_t)(rows * stride) ||
+        reinterpret_cast<uintptr_t>(c->const_data_ptr()) % 16)
+      return value_error("%s must have rows that begin on 16 bytes and are padded to a multiple of them", name);
+  }
+  if (!same_device(*s, *c, scales_name)) return false;
+  if (s->scalar_type() != at::kFloat8_e8m0fnu || s->dim() != 2 || s->size(0) != blocks_of(rows) || s->size(1) != blocks_of(cols))
+    return value_error("%s must be float8_e8m0fnu, one for each block of 128 x 128 codes", scales_name);
+  if (!require_flat(*s, scales_name)) return false;
+  *t = c;
+  *m = {ptr(*c), ptr(*s), (size_t)rows, (size_t)cols, (size_t)stride, 0};
+  return true;
+}
+
+bool dtype_of(PyObject* o, at::ScalarType* kind, int* type) {
+  if (!THPDtype_Check(o)) {
+    PyErr_SetString(PyExc_TypeError, "dtype must be a torch.dtype");
+    return false;
+  }
+  *kind = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  *type = type_code(*kind);
+  return *type >= 0 || value_error("%s must be float32, float16 or bfloat16", "dtype");
+}
+
+// fp8_quantize(x, sums) -> (codes, scales), or with their columns' sums
+PyObject* fp8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int type;
+    if (!arg_count(n, 2)) return nullptr;
+    const at::Tensor* x = as_tensor(a[0], "x");
+    if (!x || !require_values(*x, "x", &type)) return nullptr;
+    const int wanted = PyObject_IsTrue(a[1]);
+    if (wanted < 0) return nullptr;
+    if (x->dim() < 1) {
+      value_error("x needs one axis at least");
+      return nullptr;
+    }
+    const int64_t cols = x->size(-1), rows = cols ? x->numel() / cols : x->dim() == 2 ? x->size(0) : 0;
+    int64_t stride = cols;
+    if (x->dim() == 2 && rows > 1 && (cols == 1 || x->stride(1) == 1) && x->stride(0) >= cols) stride = x->stride(0);
+    else if (!require_flat(*x, "x")) return nullptr;
+    size_t need;
+    if (!status_ok(csw_fp8_quantize_workspace(rows, cols, &need), "csw_fp8_quantize_workspace")) return nullptr;
+    const int64_t code_stride = padded(cols);
+    at::Tensor codes = fresh(*x, {rows, code_stride}, at::kFloat8_e4m3fn);
+    at::Tensor scales = fresh(*x, {blocks_of(rows), blocks_of(cols)}, at::kFloat8_e8m0fnu), sums, space;
+    void *to = out(codes), *powers = out(scales), *ws = nullptr;
+    float* totals = nullptr;
+    if (wanted) {
+      sums = fresh(*x, {cols}, at::kFloat);
+      totals = static_cast<float*>(out(sums));
+      if (need) {
+        space = fresh(*x, {(int64_t)need}, at::kByte);
+        ws = out(space);
+      }
+    }
+    const void* from = ptr(*x);
+    if (!launch(*x, "csw_fp8_quantize", [&](csw_stream_t s) {
+          return csw_fp8_quantize(from, type, rows, cols, stride, to, code_stride, powers, totals, ws, need, s);
+        }))
+      return nullptr;
+    if (code_stride != cols) codes = codes.narrow(1, 0, cols);
+    return wanted ? tuple_of({codes, scales, sums}) : tuple_of({codes, scales});
+  });
+}
+
+// fp8_dequantize(codes, scales, dtype) -> tensor
+PyObject* fp8_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* codes;
+    csw_fp8_matrix m;
+    at::ScalarType kind;
+    int type;
+    if (!arg_count(n, 3) || !matrix_of(a[0], a[1], "codes", "scales", &codes, &m) || !dtype_of(a[2], &kind, &type))
+      return nullptr;
+    at::Tensor dst = fresh(*codes, codes->sizes(), kind);
+    void* to = out(dst);
+    if (!launch(*codes, "csw_fp8_dequantize", [&](csw_stream_t s) {
+          return csw_fp8_dequantize(m.codes, m.code_stride, m.scales, m.rows, m.cols, to, type, s);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(dst);
+  });
+}
+
+// fp8_matmul(a, a_scales, b, b_scales, transpose_a, transpose_b, bias, dtype) -> tensor
+PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *l, *r, *bias;
+    csw_fp8_matrix left, right;
+    at::ScalarType kind;
+    int type, bias_type = 0;
+    if (!arg_count(n, 8) || !matrix_of(a[0], a[1], "a", "a_scales", &l, &left) ||
+        !matrix_of(a[2], a[3], "b", "b_scales", &r, &right) || !same_device(*r, *l, "b") ||
+        !optional_tensor(a[6], "bias", &bias) || !dtype_of(a[7], &kind, &type))
+      return nullptr;
+    left.transposed = PyObject_IsTrue(a[4]), right.transposed = PyObject_IsTrue(a[5]);
+    if (left.transposed < 0 || right.transposed < 0) return nullptr;
+    const size_t rows = left.transposed ? left.cols : left.rows, inner = left.transposed ? left.rows : left.cols;
+    const size_t cols = right.transposed ? right.rows : right.cols;
+    if (inner != (right.transposed ? right.cols : right.rows)) {
+      value_error("a and b do not fit: the columns of the one must be the rows of the other");
+      return nullptr;
+    }
+    if (bias) {
+      if (!require_values(*bias, "bias", &bias_type) || !same_device(*bias, *l, "bias") || !require_flat(*bias, "bias"))
+        return nullptr;
+      if (bias->dim() != 1 || (size_t)bias->numel() != cols) {
+        value_error("%s must hold one value for each column of the product", "bias");
+        return nullptr;
+      }
+    }
+    at::Tensor dst = fresh(*l, {(int64_t)rows, (int64_t)cols}, kind);
+    void* to = out(dst);
+    const void* more = bias ? ptr(*bias) : nullptr;
+    if (!launch(*l, "csw_fp8_matmul", [&](csw_stream_t s) {
+          return csw_fp8_matmul(&left, &right, more, bias_type, to, type, s);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(dst);
+  });
+}
+
+// ---- the optimizer's step ------------------------------------------------------------------------------------------
+// The tensors of a list or tuple; what they are checked for is their caller's.
+struct List {
+  PyObject* fast = nullptr;
+  Py_ssize_t size = 0;
+  bool of(PyObject* o, const char* name) {
+    fast = PySequence_Fast(o, "a list of tensors is wanted");
+    if (!fast) return false;
+    size = PySequence_Fast_GET_SIZE(fast);
+    return true;
+  }
+  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
+  ~List() { Py_XDECREF(fast); }
+};
+bool same_size(const List& l, Py_ssize_t n, const char* name) {
+  return l.size == n || value_error("%s must have an entry for each parameter", name);
+}
+
+// What is written by a call, apart: a range for each tensor, by its role.
+struct Written {
+  using Range = std::pair<const char*, const char*>;
+  std::vector<std::vector<Range>> roles;
+  explicit Written(size_t n) : roles(n) {}
+  void add(size_t role, const at::Tensor& t) {
+    const char* p = static_cast<const char*>(t.const_data_ptr());
+    if (t.numel()) roles[role].push_back({p, p + t.nbytes()});
+  }
+  static bool ascend(const std::vector<Range>& r) {
+    for (size_t i = 1; i < r.size(); ++i)
+      if (r[i].first < r[i - 1].second) return false;
+    return true;
+  }
+  // Most programs' tensors of one role ascend in memory, apart from those of the others: no need to sort them then.
+  bool apart() {
+    std::vector<Range> hulls, all;
+    bool plain = true;
+    for (const auto& r : roles) {
+      plain = plain && ascend(r);
+      if (!r.empty()) hulls.push_back({r.front().first, r.back().second});
+    }
+    std::sort(hulls.begin(), hulls.end());
+    if (plain && ascend(hulls)) return true;
+    for (const auto& r : roles) all.insert(all.end(), r.begin(), r.end());
+    std::sort(all.begin(), all.end());
+    return ascend(all) || value_error("the tensors that the step writes overlap");
+  }
+};
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// a tensor that lies as `as` does: the same shape and order in memory
+bool lies_like(const at::Tensor& t, const at::Tensor& as, const char* name) {
+  if (!same_device(t, as, name)) return false;
+  if (!t.sizes().equals(as.sizes())) return value_error("%s has another shape than its parameter", name);
+  if (t.is_contiguous() && as.is_contiguous()) return true;
+  return t.strides().equals(as.strides()) || value_error("%s lies in another order than its parameter", name);
+}
+bool require_dense(const at::Tensor& t, const char* name) {
+  return t.is_contiguous() || t.is_non_overlapping_and_dense() || value_error("%s must lie densely", name);
+}
+// codes (n) or scales (one for 128) of a state
+bool bytes_of(const at::Tensor& t, const at::Tensor& on, int64_t n, const char* name) {
+  if (!same_device(t, on, name)) return false;
+  if (t.scalar_type() != at::kByte || t.numel() != n) return value_error("%s has another type or size than its parameter asks for", name);
+  return require_flat(t, name);
+}
+bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, size_t role) {
+  List l;
+  if (!l.of(o, "states")) return false;
+  if (l.size != 4) return value_error("a state is (exp_avg, exp_avg_sq, their scales)");
+  void** const to[4] = {&t->exp_avg, &t->exp_avg_sq, &t->exp_avg_scale, &t->exp_avg_sq_scale};
+  const int64_t n = on.numel();
+  for (int i = 0; i < 4; ++i) {
+    const at::Tensor* s = as_tensor(l[i], "a state");
+    if (!s || !bytes_of(*s, on, i < 2 ? n : blocks_of(n), "a state")) return false;
+    *to[i] = ptr(*s);
+    if (written) {
+      written->add(role + i, *s);
+      changed(*s);
+    }
+  }
+  return true;
+}
+bool floats_of(PyObject* o, const at::Tensor& as, const char* name, const at::Tensor** t) {
+  *t = as_tensor(o, name);
+  if (!*t || !lies_like(**t, as, name)) return false;
+  return (*t)->scalar_type() == at::kFloat || value_error("%s must be float32", name);
+}
+bool number(PyObject* o, double* v) {
+  *v = PyFloat_AsDouble(o);
+  return !(*v == -1.0 && PyErr_Occurred());
+}
+// a number on the device that takes the place of one of the host's
+bool on_device(const at::Tensor& t, const at::Tensor& on, at::ScalarType kind, const char* name, const void** p) {
+  if (!same_device(t, on, name)) return false;
+  if (t.scalar_type() != kind || t.numel() != 1)
+    return value_error(kind == at::kLong ? "%s must be a number or one int64 on the device" : "%s must be a number or one float32 on the device", name);
+  *p = t.const_data_ptr();
+  return true;
+}
+
+// The tail of both steps' arguments: step, lr, beta1, beta2, eps, weight_decay, norm, max_norm
+bool options_of(PyObject* const* a, const at::Tensor* on, csw_adamw_options* o) {
+  double v[5];
+  const void* p;
+  if (THPVariable_Check(a[0])) {
+    if (on && !on_device(THPVariable_Unpack(a[0]), *on, at::kLong, "step", &p)) return false;
+    o->d_step = on ? static_cast<const int64_t*>(p) : nullptr;
+    o->step = 1;
+  } else {
+    o->step = PyLong_AsLongLong(a[0]);
+    if (o->step == -1 && PyErr_Occurred()) return false;
+    if (o->step < 1) return value_error("step counts from 1");
+  }
+  if (THPVariable_Check(a[1])) {
+    if (on && !on_device(THPVariable_Unpack(a[1]), *on, at::kFloat, "lr", &p)) return false;
+    o->d_lr = on ? static_cast<const float*>(p) : nullptr;
+    o->lr = 0.0;
+  } else if (!number(a[1], &o->lr)) {
+    return false;
+  }
+  for (int i = 0; i < 4; ++i)
+    if (!number(a[2 + i], &v[i])) return false;
+  o->beta1 = v[0], o->beta2 = v[1], o->eps = v[2], o->weight_decay = v[3];
+  auto fine = [](double x) { return x >= 0.0 && x <= 3.4e38; };
+  if (!fine(o->lr)) return value_error("lr must not be negative");
+  for (int i = 0; i < 2; ++i)
+    if (!(v[i] >= 0.0 && v[i] < 1.0)) return value_error("betas must be at least 0 and below 1");
+  if (!fine(v[2])) return value_error("eps must not be negative");
+  if (!fine(v[3])) return value_error("weight_decay must not be negative");
+  o->max_norm = 0.0;
+  if (a[6] != Py_None) {
+    const at::Tensor* t = as_tensor(a[6], "norm");
+    if (!t || !number(a[7], &o->max_norm)) return false;
+    if (on && !on_device(*t, *on, at::kFloat, "norm", &p)) return false;
+    o->d_norm = on ? static_cast<const float*>(p) : nullptr;
+    if (!fine(o->max_norm)) return value_error("max_norm must not be negative");
+  }
+  return true;
+}
+
+// params, grads and copies of a call; the first parameter in *on
+bool tensors_of(const List& params, PyObject* grads, PyObject* copies, std::vector<csw_adamw_tensor>* to, Written* written,
+                const at::Tensor** on) {
+  List g, c;
+  if (!g.of(grads, "grads") || !same_size(g, params.size, "grads")) return false;
+  const bool with_copies = copies != Py_None;
+  if (with_copies && (!c.of(copies, "copies") || !same_size(c, params.size, "copies"))) return false;
+  to->resize(params.size);
+  *on = nullptr;
+  for (Py_ssize_t i = 0; i < params.size; ++i) {
+    csw_adamw_tensor& t = (*to)[i];
+    t = {};
+    const at::Tensor* p = as_tensor(params[i], "a parameter");
+    const at::Tensor* d = p ? as_tensor(g[i], "a gradient") : nullptr;
+    if (!d || !require_values(*p, "a parameter", &t.param_type) || !require_dense(*p, "a parameter") ||
+        !require_values(*d, "a gradient", &t.grad_type) || !lies_like(*d, *p, "a gradient"))
+      return false;
+    if (!*on) *on = p;
+    if (!same_device(*p, **on, "a parameter")) return false;
+    t.param = ptr(*p), t.grad = ptr(*d), t.numel = (size_t)p->numel();
+    written->add(0, *p);
+    if (with_copies && c[i] != Py_None) {
+      const at::Tensor* k = as_tensor(c[i], "a copy");
+      if (!k || !require_values(*k, "a copy", &t.copy_type) || !lies_like(*k, *p, "a copy")) return false;
+      t.copy = ptr(*k);
+      written->add(1, *k);
+    }
+  }
+  return true;
+}
+void all_changed(const List& params, PyObject* copies) {
+  for (Py_ssize_t i = 0; i < params.size; ++i) changed(THPVariable_Unpack(params[i]));
+  if (copies == Py_None) return;
+  List c;
+  if (!c.of(copies, "copies")) return;
+  for (Py_ssize_t i = 0; i < c.size; ++i)
+    if (THPVariable_Check(c[i])) changed(THPVariable_Unpack(c[i]));
+}
+
+bool step_of(const std::vector<csw_adamw_tensor>& tensors, const csw_adamw_options& o, const at::Tensor* on) {
+  return !on || launch(*on, "csw_adamw_step",
+                       [&](csw_stream_t s) { return csw_adamw_step(tensors.data(), tensors.size(), &o, s); });
+}
+
+// adamw_step(params, grads, exp_avgs, exp_avg_sqs, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm) -> None
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    List params, m, v;
+    std::vector<csw_adamw_tensor> tensors;
+    Written written(4);
+    const at::Tensor *on, *t;
+    csw_adamw_options o{};
+    o.bits = 32;
+    if (!arg_count(n, 13) || !params.of(a[0], "params") || !tensors_of(params, a[1], a[4], &tensors, &written, &on) ||
+        !m.of(a[2], "exp_avgs") || !v.of(a[3], "exp_avg_sqs") || !same_size(m, params.size, "exp_avgs") ||
+        !same_size(v, params.size, "exp_avg_sqs") || !options_of(a + 5, on, &o))
+      return nullptr;
+    for (Py_ssize_t i = 0; i < params.size; ++i) {
+      const at::Tensor& p = THPVariable_Unpack(params[i]);
+      if (!floats_of(m[i], p, "exp_avg", &t)) return nullptr;
+      tensors[i].exp_avg = ptr(*t);
+      written.add(2, *t);
+      if (!floats_of(v[i], p, "exp_avg_sq", &t)) return nullptr;
+      tensors[i].exp_avg_sq = ptr(*t);
+      written.add(3, *t);
+    }
+    if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
+    all_changed(params, a[4]);
+    for (Py_ssize_t i = 0; i < params.size; ++i) changed(THPVariable_Unpack(m[i])), changed(THPVariable_Unpack(v[i]));
+    Py_RETURN_NONE;
+  });
+}
+
+// adamw8_step(params, grads, states, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed) -> None
+PyObject* adamw8_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    List params, states;
+    std::vector<csw_adamw_tensor> tensors;
+    Written written(6);
+    const at::Tensor* on;
+    csw_adamw_options o{};
+    o.bits = 8;
+    if (!arg_count(n, 13) || !params.of(a[0], "params") || !tensors_of(params, a[1], a[3], &tensors, &written, &on) ||
+        !states.of(a[2], "states") || !same_size(states, params.size, "states") || !options_of(a + 4, on, &o))
+      return nullptr;
+    const unsigned long long seed = PyLong_AsUnsignedLongLong(a[12]);
+    if (PyErr_Occurred()) return nullptr;
+    if (seed >> 32) {
+      value_error("seed must be below 2^32");
+      return nullptr;
+    }
+    o.seed = (uint32_t)seed;
+    for (Py_ssize_t i = 0; i < params.size; ++i)
+      if (!eight_of(states[i], THPVariable_Unpack(params[i]), &tensors[i], &written, 2)) return nullptr;
+    if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
+    all_changed(params, a[3]);
+    Py_RETURN_NONE;
+  });
+}
+
+// adamw8_convert(states, exp_avgs, exp_avg_sqs, pack) -> None
+PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    List states, m, v;
+    if (!arg_count(n, 4) || !states.of(a[0], "states") || !m.of(a[1], "exp_avgs") || !v.of(a[2], "exp_avg_sqs") ||
+        !same_size(m, states.size, "exp_avgs") || !same_size(v, states.size, "exp_avg_sqs"))
+      return nullptr;
+    const int pack = PyObject_IsTrue(a[3]);
+    if (pack < 0) return nullptr;
+    std::vector<csw_adamw_tensor> tensors(states.size);
+    Written written(4);
+    const at::Tensor* on = nullptr;
+    for (Py_ssize_t i = 0; i < states.size; ++i) {
+      csw_adamw_tensor& t = tensors[i];
+      t = {};
+      const at::Tensor* first = as_tensor(m[i], "exp_avg");
+      const at::Tensor* second;
+      int type;
+      if (!first || !require_values(*first, "exp_avg", &type) || !require_dense(*first, "exp_avg") ||
+          !floats_of(m[i], *first, "exp_avg", &first) || !floats_of(v[i], *first, "exp_avg_sq", &second))
+        return nullptr;
+      if (!on) on = first;
+      if (!same_device(*first, *on, "exp_avg") || !eight_of(states[i], *first, &t, pack ? &written : nullptr, 0)) return nullptr;
+      t.param = ptr(*first), t.copy = ptr(*second), t.numel = (size_t)first->numel();
+      if (!pack) {
+        written.add(0, *first), written.add(1, *second);
+        changed(*first), changed(*second);
+      }
+    }
+    if (!written.apart()) return nullptr;
+    if (on && !launch(*on, pack ? "csw_adamw8_pack" : "csw_adamw8_unpack", [&](csw_stream_t s) {
+          return pack ? csw_adamw8_pack(tensors.data(), tensors.size(), s) : csw_adamw8_unpack(tensors.data(), tensors.size(), s);
+        }))
+      return nullptr;
+    Py_RETURN_NONE;
+  });
+}
+
+// gradient_norm(tensors) -> float32
+PyObject* gradient_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    List grads;
+    if (!arg_count(n, 1) || !grads.of(a[0], "tensors")) return nullptr;
+    if (grads.size == 0) {
+      value_error("a norm needs a tensor at least");
+      return nullptr;
+    }
+    std::vector<csw_adamw_tensor> tensors(grads.size);
+    const at::Tensor* on = nullptr;
+    for (Py_ssize_t i = 0; i < grads.size; ++i) {
+      csw_adamw_tensor& t = tensors[i];
+      t = {};
+      const at::Tensor* g = as_tensor(grads[i], "a gradient");
+      if (!g || !require_values(*g, "a gradient", &t.grad_type) || !require_dense(*g, "a gradient")) return nullptr;
+      if (!on) on = g;
+      if (!same_device(*g, *on, "a gradient")) return nullptr;
+      t.grad = ptr(*g), t.numel = (size_t)g->numel();
+    }
+    const c10::cuda::CUDAGuard guard(on->device());  // the size goes by the device's SMs
+    size_t need;
+    if (!status_ok(csw_gradient_norm_workspace(tensors.data(), tensors.size(), &need), "csw_gradient_norm_workspace"))
+      return nullptr;
+    at::Tensor norm = fresh(*on, {}, at::kFloat), space = fresh(*on, {(int64_t)need}, at::kByte);
+    float* to = static_cast<float*>(out(norm));
+    void* ws = out(space);
+    if (!launch(*on, "csw_gradient_norm",
+                [&](csw_stream_t s) { return csw_gradient_norm(tensors.data(), tensors.size(), to, ws, need, s); }))
+      return nullptr;
+    return THPVariable_Wrap(norm);
+  });
+}
+
+}  // namespace
+
+PyMethodDef cswap_step_methods[] = {
+    CSW_METHOD(fp8_quantize, "(x, sums) -> (codes, scales) or (codes, scales, sums)"),
+    CSW_METHOD(fp8_dequantize, "(codes, scales, dtype) -> tensor"),
+    CSW_METHOD(fp8_matmul, "(a, a_scales, b, b_scales, transpose_a, transpose_b, bias, dtype) -> tensor"),
+    CSW_METHOD(adamw_step, "(params, grads, exp_avgs, exp_avg_sqs, copies, step, lr, beta1, beta2, eps, weight_decay, norm, "
+                           "max_norm) -> None"),
+    CSW_METHOD(adamw8_step, "(params, grads, states, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed) "
+                            "-> None"),
+    CSW_METHOD(adamw8_convert, "(states, exp_avgs, exp_avg_sqs, pack) -> None"),
+    CSW_METHOD(gradient_norm, "(tensors) -> float32"),
+    {nullptr, nullptr, 0, nullptr}};

@@ -1,4 +1,4 @@
-// The instructions that the attention kernels are built on: mbarriers, tile copies (TMA), and the fifth-generation
+// The instructions that the attention kernels and the 8-bit products are built on: mbarriers, tile copies (TMA), and the fifth-generation
 // tensor cores with their accumulators in tensor memory (tcgen05).
 //
 // Every wait on an mbarrier is bounded: where it runs out, the kernel sets a status word in host memory (the next call and
@@ -60,6 +60,13 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, 
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar), "r"(dim), "r"(token), "r"(head), "r"(batch)
+      : "memory");
+}
+// a tile of a matrix of bytes, columns x (a multiple of 16) and rows y
+__device__ __forceinline__ void copy_bytes_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
 // bytes (a multiple of 16) from a 16-byte boundary
@@ -216,6 +223,30 @@ __device__ __forceinline__ void mma_tmem(uint32_t acc, uint32_t a, uint64_t b, u
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(acc),
       "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
       : "memory");
+}
+// 128 x N products of e4m3 values with a scale 2^(s - 127) for 32 of them along the reduction, sums in float32; across as
+// above, for each operand.
+__host__ __device__ constexpr uint32_t scaled_desc(int n, bool a_across, bool b_across) {
+  return (a_across ? 1u << 15 : 0u) | (b_across ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | 1u << 23 |
+         (uint32_t)(128 / 16) << 24;
+}
+// One reduction step of 32, 32 bytes further along a row or 32 rows, 4096 bytes, across.  The operands' scales lie in tensor
+// memory, one of a row (a column of the result) in lane row % 32 of column row / 32, each byte of it for a step of its own.
+__device__ __forceinline__ void mma_scaled(uint32_t acc, uint64_t a, uint64_t b, uint32_t desc, uint32_t a_scales,
+                                           uint32_t b_scales, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(a_scales), "r"(b_scales)
+      : "memory");
+}
+// 512 bytes of scales to four columns of tensor memory, behind the products and copies issued before: rows of 16 bytes, a
+// row to a lane, the same for all four warps' lanes.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t at) {
+  return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t from) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from) : "memory");
 }
 // arrives at `bar` when all products issued before have ended
 __device__ __forceinline__ void commit(uint32_t bar) {

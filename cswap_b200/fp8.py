@@ -1,0 +1,116 @@
+"""Linear layers whose products take 8-bit floating-point operands.
+
+* ``fp8_quantize`` / ``fp8_dequantize``: a matrix as e4m3 codes with a power of two for each block of 128 x 128 values.
+* ``fp8_matmul``: the product of two such matrices, either one taken transposed, on the tensor cores.
+* ``fp8_linear``: a linear layer on them, differentiable (once).  All three of its products run in 8 bits, and of its input
+  it keeps what its forward product read: 1.00006 bytes a value.
+
+A block's scale 2^E is the least power of two (2^-126 at least) for which its largest magnitude is at most 448 2^E; a value's
+code is the e4m3 number nearest to x / 2^E, ties to even.  A value of at least 2^-14.8 of its block's largest is off by at most
+a sixteenth of itself, a smaller one by 2^-19 of the block's largest or so.  A NaN or an infinity is held as NaN, and shows in
+every result that it goes into; the scale goes by the others.
+
+Everything runs on torch's current stream of the tensors' device, on float32, float16 and bfloat16 values, sums in float32 and
+rounds a result to its type once.  The same call gives the same bits every time.  There is no CPU implementation.  Waits inside
+the products are bounded as those of attention are (``device_status``).
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.amp import custom_bwd, custom_fwd
+from torch.autograd.function import once_differentiable
+
+from . import codec
+
+FP8_BLOCK = 128
+
+Quantized = Tuple[torch.Tensor, torch.Tensor]
+
+
+def _ext():
+    return codec._native or codec._load()
+
+
+def fp8_quantize(x: torch.Tensor, sums: bool = False):
+    """(codes, scales) of x as a matrix of rows of its last axis; with `sums` also the float32 sum of each column.
+
+    codes is float8_e4m3fn [rows, cols], whose rows begin on 16 bytes (they are padded to that in memory), scales
+    float8_e8m0fnu [blocks of rows, blocks of columns].  A matrix may have any distance between its rows; other tensors are
+    contiguous."""
+    return _ext().fp8_quantize(x, sums)
+
+
+def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that codes and scales stand for, rounded to `dtype`."""
+    return _ext().fp8_dequantize(codes, scales, dtype)
+
+
+def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, transpose_a: bool = False,
+               transpose_b: bool = False, bias: Optional[torch.Tensor] = None,
+               dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a b + bias in `dtype`, a and b as fp8_quantize gives them, or transposed."""
+    return _ext().fp8_matmul(a, a_scales, b, b_scales, transpose_a, transpose_b, bias, dtype)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, bias):
+        ext = _ext()
+        held = ext.fp8_quantize(x, False)
+        w = ext.fp8_quantize(weight, False)
+        y = ext.fp8_matmul(*held, *w, False, True, bias, x.dtype)
+        # what a gradient that is not asked for would need is not kept
+        keep_x = held if weight.requires_grad else (None, None)
+        keep_w = w if x.requires_grad else (None, None)
+        ctx.save_for_backward(*keep_x, *keep_w)
+        ctx.shape, ctx.types = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    @once_differentiable
+    def backward(ctx, dy):
+        ext = _ext()
+        x, x_scales, w, w_scales = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad
+        kind, weight_kind, bias_kind = ctx.types
+        dx = dw = db = None
+        g = ext.fp8_quantize(_rows(dy.reshape(-1, dy.shape[-1])), want_b)
+        if want_x:
+            dx = ext.fp8_matmul(g[0], g[1], w, w_scales, False, False, None, kind).view(ctx.shape)
+        if want_w:
+            dw = ext.fp8_matmul(g[0], g[1], x, x_scales, True, False, None, weight_kind)
+        if want_b:
+            db = g[2].to(bias_kind)
+        return dx, dw, db
+
+
+def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Quantized], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x weight^T + bias in the type of x, every product on operands in 8 bits.
+
+    x is [..., in], weight [out, in], bias [out], each of its own type; their gradients have it, too.  x is kept as codes, and
+    the weight's are for the input's gradient.  A weight that does not change may be given as fp8_quantize(weight), and takes no
+    gradient then (nor do x and the bias)."""
+    if isinstance(weight, torch.Tensor):
+        if x.dim() < 2 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+            raise ValueError("x needs two axes at least, and a weight of [out, in] for its last one")
+        _ext().check_capture(x, weight, bias)
+        return _Fp8Linear.apply(_rows(x), _rows(weight), bias)
+    codes, scales = weight
+    if x.dim() < 2 or codes.dim() != 2 or x.shape[-1] != codes.shape[1]:
+        raise ValueError("x needs two axes at least, and a weight of [out, in] for its last one")
+    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
+        raise ValueError("no gradient passes through a weight that was quantized before: call under torch.no_grad()")
+    ext = _ext()
+    y = ext.fp8_matmul(*ext.fp8_quantize(_rows(x), False), codes, scales, False, True, bias, x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], codes.shape[0])
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as the quantizer takes it: a matrix of rows at any distance, or contiguous."""
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
+        return t
+    return t.contiguous()

@@ -407,8 +407,8 @@ typedef struct {
 /* The kernels' warps wait for one another's copies and products, each time for two seconds or so at the most.  Where that
  * runs out, which takes a fault of the device, what the CTA in question had to compute is NaN, in the results and in the
  * gradients that follow from them, and the next call of csw_attention_forward or csw_attention_backward on that device,
- * or csw_device_status, returns CSW_ERR_TIMEOUT, once; that call launches nothing.  csw_attention_wait_limit sets the time
- * for the calls of this process from now on, in clocks of an SM (2^32 to begin with).  A negative one lets the waits run
+ * of csw_fp8_matmul, or csw_device_status, returns CSW_ERR_TIMEOUT, once; that call launches nothing.
+ * csw_attention_wait_limit sets the time for the calls of this process (csw_fp8_matmul's, too) from now on, in clocks of an SM (2^32 to begin with).  A negative one lets the waits run
  * out after -clocks, since the copies they are for are not begun: what a program does then can be tried out with it. */
 csw_status csw_attention_wait_limit(int64_t clocks);
 /* d_lse: batch x heads x q_len float32, the natural logarithm of each row's sum of exp(scale q.k). */
@@ -425,6 +425,83 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
                                   const csw_attention_operand* dq, const csw_attention_operand* dk,
                                   const csw_attention_operand* dv, void* d_workspace, size_t workspace_bytes,
                                   csw_stream_t stream);
+
+/* ---- 8. matrices in 8-bit floating point ------------------------------------ */
+/* A matrix as codes and scales.  Blocks of 128 x 128 values (those at the ends smaller) share a scale 2^E, held as the byte
+ * E + 127 in [blocks of rows][blocks of columns].  With a the block's largest finite magnitude, E is the least for which
+ * a <= 448 2^E, but -126 at least; a value's code is the e4m3 number (1 bit of sign, 4 of exponent with bias 7, 3 of mantissa,
+ * no infinities) nearest to x 2^-E, ties to even; a NaN or an infinity is held as NaN.  Rows of codes begin code_stride bytes
+ * apart, a multiple of 16 and not less than cols rounded up to 8; the codes lie on 16 bytes.  What lies between a row's last
+ * code and the next row is not used (up to 7 bytes of it are written). */
+/* d_x: rows of cols values, x_stride values apart (cols at least).  Where d_sums is given it receives the sum of each column
+ * in float32, by way of a workspace of csw_fp8_quantize_workspace bytes (none for up to 128 rows). */
+csw_status csw_fp8_quantize_workspace(size_t rows, size_t cols, size_t* bytes);
+csw_status csw_fp8_quantize(const void* d_x, int type, size_t rows, size_t cols, size_t x_stride, void* d_codes,
+                            size_t code_stride, void* d_scales, float* d_sums, void* d_workspace, size_t workspace_bytes,
+                            csw_stream_t stream);
+/* The values that codes and scales stand for, rounded to the type, row behind row. */
+csw_status csw_fp8_dequantize(const void* d_codes, size_t code_stride, const void* d_scales, size_t rows, size_t cols,
+                              void* d_out, int type, csw_stream_t stream);
+/* A matrix of rows x cols as it is stored; transposed: the product takes it as cols x rows. */
+typedef struct {
+  const void* codes;
+  const void* scales;
+  size_t rows, cols, code_stride;
+  int transposed;
+} csw_fp8_matrix;
+/* out = a b + bias, with a taken as m x k, b as k x n, out m x n row behind row; the bias (n values of bias_type) may be NULL.
+ * Products are exact and summed in float32 by the tensor cores; the sum is rounded to the type once.  m and n are at most 2^31 - 129, k at
+ * most 2^31 - 1.  The same call gives the same bits every time.  Waits are bounded as those of attention (section 7). */
+csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, const void* d_bias, int bias_type, void* d_out,
+                          int type, csw_stream_t stream);
+
+/* ---- 9. the optimizer's step over many tensors ------------------------------- */
+/* A parameter with its gradient and state, each numel values in the same order in memory, each of its own type where there is
+ * one.  copy may be NULL, else it receives the new parameter in its type.  State in 32 bits: exp_avg (m) and exp_avg_sq (v)
+ * are float32, the scales NULL.  State in 8 bits: exp_avg and exp_avg_sq are numel codes, the scales ceil(numel / 128) bytes;
+ * all zero is a state of zeros.  Groups of 128 consecutive values share a scale 2^E, held as the byte E + 127, E the least for
+ * which the group's largest magnitude is at most 1.75 2^E, but -126 at least; the byte is 0 for a group of zeros, and 255 for one
+ * with a number that is not finite or beyond 1.75 2^126, which reads as NaN.  A code of m is a sign, 4 bits of exponent x and
+ * 3 of mantissa f and stands for (1 + f / 8) 2^(x - 15 + E), or f / 8 2^(-14 + E) where x is 0; one of v has 5 bits and 3 and
+ * stands for (1 + f / 8) 2^(x - 31 + E), or f / 8 2^(-30 + E).  No tensor that is written overlaps another one of the call. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* copy;
+  void *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale;
+  size_t numel;
+  int param_type, grad_type, copy_type;
+} csw_adamw_tensor;
+/* d_step, d_lr and d_norm may be NULL: where one is given it is read on the device, d_step and d_lr in place of step and lr
+ * (a step below 1 counts as 1). */
+typedef struct {
+  int bits; /* of the state: 8 or 32 */
+  uint32_t seed;
+  int64_t step; /* t, from 1 on */
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  const int64_t* d_step;
+  const float* d_lr;
+  const float* d_norm;
+} csw_adamw_options;
+/* With c = min(1, max_norm / (norm + 1e-6)) where a norm is given, else 1, and every operation on averages one of float32:
+ *   m = beta1 m + (1 - beta1) (c g),  v = beta2 v + ((1 - beta2) (c g)) (c g)
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * State in 8 bits is rounded up or down at random: with u the 20 bits of a value's float32 mantissa (of one that is scaled to
+ * where its code's lowest bit is the 2^20's) that its code has no room for, the code is one larger where u + 16 r + 8 >= 2^20; a
+ * code of v is 1 at least unless its group is zero.  r is 16 bits of mix(k + i), the upper ones for m, the lower for v, with i the
+ * value's index, k = mix(mix(seed + 0x9e3779b9 t) + 0x9e3779b9 j) for the j-th tensor of the call and, modulo 2^32,
+ * mix(x): x ^= x >> 16, x *= 0x9e3779b1, x ^= x >> 15, x *= 0x85ebca77, x ^= x >> 16. */
+csw_status csw_adamw_step(const csw_adamw_tensor* tensors, size_t count, const csw_adamw_options* options,
+                          csw_stream_t stream);
+/* State in 8 bits from averages in float32 (exp_avg in the place of param, exp_avg_sq of copy), rounded to the nearest with
+ * halves away from zero; and the averages that it stands for.  Gradients and types are not looked at. */
+csw_status csw_adamw8_pack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream);
+csw_status csw_adamw8_unpack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream);
+/* The square root of the sum of all gradients' squares, summed in float64; the workspace holds csw_gradient_norm_workspace bytes (of the
+ * current device). */
+csw_status csw_gradient_norm_workspace(const csw_adamw_tensor* tensors, size_t count, size_t* bytes);
+csw_status csw_gradient_norm(const csw_adamw_tensor* tensors, size_t count, float* d_norm, void* d_workspace,
+                             size_t workspace_bytes, csw_stream_t stream);
 
 /* ---- pinned host memory helpers (for callers without a CUDA binding) ------ */
 csw_status csw_host_alloc(size_t bytes, void** p);
