@@ -248,7 +248,6 @@ csw_status csw_fp8_dequantize(const void* d_codes, size_t code_stride, const voi
                               void* d_out, int type, csw_stream_t stream) {
   if (!known_type(type) || !matrix(d_codes, d_scales, rows, cols, code_stride)) return CSW_ERR_ARG;
   if (rows && cols && !good(d_out, type)) return CSW_ERR_ARG;
-  if (rows && (cols + 7) / 8 > (kMostRows * 256) / rows) return CSW_ERR_ARG;
   return done(fp8_dequantize_launch(d_codes, code_stride, static_cast<const uint8_t*>(d_scales), rows, cols, d_out, type,
                                     stream));
 }

@@ -167,59 +167,99 @@ __device__ __forceinline__ void store_codes(void* to, uint64_t i, int live, bool
       if (j < live) p[j] = (uint8_t)((j < 4 ? codes.x : codes.y) >> (j % 4 * 8));
   }
 }
-// SIGNED: m, else v
+// SIGNED: m, else v.  The exponent of the foot of float32's range, seen from a group's scale.
 template <bool SIGNED>
-constexpr float kFoot = SIGNED ? 0x1p-112f : 0x1p-96f;  // from a group's scale to the foot of float32's range
+constexpr int kFoot = SIGNED ? 112 : 96;
+__device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Both ways a value is multiplied with a power of two that may be beyond float32: in one step where it is not (averages below
+// 2^15 and 2^31), else in two.  The first of two steps is exact, or what it leaves ends as zero in either way.
 template <bool SIGNED>
 __device__ __forceinline__ void values_of(uint2 codes, uint32_t scale, float (&f)[kEach]) {
-  const float power = __uint_as_float(scale == 255 ? 0x7fc00000u : scale << 23);
+  const int e = (int)scale - 127;
+  const bool once = e + kFoot<SIGNED> <= 127;
+  const float power = scale == 0     ? 0.0f
+                      : scale == 255 ? __uint_as_float(0x7fc00000u)
+                                     : power_of(once ? e + kFoot<SIGNED> : e);
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    const uint32_t c = (j < 4 ? codes.x : codes.y) >> (j % 4 * 8);
-    const uint32_t bits = SIGNED ? (c & 0x80u) << 24 | (c & 0x7fu) << 20 : (c & 0xffu) << 20;
-    f[j] = __fmul_rn(__fmul_rn(__uint_as_float(bits), 1.0f / kFoot<SIGNED>), power);
+    const uint32_t top = __byte_perm(j < 4 ? codes.x : codes.y, 0, 0x0444u | (uint32_t)(j % 4) << 12);  // the code on top
+    const uint32_t bits = SIGNED ? (uint32_t)((int)top >> 4) & 0x87f00000u : top >> 4;
+    f[j] = __uint_as_float(bits);
   }
+  if (!once) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) f[j] = __fmul_rn(f[j], power_of(kFoot<SIGNED>));
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) f[j] = __fmul_rn(f[j], power);
 }
 // The largest magnitude of a group's 16 threads, as bits; a NaN's are above all others.
 __device__ __forceinline__ uint32_t top_of(const float (&f)[kEach]) {
-  uint32_t top = 0;
+  float top = fabsf(f[0]);
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+  for (int j = 1; j < kEach; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[j])));
+  uint32_t bits = __float_as_uint(top);
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-  return top;
+  for (int d = 1; d < 16; d *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+  return bits;
 }
-// codes of a group whose largest magnitude is top, and its scale; cut[j]: what is added to the 20 bits that are cut off
-template <bool SIGNED>
-__device__ __forceinline__ uint2 codes_of(const float (&f)[kEach], uint32_t top, const uint32_t (&cut)[kEach],
-                                          uint32_t* scale) {
+// Codes of a group whose largest magnitude is top, and its scale; cut(j): what is added to the 20 bits that are cut off.
+template <bool SIGNED, class F>
+__device__ __forceinline__ uint2 codes_of(float (&f)[kEach], uint32_t top, F&& cut, uint32_t* scale) {
   const int e = max((int)(top >> 23) - 127 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
   *scale = top == 0 ? 0 : e > 126 ? 255 : (uint32_t)(e + 127);
   if (*scale == 0 || *scale == 255) return make_uint2(0, 0);
-  const float power = __uint_as_float((uint32_t)(127 - e) << 23);
-  uint32_t w[2] = {0, 0};
+  const bool once = e + kFoot<SIGNED> <= 126;
+  const float power = power_of(once ? -e - kFoot<SIGNED> : -e);
+  uint32_t w[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(fabsf(f[j]), power), kFoot<SIGNED>));
-    uint32_t code = (bits + cut[j]) >> 20;
-    if (SIGNED) code |= __float_as_uint(f[j]) >> 24 & 0x80u;
-    else code = max(code, 1u);
-    w[j / 4] |= code << (j % 4 * 8);
+    float size = __fmul_rn(fabsf(f[j]), power);
+    if (!once) size = __fmul_rn(size, power_of(-kFoot<SIGNED>));
+    uint32_t bits = __float_as_uint(size) + cut(j);
+    if (!SIGNED) bits = max(bits, 1u << 20);
+    w[j] = bits << 4;  // the code on top
+    if (SIGNED) w[j] |= __float_as_uint(f[j]) & 0x80000000u;
   }
-  return make_uint2(w[0], w[1]);
+  auto four = [](const uint32_t* v) {
+    return __byte_perm(__byte_perm(v[0], v[1], 0x0073u), __byte_perm(v[2], v[3], 0x0073u), 0x5410u);
+  };
+  return make_uint2(four(w), four(w + 4));
 }
 
 // ---- the step -----------------------------------------------------------------------------------------------------------
+// The unit's square root and reciprocal, off by 2^-23 at most: a parameter's move is added to something much larger.
+__device__ __forceinline__ float root_of(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse_of(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A CTA's pieces, one behind the other: f(tensor, its index in the table, first value of this thread, how many).
+template <int N, class F>
+__device__ __forceinline__ void over_pieces(const Table<N>& table, uint32_t run, F&& f) {
+  uint32_t piece = blockIdx.x * run;
+  const uint32_t end = min(piece + run, table.first[table.count]);
+  int at = tensor_of(table, piece);
+  for (; piece < end; ++piece) {
+    while (piece >= table.first[at + 1]) ++at;
+    const Entry& t = table.tensor[at];
+    const uint64_t i = (uint64_t)(piece - table.first[at]) * kPiece + threadIdx.x * kEach;
+    f(t, at, i, i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0);
+  }
+}
+
 template <int N, bool EIGHT>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> table,
-                                                         const __grid_constant__ Step given) {
+                                                         const __grid_constant__ Step given, uint32_t run) {
   __shared__ Step computed;
   pdl_wait();
-  const int at = tensor_of(table, blockIdx.x);
-  const Entry& t = table.tensor[at];
-  const uint64_t i = (uint64_t)(blockIdx.x - table.first[at]) * kPiece + threadIdx.x * kEach;
-  const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
   float decay = given.decay, size = given.size, root = given.root;
   uint32_t call = given.call;
   if (given.step || given.lr) {
@@ -235,75 +275,79 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     const float q = __fdiv_rn(given.max_norm, __fadd_rn(*given.norm, 1e-6f));
     c = q >= 1.0f ? 1.0f : q;  // NaN of a norm that is none
   }
-  float g[kEach], p[kEach], m[kEach], v[kEach];
-  load_any(t.grad, t.grad_type, i, live, t.packs, g);
-  load_any(t.param, t.param_type, i, live, t.packs, p);
-  if constexpr (EIGHT) {
-    const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
-    values_of<true>(mc, live ? t.m_scale[i / kGroup] : 0, m);
-    values_of<false>(vc, live ? t.v_scale[i / kGroup] : 0, v);
-  } else {
-    load_of<float>(t.m, i, live, t.packs, m);
-    load_of<float>(t.v, i, live, t.packs, v);
-  }
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const float s = __fmul_rn(g[j], c);
-    m[j] = __fadd_rn(__fmul_rn(m[j], given.b1), __fmul_rn(s, given.rest1));
-    v[j] = __fadd_rn(__fmul_rn(v[j], given.b2), __fmul_rn(__fmul_rn(s, given.rest2), s));
-    p[j] = p[j] * decay - size * (m[j] / (sqrtf(v[j]) * root + given.eps));
-  }
-  store_any(t.param, t.param_type, i, live, t.packs, p);
-  if (t.copy) store_any(t.copy, t.copy_type, i, live, t.packs, p);
-  if constexpr (EIGHT) {
-    const uint32_t key = random_of(call, table.place + at) + (uint32_t)i;
-    uint32_t up[kEach], low[kEach], scale;
+  over_pieces(table, run, [&](const Entry& t, int at, uint64_t i, int live) {
+    float g[kEach], p[kEach], m[kEach], v[kEach];
+    uint2 mc, vc;
+    uint32_t m_scale = 0, v_scale = 0;
+    if constexpr (EIGHT) {
+      mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
+      if (live) m_scale = t.m_scale[i / kGroup], v_scale = t.v_scale[i / kGroup];
+    } else {
+      load_of<float>(t.m, i, live, t.packs, m);
+      load_of<float>(t.v, i, live, t.packs, v);
+    }
+    load_any(t.grad, t.grad_type, i, live, t.packs, g);
+    load_any(t.param, t.param_type, i, live, t.packs, p);
+    if constexpr (EIGHT) {
+      values_of<true>(mc, m_scale, m);
+      values_of<false>(vc, v_scale, v);
+    }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const uint32_t r = mix(key + j);
-      up[j] = r >> 16 << 4 | 8, low[j] = (r & 0xffffu) << 4 | 8;
-      if (j >= live) m[j] = v[j] = 0.0f;
+      const float s = __fmul_rn(g[j], c);
+      m[j] = __fadd_rn(__fmul_rn(m[j], given.b1), __fmul_rn(s, given.rest1));
+      v[j] = __fadd_rn(__fmul_rn(v[j], given.b2), __fmul_rn(__fmul_rn(s, given.rest2), s));
+      p[j] = fmaf(p[j], decay, -size * (m[j] * inverse_of(fmaf(root_of(v[j]), root, given.eps))));
     }
-    const uint2 mc = codes_of<true>(m, top_of(m), up, &scale);
-    store_codes(t.m, i, live, t.packs, mc);
-    if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)scale;
-    const uint2 vc = codes_of<false>(v, top_of(v), low, &scale);
-    store_codes(t.v, i, live, t.packs, vc);
-    if (live && threadIdx.x % 16 == 0) t.v_scale[i / kGroup] = (uint8_t)scale;
-  } else {
-    store_of<float>(t.m, i, live, t.packs, m);
-    store_of<float>(t.v, i, live, t.packs, v);
-  }
+    store_any(t.param, t.param_type, i, live, t.packs, p);
+    if (t.copy) store_any(t.copy, t.copy_type, i, live, t.packs, p);
+    if constexpr (EIGHT) {
+      if (live < kEach) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+          if (j >= live) m[j] = v[j] = 0.0f;
+      }
+      const uint32_t m_top = top_of(m), v_top = top_of(v);
+      const uint32_t key = random_of(call, table.place + at) + (uint32_t)i;
+      uint32_t r[kEach];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) r[j] = mix(key + j);
+      mc = codes_of<true>(m, m_top, [&](int j) { return (r[j] >> 12 & 0xffff0u) | 8u; }, &m_scale);
+      vc = codes_of<false>(v, v_top, [&](int j) { return (r[j] << 4 & 0xffff0u) | 8u; }, &v_scale);
+      store_codes(t.m, i, live, t.packs, mc);
+      store_codes(t.v, i, live, t.packs, vc);
+      if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)m_scale, t.v_scale[i / kGroup] = (uint8_t)v_scale;
+    } else {
+      store_of<float>(t.m, i, live, t.packs, m);
+      store_of<float>(t.v, i, live, t.packs, v);
+    }
+  });
 }
 
 // The state in 8 bits from and to averages in 32, which stand in the places of param and copy; rounded to the nearest.
 template <int N, bool PACK>
-__global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table) {
+__global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table, uint32_t run) {
   pdl_wait();
-  const int at = tensor_of(table, blockIdx.x);
-  const Entry& t = table.tensor[at];
-  const uint64_t i = (uint64_t)(blockIdx.x - table.first[at]) * kPiece + threadIdx.x * kEach;
-  const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
-  float m[kEach], v[kEach];
-  if constexpr (PACK) {
-    load_of<float>(t.param, i, live, t.packs, m);
-    load_of<float>(t.copy, i, live, t.packs, v);
-    uint32_t half[kEach], scale;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) half[j] = 1u << 19;
-    const uint2 mc = codes_of<true>(m, top_of(m), half, &scale);
-    store_codes(t.m, i, live, t.packs, mc);
-    if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)scale;
-    const uint2 vc = codes_of<false>(v, top_of(v), half, &scale);
-    store_codes(t.v, i, live, t.packs, vc);
-    if (live && threadIdx.x % 16 == 0) t.v_scale[i / kGroup] = (uint8_t)scale;
-  } else {
-    const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
-    values_of<true>(mc, live ? t.m_scale[i / kGroup] : 0, m);
-    values_of<false>(vc, live ? t.v_scale[i / kGroup] : 0, v);
-    store_of<float>(t.param, i, live, t.packs, m);
-    store_of<float>(t.copy, i, live, t.packs, v);
-  }
+  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, int live) {
+    float m[kEach], v[kEach];
+    uint32_t m_scale = 0, v_scale = 0;
+    if constexpr (PACK) {
+      load_of<float>(t.param, i, live, t.packs, m);
+      load_of<float>(t.copy, i, live, t.packs, v);
+      auto half = [](int) { return 1u << 19; };
+      const uint2 mc = codes_of<true>(m, top_of(m), half, &m_scale), vc = codes_of<false>(v, top_of(v), half, &v_scale);
+      store_codes(t.m, i, live, t.packs, mc);
+      store_codes(t.v, i, live, t.packs, vc);
+      if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)m_scale, t.v_scale[i / kGroup] = (uint8_t)v_scale;
+    } else {
+      const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
+      if (live) m_scale = t.m_scale[i / kGroup], v_scale = t.v_scale[i / kGroup];
+      values_of<true>(mc, m_scale, m);
+      values_of<false>(vc, v_scale, v);
+      store_of<float>(t.param, i, live, t.packs, m);
+      store_of<float>(t.copy, i, live, t.packs, v);
+    }
+  });
 }
 
 // ---- the norm -----------------------------------------------------------------------------------------------------------
@@ -319,21 +363,18 @@ __device__ __forceinline__ double sum_of_threads(double s) {
 }
 // Squares are summed in 64 bits: a norm that goes into every value must not depend on the order of its sum.
 template <int N>
-__global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ Table<N> table, double* parts) {
+__global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ Table<N> table, uint32_t run,
+                                                              double* parts) {
   pdl_wait();
-  double s = 0.0;
-  for (uint32_t piece = blockIdx.x; piece < table.first[table.count]; piece += gridDim.x) {
-    const int at = tensor_of(table, piece);
-    const Entry& t = table.tensor[at];
-    const uint64_t i = (uint64_t)(piece - table.first[at]) * kPiece + threadIdx.x * kEach;
-    const int live = i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of their own, so that one need not wait for the other
+  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, int live) {
     float g[kEach];
     load_any(t.grad, t.grad_type, i, live, t.packs, g);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) s = fma((double)g[j], (double)g[j], s);
-  }
-  s = sum_of_threads(s);
-  if (threadIdx.x == 0) parts[blockIdx.x] = s;
+    for (int j = 0; j < kEach; ++j) s[j % 4] = fma((double)g[j], (double)g[j], s[j % 4]);
+  });
+  const double sum = sum_of_threads((s[0] + s[1]) + (s[2] + s[3]));
+  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 __global__ void __launch_bounds__(kThreads) norm_sum_kernel(const double* __restrict__ parts, uint32_t count, float* norm) {
   pdl_wait(parts);
@@ -379,7 +420,9 @@ template <class F>
 cudaError_t in_any_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch) {
   return count <= kFew ? in_tables<kFew>(tensors, count, launch) : in_tables<kMany>(tensors, count, launch);
 }
-uint32_t norm_grid(uint64_t pieces) { return (uint32_t)std::min<uint64_t>(pieces, (uint64_t)sm_count() * 8); }
+// Pieces of a CTA: the search for its tensor is spread over some, as long as there are CTAs for eight an SM.
+uint32_t run_of(uint32_t pieces) { return std::min(std::max(pieces / (8u * (uint32_t)sm_count()), 1u), 8u); }
+uint32_t grid_of(uint32_t pieces, uint32_t run) { return pieces / run + (pieces % run != 0); }
 
 }  // namespace
 
@@ -392,22 +435,25 @@ cudaError_t adamw_launch(const csw_adamw_tensor* tensors, size_t count, const cs
   settle(s, o.step, o.lr);
   return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
     constexpr int N = std::decay_t<decltype(table)>::kSize;
-    return pdl_launch(o.bits == 8 ? adamw_kernel<N, true> : adamw_kernel<N, false>, pieces, kThreads, 0, stream, table, s);
+    const uint32_t run = run_of(pieces);
+    return pdl_launch(o.bits == 8 ? adamw_kernel<N, true> : adamw_kernel<N, false>, grid_of(pieces, run), kThreads, 0, stream,
+                      table, s, run);
   });
 }
 
 cudaError_t adamw8_convert_launch(const csw_adamw_tensor* tensors, size_t count, bool pack, cudaStream_t stream) {
   return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
     constexpr int N = std::decay_t<decltype(table)>::kSize;
-    return pdl_launch(pack ? adamw8_convert_kernel<N, true> : adamw8_convert_kernel<N, false>, pieces, kThreads, 0, stream,
-                      table);
+    const uint32_t run = run_of(pieces);
+    return pdl_launch(pack ? adamw8_convert_kernel<N, true> : adamw8_convert_kernel<N, false>, grid_of(pieces, run), kThreads,
+                      0, stream, table, run);
   });
 }
 
 uint64_t gradient_norm_partials(const csw_adamw_tensor* tensors, size_t count) {
   uint64_t parts = 0;
   in_any_tables(tensors, count, [&](const auto&, uint32_t pieces) {
-    parts += norm_grid(pieces);
+    parts += grid_of(pieces, run_of(pieces));
     return cudaSuccess;
   });
   return parts;
@@ -418,8 +464,8 @@ cudaError_t gradient_norm_launch(const csw_adamw_tensor* tensors, size_t count, 
   uint32_t parts = 0;
   const cudaError_t e = in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
     constexpr int N = std::decay_t<decltype(table)>::kSize;
-    const uint32_t grid = norm_grid(pieces);
-    const cudaError_t e = pdl_launch(norm_parts_kernel<N>, grid, kThreads, 0, stream, table, partials + parts);
+    const uint32_t run = run_of(pieces), grid = grid_of(pieces, run);
+    const cudaError_t e = pdl_launch(norm_parts_kernel<N>, grid, kThreads, 0, stream, table, run, partials + parts);
     parts += grid;
     return e;
   });

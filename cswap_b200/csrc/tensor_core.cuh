@@ -62,11 +62,20 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, 
       ::"r"(dst), "l"(map), "r"(bar), "r"(dim), "r"(token), "r"(head), "r"(batch)
       : "memory");
 }
+// For one lane alone, the others passing by: me is true for that lane (elected(), once).  A branch around the instruction
+// instead costs a warp that issues step after step some 50 clocks each time.
+#define CSW_MINE(me_operand) "{\n\t.reg .pred me;\n\tsetp.ne.b32 me, " me_operand ", 0;\n\t@me "
+__device__ __forceinline__ void bar_expect_by(bool me, uint32_t bar, uint32_t bytes) {
+  asm volatile(CSW_MINE("%2") "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes),
+               "r"((uint32_t)me)
+               : "memory");
+}
 // a tile of a matrix of bytes, columns x (a multiple of 16) and rows y
-__device__ __forceinline__ void copy_bytes_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+__device__ __forceinline__ void copy_bytes_tile_by(bool me, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(x), "r"(y)
+      CSW_MINE("%5") "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];\n\t}" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"((uint32_t)me)
       : "memory");
 }
 // bytes (a multiple of 16) from a 16-byte boundary
@@ -84,6 +93,14 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, uint32_t src,
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// columns x and rows y of a matrix
+__device__ __forceinline__ void store_matrix_tile(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x),
+               "r"(y)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // the source of this thread's stores may be written again
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
@@ -230,14 +247,16 @@ __host__ __device__ constexpr uint32_t scaled_desc(int n, bool a_across, bool b_
   return (a_across ? 1u << 15 : 0u) | (b_across ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | 1u << 23 |
          (uint32_t)(128 / 16) << 24;
 }
+// which byte of the scales' words counts, for both operands
+__device__ __forceinline__ uint32_t scales_of(uint32_t which) { return which << 4 | which << 29; }
 // One reduction step of 32, 32 bytes further along a row or 32 rows, 4096 bytes, across.  The operands' scales lie in tensor
-// memory, one of a row (a column of the result) in lane row % 32 of column row / 32, each byte of it for a step of its own.
-__device__ __forceinline__ void mma_scaled(uint32_t acc, uint64_t a, uint64_t b, uint32_t desc, uint32_t a_scales,
-                                           uint32_t b_scales, bool add) {
+// memory, a word for a row (a column of the result) in lane row % 32 of column row / 32.
+__device__ __forceinline__ void mma_scaled_by(bool me, uint32_t acc, uint64_t a, uint64_t b, uint32_t desc,
+                                              uint32_t a_scales, uint32_t b_scales, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
-      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(a_scales), "r"(b_scales)
+      "{\n\t.reg .pred me, p;\n\tsetp.ne.b32 me, %7, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@me tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(a_scales), "r"(b_scales), "r"((uint32_t)me)
       : "memory");
 }
 // 512 bytes of scales to four columns of tensor memory, behind the products and copies issued before: rows of 16 bytes, a
@@ -248,9 +267,106 @@ __device__ __forceinline__ uint64_t scales_desc(uint32_t at) {
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t from) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from) : "memory");
 }
+__device__ __forceinline__ void commit_by(bool me, uint32_t bar) {
+  asm volatile(CSW_MINE("%1") "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+               "r"((uint32_t)me)
+               : "memory");
+}
 // arrives at `bar` when all products issued before have ended
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- two CTAs on one product -----------------------------------------------------------------------------------------
+// A cluster of two CTAs on neighbouring SMs: the first one issues products of 256 rows, of which each has 128, in its own
+// shared and tensor memory; of the columns' operand each brings half.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// where a CTA of the cluster has what this one has at an address of its shared memory
+__device__ __forceinline__ uint32_t peer_at(uint32_t at, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same where no ordinary stores of this thread have to be seen there: a release to the whole cluster waits for them, for
+// some 2000 clocks.
+__device__ __forceinline__ void peer_arrive_near(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+// bar_wait for a barrier that CTAs of the cluster arrive at
+__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, long long patience) {
+  if (bar_try_cluster(bar, parity)) return true;
+  const long long start = clock64();
+  do {
+    if (bar_try_cluster(bar, parity)) return true;
+  } while (clock64() - start < patience);
+  return false;
+}
+// copy_bytes_tile_by into this CTA's shared memory, told at a barrier of either
+__device__ __forceinline__ void copy_bytes_tile_pair_by(bool me, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                                        int y) {
+  asm volatile(
+      CSW_MINE("%5") "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"((uint32_t)me)
+      : "memory");
+}
+// bytes (a multiple of 16) from this CTA's shared memory to another one's, told there
+__device__ __forceinline__ void send_bytes(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "r"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t at) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "n"(COLUMNS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_free_pair(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS));
+}
+__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t from) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(from) : "memory");
+}
+// scaled_desc of 128 rows plus this: 256 rows
+constexpr uint32_t kPairRows = (uint32_t)(128 / 16) << 24;
+__device__ __forceinline__ void mma_scaled_pair_by(bool me, uint32_t acc, uint64_t a, uint64_t b, uint32_t desc,
+                                                   uint32_t a_scales, uint32_t b_scales, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred me, p;\n\tsetp.ne.b32 me, %7, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@me tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(a_scales), "r"(b_scales), "r"((uint32_t)me)
+      : "memory");
+}
+// arrives at this barrier of both CTAs when all products issued before have ended
+__device__ __forceinline__ void commit_pair_by(bool me, uint32_t bar) {
+  asm volatile(
+      CSW_MINE("%2") "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+          "r"(bar),
+      "h"((uint16_t)3), "r"((uint32_t)me)
+      : "memory");
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {

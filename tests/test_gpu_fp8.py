@@ -319,3 +319,19 @@ def test_a_last_row_without_its_padding_is_refused(cs):
     one = torch.zeros(1, 50, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
     with pytest.raises(ValueError, match="padded"):
         cs.fp8_dequantize(one, scales)
+
+
+@pytest.mark.parametrize("ta,tb", [(False, True), (False, False), (True, False), (True, True)],
+                         ids=["nt", "nn", "tn", "tt"])
+@pytest.mark.parametrize("m,n,k", [(2304, 2048, 640), (3000, 1700, 300), (2500, 1801, 4500), (1025, 5000, 100)])
+def test_products_of_many_tiles(cs, m, n, k, ta, tb):
+    """Tiles that two CTAs share, one behind the other on the same pair; results whose rows begin on 16 bytes and anywhere."""
+    a, b, A, B = operands(cs, m, n, k, ta, tb)
+    for kind in KINDS:
+        bias = normal(n, seed=9, kind=kind)
+        got = cs.fp8_matmul(*a, *b, transpose_a=ta, transpose_b=tb, bias=bias, dtype=kind)
+        want, bound = R.product(A, B, bias, kind)
+        if kind == torch.float16:  # what half precision cannot hold
+            bound = bound.masked_fill(want.abs() > 65000, math.inf)
+            got, want = got.clamp(-65504, 65504), want.clamp(-65504, 65504)
+        R.close(got, want, bound)
