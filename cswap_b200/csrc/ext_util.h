@@ -57,6 +57,16 @@ inline at::Tensor new_on(const at::Tensor& like, int64_t n, at::ScalarType type)
   return at::empty({n}, at::TensorOptions().dtype(type).device(like.device()));
 }
 
+// The same outside of Python's calls, in a thread of autograd's: the exception that g_check raises, thrown
+inline void require_ok(csw_status st, const char* what) {
+  if (st == CSW_OK) return;
+  PyGILState_STATE gil = PyGILState_Ensure();
+  python_error err;
+  if (!status_ok(st, what)) err.persist();
+  PyGILState_Release(gil);
+  throw err;
+}
+
 // What every call ends with: the ABI call on the tensor's device and torch's
 // current stream there, without the interpreter lock.
 template <class F>
@@ -126,6 +136,11 @@ inline PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
   }
   return r;
 }
+
+// While a graph is captured, refuses a leaf, also behind views and copies, whose gradient accumulator a graph of another
+// stream keeps (with a Python exception set).  Backward would hand the gradient over to that stream in the middle of the
+// capture, an error that autograd's threads do not survive.  (ops_ext.cpp)
+bool capture_allows(const at::Tensor& t);
 
 #define CSW_METHOD(name, doc) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, doc}
 

@@ -55,12 +55,18 @@ struct Eight {
   }
   __device__ __forceinline__ void load(const T* from, int live) {
     using Bits = typename Words<sizeof(T)>::type;
-    const Bits* bits = reinterpret_cast<const Bits*>(from);
+    uint32_t bits[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bits[j] = 0;
+      if (j < live) bits[j] = reinterpret_cast<const Bits*>(from)[j];
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = sizeof(T) == 4 ? bits[i] : bits[2 * i] | bits[2 * i + 1] << 16;
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < live) w[j * sizeof(T) / 4] |= (uint32_t)bits[j] << (j * sizeof(T) % 4 * 8);
   }
   // from any place, by the packs of 16 bytes that it lies in
   __device__ __forceinline__ void load_across(const T* from) {
@@ -101,6 +107,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T*
                                                                         uint64_t code_stride, uint8_t* scales, float* sums) {
   __shared__ uint32_t tops[kQuantizeThreads / 32];
   __shared__ float column[SUMS ? 16 : 1][SUMS ? kBlock : 1];
+  pdl_trigger_if_few();
   pdl_wait(x);
   const uint32_t blocks = (uint32_t)((cols + kBlock - 1) / kBlock);
   const uint64_t bi = blockIdx.x / blocks, bj = blockIdx.x % blocks;
@@ -112,16 +119,20 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T*
 #pragma unroll
     for (int i = 0; i < kRowsEach; ++i) v[i].load(from + 16 * i * stride);
   } else {
-    // Rows that begin anywhere, or end in the block.  Packs that a value lies in are read whole where they are x's.
+    // Rows that begin anywhere, or end in the block: packs that a value lies in are read whole where they are x's.
     const int live = (int)min((int64_t)8, max((int64_t)cols - (int64_t)col, (int64_t)0));  // of this thread's columns
+    const int here = row < rows ? (int)min((rows - 1 - row) / 16, (uint64_t)(kRowsEach - 1)) : -1;  // its last row
     const uintptr_t begin = reinterpret_cast<uintptr_t>(x), end = begin + ((rows - 1) * stride + cols) * sizeof(T);
+    const uintptr_t first = reinterpret_cast<uintptr_t>(from), last = reinterpret_cast<uintptr_t>(from + 16 * here * (int64_t)stride);
+    if (live == 8 && here >= 0 && (first & ~(uintptr_t)15) >= begin && (last & ~(uintptr_t)15) + 8 * sizeof(T) + 16 <= end) {
 #pragma unroll
-    for (int i = 0; i < kRowsEach; ++i) {
-      const T* at = from + 16 * i * stride;
-      const int here = row + 16 * i < rows ? live : 0;
-      const uintptr_t first = reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)15;
-      if (here == 8 && first >= begin && first + 8 * sizeof(T) + 16 <= end) v[i].load_across(at);
-      else v[i].load(at, here);
+      for (int i = 0; i < kRowsEach; ++i) {
+        v[i].load_across(from + 16 * min(i, here) * stride);
+        if (i > here) v[i].clear();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowsEach; ++i) v[i].load(from + 16 * i * stride, i <= here ? live : 0);
     }
   }
   uint32_t top = 0;
@@ -188,6 +199,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T*
 __global__ void __launch_bounds__(256) fp8_sums_kernel(const float* __restrict__ partials, uint64_t parts, uint64_t cols,
                                                        float* sums) {
   __shared__ float part[8][32];
+  pdl_trigger_if_few();
   pdl_wait(partials);
   const uint64_t col = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
   const int p = threadIdx.x / 32;
@@ -209,6 +221,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_dequantize_kernel(const 
                                                                           uint64_t code_stride,
                                                                           const uint8_t* __restrict__ scales, uint64_t rows,
                                                                           uint64_t cols, bool packs, T* out) {
+  pdl_trigger_if_few();
   pdl_wait(codes);
   pdl_behind(scales);
   const uint32_t blocks = (uint32_t)((cols + kBlock - 1) / kBlock);
@@ -443,6 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
   // Every CTA's barriers are there.  From here to where tensor memory is freed no CTA waits for another one, which might wait
   // for that memory.
   if (p.parts > 1) cluster_meet();
+  pdl_trigger_if_few();
   pdl_wait();  // before tensor memory is taken, which a kernel in front may still hold
   if (warp == 3) tmem_alloc<L::kColumns>(smem_at(&tmem_at));
   fence_before();

@@ -14,6 +14,24 @@
 using namespace cswext;
 
 namespace {
+std::shared_ptr<torch::autograd::Node> accumulator_of(const at::Tensor& t);
+}  // namespace
+
+bool cswext::capture_allows(const at::Tensor& t) {
+  if (!t.is_cuda() || !t.requires_grad()) return true;
+  const c10::cuda::CUDAGuard on(t.device());  // the operands of a call are on one device, and refused otherwise
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return true;
+  const auto node = accumulator_of(t);
+  if (!node) return true;
+  const auto stream = node->stream();
+  if (!stream || *stream == c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap()) return true;
+  PyErr_SetString(PyExc_RuntimeError,
+                  "a leaf of this captured step is also a leaf of a live graph of another stream: "
+                  "let go of that graph (its outputs and losses) before the capture");
+  return false;
+}
+
+namespace {
 
 bool require_like(const at::Tensor& t, const at::Tensor& as, const char* name) {
   if (!same_device(t, as, name)) return false;
@@ -408,27 +426,11 @@ std::shared_ptr<torch::autograd::Node> accumulator_of(const at::Tensor& t) {
   return node && dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()) ? node : nullptr;
 }
 
-// check_capture(tensors): while a graph is captured, refuses leaves, also behind views and copies, whose gradient
-// accumulator a graph of another stream keeps.  Backward would hand the gradient over to that stream in the middle of the
-// capture, an error that autograd's threads do not survive.
+// check_capture(tensors): capture_allows
 PyObject* check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      if (!THPVariable_Check(a[i])) continue;
-      const at::Tensor& t = THPVariable_Unpack(a[i]);
-      if (!t.is_cuda() || !t.requires_grad()) continue;
-      const c10::cuda::CUDAGuard on(t.device());  // the operands of a call are on one device, and refused otherwise
-      if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) break;
-      const auto node = accumulator_of(t);
-      if (!node) continue;
-      const auto stream = node->stream();
-      if (stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap()) {
-        PyErr_SetString(PyExc_RuntimeError,
-                        "a leaf of this captured step is also a leaf of a live graph of another stream: "
-                        "let go of that graph (its outputs and losses) before the capture");
-        return nullptr;
-      }
-    }
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (THPVariable_Check(a[i]) && !capture_allows(THPVariable_Unpack(a[i]))) return nullptr;
     Py_RETURN_NONE;
   });
 }

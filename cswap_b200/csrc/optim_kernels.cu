@@ -16,12 +16,19 @@
 // not rounded to zero in a group that has anything: m's smallest step is 2^-17 of its group's scale, the root of v's smallest
 // 2^-16.5, so that m / sqrt(v) stays of the size that it has for the group's largest.
 //
+// What bounds it.  In 32 bits HBM: 28 bytes a value, 447 us for the 110 M float32 parameters of a BERT-base-shaped encoder, 6.8
+// TB/s.  In 8 bits the instructions, some 70 a value (8 of them for its random bits, 20 for both codes): as many with 16-bit
+// gradients and copies 350 us, 1.3 times what its bytes take; 40 registers a thread, so that six CTAs an SM cover one another's
+// loads (64 registers, four CTAs: a tenth longer).
+//
 // Every 32-bit operation that a code depends on is rounded by itself (no fused multiply-add), so that the codes follow from
 // the definition whatever a compiler does.
 //
 // One launch takes hundreds of tensors: where they lie travels in the kernel's parameters, so that nothing is copied to the
 // device and a captured call holds all that it needs.
 #include "optim_kernels.h"
+
+#include <cuda_fp8.h>
 
 #include <algorithm>
 #include <cmath>
@@ -34,9 +41,13 @@
 namespace csw {
 namespace {
 
-constexpr int kThreads = 256, kEach = 8;  // values of a thread: a sixteenth of a group
-constexpr uint32_t kPiece = kThreads * kEach;
-constexpr int kGroup = 128;
+// A piece of a tensor is 2048 values, 8 a thread: a group of 128 belongs to half a warp, whose lanes have four neighbours of its
+// first half and four of its second, so that loads and stores of any type are runs of whole lines.
+constexpr int kThreads = 256, kGroup = 128;
+constexpr uint32_t kPiece = kThreads * 8;
+// a thread's first value in a piece; the second four are kNext further on
+__device__ __forceinline__ uint32_t first_value() { return threadIdx.x / 16 * kGroup + threadIdx.x % 16 * 4; }
+constexpr uint32_t kNext = kGroup / 2;
 
 struct Entry {
   const void* grad;
@@ -44,7 +55,7 @@ struct Entry {
   uint8_t *m_scale, *v_scale;
   uint64_t numel;
   uint8_t param_type, grad_type, copy_type;  // CSW_TYPE_*
-  bool packs;                                // all of the tensors lie so that 8 values of one are whole packs
+  bool packs;                                // all of the tensors lie so that four values are one load
 };
 template <int N>
 struct Table {
@@ -54,7 +65,7 @@ struct Table {
   int count;
   uint32_t place;  // of the first tensor in the call
 };
-// Kernel parameters are 32764 bytes at most.  A launch with the large table costs the host 2 us more.
+// Kernel parameters are 32764 bytes at most.
 constexpr int kFew = 40, kMany = 380;
 
 struct Step {
@@ -100,71 +111,83 @@ __device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t piece) {
   return lo;
 }
 
-// 8 values from index i on, zeros behind the last one
-template <class T>
-__device__ __forceinline__ void load_of(const void* from, uint64_t i, int live, bool packs, float (&f)[kEach]) {
+// Eight values of a thread, from index i and i + kNext on.  WHOLE: all of a tensor that lies in packs; else those below n, and
+// zeros for the others.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load_of(const void* from, uint64_t i, uint64_t n, bool packs, float (&f)[8]) {
   const T* p = static_cast<const T*>(from) + i;
-  if (packs && live == kEach) {
-    constexpr int kPack = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < kEach; j += kPack) {
-      float v[kPack];
-      load_pack(p + j, v);
+  for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (WHOLE || (packs && i + 4 <= n)) {
+      load_pack(p, v);
+    } else {
 #pragma unroll
-      for (int k = 0; k < kPack; ++k) f[j + k] = v[k];
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) v[j] = widen(p[j]);
     }
-  } else {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) f[j] = j < live ? widen(p[j]) : 0.0f;
+    for (int j = 0; j < 4; ++j) f[4 * q + j] = v[j];
   }
 }
-template <class T>
-__device__ __forceinline__ void store_of(void* to, uint64_t i, int live, bool packs, const float (&f)[kEach]) {
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store_of(void* to, uint64_t i, uint64_t n, bool packs, const float (&f)[8]) {
   T* p = static_cast<T*>(to) + i;
-  if (packs && live == kEach) {
-    constexpr int kPack = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < kEach; j += kPack) {
-      float v[kPack];
+  for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
+    const float v[4] = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
+    if (WHOLE || (packs && i + 4 <= n)) {
+      store_pack(p, v);
+    } else {
 #pragma unroll
-      for (int k = 0; k < kPack; ++k) v[k] = f[j + k];
-      store_pack(p + j, v);
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) p[j] = narrow<T>(v[j]);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (j < live) p[j] = narrow<T>(f[j]);
   }
 }
-__device__ __forceinline__ void load_any(const void* from, int type, uint64_t i, int live, bool packs, float (&f)[kEach]) {
-  if (type == CSW_TYPE_F32) load_of<float>(from, i, live, packs, f);
-  else if (type == CSW_TYPE_F16) load_of<__half>(from, i, live, packs, f);
-  else load_of<__nv_bfloat16>(from, i, live, packs, f);
+template <bool WHOLE>
+__device__ __forceinline__ void load_any(const void* from, int type, uint64_t i, uint64_t n, bool packs, float (&f)[8]) {
+  if (type == CSW_TYPE_F32) load_of<float, WHOLE>(from, i, n, packs, f);
+  else if (type == CSW_TYPE_F16) load_of<__half, WHOLE>(from, i, n, packs, f);
+  else load_of<__nv_bfloat16, WHOLE>(from, i, n, packs, f);
 }
-__device__ __forceinline__ void store_any(void* to, int type, uint64_t i, int live, bool packs, const float (&f)[kEach]) {
-  if (type == CSW_TYPE_F32) store_of<float>(to, i, live, packs, f);
-  else if (type == CSW_TYPE_F16) store_of<__half>(to, i, live, packs, f);
-  else store_of<__nv_bfloat16>(to, i, live, packs, f);
+template <bool WHOLE>
+__device__ __forceinline__ void store_any(void* to, int type, uint64_t i, uint64_t n, bool packs, const float (&f)[8]) {
+  if (type == CSW_TYPE_F32) store_of<float, WHOLE>(to, i, n, packs, f);
+  else if (type == CSW_TYPE_F16) store_of<__half, WHOLE>(to, i, n, packs, f);
+  else store_of<__nv_bfloat16, WHOLE>(to, i, n, packs, f);
 }
 
 // ---- 8-bit codes ------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint2 load_codes(const void* from, uint64_t i, int live, bool packs) {
+template <bool WHOLE>
+__device__ __forceinline__ uint2 load_codes(const void* from, uint64_t i, uint64_t n, bool packs) {
   const uint8_t* p = static_cast<const uint8_t*>(from) + i;
-  if (packs && live == kEach) return *reinterpret_cast<const uint2*>(p);
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    if (j < live) w[j / 4] |= (uint32_t)p[j] << (j % 4 * 8);
+  for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
+    if (WHOLE || (packs && i + 4 <= n)) {
+      w[q] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) w[q] |= (uint32_t)p[j] << 8 * j;
+    }
+  }
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void store_codes(void* to, uint64_t i, int live, bool packs, uint2 codes) {
+template <bool WHOLE>
+__device__ __forceinline__ void store_codes(void* to, uint64_t i, uint64_t n, bool packs, uint2 codes) {
   uint8_t* p = static_cast<uint8_t*>(to) + i;
-  if (packs && live == kEach) {
-    *reinterpret_cast<uint2*>(p) = codes;
-  } else {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (j < live) p[j] = (uint8_t)((j < 4 ? codes.x : codes.y) >> (j % 4 * 8));
+  for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
+    const uint32_t w = q ? codes.y : codes.x;
+    if (WHOLE || (packs && i + 4 <= n)) {
+      *reinterpret_cast<uint32_t*>(p) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) p[j] = (uint8_t)(w >> 8 * j);
+    }
   }
 }
 // SIGNED: m, else v.  The exponent of the foot of float32's range, seen from a group's scale.
@@ -172,76 +195,97 @@ template <bool SIGNED>
 constexpr int kFoot = SIGNED ? 112 : 96;
 __device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Both ways a value is multiplied with a power of two that may be beyond float32: in one step where it is not (averages below
-// 2^15 and 2^31), else in two.  The first of two steps is exact, or what it leaves ends as zero in either way.
+// Both ways a value is multiplied with a power of two that may be beyond float32: in one step where it is not (averages from
+// 2^-118 to 2^15 and 2^31, for all of a warp), else in two, of which the first is exact or what it leaves ends as zero in
+// either way; and with what stands for no scale.
 template <bool SIGNED>
-__device__ __forceinline__ void values_of(uint2 codes, uint32_t scale, float (&f)[kEach]) {
-  const int e = (int)scale - 127;
-  const bool once = e + kFoot<SIGNED> <= 127;
-  const float power = scale == 0     ? 0.0f
-                      : scale == 255 ? __uint_as_float(0x7fc00000u)
-                                     : power_of(once ? e + kFoot<SIGNED> : e);
+__device__ __forceinline__ void values_of(uint2 codes, uint32_t scale, float (&f)[8]) {
+  constexpr int kOnce = SIGNED ? -8 : kFoot<SIGNED>;  // from a scale's exponent to that of the one factor
+  if (SIGNED) {  // these codes are e4m3 numbers with the exponent's bias 8 lower (and never that format's NaN)
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const uint32_t top = __byte_perm(j < 4 ? codes.x : codes.y, 0, 0x0444u | (uint32_t)(j % 4) << 12);  // the code on top
-    const uint32_t bits = SIGNED ? (uint32_t)((int)top >> 4) & 0x87f00000u : top >> 4;
-    f[j] = __uint_as_float(bits);
+    for (int j = 0; j < 8; j += 2) {
+      const __half2_raw h =
+          __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 4 ? codes.x : codes.y) >> (j % 4 * 8)), __NV_E4M3);
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      f[j] = v.x, f[j + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      f[j] = __uint_as_float(__byte_perm(j < 4 ? codes.x : codes.y, 0, 0x0444u | (uint32_t)(j % 4) << 12) >> 4);
   }
-  if (!once) {
+  const int e = (int)scale - 127 + kOnce;
+  float power;
+  if (__all_sync(0xffffffffu, scale - 1 < 254 && e >= -126 && e <= 127)) {
+    power = power_of(e);
+  } else {
+    const float exact = scale == 0 ? 0.0f : scale == 255 ? __uint_as_float(0x7fc00000u) : power_of((int)scale - 127);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) f[j] = __fmul_rn(f[j], power_of(kFoot<SIGNED>));
+    for (int j = 0; j < 8; ++j) f[j] = __fmul_rn(f[j], power_of(kOnce));
+    power = exact;
   }
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) f[j] = __fmul_rn(f[j], power);
+  for (int j = 0; j < 8; j += 2) {
+    const Pair v = mul2({f[j], f[j + 1]}, both(power));
+    f[j] = v.x, f[j + 1] = v.y;
+  }
 }
 // The largest magnitude of a group's 16 threads, as bits; a NaN's are above all others.
-__device__ __forceinline__ uint32_t top_of(const float (&f)[kEach]) {
+__device__ __forceinline__ uint32_t top_of(const float (&f)[8]) {
   float top = fabsf(f[0]);
 #pragma unroll
-  for (int j = 1; j < kEach; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[j])));
+  for (int j = 1; j < 8; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[j])));
   uint32_t bits = __float_as_uint(top);
 #pragma unroll
   for (int d = 1; d < 16; d *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
   return bits;
 }
-// Codes of a group whose largest magnitude is top, and its scale; cut(j): what is added to the 20 bits that are cut off.
+// Codes of a group whose largest magnitude is top, and its scale; cut(j): what is added to the 20 bits that are cut off, four
+// bits further up.
 template <bool SIGNED, class F>
-__device__ __forceinline__ uint2 codes_of(float (&f)[kEach], uint32_t top, F&& cut, uint32_t* scale) {
+__device__ __forceinline__ uint2 codes_of(const float (&f)[8], uint32_t top, F&& cut, uint32_t* scale) {
   const int e = max((int)(top >> 23) - 127 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
   *scale = top == 0 ? 0 : e > 126 ? 255 : (uint32_t)(e + 127);
-  if (*scale == 0 || *scale == 255) return make_uint2(0, 0);
-  const bool once = e + kFoot<SIGNED> <= 126;
-  const float power = power_of(once ? -e - kFoot<SIGNED> : -e);
-  uint32_t w[kEach];
+  const bool none = *scale == 0 || *scale == 255;
+  float size[8];
+  if (__all_sync(0xffffffffu, !none && e + kFoot<SIGNED> <= 126)) {
+    const float power = power_of(-e - kFoot<SIGNED>);
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    float size = __fmul_rn(fabsf(f[j]), power);
-    if (!once) size = __fmul_rn(size, power_of(-kFoot<SIGNED>));
-    uint32_t bits = __float_as_uint(size) + cut(j);
-    if (!SIGNED) bits = max(bits, 1u << 20);
-    w[j] = bits << 4;  // the code on top
+    for (int j = 0; j < 8; ++j) size[j] = __fmul_rn(fabsf(f[j]), power);
+  } else {
+    const float power = none ? 0.0f : power_of(-e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) size[j] = __fmul_rn(__fmul_rn(fabsf(f[j]), power), power_of(-kFoot<SIGNED>));
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w[j] = __float_as_uint(size[j]) * 16u + cut(j);  // the code on top
     if (SIGNED) w[j] |= __float_as_uint(f[j]) & 0x80000000u;
+    else w[j] = max(w[j], 1u << 24);
   }
   auto four = [](const uint32_t* v) {
     return __byte_perm(__byte_perm(v[0], v[1], 0x0073u), __byte_perm(v[2], v[3], 0x0073u), 0x5410u);
   };
-  return make_uint2(four(w), four(w + 4));
+  return none ? make_uint2(0, 0) : make_uint2(four(w), four(w + 4));
 }
 
 // ---- the step -----------------------------------------------------------------------------------------------------------
-// The unit's square root and reciprocal, off by 2^-23 at most: a parameter's move is added to something much larger.
+// The unit's square root and reciprocal, off by 2^-23 at most: a parameter's move is added to something much larger.  They take
+// what is below 2^-126 for zero, which an epsilon from 2^-40 on does not notice; below that the exact ones are taken.
 __device__ __forceinline__ float root_of(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float inverse_of(float x) {
   float y;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// A CTA's pieces, one behind the other: f(tensor, its index in the table, first value of this thread, how many).
+// A CTA's pieces, one behind the other: f(tensor, its index in the table, this thread's first value in it, whole), whole as
+// std::true_type for a piece that has nothing but values in packs: there is then nothing to ask for each of them.
 template <int N, class F>
 __device__ __forceinline__ void over_pieces(const Table<N>& table, uint32_t run, F&& f) {
   uint32_t piece = blockIdx.x * run;
@@ -250,102 +294,131 @@ __device__ __forceinline__ void over_pieces(const Table<N>& table, uint32_t run,
   for (; piece < end; ++piece) {
     while (piece >= table.first[at + 1]) ++at;
     const Entry& t = table.tensor[at];
-    const uint64_t i = (uint64_t)(piece - table.first[at]) * kPiece + threadIdx.x * kEach;
-    f(t, at, i, i < t.numel ? (int)min(t.numel - i, (uint64_t)kEach) : 0);
+    const uint64_t begin = (uint64_t)(piece - table.first[at]) * kPiece, i = begin + first_value();
+    if (t.packs && begin + kPiece <= t.numel) f(t, at, i, std::true_type());
+    else f(t, at, i, std::false_type());
+  }
+}
+
+// What a CTA knows of the step.
+struct Now {
+  float b1, rest1, b2, rest2, eps, decay, size, root, factor;
+  uint32_t call;
+};
+template <bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void adamw_piece(const Entry& t, uint32_t place, uint64_t i, const Now& now) {
+  const uint64_t n = t.numel, group = i / kGroup;
+  const bool some = WHOLE || group * kGroup < n;
+  float g[8], p[8], m[8], v[8];
+  uint2 mc, vc;
+  uint32_t m_scale = 0, v_scale = 0;
+  if constexpr (EIGHT) {
+    mc = load_codes<WHOLE>(t.m, i, n, t.packs), vc = load_codes<WHOLE>(t.v, i, n, t.packs);
+    if (some) m_scale = t.m_scale[group], v_scale = t.v_scale[group];
+  } else {
+    load_of<float, WHOLE>(t.m, i, n, t.packs, m);
+    load_of<float, WHOLE>(t.v, i, n, t.packs, v);
+  }
+  load_any<WHOLE>(t.grad, t.grad_type, i, n, t.packs, g);
+  load_any<WHOLE>(t.param, t.param_type, i, n, t.packs, p);
+  if constexpr (EIGHT) {
+    values_of<true>(mc, m_scale, m);
+    values_of<false>(vc, v_scale, v);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    // Two at a time only where no sum follows: a product and a sum of pairs become one operation, whatever their rounding says.
+    const Pair s = mul2({g[j], g[j + 1]}, both(now.factor)), r = mul2(s, both(now.rest2));
+    m[j] = __fadd_rn(__fmul_rn(m[j], now.b1), __fmul_rn(s.x, now.rest1));
+    m[j + 1] = __fadd_rn(__fmul_rn(m[j + 1], now.b1), __fmul_rn(s.y, now.rest1));
+    v[j] = __fadd_rn(__fmul_rn(v[j], now.b2), __fmul_rn(r.x, s.x));
+    v[j + 1] = __fadd_rn(__fmul_rn(v[j + 1], now.b2), __fmul_rn(r.y, s.y));
+  }
+  if (now.eps >= 0x1p-40f) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const Pair below = fma2({root_of(v[j]), root_of(v[j + 1])}, both(now.root), both(now.eps));
+      const Pair move = mul2({m[j], m[j + 1]}, {inverse_of(below.x), inverse_of(below.y)});
+      const Pair r = fma2(both(-now.size), move, mul2({p[j], p[j + 1]}, both(now.decay)));
+      p[j] = r.x, p[j + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      p[j] = fmaf(-now.size, m[j] / fmaf(sqrtf(v[j]), now.root, now.eps), p[j] * now.decay);
+  }
+  store_any<WHOLE>(t.param, t.param_type, i, n, t.packs, p);
+  if (t.copy) store_any<WHOLE>(t.copy, t.copy_type, i, n, t.packs, p);
+  if constexpr (EIGHT) {
+    if (!WHOLE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j / 4 * kNext + j % 4 >= n) m[j] = v[j] = 0.0f;
+    }
+    const uint32_t key = random_of(now.call, place) + (uint32_t)i;
+    uint32_t r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = mix(key + j / 4 * kNext + j % 4);
+    mc = codes_of<true>(m, top_of(m), [&](int j) { return (r[j] >> 8 & 0xffff00u) | 0x80u; }, &m_scale);
+    vc = codes_of<false>(v, top_of(v), [&](int j) { return (r[j] << 8 & 0xffff00u) | 0x80u; }, &v_scale);
+    store_codes<WHOLE>(t.m, i, n, t.packs, mc);
+    store_codes<WHOLE>(t.v, i, n, t.packs, vc);
+    if (some && threadIdx.x % 16 == 0) t.m_scale[group] = (uint8_t)m_scale, t.v_scale[group] = (uint8_t)v_scale;
+  } else {
+    store_of<float, WHOLE>(t.m, i, n, t.packs, m);
+    store_of<float, WHOLE>(t.v, i, n, t.packs, v);
   }
 }
 
 template <int N, bool EIGHT>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> table,
-                                                         const __grid_constant__ Step given, uint32_t run) {
+__global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constant__ Table<N> table,
+                                                         const __grid_constant__ Step given) {
   __shared__ Step computed;
+  pdl_trigger_if_few();
   pdl_wait();
-  float decay = given.decay, size = given.size, root = given.root;
-  uint32_t call = given.call;
+  Now now{given.b1, given.rest1, given.b2, given.rest2, given.eps, given.decay, given.size, given.root, 1.0f, given.call};
   if (given.step || given.lr) {
     if (threadIdx.x == 0) {
       computed = given;
       settle(computed, given.step ? *given.step : given.host_step, given.lr ? (double)*given.lr : given.wide_lr);
     }
     __syncthreads();
-    decay = computed.decay, size = computed.size, root = computed.root, call = computed.call;
+    now.decay = computed.decay, now.size = computed.size, now.root = computed.root, now.call = computed.call;
   }
-  float c = 1.0f;
   if (given.norm) {
     const float q = __fdiv_rn(given.max_norm, __fadd_rn(*given.norm, 1e-6f));
-    c = q >= 1.0f ? 1.0f : q;  // NaN of a norm that is none
+    now.factor = q >= 1.0f ? 1.0f : q;  // NaN of a norm that is none
   }
-  over_pieces(table, run, [&](const Entry& t, int at, uint64_t i, int live) {
-    float g[kEach], p[kEach], m[kEach], v[kEach];
-    uint2 mc, vc;
-    uint32_t m_scale = 0, v_scale = 0;
-    if constexpr (EIGHT) {
-      mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
-      if (live) m_scale = t.m_scale[i / kGroup], v_scale = t.v_scale[i / kGroup];
-    } else {
-      load_of<float>(t.m, i, live, t.packs, m);
-      load_of<float>(t.v, i, live, t.packs, v);
-    }
-    load_any(t.grad, t.grad_type, i, live, t.packs, g);
-    load_any(t.param, t.param_type, i, live, t.packs, p);
-    if constexpr (EIGHT) {
-      values_of<true>(mc, m_scale, m);
-      values_of<false>(vc, v_scale, v);
-    }
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const float s = __fmul_rn(g[j], c);
-      m[j] = __fadd_rn(__fmul_rn(m[j], given.b1), __fmul_rn(s, given.rest1));
-      v[j] = __fadd_rn(__fmul_rn(v[j], given.b2), __fmul_rn(__fmul_rn(s, given.rest2), s));
-      p[j] = fmaf(p[j], decay, -size * (m[j] * inverse_of(fmaf(root_of(v[j]), root, given.eps))));
-    }
-    store_any(t.param, t.param_type, i, live, t.packs, p);
-    if (t.copy) store_any(t.copy, t.copy_type, i, live, t.packs, p);
-    if constexpr (EIGHT) {
-      if (live < kEach) {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (j >= live) m[j] = v[j] = 0.0f;
-      }
-      const uint32_t m_top = top_of(m), v_top = top_of(v);
-      const uint32_t key = random_of(call, table.place + at) + (uint32_t)i;
-      uint32_t r[kEach];
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) r[j] = mix(key + j);
-      mc = codes_of<true>(m, m_top, [&](int j) { return (r[j] >> 12 & 0xffff0u) | 8u; }, &m_scale);
-      vc = codes_of<false>(v, v_top, [&](int j) { return (r[j] << 4 & 0xffff0u) | 8u; }, &v_scale);
-      store_codes(t.m, i, live, t.packs, mc);
-      store_codes(t.v, i, live, t.packs, vc);
-      if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)m_scale, t.v_scale[i / kGroup] = (uint8_t)v_scale;
-    } else {
-      store_of<float>(t.m, i, live, t.packs, m);
-      store_of<float>(t.v, i, live, t.packs, v);
-    }
+  over_pieces(table, 1, [&](const Entry& t, int at, uint64_t i, auto whole) {
+    adamw_piece<EIGHT, decltype(whole)::value>(t, table.place + at, i, now);
   });
 }
 
 // The state in 8 bits from and to averages in 32, which stand in the places of param and copy; rounded to the nearest.
 template <int N, bool PACK>
-__global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table, uint32_t run) {
+__global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table) {
+  pdl_trigger_if_few();
   pdl_wait();
-  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, int live) {
-    float m[kEach], v[kEach];
+  over_pieces(table, 1, [&](const Entry& t, int, uint64_t i, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    const uint64_t n = t.numel, group = i / kGroup;
+    const bool some = kWhole || group * kGroup < n;
+    float m[8], v[8];
     uint32_t m_scale = 0, v_scale = 0;
     if constexpr (PACK) {
-      load_of<float>(t.param, i, live, t.packs, m);
-      load_of<float>(t.copy, i, live, t.packs, v);
-      auto half = [](int) { return 1u << 19; };
-      const uint2 mc = codes_of<true>(m, top_of(m), half, &m_scale), vc = codes_of<false>(v, top_of(v), half, &v_scale);
-      store_codes(t.m, i, live, t.packs, mc);
-      store_codes(t.v, i, live, t.packs, vc);
-      if (live && threadIdx.x % 16 == 0) t.m_scale[i / kGroup] = (uint8_t)m_scale, t.v_scale[i / kGroup] = (uint8_t)v_scale;
+      load_of<float, kWhole>(t.param, i, n, t.packs, m);
+      load_of<float, kWhole>(t.copy, i, n, t.packs, v);
+      auto half = [](int) { return 1u << 23; };
+      store_codes<kWhole>(t.m, i, n, t.packs, codes_of<true>(m, top_of(m), half, &m_scale));
+      store_codes<kWhole>(t.v, i, n, t.packs, codes_of<false>(v, top_of(v), half, &v_scale));
+      if (some && threadIdx.x % 16 == 0) t.m_scale[group] = (uint8_t)m_scale, t.v_scale[group] = (uint8_t)v_scale;
     } else {
-      const uint2 mc = load_codes(t.m, i, live, t.packs), vc = load_codes(t.v, i, live, t.packs);
-      if (live) m_scale = t.m_scale[i / kGroup], v_scale = t.v_scale[i / kGroup];
+      const uint2 mc = load_codes<kWhole>(t.m, i, n, t.packs), vc = load_codes<kWhole>(t.v, i, n, t.packs);
+      if (some) m_scale = t.m_scale[group], v_scale = t.v_scale[group];
       values_of<true>(mc, m_scale, m);
       values_of<false>(vc, v_scale, v);
-      store_of<float>(t.param, i, live, t.packs, m);
-      store_of<float>(t.copy, i, live, t.packs, v);
+      store_of<float, kWhole>(t.param, i, n, t.packs, m);
+      store_of<float, kWhole>(t.copy, i, n, t.packs, v);
     }
   });
 }
@@ -365,18 +438,20 @@ __device__ __forceinline__ double sum_of_threads(double s) {
 template <int N>
 __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ Table<N> table, uint32_t run,
                                                               double* parts) {
+  pdl_trigger_if_few();
   pdl_wait();
   double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of their own, so that one need not wait for the other
-  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, int live) {
-    float g[kEach];
-    load_any(t.grad, t.grad_type, i, live, t.packs, g);
+  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, auto whole) {
+    float g[8];
+    load_any<decltype(whole)::value>(t.grad, t.grad_type, i, t.numel, t.packs, g);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) s[j % 4] = fma((double)g[j], (double)g[j], s[j % 4]);
+    for (int j = 0; j < 8; ++j) s[j % 4] = fma((double)g[j], (double)g[j], s[j % 4]);
   });
   const double sum = sum_of_threads((s[0] + s[1]) + (s[2] + s[3]));
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 __global__ void __launch_bounds__(kThreads) norm_sum_kernel(const double* __restrict__ parts, uint32_t count, float* norm) {
+  pdl_trigger();
   pdl_wait(parts);
   double s = 0.0;
   for (uint32_t i = threadIdx.x; i < count; i += kThreads) s += parts[i];
@@ -403,9 +478,10 @@ cudaError_t in_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch)
       e = {t.grad,  t.param, t.copy, t.exp_avg, t.exp_avg_sq, static_cast<uint8_t*>(t.exp_avg_scale),
            static_cast<uint8_t*>(t.exp_avg_sq_scale), t.numel, (uint8_t)t.param_type, (uint8_t)t.grad_type,
            (uint8_t)t.copy_type, true};
-      const size_t state = t.exp_avg_scale ? 8 : 16;
-      e.packs = lies_on(t.grad, 16) && lies_on(t.param, 16) && lies_on(t.copy, 16) && lies_on(t.exp_avg, state) &&
-                lies_on(t.exp_avg_sq, state);
+      const size_t state = t.exp_avg_scale ? 4 : 16;
+      auto four = [](int type) { return type == CSW_TYPE_F32 ? (size_t)16 : (size_t)8; };
+      e.packs = lies_on(t.grad, four(t.grad_type)) && lies_on(t.param, four(t.param_type)) &&
+                lies_on(t.copy, four(t.copy_type)) && lies_on(t.exp_avg, state) && lies_on(t.exp_avg_sq, state);
       table.first[n] = (uint32_t)pieces;
       pieces += more;
     }
@@ -420,7 +496,9 @@ template <class F>
 cudaError_t in_any_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch) {
   return count <= kFew ? in_tables<kFew>(tensors, count, launch) : in_tables<kMany>(tensors, count, launch);
 }
-// Pieces of a CTA: the search for its tensor is spread over some, as long as there are CTAs for eight an SM.
+// Pieces of a CTA of the norm: the search for its tensor and its sum's way out are spread over some, as long as there are CTAs
+// for eight an SM.  (92 us for 110 M bfloat16 values with one piece each, 51 with eight.  The step wants one: 470 us with eight,
+// 447 with one, since new CTAs load while others compute.)
 uint32_t run_of(uint32_t pieces) { return std::min(std::max(pieces / (8u * (uint32_t)sm_count()), 1u), 8u); }
 uint32_t grid_of(uint32_t pieces, uint32_t run) { return pieces / run + (pieces % run != 0); }
 
@@ -435,18 +513,15 @@ cudaError_t adamw_launch(const csw_adamw_tensor* tensors, size_t count, const cs
   settle(s, o.step, o.lr);
   return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
     constexpr int N = std::decay_t<decltype(table)>::kSize;
-    const uint32_t run = run_of(pieces);
-    return pdl_launch(o.bits == 8 ? adamw_kernel<N, true> : adamw_kernel<N, false>, grid_of(pieces, run), kThreads, 0, stream,
-                      table, s, run);
+    return pdl_launch(o.bits == 8 ? adamw_kernel<N, true> : adamw_kernel<N, false>, pieces, kThreads, 0, stream, table, s);
   });
 }
 
 cudaError_t adamw8_convert_launch(const csw_adamw_tensor* tensors, size_t count, bool pack, cudaStream_t stream) {
   return in_any_tables(tensors, count, [&](const auto& table, uint32_t pieces) {
     constexpr int N = std::decay_t<decltype(table)>::kSize;
-    const uint32_t run = run_of(pieces);
-    return pdl_launch(pack ? adamw8_convert_kernel<N, true> : adamw8_convert_kernel<N, false>, grid_of(pieces, run), kThreads,
-                      0, stream, table, run);
+    return pdl_launch(pack ? adamw8_convert_kernel<N, true> : adamw8_convert_kernel<N, false>, pieces, kThreads, 0, stream,
+                      table);
   });
 }
 

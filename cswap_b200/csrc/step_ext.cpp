@@ -2,6 +2,9 @@
 // keep the documented signatures; these functions take every argument by position).
 #include "ext_util.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <algorithm>
 #include <cmath>
 #include <utility>
@@ -51,6 +54,57 @@ bool dtype_of(PyObject* o, at::ScalarType* kind, int* type) {
   return *type >= 0 || value_error("%s must be float32, float16 or bfloat16", "dtype");
 }
 
+struct Quantized {
+  at::Tensor codes, scales, sums;
+};
+// A matrix of rows that lie `stride` values apart.  The values are checked; what the call itself finds wrong is thrown.
+Quantized quantized(const at::Tensor& x, int type, int64_t rows, int64_t cols, int64_t stride, bool sums) {
+  const c10::cuda::CUDAGuard on(x.device());
+  size_t need;
+  require_ok(csw_fp8_quantize_workspace(rows, cols, &need), "csw_fp8_quantize_workspace");
+  const int64_t code_stride = padded(cols);
+  Quantized q{fresh(x, {rows, code_stride}, at::kFloat8_e4m3fn), fresh(x, {blocks_of(rows), blocks_of(cols)}, at::kFloat8_e8m0fnu), {}};
+  at::Tensor space;
+  void* ws = nullptr;
+  float* totals = nullptr;
+  if (sums) {
+    q.sums = fresh(x, {cols}, at::kFloat);
+    totals = static_cast<float*>(out(q.sums));
+    if (need) {
+      space = fresh(x, {(int64_t)need}, at::kByte);
+      ws = out(space);
+    }
+  }
+  require_ok(csw_fp8_quantize(ptr(x), type, rows, cols, stride, out(q.codes), code_stride, out(q.scales), totals, ws, need,
+                              c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+             "csw_fp8_quantize");
+  if (code_stride != cols) q.codes = q.codes.as_strided({rows, cols}, {code_stride, 1});
+  return q;
+}
+// whether t is a matrix whose rows lie apart by some distance, or one behind the other
+bool lies_in_rows(const at::Tensor& t) {
+  return t.is_contiguous() ||
+         (t.dim() == 2 && t.size(0) > 1 && (t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) >= t.size(1));
+}
+Quantized quantized(const at::Tensor& x, int type, bool sums) {
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  const int64_t cols = x.size(-1);
+  return quantized(x, type, rows, cols, x.is_contiguous() ? cols : x.stride(0), sums);
+}
+csw_fp8_matrix matrix_of(const at::Tensor& codes, const at::Tensor& scales, bool transposed) {
+  return {ptr(codes), ptr(scales), (size_t)codes.size(0), (size_t)codes.size(1), (size_t)padded(codes.size(1)), transposed};
+}
+at::Tensor product(const csw_fp8_matrix& a, const csw_fp8_matrix& b, const at::Tensor* bias, const at::Tensor& like,
+                   at::ScalarType kind, at::IntArrayRef sizes) {
+  const c10::cuda::CUDAGuard on(like.device());
+  at::Tensor dst = fresh(like, sizes, kind);
+  require_ok(csw_fp8_matmul(&a, &b, bias ? ptr(*bias) : nullptr, bias ? type_code(bias->scalar_type()) : 0, out(dst),
+                            type_code(kind), c10::cuda::getCurrentCUDAStream(like.device().index()).stream()),
+             "csw_fp8_matmul");
+  return dst;
+}
+
 // fp8_quantize(x, sums) -> (codes, scales), or with their columns' sums
 PyObject* fp8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -64,32 +118,12 @@ PyObject* fp8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
       value_error("x needs one axis at least");
       return nullptr;
     }
-    const int64_t cols = x->size(-1), rows = cols ? x->numel() / cols : x->dim() == 2 ? x->size(0) : 0;
-    int64_t stride = cols;
-    if (x->dim() == 2 && rows > 1 && (cols == 1 || x->stride(1) == 1) && x->stride(0) >= cols) stride = x->stride(0);
-    else if (!require_flat(*x, "x")) return nullptr;
-    size_t need;
-    if (!status_ok(csw_fp8_quantize_workspace(rows, cols, &need), "csw_fp8_quantize_workspace")) return nullptr;
-    const int64_t code_stride = padded(cols);
-    at::Tensor codes = fresh(*x, {rows, code_stride}, at::kFloat8_e4m3fn);
-    at::Tensor scales = fresh(*x, {blocks_of(rows), blocks_of(cols)}, at::kFloat8_e8m0fnu), sums, space;
-    void *to = out(codes), *powers = out(scales), *ws = nullptr;
-    float* totals = nullptr;
-    if (wanted) {
-      sums = fresh(*x, {cols}, at::kFloat);
-      totals = static_cast<float*>(out(sums));
-      if (need) {
-        space = fresh(*x, {(int64_t)need}, at::kByte);
-        ws = out(space);
-      }
-    }
-    const void* from = ptr(*x);
-    if (!launch(*x, "csw_fp8_quantize", [&](csw_stream_t s) {
-          return csw_fp8_quantize(from, type, rows, cols, stride, to, code_stride, powers, totals, ws, need, s);
-        }))
+    if (!lies_in_rows(*x)) {
+      value_error("%s must be contiguous", "x");
       return nullptr;
-    if (code_stride != cols) codes = codes.narrow(1, 0, cols);
-    return wanted ? tuple_of({codes, scales, sums}) : tuple_of({codes, scales});
+    }
+    const Quantized q = quantized(*x, type, wanted);
+    return wanted ? tuple_of({q.codes, q.scales, q.sums}) : tuple_of({q.codes, q.scales});
   });
 }
 
@@ -147,6 +181,118 @@ PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }))
       return nullptr;
     return THPVariable_Wrap(dst);
+  });
+}
+
+// The linear layer as a node of autograd's, without Python in its backward pass: a layer of a few hundred rows takes less time
+// than a function of Python's there.
+struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
+  using Context = torch::autograd::AutogradContext;
+  static at::Tensor forward(Context* ctx, const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
+    const Quantized held = quantized(x, type_code(x.scalar_type()), false);
+    const Quantized w = quantized(weight, type_code(weight.scalar_type()), false);
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = weight.size(0);
+    // what a gradient that is not asked for would need is not kept
+    const bool keep_x = weight.requires_grad(), keep_w = x.requires_grad();
+    ctx->save_for_backward({keep_x ? held.codes : at::Tensor(), keep_x ? held.scales : at::Tensor(),
+                            keep_w ? w.codes : at::Tensor(), keep_w ? w.scales : at::Tensor()});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
+                                                    bias ? (int64_t)bias->scalar_type() : -1};
+    return product(matrix_of(held.codes, held.scales, false), matrix_of(w.codes, w.scales, true), bias ? &*bias : nullptr, x,
+                   x.scalar_type(), sizes);
+  }
+  static torch::autograd::variable_list backward(Context* ctx, const torch::autograd::variable_list& grads) {
+    const bool again = at::GradMode::is_enabled();
+    torch::autograd::variable_list r(3);
+    if (!grads[0].defined()) return r;
+    {
+      at::NoGradGuard none;
+      const auto saved = ctx->get_saved_variables();
+      const auto shape = ctx->saved_data["shape"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+      const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = types[2] >= 0 && ctx->needs_input_grad(2);
+      const at::Tensor rows = grads[0].dim() == 2 ? grads[0] : grads[0].flatten(0, -2);
+      const at::Tensor dy = lies_in_rows(rows) ? rows : rows.contiguous();
+      const Quantized g = quantized(dy, type_code(dy.scalar_type()), want_b);
+      const csw_fp8_matrix along = matrix_of(g.codes, g.scales, false), across = matrix_of(g.codes, g.scales, true);
+      if (want_x)
+        r[0] = product(along, matrix_of(saved[2], saved[3], false), nullptr, dy, (at::ScalarType)types[0], shape);
+      if (want_w)
+        r[1] = product(across, matrix_of(saved[0], saved[1], false), nullptr, dy, (at::ScalarType)types[1],
+                       {dy.size(1), saved[0].size(1)});
+      if (want_b) r[2] = g.sums.to((at::ScalarType)types[2]);
+    }
+    if (again) {  // a gradient of these gradients is an error, where one is asked for
+      for (at::Tensor& t : r)
+        if (t.defined()) t.requires_grad_(true);
+      r = (*std::make_shared<torch::autograd::DelayedError>("fp8_linear is differentiable once", (int64_t)r.size()))(std::move(r));
+    }
+    return r;
+  }
+};
+
+bool layer_of(const at::Tensor* x, const at::Tensor* bias, int64_t in, int64_t outs, const at::Tensor& on) {
+  int type;
+  if (!require_values(*x, "x", &type) || !same_device(on, *x, "weight")) return false;
+  if (x->dim() < 2 || x->size(-1) != in)
+    return value_error("x needs two axes at least, and a weight of [out, in] for its last one");
+  if (!bias) return true;
+  if (!require_values(*bias, "bias", &type) || !same_device(*bias, *x, "bias")) return false;
+  return (bias->dim() == 1 && bias->numel() == outs) || value_error("%s must hold one value for each row of the weight", "bias");
+}
+at::Tensor in_rows(const at::Tensor& t) { return lies_in_rows(t) ? t : t.contiguous(); }
+
+// fp8_linear(x, weight, bias) -> y
+PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* bias;
+    int type;
+    if (!arg_count(n, 3)) return nullptr;
+    const at::Tensor* x = as_tensor(a[0], "x");
+    const at::Tensor* w = x ? as_tensor(a[1], "weight") : nullptr;
+    if (!w || !optional_tensor(a[2], "bias", &bias) || !require_values(*w, "weight", &type)) return nullptr;
+    if (w->dim() != 2) {
+      value_error("weight must be [out, in]");
+      return nullptr;
+    }
+    if (!layer_of(x, bias, w->size(1), w->size(0), *w)) return nullptr;
+    for (const at::Tensor* t : {x, w, bias})
+      if (t && !capture_allows(*t)) return nullptr;
+    at::Tensor y;
+    {
+      pybind11::gil_scoped_release free;
+      y = Fp8Linear::apply(in_rows(*x), in_rows(*w), bias ? std::optional<at::Tensor>(bias->contiguous()) : std::nullopt);
+    }
+    return THPVariable_Wrap(y);
+  });
+}
+
+// fp8_linear_held(x, codes, scales, bias) -> y
+PyObject* fp8_linear_held(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *codes, *bias;
+    csw_fp8_matrix m;
+    if (!arg_count(n, 4)) return nullptr;
+    const at::Tensor* x = as_tensor(a[0], "x");
+    if (!x || !optional_tensor(a[3], "bias", &bias) || !matrix_of(a[1], a[2], "weight", "scales", &codes, &m) ||
+        !layer_of(x, bias, codes->size(1), codes->size(0), *codes))
+      return nullptr;
+    if (at::GradMode::is_enabled() && (x->requires_grad() || (bias && bias->requires_grad()))) {
+      value_error("no gradient passes through a weight that was quantized before: call under torch.no_grad()");
+      return nullptr;
+    }
+    at::Tensor y;
+    {
+      pybind11::gil_scoped_release free;
+      const at::Tensor rows = in_rows(*x), b = bias ? bias->contiguous() : at::Tensor();
+      const Quantized q = quantized(rows, type_code(rows.scalar_type()), false);
+      std::vector<int64_t> sizes = x->sizes().vec();
+      sizes.back() = codes->size(0);
+      m.transposed = 1;
+      y = product(matrix_of(q.codes, q.scales, false), m, bias ? &b : nullptr, rows, rows.scalar_type(), sizes);
+    }
+    return THPVariable_Wrap(y);
   });
 }
 
@@ -470,6 +616,8 @@ PyMethodDef cswap_step_methods[] = {
     CSW_METHOD(fp8_quantize, "(x, sums) -> (codes, scales) or (codes, scales, sums)"),
     CSW_METHOD(fp8_dequantize, "(codes, scales, dtype) -> tensor"),
     CSW_METHOD(fp8_matmul, "(a, a_scales, b, b_scales, transpose_a, transpose_b, bias, dtype) -> tensor"),
+    CSW_METHOD(fp8_linear, "(x, weight, bias) -> tensor"),
+    CSW_METHOD(fp8_linear_held, "(x, codes, scales, bias) -> tensor"),
     CSW_METHOD(adamw_step, "(params, grads, exp_avgs, exp_avg_sqs, copies, step, lr, beta1, beta2, eps, weight_decay, norm, "
                            "max_norm) -> None"),
     CSW_METHOD(adamw8_step, "(params, grads, states, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed) "

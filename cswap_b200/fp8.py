@@ -19,8 +19,6 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.amp import custom_bwd, custom_fwd
-from torch.autograd.function import once_differentiable
 
 from . import codec
 
@@ -54,40 +52,6 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     return _ext().fp8_matmul(a, a_scales, b, b_scales, transpose_a, transpose_b, bias, dtype)
 
 
-class _Fp8Linear(torch.autograd.Function):
-    @staticmethod
-    @custom_fwd(device_type="cuda")
-    def forward(ctx, x, weight, bias):
-        ext = _ext()
-        held = ext.fp8_quantize(x, False)
-        w = ext.fp8_quantize(weight, False)
-        y = ext.fp8_matmul(*held, *w, False, True, bias, x.dtype)
-        # what a gradient that is not asked for would need is not kept
-        keep_x = held if weight.requires_grad else (None, None)
-        keep_w = w if x.requires_grad else (None, None)
-        ctx.save_for_backward(*keep_x, *keep_w)
-        ctx.shape, ctx.types = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
-
-    @staticmethod
-    @custom_bwd(device_type="cuda")
-    @once_differentiable
-    def backward(ctx, dy):
-        ext = _ext()
-        x, x_scales, w, w_scales = ctx.saved_tensors
-        want_x, want_w, want_b = ctx.needs_input_grad
-        kind, weight_kind, bias_kind = ctx.types
-        dx = dw = db = None
-        g = ext.fp8_quantize(_rows(dy.reshape(-1, dy.shape[-1])), want_b)
-        if want_x:
-            dx = ext.fp8_matmul(g[0], g[1], w, w_scales, False, False, None, kind).view(ctx.shape)
-        if want_w:
-            dw = ext.fp8_matmul(g[0], g[1], x, x_scales, True, False, None, weight_kind)
-        if want_b:
-            db = g[2].to(bias_kind)
-        return dx, dw, db
-
-
 def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Quantized], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x weight^T + bias in the type of x, every product on operands in 8 bits.
 
@@ -95,22 +59,6 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Quantized], bias: Op
     the weight's are for the input's gradient.  A weight that does not change may be given as fp8_quantize(weight), and takes no
     gradient then (nor do x and the bias)."""
     if isinstance(weight, torch.Tensor):
-        if x.dim() < 2 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-            raise ValueError("x needs two axes at least, and a weight of [out, in] for its last one")
-        _ext().check_capture(x, weight, bias)
-        return _Fp8Linear.apply(_rows(x), _rows(weight), bias)
+        return _ext().fp8_linear(x, weight, bias)
     codes, scales = weight
-    if x.dim() < 2 or codes.dim() != 2 or x.shape[-1] != codes.shape[1]:
-        raise ValueError("x needs two axes at least, and a weight of [out, in] for its last one")
-    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
-        raise ValueError("no gradient passes through a weight that was quantized before: call under torch.no_grad()")
-    ext = _ext()
-    y = ext.fp8_matmul(*ext.fp8_quantize(_rows(x), False), codes, scales, False, True, bias, x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], codes.shape[0])
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as the quantizer takes it: a matrix of rows at any distance, or contiguous."""
-    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
-        return t
-    return t.contiguous()
+    return _ext().fp8_linear_held(x, codes, scales, bias)

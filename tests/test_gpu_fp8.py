@@ -211,6 +211,14 @@ def test_codes_of_a_program_that_pads_its_rows_otherwise(cs):
 
 # ---- the layer -----------------------------------------------------------------------------------------------------
 
+def keeping(f):
+    """What f() returns, and the tensors that autograd keeps for it."""
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        y = f()
+    return y, kept
+
+
 @kinds
 @pytest.mark.parametrize("bias", [True, False])
 @pytest.mark.parametrize("shape,out", [((3, 33, 64), 40), ((300, 130), 257), ((1, 1000), 200)])
@@ -219,8 +227,8 @@ def test_linear_and_its_gradients(cs, kind, bias, shape, out):
     x, w = normal(*shape, seed=1, kind=kind).requires_grad_(True), normal(out, shape[-1], seed=2, kind=kind).requires_grad_(True)
     b = normal(out, seed=3, kind=kind).requires_grad_(True) if bias else None
     dy = normal(*shape[:-1], out, seed=4, kind=kind)
-    y = cs.fp8_linear(x, w, b)
-    kept = sum(t.numel() * t.element_size() for t in y.grad_fn.saved_tensors if t is not None)
+    y, kept = keeping(lambda: cs.fp8_linear(x, w, b))
+    kept = sum(t.numel() * t.element_size() for t in kept)
     blocks = lambda r, c: -(-r // 128) * -(-c // 128)
     rows, cols = x.numel() // shape[-1], shape[-1]
     assert kept == rows * cols + out * cols + blocks(rows, cols) + blocks(out, cols)
@@ -256,10 +264,26 @@ def test_linear_gradients_by_differences(cs):
 def test_linear_keeps_what_its_gradients_need(cs):
     x, w = normal(9, 64), normal(5, 64, seed=1)
     for gx, gw in ((True, False), (False, True)):
-        y = cs.fp8_linear(x.clone().requires_grad_(gx), w.clone().requires_grad_(gw))
-        kept = [t for t in y.grad_fn.saved_tensors if t is not None]
+        y, kept = keeping(lambda: cs.fp8_linear(x.clone().requires_grad_(gx), w.clone().requires_grad_(gw)))
         assert len(kept) == 2 and kept[0].numel() == (w.numel() if gx else x.numel())
     assert cs.fp8_linear(x, w).grad_fn is None
+
+
+def test_linear_is_differentiable_once(cs):
+    x, w = normal(9, 64).requires_grad_(True), normal(5, 64, seed=1).requires_grad_(True)
+    dx, = torch.autograd.grad(cs.fp8_linear(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dx.sum().backward()
+
+
+def test_linear_of_nothing(cs):
+    w, b = normal(5, 64, seed=1).requires_grad_(True), normal(5).requires_grad_(True)
+    x = torch.empty(2, 0, 64, device="cuda").requires_grad_(True)
+    y = cs.fp8_linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == (2, 0, 5) and dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
+    y = cs.fp8_linear(torch.empty(2, 3, 0, device="cuda"), torch.empty(5, 0, device="cuda"), b)
+    assert torch.equal(y, b.expand(2, 3, 5))
 
 
 def test_linear_of_a_weight_quantized_before(cs):
