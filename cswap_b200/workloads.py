@@ -8,7 +8,8 @@ by layer in Execution.pre/post exactly the way the reference's drivers do.
   layer-norm / activation wrapped, as CSWAP+/bert.cpp:370-801 does, with the
   dimensions left to the caller (the benchmark uses the BERT-base shape).  With
   `lean` its attention, feed-forward part and norms are the operators of ops.py,
-  which save little for backward in the first place.
+  which save little for backward in the first place, with `fp8` its linear
+  layers those of fp8.py.
 
 Inputs are synthetic (the datasets are not part of this repository) and
 weights are randomly initialised.
@@ -24,7 +25,8 @@ import torch.nn.functional as F
 
 from .codec import POLICY_KEEP, POLICY_RAW, POLICY_ZFP
 from .execution import Execution, LayerType
-from .ops import attention, gelu_linear, layer_norm
+from .fp8 import fp8_linear
+from .ops import attention, gelu, gelu_linear, layer_norm
 
 
 # ---------------------------------------------------------------------------
@@ -120,15 +122,15 @@ def vgg16_reference_policy(exe: Execution, compressed: int = POLICY_ZFP) -> None
 class BertEncoder(nn.Module):
     """`lean`: attention that keeps its output and one number a row besides its operands (in bfloat16, its probabilities
     without dropout, of which a warning tells where `dropout` is not 0), a feed-forward part that keeps its activation in 8
-    bits, norms that take the residual's sum with them.  The parameters are the same, so that a state of one kind loads
-    into the other."""
+    bits, norms that take the residual's sum with them.  `fp8`: the layers' products take operands in 8 bits, and keep them
+    as that; lean or not.  The parameters are the same, so that a state of one kind loads into the other."""
 
     def __init__(self, vocab: int = 30522, hidden: int = 768, layers: int = 12, heads: int = 12, ffn: int = 3072,
-                 max_seq: int = 512, dropout: float = 0.1, lean: bool = False):
+                 max_seq: int = 512, dropout: float = 0.1, lean: bool = False, fp8: bool = False):
         super().__init__()
         if lean and dropout > 0:
             warnings.warn("BertEncoder(lean=True) drops out activations alone: its attention has no dropout on probabilities")
-        self.lean = lean
+        self.lean, self.fp8 = lean, fp8
         self.hidden, self.heads, self.nlayers, self.p = hidden, heads, layers, dropout
         self.tok = nn.Embedding(vocab, hidden)
         self.pos = nn.Embedding(max_seq, hidden)
@@ -166,18 +168,23 @@ class BertEncoder(nn.Module):
         def norm(ln, a, b):  # under autocast a product's type is not that of the sum it goes into
             return layer_norm(a.to(b.dtype), ln.weight, ln.bias, ln.eps, residual=b)
 
+        def linear(m):
+            return (lambda t: fp8_linear(t, m.weight, m.bias)) if self.fp8 else m
+
         for l in range(self.nlayers):
-            q = step(self.q[l], x, LayerType.FC)
-            k = step(self.k[l], x, LayerType.FC)
-            v = step(self.v[l], x, LayerType.FC)
+            q = step(linear(self.q[l]), x, LayerType.FC)
+            k = step(linear(self.k[l]), x, LayerType.FC)
+            v = step(linear(self.v[l]), x, LayerType.FC)
             if self.lean:
                 ctx = step(lambda a, b, c: attention(heads(a), heads(b), heads(c)).transpose(1, 2).reshape(B, S, H)
                            .to(x.dtype), [q, k, v], LayerType.FC)
-                ao = step(self.o[l], ctx, LayerType.FC)
+                ao = step(linear(self.o[l]), ctx, LayerType.FC)
                 ao = step(lambda t: F.dropout(t, self.p, self.training), ao)
                 x = step(lambda a, b: norm(self.ln1[l], a, b), [ao, x], LayerType.BN)
-                h = step(self.f1[l], x, LayerType.FC)
-                h = step(lambda t: gelu_linear(t, self.f2[l].weight, self.f2[l].bias), h, LayerType.FC)
+                h = step(linear(self.f1[l]), x, LayerType.FC)
+                second = (lambda t: linear(self.f2[l])(gelu(t))) if self.fp8 else (
+                    lambda t: gelu_linear(t, self.f2[l].weight, self.f2[l].bias))
+                h = step(second, h, LayerType.FC)
                 h = step(lambda t: F.dropout(t, self.p, self.training), h)
                 x = step(lambda a, b: norm(self.ln2[l], a, b), [h, x], LayerType.BN)
                 continue
@@ -189,12 +196,12 @@ class BertEncoder(nn.Module):
             pr = step(lambda t: F.dropout(t, self.p, self.training), pr)
             ctx = step(lambda a, b: torch.matmul(a, b), [pr, vh], LayerType.FC)
             ctx = step(lambda t: t.transpose(1, 2).reshape(B, S, H), ctx)
-            ao = step(self.o[l], ctx, LayerType.FC)
+            ao = step(linear(self.o[l]), ctx, LayerType.FC)
             ao = step(lambda t: F.dropout(t, self.p, self.training), ao)
             x = step(lambda a, b: self.ln1[l](a + b), [ao, x], LayerType.BN)
-            h = step(self.f1[l], x, LayerType.FC)
+            h = step(linear(self.f1[l]), x, LayerType.FC)
             h = step(F.gelu, h)
-            h = step(self.f2[l], h, LayerType.FC)
+            h = step(linear(self.f2[l]), h, LayerType.FC)
             h = step(lambda t: F.dropout(t, self.p, self.training), h)
             x = step(lambda a, b: self.ln2[l](a + b), [h, x], LayerType.BN)
         cls = step(lambda t: t[:, 0], x, LayerType.ACT, True)
@@ -208,8 +215,9 @@ class BertEncoder(nn.Module):
 # measuring a swapped step
 # ---------------------------------------------------------------------------
 def timed_steps(model: nn.Module, exe: Execution, make_batch: Callable[[], Tuple[torch.Tensor, torch.Tensor]],
-                steps: int, warmup: int) -> dict:
-    """Run forward + backward `steps` times under `exe`'s policy.  Each step
+                steps: int, warmup: int, optimizer: Optional[torch.optim.Optimizer] = None) -> dict:
+    """Run forward + backward `steps` times under `exe`'s policy, and the step of an `optimizer` where one is given (the
+    one of optim.py holds its state in 8 bits, if asked to).  Each step
     takes its batch from pinned host memory (non-blocking copy) and reads the
     loss back, so the numbers include the step's host traffic."""
     times = []
@@ -231,6 +239,8 @@ def timed_steps(model: nn.Module, exe: Execution, make_batch: Callable[[], Tuple
             p.grad = None
         loss = model.forward_with(exe, x, y)
         loss.backward()
+        if optimizer is not None:
+            optimizer.step()
         loss_val = float(loss.detach())  # device -> host read of the step's result
         e1.record()
         torch.cuda.synchronize()
