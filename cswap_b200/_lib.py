@@ -184,6 +184,8 @@ SIGNATURES = {
     "csw_fp8_quantize": (_I, [_P, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _P, _SZ, _P]),
     "csw_fp8_dequantize": (_I, [_P, _SZ, _P, _SZ, _SZ, _P, _I, _P]),
     "csw_fp8_matmul": (_I, [_MX, _MX, _P, _I, _P, _I, _P]),
+    "csw_fp8_linear_workspace": (_I, [_SZ, _SZ, _SZ, C.POINTER(_SZ)]),
+    "csw_fp8_linear": (_I, [_P, _I, _SZ, _SZ, _MX, _P, _I, _P, _I, _P, _SZ, _P]),
     "csw_adamw_step": (_I, [_AT, _SZ, C.POINTER(AdamwOptions), _P]),
     "csw_adamw8_pack": (_I, [_AT, _SZ, _P]),
     "csw_adamw8_unpack": (_I, [_AT, _SZ, _P]),

@@ -321,6 +321,11 @@ struct Product {
   const void* bias;
   int type, bias_type;
   bool exchanged, packs;  // packs: rows of the result begin on 16 bytes
+  // the column operand as values that are yet to be quantized: p.n rows, x_cols of the reduction, x_stride apart
+  const void* x;
+  uint64_t x_stride;
+  uint32_t x_cols;
+  bool x_packs;  // four of them lie so that they are one load
   long long patience;
   bool idle;
   uint32_t* status;
@@ -425,14 +430,71 @@ __device__ __forceinline__ void write_scales(char* to, const uint32_t (&held)[OP
   __syncwarp();
 }
 
+// The warp that writes scales and the four that quantize meet once; nothing in front of it can fail.
+__device__ __forceinline__ void values_meet() { asm volatile("bar.sync 1, 160;" ::: "memory"); }
+
 // One warp copies tiles, one writes their scales, one issues the products, four take the sums out.  Where there are few
 // tiles, a cluster of `parts` CTAs shares one: each takes a part of the reduction, and the parts' sums, in shared memory, are
 // added in their order, each CTA a part of the columns.
-template <int BN>
+// A few rows of values (tokens, in generation) need not be quantized by a launch of their own: with X their type, the warps that
+// wait for the sums do it before, every CTA for its part of the reduction.  First the scales of all its blocks, then the codes,
+// a warp a block, into the stage that the other operand's tile is copied to.  (1 x 4096 x 4096: 7.2 us of product behind 4 of
+// quantizing, 8.4 together.)
+constexpr int kMostHeld = 512;  // blocks of a CTA's part of the reduction, with X
+template <class X>
+struct Block {  // four columns of each row
+  const Product& p;
+  uint32_t col;
+  __device__ Block(const Product& q, uint32_t block) : p(q), col(block * kBlock + threadIdx.x % 32 * 4) {}
+  __device__ __forceinline__ void load(uint32_t row, float (&f)[4]) const {
+    const X* from = static_cast<const X*>(p.x) + row * p.x_stride + col;
+    if (p.x_packs && col + 4 <= p.x_cols) {
+      load_pack(from, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = col + j < p.x_cols ? widen(from[j]) : 0.0f;
+    }
+  }
+  __device__ __forceinline__ int exponent() const {
+    uint32_t top = 0;
+#pragma unroll 4
+    for (uint32_t r = 0; r < p.n; ++r) {
+      float f[4];
+      load(r, f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t bits = __float_as_uint(f[j]) & 0x7fffffffu;
+        top = max(top, bits < 0x7f800000u ? bits : 0u);
+      }
+    }
+    return exponent_of(__reduce_max_sync(0xffffffffu, top));
+  }
+  // to a tile of rows of 128 bytes, swizzled as the tile copies leave them
+  __device__ __forceinline__ void write(char* tile, int e) const {
+    const float factor = power_of(-e);
+    const uint32_t lane = threadIdx.x % 32;
+#pragma unroll 4
+    for (uint32_t r = 0; r < p.n; ++r) {
+      float f[4];
+      load(r, f);
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float2 v = {isinf(f[j]) ? NAN : f[j] * factor, isinf(f[j + 1]) ? NAN : f[j + 1] * factor};
+        word |= (uint32_t)__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3) << 8 * j;
+      }
+      *reinterpret_cast<uint32_t*>(tile + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4) = word;
+    }
+  }
+};
+
+template <int BN, class X = void>
 __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_constant__ Product p) {
   using L = Plan<BN>;
+  constexpr bool kValues = !std::is_same<X, void>::value;
   extern __shared__ char shared[];
   __shared__ uint64_t bars[2 * kMostStages + 6];
+  __shared__ uint8_t held_scales[kValues ? kMostHeld : 1];
   __shared__ uint32_t tmem_at, flag;
   char* const ring = shared + (1024 - smem_at(shared) % 1024) % 1024;
   const uint32_t ring_at = smem_at(ring);
@@ -445,14 +507,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
   const uint32_t row = place.row * kBlock, col = place.col * BN;
   const uint32_t begin = (uint64_t)p.steps * part / p.parts, count = (uint32_t)((uint64_t)p.steps * (part + 1) / p.parts) - begin;
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < p.stages; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
+    for (uint32_t s = 0; s < p.stages; ++s) bar_init(full + 8 * s, kValues ? 2 : 1), bar_init(empty + 8 * s, 1);
     for (int b = 0; b < 2; ++b) bar_init(scaled + 8 * b, 1), bar_init(unscaled + 8 * b, 1);
     bar_init(done, 1);
     bar_init(received, 1);
     flag = 0;
     init_visible();
     prefetch_map(&p.r.map);
-    prefetch_map(&p.c.map);
+    if (!kValues) prefetch_map(&p.c.map);
   }
   // Every CTA's barriers are there.  From here to where tensor memory is freed no CTA waits for another one, which might wait
   // for that memory.
@@ -474,15 +536,16 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
         if (p.idle) return;
         const uint32_t bar = full + 8 * s, to = ring_at + s * stage;
         const int k = (int)(begin + i) * kBlock;
-        bar_expect_by(me, bar, stage);
+        bar_expect_by(me, bar, kValues ? kTileBytes : stage);
         copy_bytes_tile_by(me, to, &p.r.map, bar, p.r.across ? (int)row : k, p.r.across ? k : (int)row);
 #pragma unroll
-        for (int j = 0; j < L::kPanels; ++j)
+        for (int j = 0; j < L::kPanels && !kValues; ++j)
           copy_bytes_tile_by(me, to + (1 + j) * kTileBytes, &p.c.map, bar, p.c.across ? (int)col + j * kBlock : k,
                              p.c.across ? k : (int)col + j * kBlock);
       }
     }();
   } else if (warp == 2) {
+    if (kValues) values_meet();
     [&] {
       for (uint32_t i = 0, n = 0; i < count; i += kBatch, ++n) {
         const uint32_t mine = begin + i + lane % kBatch;  // a block's scales to a lane
@@ -491,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
         held[0] = is ? p.r.scales[(uint64_t)(row / kBlock) * p.r.scale_step + (uint64_t)mine * p.r.scale_k_step] : 0;
 #pragma unroll
         for (int j = 0; j < L::kPanels; ++j)
-          held[1 + j] = is && col + j * kBlock < p.n
+          held[1 + j] = kValues ? (is ? held_scales[mine - begin] : 0)
+                        : is && col + j * kBlock < p.n
                             ? p.c.scales[(uint64_t)(col / kBlock + j) * p.c.scale_step + (uint64_t)mine * p.c.scale_k_step]
                             : 0;
         if (n > 1) CSW_WAIT_WARP(unscaled + 8 * (n % 2), (n / 2 - 1) & 1);
@@ -531,7 +595,24 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
       }
     }();
   } else if (warp >= 4) {
+    if constexpr (kValues) {
+      for (uint32_t i = warp - 4; i < count; i += 4) {
+        const int e = Block<X>(p, begin + i).exponent();
+        if (lane == 0) held_scales[i] = (uint8_t)(e + 127);
+      }
+      values_meet();
+    }
     [&] {
+      if constexpr (kValues) {
+        for (uint32_t i = warp - 4; i < count; i += 4) {
+          const uint32_t round = i / p.stages, s = i - round * p.stages;
+          if (round) CSW_WAIT_WARP(empty + 8 * s, (round - 1) & 1);
+          Block<X>(p, begin + i).write(ring + s * stage + kTileBytes, (int)held_scales[i] - 127);
+          async_fence();
+          __syncwarp();
+          if (lane == 0) bar_arrive(full + 8 * s);
+        }
+      }
       if (count) CSW_WAIT_WARP(done, 0);
       fence_after();
       const uint32_t lanes = (uint32_t)(32 * (warp % 4)) << 16, line = 32 * (warp % 4) + lane;
@@ -865,11 +946,11 @@ Way way_for(const Product& p) {
   return best;
 }
 
-template <int BN>
+template <int BN, class X = void>
 cudaError_t product(Product& p, const Fp8Matrix& r, const Fp8Matrix& c, bool r_across, bool c_across, cudaStream_t stream) {
   using L = Plan<BN>;
-  if (p.steps && (!operand_of(&p.r, r, r_across, kBlock) || !operand_of(&p.c, c, c_across, std::min(BN, kBlock))))
-    return cudaErrorInvalidValue;
+  if (p.steps && !operand_of(&p.r, r, r_across, kBlock)) return cudaErrorInvalidValue;
+  if (p.steps && !p.x && !operand_of(&p.c, c, c_across, std::min(BN, kBlock))) return cudaErrorInvalidValue;
   p.col_tiles = (p.n + BN - 1) / BN;
   const uint32_t ctas = p.row_tiles * p.col_tiles * p.parts;
   const bool alone = BN > kBlock || p.parts > 1 || ctas <= (uint32_t)sm_count();
@@ -877,9 +958,9 @@ cudaError_t product(Product& p, const Fp8Matrix& r, const Fp8Matrix& c, bool r_a
   const size_t shared = L::shared(c_across, p.parts > 1, p.stages);
   // the most of any call, so that calls at the same time need not agree
   if (const cudaError_t e = taken(
-          cudaFuncSetAttribute(fp8_product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024)))
+          cudaFuncSetAttribute(fp8_product_kernel<BN, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024)))
     return e;
-  return pdl_launch_clusters(fp8_product_kernel<BN>, ctas, p.parts, kThreads, shared, stream, p);
+  return pdl_launch_clusters(fp8_product_kernel<BN, X>, ctas, p.parts, kThreads, shared, stream, p);
 }
 
 template <class T>
@@ -937,24 +1018,33 @@ cudaError_t fp8_dequantize_launch(const void* codes, uint64_t code_stride, const
   return e;
 }
 
+namespace {
+// what a product of m x k and k x n needs besides its operands
+cudaError_t begin_product(Product* p, uint64_t m, uint64_t n, uint64_t k, const void* bias, int bias_type, void* out, int type) {
+  if (const cudaError_t e = bind_context()) return e;
+  *p = Product{};
+  if (const cudaError_t e = status_word(&p->status)) return e;
+  const long long limit = wait_limit();
+  p->patience = limit < 0 ? -limit : limit, p->idle = limit < 0;
+  p->out = out, p->bias = bias, p->type = type, p->bias_type = bias_type;
+  p->steps = (uint32_t)fp8_blocks(k);
+  p->exchanged = m <= 64 && n > m;
+  p->packs = n * (type == 0 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  p->m = (uint32_t)(p->exchanged ? n : m), p->n = (uint32_t)(p->exchanged ? m : n);
+  p->row_tiles = (uint32_t)fp8_blocks(p->m);
+  return cudaSuccess;
+}
+}  // namespace
+
 cudaError_t fp8_matmul_launch(const Fp8Matrix& a, const Fp8Matrix& b, const void* bias, int bias_type, void* out, int type,
                               cudaStream_t stream) {
   const uint64_t m = a.transposed ? a.cols : a.rows, k = a.transposed ? a.rows : a.cols;
   const uint64_t n = b.transposed ? b.rows : b.cols;
   if (m == 0 || n == 0) return cudaSuccess;
-  if (const cudaError_t e = bind_context()) return e;
-  Product p{};
-  if (const cudaError_t e = status_word(&p.status)) return e;
-  const long long limit = wait_limit();
-  p.patience = limit < 0 ? -limit : limit, p.idle = limit < 0;
-  p.out = out, p.bias = bias, p.type = type, p.bias_type = bias_type;
-  p.steps = (uint32_t)fp8_blocks(k);
-  p.exchanged = m <= 64 && n > m;
-  p.packs = n * (type == 0 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  Product p;
+  if (const cudaError_t e = begin_product(&p, m, n, k, bias, bias_type, out, type)) return e;
   const Fp8Matrix &r = p.exchanged ? b : a, &c = p.exchanged ? a : b;
   const bool r_across = p.exchanged ? !b.transposed : a.transposed, c_across = p.exchanged ? a.transposed : !b.transposed;
-  p.m = (uint32_t)(p.exchanged ? n : m), p.n = (uint32_t)(p.exchanged ? m : n);
-  p.row_tiles = (uint32_t)fp8_blocks(p.m);
   const Way way = way_for(p);
   p.parts = way.parts;
   switch (way.columns) {
@@ -965,6 +1055,31 @@ cudaError_t fp8_matmul_launch(const Fp8Matrix& a, const Fp8Matrix& b, const void
   }
   cudaError_t e = cudaErrorInvalidValue;
   with_type(type, [&](auto v) { e = pair_product<decltype(v)>(p, r, c, r_across, c_across, stream); });
+  return e;
+}
+
+bool fp8_linear_at_once(uint64_t rows, uint64_t cols, uint64_t outs) {
+  return rows <= 32 && outs > rows && fp8_blocks(cols) <= kMostHeld;
+}
+
+cudaError_t fp8_linear_launch(const Fp8Quantize& x, const Fp8Matrix& weight, const void* bias, int bias_type, void* out,
+                              int type, cudaStream_t stream) {
+  if (x.rows == 0 || weight.rows == 0) return cudaSuccess;
+  if (!fp8_linear_at_once(x.rows, x.cols, weight.rows)) {
+    const cudaError_t e = fp8_quantize_launch(x, stream);
+    const Fp8Matrix held{x.codes, x.scales, x.rows, x.cols, x.code_stride, false};
+    return e != cudaSuccess ? e : fp8_matmul_launch(held, weight, bias, bias_type, out, type, stream);
+  }
+  Product p;
+  if (const cudaError_t e = begin_product(&p, x.rows, weight.rows, x.cols, bias, bias_type, out, type)) return e;
+  p.parts = way_for(p).parts;
+  p.x = x.x, p.x_stride = x.stride, p.x_cols = (uint32_t)x.cols;
+  cudaError_t e = cudaErrorInvalidValue;
+  with_type(x.type, [&](auto v) {
+    using X = decltype(v);
+    p.x_packs = reinterpret_cast<uintptr_t>(x.x) % (4 * sizeof(X)) == 0 && x.stride % 4 == 0;
+    e = product<32, X>(p, weight, Fp8Matrix{}, false, false, stream);
+  });
   return e;
 }
 

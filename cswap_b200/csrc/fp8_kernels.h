@@ -35,4 +35,10 @@ struct Fp8Matrix {
 cudaError_t fp8_matmul_launch(const Fp8Matrix& a, const Fp8Matrix& b, const void* bias, int bias_type, void* out, int type,
                               cudaStream_t stream);
 
+// Whether x weight^T is one launch, which quantizes x itself: x.codes and x.scales are then not used.
+bool fp8_linear_at_once(uint64_t rows, uint64_t cols, uint64_t outs);
+// out = x weight^T + bias; weight is taken transposed
+cudaError_t fp8_linear_launch(const Fp8Quantize& x, const Fp8Matrix& weight, const void* bias, int bias_type, void* out,
+                              int type, cudaStream_t stream);
+
 }  // namespace csw

@@ -273,6 +273,38 @@ csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, cons
   return done(fp8_matmul_launch(of(*a), of(*b), d_bias, bias_type, d_out, type, stream));
 }
 
+csw_status csw_fp8_linear_workspace(size_t rows, size_t cols, size_t outs, size_t* bytes) {
+  if (!bytes || rows > kMostRows || cols > kMostRows || outs > kMostRows) return CSW_ERR_ARG;
+  if (rows && (cols + 15 > kMostValues / rows || fp8_blocks(rows) > kMostRows / (fp8_blocks(cols) + 1))) return CSW_ERR_ARG;
+  *bytes = rows == 0 || fp8_linear_at_once(rows, cols, outs) ? 0 : (cols + 15) / 16 * 16 * rows + fp8_blocks(rows) * fp8_blocks(cols);
+  return CSW_OK;
+}
+
+csw_status csw_fp8_linear(const void* d_x, int type, size_t rows, size_t x_stride, const csw_fp8_matrix* weight,
+                          const void* d_bias, int bias_type, void* d_out, int out_type, void* d_workspace,
+                          size_t workspace_bytes, csw_stream_t stream) {
+  if (!weight || !known_type(type) || !known_type(out_type) || weight->transposed) return CSW_ERR_ARG;
+  const size_t outs = weight->rows, cols = weight->cols;
+  size_t need;
+  if (!matrix(weight->codes, weight->scales, outs, cols, weight->code_stride) ||
+      csw_fp8_linear_workspace(rows, cols, outs, &need) != CSW_OK)
+    return CSW_ERR_ARG;
+  if (rows == 0 || outs == 0) return CSW_OK;
+  constexpr size_t kMost = kMostRows - 128;
+  if (rows > kMost || outs > kMost || fp8_blocks(rows) > kMostRows / 32 / ((outs + 31) / 32)) return CSW_ERR_ARG;
+  if (cols && (!good(d_x, type) || x_stride < cols || x_stride > kMostValues / rows)) return CSW_ERR_ARG;
+  if (!good(d_out, out_type) || (d_bias && (!known_type(bias_type) || !good(d_bias, bias_type)))) return CSW_ERR_ARG;
+  if (need && (!d_workspace || !aligned(d_workspace, 16))) return CSW_ERR_ARG;
+  if (workspace_bytes < need) return CSW_ERR_SIZE;
+  const csw_status st = before_waits();
+  if (st != CSW_OK) return st;
+  const size_t stride = (cols + 15) / 16 * 16;
+  return done(fp8_linear_launch({d_x, type, rows, cols, x_stride, d_workspace, stride,
+                                 static_cast<uint8_t*>(d_workspace) + stride * rows, nullptr, nullptr},
+                                {weight->codes, static_cast<const uint8_t*>(weight->scales), outs, cols, weight->code_stride, true},
+                                d_bias, bias_type, d_out, out_type, stream));
+}
+
 csw_status csw_adamw_step(const csw_adamw_tensor* tensors, size_t count, const csw_adamw_options* options,
                           csw_stream_t stream) {
   if (!options || (options->bits != 8 && options->bits != 32) || !gradients(tensors, count)) return CSW_ERR_ARG;

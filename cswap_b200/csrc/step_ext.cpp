@@ -286,11 +286,20 @@ PyObject* fp8_linear_held(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
       pybind11::gil_scoped_release free;
       const at::Tensor rows = in_rows(*x), b = bias ? bias->contiguous() : at::Tensor();
-      const Quantized q = quantized(rows, type_code(rows.scalar_type()), false);
+      const c10::cuda::CUDAGuard on(rows.device());
       std::vector<int64_t> sizes = x->sizes().vec();
       sizes.back() = codes->size(0);
-      m.transposed = 1;
-      y = product(matrix_of(q.codes, q.scales, false), m, bias ? &b : nullptr, rows, rows.scalar_type(), sizes);
+      int64_t count = 1;
+      for (size_t i = 0; i + 1 < sizes.size(); ++i) count *= sizes[i];
+      size_t need;
+      require_ok(csw_fp8_linear_workspace(count, m.cols, m.rows, &need), "csw_fp8_linear_workspace");
+      at::Tensor space = need ? fresh(rows, {(int64_t)need}, at::kByte) : at::Tensor();
+      y = fresh(rows, sizes, rows.scalar_type());
+      const int type = type_code(rows.scalar_type());
+      require_ok(csw_fp8_linear(ptr(rows), type, count, rows.is_contiguous() ? m.cols : rows.stride(0), &m,
+                                bias ? ptr(b) : nullptr, bias ? type_code(b.scalar_type()) : 0, out(y), type,
+                                need ? out(space) : nullptr, need, c10::cuda::getCurrentCUDAStream(rows.device().index()).stream()),
+                 "csw_fp8_linear");
     }
     return THPVariable_Wrap(y);
   });

@@ -455,6 +455,14 @@ typedef struct {
 csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, const void* d_bias, int bias_type, void* d_out,
                           int type, csw_stream_t stream);
 
+/* out = x weight^T + bias for rows of values, x_stride apart, and a weight held as codes (outs x cols, transposed 0): what
+ * csw_fp8_quantize of x and csw_fp8_matmul give, bit by bit, and for up to 32 rows in one launch.  The workspace
+ * (csw_fp8_linear_workspace bytes) is 16-byte aligned. */
+csw_status csw_fp8_linear_workspace(size_t rows, size_t cols, size_t outs, size_t* bytes);
+csw_status csw_fp8_linear(const void* d_x, int type, size_t rows, size_t x_stride, const csw_fp8_matrix* weight,
+                          const void* d_bias, int bias_type, void* d_out, int out_type, void* d_workspace,
+                          size_t workspace_bytes, csw_stream_t stream);
+
 /* ---- 9. the optimizer's step over many tensors ------------------------------- */
 /* A parameter with its gradient and state, each numel values in the same order in memory, each of its own type where there is
  * one.  copy may be NULL, else it receives the new parameter in its type.  State in 32 bits: exp_avg (m) and exp_avg_sq (v)

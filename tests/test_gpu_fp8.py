@@ -296,6 +296,27 @@ def test_linear_of_a_weight_quantized_before(cs):
         cs.fp8_linear(normal(2, 136).requires_grad_(True), q)
 
 
+@kinds
+@pytest.mark.parametrize("rows,cols,out", [(1, 4096, 4096), (1, 1, 2), (2, 127, 300), (7, 515, 1030), (32, 2000, 640), (33, 300, 520),
+                                           (5, 9000, 130), (31, 640, 31), (3, 70000, 40), (1, 0, 5)])
+def test_linear_of_a_few_rows(cs, kind, rows, cols, out):
+    """What quantizing and the product give one after the other, bit by bit, also where one launch does both; rows that lie
+    apart, and off their alignment."""
+    w = cs.fp8_quantize(normal(out, cols, seed=1, kind=kind))
+    whole = (normal(rows, cols + 9, seed=2) * torch.exp(2 * normal(cols + 9, seed=3))).to(kind)
+    for x in (whole[:, :cols].contiguous(), whole[:, :cols], whole[:, 3:cols + 3]):
+        for bias in (None, normal(out, seed=4, kind=kind)):
+            want = cs.fp8_matmul(*cs.fp8_quantize(x.contiguous()), *w, transpose_b=True, bias=bias, dtype=kind)
+            assert R.bits_equal(cs.fp8_linear(x, w, bias), want)
+
+
+def test_linear_of_a_few_rows_that_hold_no_numbers(cs):
+    x, w = normal(4, 300, seed=1), cs.fp8_quantize(normal(200, 300, seed=2))
+    x[1, 200], x[2, 5], x[3, :] = math.nan, -math.inf, 0.0
+    y = cs.fp8_linear(x, w)
+    assert torch.isfinite(y[0]).all() and torch.isnan(y[1]).all() and torch.isnan(y[2]).all() and (y[3] == 0).all()
+
+
 def test_linear_under_autocast_and_of_a_transposed_input(cs):
     x, w = normal(24, 10, seed=1).requires_grad_(True), normal(6, 24, seed=2).requires_grad_(True)
     y = cs.fp8_linear(x.t(), w)

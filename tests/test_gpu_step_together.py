@@ -119,7 +119,7 @@ def test_a_training_step_with_the_optimizer(cs):
     out = timed_steps(model, exe, batch, steps=3, warmup=1, optimizer=opt)
     assert math.isfinite(out["loss"])
     for old, (name, p) in zip(before, model.named_parameters()):
-        moved = float((p - old).abs().max())
+        moved = float((p.detach() - old).abs().max())
         assert moved <= 4 * 2.2e-3 and (moved > 0 or p.grad is None or not p.grad.any()), name
 
 
@@ -251,6 +251,17 @@ def test_results_are_nan_and_the_status_is_told_once(cs, limit, kind, m, n, k):
     limit(LIMIT)
     assert torch.equal(product(), want)
     cs.device_status()
+
+
+def test_a_layer_of_a_few_rows_is_nan_too(cs, limit):
+    x, w = normal(3, 2000), cs.fp8_quantize(normal(600, 2000, seed=1))
+    want = cs.fp8_linear(x, w)
+    limit(SHORT)
+    assert torch.isnan(cs.fp8_linear(x, w)).all()
+    limit(LIMIT)
+    with raises(cs):
+        cs.fp8_linear(x, w)
+    assert torch.equal(cs.fp8_linear(x, w), want)
 
 
 def test_the_next_call_raises(cs, limit):

@@ -78,6 +78,26 @@ def test_matmul_arguments(L, mem):
     assert matmul(a=empty, out=None) == 0
 
 
+def test_linear_arguments(L, mem):
+    from cswap_b200._lib import Fp8Matrix
+    x, p, s, out, ws = (mem + 8192 * i for i in range(5))
+
+    def linear(x=x, t=F32, rows=40, stride=6, w=Fp8Matrix(p, s, 9, 6, 16, 0), bias=None, bt=F32, out=out, ot=BF16, ws=ws, size=4096):
+        return L.csw_fp8_linear(x, t, rows, stride, C.byref(w) if w is not None else None, bias, bt, out, ot, ws, size, None)
+
+    for bad in (dict(x=None), dict(x=x + 2), dict(t=3), dict(stride=5), dict(w=None), dict(w=Fp8Matrix(p, s, 9, 6, 16, 1)),
+                dict(w=Fp8Matrix(p + 4, s, 9, 6, 16, 0)), dict(w=Fp8Matrix(p, None, 9, 6, 16, 0)), dict(w=Fp8Matrix(p, s, 9, 6, 8, 0)),
+                dict(bias=p + 2), dict(bias=p, bt=4), dict(out=None), dict(out=out + 1), dict(ot=9), dict(ws=None), dict(ws=ws + 8),
+                dict(rows=1 << 31), dict(rows=(1 << 31) - 8), dict(stride=1 << 42)):
+        assert linear(**bad) == ARG, bad
+    assert linear(size=40 * 16) == SIZE and linear(rows=0, x=None, out=None, ws=None, size=0) == 0
+    b = C.c_size_t()
+    for rows, cols, outs, need in ((40, 6, 9, 40 * 16 + 1), (32, 6, 33, 0), (1, 4096, 4096, 0), (32, 6, 32, 513), (0, 6, 9, 0),
+                                   (1, 65537, 9, 65552 + 513), (300, 130, 5, 300 * 144 + 6)):
+        assert L.csw_fp8_linear_workspace(rows, cols, outs, C.byref(b)) == 0 and b.value == need
+    assert L.csw_fp8_linear_workspace(1, 1, 1, None) == ARG and L.csw_fp8_linear_workspace(1 << 31, 1, 1, C.byref(b)) == ARG
+
+
 def test_step_arguments(L, mem):
     from cswap_b200._lib import AdamwOptions, AdamwTensor
     at = [mem + 4096 * i for i in range(8)]
