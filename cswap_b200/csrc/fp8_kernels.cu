@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_dequantize_kernel(const 
   const uint32_t blocks = (uint32_t)((cols + kBlock - 1) / kBlock);
   const uint64_t row = blockIdx.x / blocks * (uint64_t)kBlock + threadIdx.x / 16;
   const uint64_t col = blockIdx.x % blocks * (uint64_t)kBlock + threadIdx.x % 16 * 4;
-  const float scale = power_of((int)scales[blockIdx.x] - 127);
+  const uint32_t byte = scales[blockIdx.x];  // 0 and 255 are no quantizer's, but a format's: 2^-127 and NaN
+  const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
   const uint8_t* from = codes + row * code_stride + col;
   uint32_t word[kRowsEach][2];
 #pragma unroll

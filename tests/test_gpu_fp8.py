@@ -77,6 +77,16 @@ def test_quantize_awkward_blocks(cs, kind):
         assert R.bits_equal(torch.nan_to_num(back, nan=-1.0), torch.nan_to_num(held.to(to), nan=-1.0))
 
 
+def test_every_code_and_scale(cs):
+    """All 256 codes under all 256 scales, as torch converts both types."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(2, 128).repeat(128 * 128, 1)[:128 * 256].contiguous()
+    scales = torch.arange(256, dtype=torch.uint8, device="cuda").view(256, 1)
+    c, s = codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu)
+    got = cs.fp8_dequantize(c, s)
+    want = (c.double() * s.double().repeat_interleave(128, 0)).float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
 @kinds
 def test_quantize_of_rows_apart_and_off_their_alignment(cs, kind):
     whole = normal(140, 300, seed=2, kind=kind)

@@ -303,6 +303,36 @@ def test_clipping(cs, bits):
             R.close(ps[i], want, R.param_bound(want, move, torch.from_numpy(olds[i]).double(), 1e-3, torch.float32))
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 2.0 ** -40, 1e-12, 1.0])
+def test_epsilons(cs, eps):
+    """Down to nothing, with averages of squares among float32's smallest numbers: the root of one is taken exactly there, and from
+    2^-40 on what lies below 2^-126 moves the sum by less than 2^-23 of it."""
+    g = torch.cat([normal(500, seed=1), normal(500, seed=2) * 1e-15, normal(500, seed=3) * 1e-19, normal(500, seed=4) * 1e15])
+    p, m, v = torch.zeros_like(g), torch.zeros_like(g), torch.zeros_like(g)
+    cs.adamw_step([p], [g], [m], [v], 1, eps=eps)
+    plain = R.Adamw(1, eps=eps)
+    zero = np.zeros(2000, np.float32)
+    a, b = plain.averages(npy(g), zero, zero)
+    assert np.array_equal(npy(m), a) and np.array_equal(npy(v), b)
+    want, move = (torch.from_numpy(x) for x in plain.param(zero, a, b))
+    R.close(p, want, R.param_bound(want, move, torch.zeros(2000).double(), 1e-3, torch.float32) + move.abs() * 2.0 ** -23)
+
+
+def test_large_and_small_gradients_in_8_bits(cs):
+    """Averages that are scaled in two steps, among others: 2^-110 to 2^60."""
+    for power in (-55, -40, -20, 10, 16, 30, 60):
+        p, g = normal(1000, seed=1), normal(1000, seed=2) * 2.0 ** power
+        state, zero = cs.adamw8_state(p), np.zeros(1000, np.float32)
+        plain, m, v = R.Adamw(1), zero, zero
+        for t in (1, 2):
+            plain.step = t
+            cs.adamw8_step([p], [g], [state], t, seed=9)
+            m, v = plain.averages(npy(g), m, v)
+            check_state(state, m, v, [b.astype(np.int64) * 16 + 8 for b in R.random_bits(9, t, 0, 1000)])
+            codes = [c.cpu().numpy() for c in state]
+            m, v = R.decode(codes[0], codes[2], 4), R.decode(codes[1], codes[3], 5)
+
+
 def test_clipping_by_a_norm_that_is_no_number(cs):
     p, g = normal(10), normal(10, seed=1)
     m, v = torch.zeros_like(p), torch.zeros_like(p)
