@@ -655,21 +655,22 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
   float* sums = reinterpret_cast<float*>(ring);
   if (*reinterpret_cast<volatile uint32_t*>(&flag)) spoil(sums, lines * pitch);
   const uint32_t rows = lines / p.parts;  // of the result, that this CTA writes
+  const uint32_t first_row = p.exchanged ? col : row, all_rows = p.exchanged ? p.n : p.m;
+  const uint32_t to_row = first_row + part * rows, to_col = p.exchanged ? row : col;
   if (p.parts > 1) {
     float* const from = reinterpret_cast<float*>(ring + scales_from + 2 * L::kBatchBytes);
     const uint32_t bytes = rows * pitch * 4;
     async_fence();
     __syncthreads();
-    if (threadIdx.x == 0) {
-      bar_expect(received, bytes * p.parts);
-      for (uint32_t q = 0; q < p.parts; ++q)
+    if (threadIdx.x == 0) {  // to those whose rows the result has
+      if (to_row < all_rows) bar_expect(received, bytes * p.parts);
+      for (uint32_t q = 0; q < p.parts && first_row + q * rows < all_rows; ++q)
         send_bytes(peer_at(smem_at(from) + part * bytes, q), ring_at + q * bytes, bytes, peer_at(received, q));
     }
-    if (!__syncthreads_and(bar_wait_cluster(received, 0, p.patience))) spoil(from, lines * pitch);
+    if (to_row < all_rows && !__syncthreads_and(bar_wait_cluster(received, 0, p.patience))) spoil(from, lines * pitch);
     sums = from;
   }
   const Sums s{sums, p.parts, rows, pitch, p.exchanged ? (uint32_t)kBlock : (uint32_t)BN};
-  const uint32_t to_row = (p.exchanged ? col : row) + part * rows, to_col = p.exchanged ? row : col;
   if (p.type == 0) emit_rows<float>(p, s, to_row, to_col);
   else if (p.type == 1) emit_rows<__half>(p, s, to_row, to_col);
   else emit_rows<__nv_bfloat16>(p, s, to_row, to_col);

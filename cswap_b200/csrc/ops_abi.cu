@@ -87,7 +87,8 @@ bool adamw_state(const csw_adamw_tensor& t, int bits) {
 csw_status adamw8_convert(const csw_adamw_tensor* t, size_t count, bool pack, csw_stream_t stream) {
   if (!adamw_list(t, count)) return CSW_ERR_ARG;
   for (size_t i = 0; i < count; ++i)
-    if (t[i].numel && (!adamw_state(t[i], 8) || !good(t[i].param, CSW_TYPE_F32) || !good(t[i].copy, CSW_TYPE_F32)))
+    if (t[i].numel && (!adamw_state(t[i], 8) || t[i].param_type != CSW_TYPE_F32 || t[i].copy_type != CSW_TYPE_F32 ||
+                       !good(t[i].param, CSW_TYPE_F32) || !good(t[i].copy, CSW_TYPE_F32)))
       return CSW_ERR_ARG;
   return done(adamw8_convert_launch(t, count, pack, stream));
 }

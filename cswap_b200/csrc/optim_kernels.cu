@@ -55,7 +55,10 @@ struct Entry {
   uint8_t *m_scale, *v_scale;
   uint64_t numel;
   uint8_t param_type, grad_type, copy_type;  // CSW_TYPE_*
-  bool packs;                                // all of the tensors lie so that four values are one load
+  // Whether four values are one load in all of the tensors, a piece beginning `shift` values before the first: tensors that lie
+  // one behind the other in flat buffers have none of them on a boundary, but all the same way off it.
+  bool packs;
+  uint8_t shift;
 };
 template <int N>
 struct Table {
@@ -111,48 +114,48 @@ __device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t piece) {
   return lo;
 }
 
-// Eight values of a thread, from index i and i + kNext on.  WHOLE: all of a tensor that lies in packs; else those below n, and
-// zeros for the others.
+// Eight values of a thread, from index i and i + kNext on.  WHOLE: all of a tensor that lies in packs; else those from 0 up to
+// n, and zeros for the others.
 template <class T, bool WHOLE>
-__device__ __forceinline__ void load_of(const void* from, uint64_t i, uint64_t n, bool packs, float (&f)[8]) {
+__device__ __forceinline__ void load_of(const void* from, int64_t i, int64_t n, bool packs, float (&f)[8]) {
   const T* p = static_cast<const T*>(from) + i;
 #pragma unroll
   for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (WHOLE || (packs && i + 4 <= n)) {
+    if (WHOLE || (packs && i >= 0 && i + 4 <= n)) {
       load_pack(p, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (i + j < n) v[j] = widen(p[j]);
+        if (i + j >= 0 && i + j < n) v[j] = widen(p[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[4 * q + j] = v[j];
   }
 }
 template <class T, bool WHOLE>
-__device__ __forceinline__ void store_of(void* to, uint64_t i, uint64_t n, bool packs, const float (&f)[8]) {
+__device__ __forceinline__ void store_of(void* to, int64_t i, int64_t n, bool packs, const float (&f)[8]) {
   T* p = static_cast<T*>(to) + i;
 #pragma unroll
   for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
     const float v[4] = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
-    if (WHOLE || (packs && i + 4 <= n)) {
+    if (WHOLE || (packs && i >= 0 && i + 4 <= n)) {
       store_pack(p, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (i + j < n) p[j] = narrow<T>(v[j]);
+        if (i + j >= 0 && i + j < n) p[j] = narrow<T>(v[j]);
     }
   }
 }
 template <bool WHOLE>
-__device__ __forceinline__ void load_any(const void* from, int type, uint64_t i, uint64_t n, bool packs, float (&f)[8]) {
+__device__ __forceinline__ void load_any(const void* from, int type, int64_t i, int64_t n, bool packs, float (&f)[8]) {
   if (type == CSW_TYPE_F32) load_of<float, WHOLE>(from, i, n, packs, f);
   else if (type == CSW_TYPE_F16) load_of<__half, WHOLE>(from, i, n, packs, f);
   else load_of<__nv_bfloat16, WHOLE>(from, i, n, packs, f);
 }
 template <bool WHOLE>
-__device__ __forceinline__ void store_any(void* to, int type, uint64_t i, uint64_t n, bool packs, const float (&f)[8]) {
+__device__ __forceinline__ void store_any(void* to, int type, int64_t i, int64_t n, bool packs, const float (&f)[8]) {
   if (type == CSW_TYPE_F32) store_of<float, WHOLE>(to, i, n, packs, f);
   else if (type == CSW_TYPE_F16) store_of<__half, WHOLE>(to, i, n, packs, f);
   else store_of<__nv_bfloat16, WHOLE>(to, i, n, packs, f);
@@ -160,7 +163,7 @@ __device__ __forceinline__ void store_any(void* to, int type, uint64_t i, uint64
 
 // ---- 8-bit codes ------------------------------------------------------------------------------------------------------
 template <bool WHOLE>
-__device__ __forceinline__ uint2 load_codes(const void* from, uint64_t i, uint64_t n, bool packs) {
+__device__ __forceinline__ uint2 load_codes(const void* from, int64_t i, int64_t n, bool packs) {
   const uint8_t* p = static_cast<const uint8_t*>(from) + i;
   uint32_t w[2] = {0, 0};
 #pragma unroll
@@ -176,7 +179,7 @@ __device__ __forceinline__ uint2 load_codes(const void* from, uint64_t i, uint64
   return make_uint2(w[0], w[1]);
 }
 template <bool WHOLE>
-__device__ __forceinline__ void store_codes(void* to, uint64_t i, uint64_t n, bool packs, uint2 codes) {
+__device__ __forceinline__ void store_codes(void* to, int64_t i, int64_t n, bool packs, uint2 codes) {
   uint8_t* p = static_cast<uint8_t*>(to) + i;
 #pragma unroll
   for (int q = 0; q < 2; ++q, p += kNext, i += kNext) {
@@ -232,10 +235,10 @@ __device__ __forceinline__ void values_of(uint2 codes, uint32_t scale, float (&f
 }
 // The largest magnitude of a group's 16 threads, as bits; a NaN's are above all others.
 __device__ __forceinline__ uint32_t top_of(const float (&f)[8]) {
-  float top = fabsf(f[0]);
+  float top = f[0];
 #pragma unroll
-  for (int j = 1; j < 8; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[j])));
-  uint32_t bits = __float_as_uint(top);
+  for (int j = 1; j < 8; ++j) asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(top) : "f"(f[j]));
+  uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
 #pragma unroll
   for (int d = 1; d < 16; d *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
   return bits;
@@ -294,8 +297,8 @@ __device__ __forceinline__ void over_pieces(const Table<N>& table, uint32_t run,
   for (; piece < end; ++piece) {
     while (piece >= table.first[at + 1]) ++at;
     const Entry& t = table.tensor[at];
-    const uint64_t begin = (uint64_t)(piece - table.first[at]) * kPiece, i = begin + first_value();
-    if (t.packs && begin + kPiece <= t.numel) f(t, at, i, std::true_type());
+    const int64_t begin = (int64_t)(piece - table.first[at]) * kPiece - t.shift, i = begin + first_value();
+    if (t.packs && begin >= 0 && begin + (int64_t)kPiece <= (int64_t)t.numel) f(t, at, i, std::true_type());
     else f(t, at, i, std::false_type());
   }
 }
@@ -306,9 +309,10 @@ struct Now {
   uint32_t call;
 };
 template <bool EIGHT, bool WHOLE>
-__device__ __forceinline__ void adamw_piece(const Entry& t, uint32_t place, uint64_t i, const Now& now) {
-  const uint64_t n = t.numel, group = i / kGroup;
-  const bool some = WHOLE || group * kGroup < n;
+__device__ __forceinline__ void adamw_piece(const Entry& t, uint32_t place, int64_t i, const Now& now) {
+  const int64_t n = (int64_t)t.numel;
+  const uint64_t group = (uint64_t)i / kGroup;  // of an 8-bit state, whose pieces are not shifted
+  const bool some = WHOLE || group * kGroup < t.numel;
   float g[8], p[8], m[8], v[8];
   uint2 mc, vc;
   uint32_t m_scale = 0, v_scale = 0;
@@ -359,8 +363,9 @@ __device__ __forceinline__ void adamw_piece(const Entry& t, uint32_t place, uint
     uint32_t r[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = mix(key + j / 4 * kNext + j % 4);
-    mc = codes_of<true>(m, top_of(m), [&](int j) { return (r[j] >> 8 & 0xffff00u) | 0x80u; }, &m_scale);
-    vc = codes_of<false>(v, top_of(v), [&](int j) { return (r[j] << 8 & 0xffff00u) | 0x80u; }, &v_scale);
+    // 16 random bits over 0x80, at the place of the bits that are cut off
+    mc = codes_of<true>(m, top_of(m), [&](int j) { return __byte_perm(r[j], 0x80u, 0x5324u); }, &m_scale);
+    vc = codes_of<false>(v, top_of(v), [&](int j) { return __byte_perm(r[j], 0x80u, 0x5104u); }, &v_scale);
     store_codes<WHOLE>(t.m, i, n, t.packs, mc);
     store_codes<WHOLE>(t.v, i, n, t.packs, vc);
     if (some && threadIdx.x % 16 == 0) t.m_scale[group] = (uint8_t)m_scale, t.v_scale[group] = (uint8_t)v_scale;
@@ -389,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constan
     const float q = __fdiv_rn(given.max_norm, __fadd_rn(*given.norm, 1e-6f));
     now.factor = q >= 1.0f ? 1.0f : q;  // NaN of a norm that is none
   }
-  over_pieces(table, 1, [&](const Entry& t, int at, uint64_t i, auto whole) {
+  over_pieces(table, 1, [&](const Entry& t, int at, int64_t i, auto whole) {
     adamw_piece<EIGHT, decltype(whole)::value>(t, table.place + at, i, now);
   });
 }
@@ -399,10 +404,11 @@ template <int N, bool PACK>
 __global__ void __launch_bounds__(kThreads) adamw8_convert_kernel(const __grid_constant__ Table<N> table) {
   pdl_trigger_if_few();
   pdl_wait();
-  over_pieces(table, 1, [&](const Entry& t, int, uint64_t i, auto whole) {
+  over_pieces(table, 1, [&](const Entry& t, int, int64_t i, auto whole) {
     constexpr bool kWhole = decltype(whole)::value;
-    const uint64_t n = t.numel, group = i / kGroup;
-    const bool some = kWhole || group * kGroup < n;
+    const int64_t n = (int64_t)t.numel;
+    const uint64_t group = (uint64_t)i / kGroup;
+    const bool some = kWhole || group * kGroup < t.numel;
     float m[8], v[8];
     uint32_t m_scale = 0, v_scale = 0;
     if constexpr (PACK) {
@@ -441,9 +447,9 @@ __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_const
   pdl_trigger_if_few();
   pdl_wait();
   double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of their own, so that one need not wait for the other
-  over_pieces(table, run, [&](const Entry& t, int, uint64_t i, auto whole) {
+  over_pieces(table, run, [&](const Entry& t, int, int64_t i, auto whole) {
     float g[8];
-    load_any<decltype(whole)::value>(t.grad, t.grad_type, i, t.numel, t.packs, g);
+    load_any<decltype(whole)::value>(t.grad, t.grad_type, i, (int64_t)t.numel, t.packs, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j % 4] = fma((double)g[j], (double)g[j], s[j % 4]);
   });
@@ -460,8 +466,6 @@ __global__ void __launch_bounds__(kThreads) norm_sum_kernel(const double* __rest
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-bool lies_on(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
 // Calls launch(table, pieces) for as many tensors at a time as a table holds; empty tensors keep their place.
 template <int N, class F>
 cudaError_t in_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch) {
@@ -472,16 +476,21 @@ cudaError_t in_tables(const csw_adamw_tensor* tensors, size_t count, F&& launch)
     int n = 0;
     for (; n < N && at < count; ++at, ++n) {
       const csw_adamw_tensor& t = tensors[at];
-      const uint64_t more = t.numel / kPiece + (t.numel % kPiece != 0);
+      // how many values each tensor lies behind a boundary of four of them
+      auto off = [](const void* p, size_t size) { return (int)(reinterpret_cast<uintptr_t>(p) / size % 4); };
+      auto size_of = [](int type) { return type == CSW_TYPE_F32 ? (size_t)4 : (size_t)2; };
+      const bool eight = t.exp_avg_scale;
+      const void* const first = t.param ? t.param : t.grad;
+      const int shift = off(first, size_of(t.param ? t.param_type : t.grad_type));
+      bool packs = !eight || shift == 0;
+      auto same = [&](const void* p, size_t size) { packs = packs && (!p || off(p, size) == shift); };
+      same(t.grad, size_of(t.grad_type)), same(t.copy, size_of(t.copy_type));
+      same(t.exp_avg, eight ? 1 : 4), same(t.exp_avg_sq, eight ? 1 : 4);
+      const uint64_t reach = t.numel + (packs ? shift : 0), more = reach / kPiece + (reach % kPiece != 0);
       if (n && pieces + more > 0x7fffffffu) break;
-      Entry& e = table.tensor[n];
-      e = {t.grad,  t.param, t.copy, t.exp_avg, t.exp_avg_sq, static_cast<uint8_t*>(t.exp_avg_scale),
-           static_cast<uint8_t*>(t.exp_avg_sq_scale), t.numel, (uint8_t)t.param_type, (uint8_t)t.grad_type,
-           (uint8_t)t.copy_type, true};
-      const size_t state = t.exp_avg_scale ? 4 : 16;
-      auto four = [](int type) { return type == CSW_TYPE_F32 ? (size_t)16 : (size_t)8; };
-      e.packs = lies_on(t.grad, four(t.grad_type)) && lies_on(t.param, four(t.param_type)) &&
-                lies_on(t.copy, four(t.copy_type)) && lies_on(t.exp_avg, state) && lies_on(t.exp_avg_sq, state);
+      table.tensor[n] = {t.grad, t.param, t.copy, t.exp_avg, t.exp_avg_sq, static_cast<uint8_t*>(t.exp_avg_scale),
+                         static_cast<uint8_t*>(t.exp_avg_sq_scale), t.numel, (uint8_t)t.param_type, (uint8_t)t.grad_type,
+                         (uint8_t)t.copy_type, packs, (uint8_t)(packs ? shift : 0)};
       table.first[n] = (uint32_t)pieces;
       pieces += more;
     }

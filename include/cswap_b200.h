@@ -502,7 +502,7 @@ typedef struct {
 csw_status csw_adamw_step(const csw_adamw_tensor* tensors, size_t count, const csw_adamw_options* options,
                           csw_stream_t stream);
 /* State in 8 bits from averages in float32 (exp_avg in the place of param, exp_avg_sq of copy), rounded to the nearest with
- * halves away from zero; and the averages that it stands for.  Gradients and types are not looked at. */
+ * halves away from zero; and the averages that it stands for.  Both types are CSW_TYPE_F32; gradients are not looked at. */
 csw_status csw_adamw8_pack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream);
 csw_status csw_adamw8_unpack(const csw_adamw_tensor* tensors, size_t count, csw_stream_t stream);
 /* The square root of the sum of all gradients' squares, summed in float64; the workspace holds csw_gradient_norm_workspace bytes (of the

@@ -104,6 +104,25 @@ def test_what_lies_between_the_tensors_stays(cs):
         assert (buffers[1][0] == 7).all()
 
 
+@kinds
+@pytest.mark.parametrize("offsets", [(1, 1, 1, 1, 1), (3, 3, 3, 3, 3), (1, 1, 1, 1, 0), (0, 2, 0, 0, 0), (2, 0, 1, 3, 2)])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 2047, 2049, 4095, 6000])
+def test_tensors_off_their_alignment(cs, kind, offsets, n):
+    """Parameter, gradient, both averages and copy so many values behind a boundary, all alike or each in its own way; their
+    neighbours stay."""
+    room = [torch.full((n + 9,), 5.0, device="cuda", dtype=k) for k in (kind, kind, torch.float32, torch.float32, torch.bfloat16)]
+    p, g, m, v, c = (r[o + 4:o + 4 + n] for r, o in zip(room, offsets))
+    p.copy_(normal(n, seed=1))
+    g.copy_(normal(n, seed=2))
+    m.copy_(normal(n, seed=3))
+    v.copy_(normal(n, seed=4).square())
+    mine = [t.clone() for t in (p, g, m, v, c)]
+    cs.adamw_step([p], [g], [m], [v], 7, copies=[c], norm=cs.gradient_norm([g]), max_norm=0.5)
+    cs.adamw_step([mine[0]], [mine[1]], [mine[2]], [mine[3]], 7, copies=[mine[4]], norm=cs.gradient_norm([mine[1]]), max_norm=0.5)
+    for r, o, t, want in zip(room, offsets, (p, g, m, v, c), mine):
+        assert R.bits_equal(t, want) and (r[:o + 4] == 5).all() and (r[o + 4 + n:] == 5).all()
+
+
 # ---- 8 bits --------------------------------------------------------------------------------------------------------
 
 def some_state(cs, n, seed):

@@ -124,7 +124,8 @@ def test_step_arguments(L, mem):
     assert step(t=None, count=0) == 0 and step(t=tensor(p=None, g=None, m=None, v=None, n=0)) == 0
     for f in (L.csw_adamw8_pack, L.csw_adamw8_unpack):
         good = dict(c=at[6], **eight)
-        for bad in (tensor(**eight), tensor(c=at[6]), tensor(p=at[0] + 2, **good), tensor(**{**good, "m": None}), tensor(n=1 << 42, **good)):
+        for bad in (tensor(**eight), tensor(c=at[6]), tensor(p=at[0] + 2, **good), tensor(**{**good, "m": None}), tensor(n=1 << 42, **good),
+                    tensor(pt=BF16, **good), tensor(ct=F16, **good)):
             assert f(C.byref(bad), 1, None) == ARG
         assert f(None, 1, None) == ARG and f(None, 0, None) == 0
     b = C.c_size_t()
