@@ -275,9 +275,9 @@ constexpr int kThreads = 256;
 // operand's (whole tiles of 128 x 128 where that is read across its rows); behind all stages two batches of scales; behind them,
 // what the CTAs of a cluster send.  A batch has the scales of 16 blocks of the reduction: a word has four blocks', of which a
 // product names one, and 128 rows or columns have 512 bytes of a word each.  (A batch a block bounded the kernel: the fence
-// between writing it and the tensor cores' reading takes 500 clocks, in which products of 128 x 128 take 256.)  Where the stages were, in the end, lie the tile's sums:
-// row by row with 16 bytes between them, so that a warp's 32 rows are in different banks, or, for a result with the operands
-// exchanged, column by column.
+// between writing it and the tensor cores' reading takes 500 clocks, in which products of 128 x 128 take 256.)  Where the
+// stages were, in the end, lie the tile's sums: row by row with 16 bytes between them, so that a warp's 32 rows are in different
+// banks, or, for a result with the operands exchanged, column by column.
 constexpr int kMostStages = 10, kBatch = 16;
 template <int BN>
 struct Plan {
@@ -288,7 +288,9 @@ struct Plan {
   static constexpr int kColumns = kNeeded > 256 ? 512 : kNeeded > 128 ? 256 : kNeeded > 64 ? 128 : 64;
   static constexpr int kPitch = BN + 4;
   static constexpr uint32_t kSums = kBlock * kPitch * 4;
-  __host__ __device__ static constexpr uint32_t stage(bool across) { return kTileBytes + (across ? kPanels * kTileBytes : BN * kBlock); }
+  __host__ __device__ static constexpr uint32_t stage(bool across) {
+    return kTileBytes + (across ? kPanels * kTileBytes : BN * kBlock);
+  }
   // As many stages as there is work for, and room: half an SM's shared memory where a CTA is not alone on it.
   static uint32_t stages(bool across, bool alone, bool parts, uint32_t steps) {
     const uint32_t room = (alone ? 224u : 110u) * 1024 - (parts ? kSums : 0) - 2 * kBatchBytes, each = stage(across);
@@ -435,12 +437,17 @@ __device__ __forceinline__ void write_scales(char* to, const uint32_t (&held)[OP
 __device__ __forceinline__ void values_meet() { asm volatile("bar.sync 1, 160;" ::: "memory"); }
 
 // One warp copies tiles, one writes their scales, one issues the products, four take the sums out.  Where there are few
-// tiles, a cluster of `parts` CTAs shares one: each takes a part of the reduction, and the parts' sums, in shared memory, are
-// added in their order, each CTA a part of the columns.
+// tiles, a cluster of `parts` CTAs shares one: each takes a part of the reduction, and sends its sums in shares, so that every
+// CTA has some rows of the result from all parts, which it adds in their order.  (Loads from the other CTAs' shared memory took
+// 460 clocks each, one after the other, copies of whole shares 1500 together.)
+//
+// What bounds it: the issue of a block's products, some 340 clocks, where BN is 128 or less (products of 128 x 128 take 256); the
+// way from L2 into an SM above; and for the smallest ones 2 us from launch to the first block, 2 from the last to the end.
+//
 // A few rows of values (tokens, in generation) need not be quantized by a launch of their own: with X their type, the warps that
 // wait for the sums do it before, every CTA for its part of the reduction.  First the scales of all its blocks, then the codes,
-// a warp a block, into the stage that the other operand's tile is copied to.  (1 x 4096 x 4096: 7.2 us of product behind 4 of
-// quantizing, 8.4 together.)
+// a warp a block, into the stage that the other operand's tile is copied to.  (One token through 4096 x 4096: 10.6 us in two
+// launches, 7.5 in one.)
 constexpr int kMostHeld = 512;  // blocks of a CTA's part of the reduction, with X
 template <class X>
 struct Block {  // four columns of each row
@@ -514,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
     bar_init(received, 1);
     flag = 0;
     init_visible();
-    prefetch_map(&p.r.map);
-    if (!kValues) prefetch_map(&p.c.map);
+    if (p.steps) prefetch_map(&p.r.map);
+    if (p.steps && !kValues) prefetch_map(&p.c.map);
   }
   // Every CTA's barriers are there.  From here to where tensor memory is freed no CTA waits for another one, which might wait
   // for that memory.
@@ -679,8 +686,12 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_product_kernel(const __grid_c
 
 // ---- two CTAs on a tile ------------------------------------------------------------------------------------------------
 // Tiles of 256 x 256, each on a pair of CTAs, which keep 128 rows and bring 128 of the columns each: a block of the reduction
-// then takes 32 KB into an SM for 512 clocks of products, where a CTA on its own takes 48.  A pair goes through tiles until there are none left.  Eight warps take a tile's
-// sums into registers, 128 a thread, and tell that the next one's may begin; they are rounded, and leave, meanwhile.
+// then takes 32 KB into an SM for 512 clocks of products, where a CTA on its own takes 48.  A pair goes through tiles until there
+// are none left.  Eight warps take a tile's sums into registers, 128 a thread, and tell that the next one's may begin; they are
+// rounded, and leave, meanwhile.
+//
+// What bounds it: the tensor cores, busy 86 % of the time, and in long runs the power limit.  8192 x 8192 x 4096: 195 us, 2.8
+// PFLOP/s; products alone would take 165, copies alone 142.
 template <class T>
 constexpr int kEachOf = 16 / sizeof(T);
 constexpr int kPairThreads = 384, kPairStages = 5, kPairTile = 2 * kBlock;

@@ -86,8 +86,9 @@ class AdamW(torch.optim.Optimizer):
 
     `max_norm`: the gradients of all groups together are scaled to that norm where theirs is larger.  `seed`: of the rounding
     in 8 bits.  A step takes the number of steps that a parameter has been through from its state; with `capturable` it is
-    counted on the device, once for all of a group, and the learning rate lies there too (`set_lr` changes it), so that a
-    captured step may be replayed."""
+    counted on the device, once for all of a group, and the learning rate lies there too, so that a captured step may be
+    replayed: `set_lr` changes it for replays, a scheduler's change of the groups arrives with the next step that is not
+    captured."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, bits: int = 32, max_norm: Optional[float] = None, seed: int = 0,
@@ -118,10 +119,12 @@ class AdamW(torch.optim.Optimizer):
             group["lr"] = lr
             if "device_lr" in group:
                 group["device_lr"].fill_(lr)
+                group["told_lr"] = lr
 
     @torch.no_grad()
     def step(self, closure=None):
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if capturing:
             fresh = any(p.grad is not None and not self.state[p] or self.capturable and "device_step" not in group
                         for group in self.param_groups for p in group["params"])
             if fresh or not self.capturable:
@@ -151,7 +154,11 @@ class AdamW(torch.optim.Optimizer):
                     device = next(iter(by_step[0]))[0].device
                     taken = max(state["step"] for _, _, state in by_step[0]) - 1
                     group["device_step"] = torch.full((1,), taken, dtype=torch.int64, device=device)
-                    group["device_lr"] = torch.full((1,), group["lr"], dtype=torch.float32, device=device)
+                    group["device_lr"] = torch.empty(1, dtype=torch.float32, device=device)
+                    group["told_lr"] = None
+                if not capturing and group["told_lr"] != group["lr"]:
+                    group["device_lr"].fill_(group["lr"])
+                    group["told_lr"] = group["lr"]
                 group["device_step"].add_(1)
             work += [(at, group, step, members) for step, members in by_step.items()]
         if not every:

@@ -451,7 +451,7 @@ typedef struct {
 } csw_fp8_matrix;
 /* out = a b + bias, with a taken as m x k, b as k x n, out m x n row behind row; the bias (n values of bias_type) may be NULL.
  * Products are exact and summed in float32 by the tensor cores; the sum is rounded to the type once.  m and n are at most 2^31 - 129, k at
- * most 2^31 - 1.  The same call gives the same bits every time.  Waits are bounded as those of attention (section 7). */
+ * most 2^31 - 1.  out overlaps no operand.  The same call gives the same bits every time.  Waits are bounded as those of attention (section 7). */
 csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, const void* d_bias, int bias_type, void* d_out,
                           int type, csw_stream_t stream);
 

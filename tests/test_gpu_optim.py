@@ -571,6 +571,23 @@ def test_a_captured_step(cs, bits):
     assert all(torch.equal(p, q) for p, q in zip(params, other))
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_scheduler_changes_the_rate(cs, capturable):
+    params, other = parameters(), parameters()
+    opt = cs.AdamW(params, lr=1e-2, capturable=capturable)
+    plan = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.5)
+    for t in (1, 3, 4):
+        set_gradients(params, t)
+        opt.step()
+        plan.step()
+    ms, vs = ([torch.zeros_like(p) for p in other] for _ in range(2))
+    for k, t in enumerate((1, 3, 4)):
+        cs.adamw_step([p.detach() for p in other], [normal(*p.shape, seed=100 * t + i) for i, p in enumerate(other)], ms, vs, k + 1,
+                      lr=1e-2 * 0.5 ** k)
+    for p, q in zip(params, other):
+        R.close(p.detach(), q.detach(), q.detach().abs() * 3 * 2.0 ** -23 + 0.07 * 2.0 ** -20)  # a rate rounded to float32
+
+
 def test_optimizer_refuses(cs):
     for bad in (dict(bits=16), dict(seed=-1), dict(seed=1 << 32), dict(max_norm=-1.0), dict(max_norm=math.nan)):
         with pytest.raises(ValueError):
