@@ -181,7 +181,7 @@ SIGNATURES = {
     "csw_attention_workspace": (_I, [_SH, C.POINTER(_SZ)]),
     "csw_attention_backward": (_I, [_SH, _OP, _OP, _OP, _OP, _P, _OP, _OP, _OP, _OP, _P, _SZ, _P]),
     "csw_fp8_quantize_workspace": (_I, [_SZ, _SZ, C.POINTER(_SZ)]),
-    "csw_fp8_quantize": (_I, [_P, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _P, _SZ, _P]),
+    "csw_fp8_quantize": (_I, [_P, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _I, _P, _SZ, _P]),
     "csw_fp8_dequantize": (_I, [_P, _SZ, _P, _SZ, _SZ, _P, _I, _P]),
     "csw_fp8_matmul": (_I, [_MX, _MX, _P, _I, _P, _I, _P]),
     "csw_fp8_linear_workspace": (_I, [_SZ, _SZ, _SZ, C.POINTER(_SZ)]),

@@ -101,10 +101,17 @@ struct Eight {
 template <class T>
 constexpr uint32_t kNoNumber = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 
+__device__ __forceinline__ void store_as(void* to, int type, uint64_t i, float v) {
+  if (type == 0) static_cast<float*>(to)[i] = v;
+  else if (type == 1) static_cast<__half*>(to)[i] = narrow<__half>(v);
+  else static_cast<__nv_bfloat16*>(to)[i] = narrow<__nv_bfloat16>(v);
+}
+
 template <class T, bool SUMS>
 __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T* __restrict__ x, uint64_t rows, uint64_t cols,
                                                                         uint64_t stride, bool packs, uint8_t* codes,
-                                                                        uint64_t code_stride, uint8_t* scales, float* sums) {
+                                                                        uint64_t code_stride, uint8_t* scales, void* sums,
+                                                                        int sums_type) {
   __shared__ uint32_t tops[kQuantizeThreads / 32];
   __shared__ float column[SUMS ? 16 : 1][SUMS ? kBlock : 1];
   pdl_trigger_if_few();
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T*
       float s = column[0][t];
 #pragma unroll
       for (int i = 1; i < 16; ++i) s += column[i][t];
-      sums[bi * cols + bj * kBlock + t] = s;
+      store_as(sums, sums_type, bi * cols + bj * kBlock + t, s);
     }
   }
   if (col >= cols) return;
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) fp8_quantize_kernel(const T*
 
 // The sums of the blocks of rows, in their order: 8 threads a column, each a part of the blocks.
 __global__ void __launch_bounds__(256) fp8_sums_kernel(const float* __restrict__ partials, uint64_t parts, uint64_t cols,
-                                                       float* sums) {
+                                                       void* sums, int type) {
   __shared__ float part[8][32];
   pdl_trigger_if_few();
   pdl_wait(partials);
@@ -212,7 +219,7 @@ __global__ void __launch_bounds__(256) fp8_sums_kernel(const float* __restrict__
   if (p || col >= cols) return;
 #pragma unroll
   for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-  sums[col] = s;
+  store_as(sums, type, col, s);
 }
 
 // The same way back, for four neighbours of a row's first half and four of its second, so that a row's float32 values leave as
@@ -1001,20 +1008,21 @@ cudaError_t pair_product(Product& p, const Fp8Matrix& r, const Fp8Matrix& c, boo
 
 cudaError_t fp8_quantize_launch(const Fp8Quantize& a, cudaStream_t stream) {
   if (a.cols == 0) return cudaSuccess;
-  if (a.rows == 0) return a.sums ? taken(cudaMemsetAsync(a.sums, 0, a.cols * sizeof(float), stream)) : cudaSuccess;
+  if (a.rows == 0)
+    return a.sums ? taken(cudaMemsetAsync(a.sums, 0, a.cols * (a.sums_type == 0 ? 4 : 2), stream)) : cudaSuccess;
   const uint64_t parts = fp8_blocks(a.rows), grid = parts * fp8_blocks(a.cols);
   cudaError_t e = cudaSuccess;
-  float* sums = parts > 1 ? a.partials : a.sums;
+  void* const sums = parts > 1 ? a.partials : a.sums;
   with_type(a.type, [&](auto v) {
     using T = decltype(v);
     const bool packs = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.stride * sizeof(T) % 16 == 0;
     const auto kernel = a.sums ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
     e = pdl_launch(kernel, (unsigned)grid, kQuantizeThreads, 0, stream, static_cast<const T*>(a.x), a.rows, a.cols, a.stride,
-                   packs, static_cast<uint8_t*>(a.codes), a.code_stride, a.scales, sums);
+                   packs, static_cast<uint8_t*>(a.codes), a.code_stride, a.scales, sums, parts > 1 ? 0 : a.sums_type);
   });
   if (e == cudaSuccess && a.sums && parts > 1)
     e = pdl_launch(fp8_sums_kernel, (unsigned)((a.cols + 31) / 32), 256, 0, stream, (const float*)a.partials, parts, a.cols,
-                   a.sums);
+                   a.sums, a.sums_type);
   return e;
 }
 

@@ -18,7 +18,9 @@ struct Fp8Quantize {
   void* codes;
   uint64_t code_stride;         // a multiple of 16, cols at least
   uint8_t* scales;              // [blocks of rows][blocks of columns]
-  float *sums, *partials;       // sums may be null; partials: fp8_blocks(rows) x cols where it is not and rows > 128
+  void* sums;                   // may be null
+  int sums_type;
+  float* partials;              // fp8_blocks(rows) x cols where sums is not null and rows > 128
 };
 cudaError_t fp8_quantize_launch(const Fp8Quantize& a, cudaStream_t stream);
 cudaError_t fp8_dequantize_launch(const void* codes, uint64_t code_stride, const uint8_t* scales, uint64_t rows, uint64_t cols,

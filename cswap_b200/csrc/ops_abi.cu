@@ -230,18 +230,18 @@ csw_status csw_fp8_quantize_workspace(size_t rows, size_t cols, size_t* bytes) {
 }
 
 csw_status csw_fp8_quantize(const void* d_x, int type, size_t rows, size_t cols, size_t x_stride, void* d_codes,
-                            size_t code_stride, void* d_scales, float* d_sums, void* d_workspace, size_t workspace_bytes,
-                            csw_stream_t stream) {
+                            size_t code_stride, void* d_scales, void* d_sums, int sums_type, void* d_workspace,
+                            size_t workspace_bytes, csw_stream_t stream) {
   size_t need;
   if (!known_type(type) || !matrix(d_codes, d_scales, rows, cols, code_stride) ||
       csw_fp8_quantize_workspace(rows, cols, &need) != CSW_OK)
     return CSW_ERR_ARG;
   if (rows && cols && (!good(d_x, type) || x_stride < cols || x_stride > kMostValues / rows)) return CSW_ERR_ARG;
-  if (d_sums && !aligned(d_sums, 4)) return CSW_ERR_ARG;
+  if (d_sums && (!known_type(sums_type) || !good(d_sums, sums_type))) return CSW_ERR_ARG;
   if (d_sums && need && !good(d_workspace, CSW_TYPE_F32)) return CSW_ERR_ARG;
   if (d_sums && workspace_bytes < need) return CSW_ERR_SIZE;
   return done(fp8_quantize_launch({d_x, type, rows, cols, x_stride, d_codes, code_stride, static_cast<uint8_t*>(d_scales),
-                                   d_sums, static_cast<float*>(d_workspace)},
+                                   d_sums, sums_type, static_cast<float*>(d_workspace)},
                                   stream));
 }
 
@@ -301,7 +301,7 @@ csw_status csw_fp8_linear(const void* d_x, int type, size_t rows, size_t x_strid
   if (st != CSW_OK) return st;
   const size_t stride = (cols + 15) / 16 * 16;
   return done(fp8_linear_launch({d_x, type, rows, cols, x_stride, d_workspace, stride,
-                                 static_cast<uint8_t*>(d_workspace) + stride * rows, nullptr, nullptr},
+                                 static_cast<uint8_t*>(d_workspace) + stride * rows, nullptr, 0, nullptr},
                                 {weight->codes, static_cast<const uint8_t*>(weight->scales), outs, cols, weight->code_stride, true},
                                 d_bias, bias_type, d_out, out_type, stream));
 }

@@ -58,7 +58,8 @@ struct Quantized {
   at::Tensor codes, scales, sums;
 };
 // A matrix of rows that lie `stride` values apart.  The values are checked; what the call itself finds wrong is thrown.
-Quantized quantized(const at::Tensor& x, int type, int64_t rows, int64_t cols, int64_t stride, bool sums) {
+Quantized quantized(const at::Tensor& x, int type, int64_t rows, int64_t cols, int64_t stride, bool sums,
+                    at::ScalarType sums_kind) {
   const c10::cuda::CUDAGuard on(x.device());
   size_t need;
   require_ok(csw_fp8_quantize_workspace(rows, cols, &need), "csw_fp8_quantize_workspace");
@@ -66,16 +67,17 @@ Quantized quantized(const at::Tensor& x, int type, int64_t rows, int64_t cols, i
   Quantized q{fresh(x, {rows, code_stride}, at::kFloat8_e4m3fn), fresh(x, {blocks_of(rows), blocks_of(cols)}, at::kFloat8_e8m0fnu), {}};
   at::Tensor space;
   void* ws = nullptr;
-  float* totals = nullptr;
+  void* totals = nullptr;
   if (sums) {
-    q.sums = fresh(x, {cols}, at::kFloat);
-    totals = static_cast<float*>(out(q.sums));
+    q.sums = fresh(x, {cols}, sums_kind);
+    totals = out(q.sums);
     if (need) {
       space = fresh(x, {(int64_t)need}, at::kByte);
       ws = out(space);
     }
   }
-  require_ok(csw_fp8_quantize(ptr(x), type, rows, cols, stride, out(q.codes), code_stride, out(q.scales), totals, ws, need,
+  require_ok(csw_fp8_quantize(ptr(x), type, rows, cols, stride, out(q.codes), code_stride, out(q.scales), totals,
+                              type_code(sums_kind), ws, need,
                               c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
              "csw_fp8_quantize");
   if (code_stride != cols) q.codes = q.codes.as_strided({rows, cols}, {code_stride, 1});
@@ -86,11 +88,11 @@ bool lies_in_rows(const at::Tensor& t) {
   return t.is_contiguous() ||
          (t.dim() == 2 && t.size(0) > 1 && (t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) >= t.size(1));
 }
-Quantized quantized(const at::Tensor& x, int type, bool sums) {
+Quantized quantized(const at::Tensor& x, int type, bool sums, at::ScalarType sums_kind = at::kFloat) {
   int64_t rows = 1;
   for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
   const int64_t cols = x.size(-1);
-  return quantized(x, type, rows, cols, x.is_contiguous() ? cols : x.stride(0), sums);
+  return quantized(x, type, rows, cols, x.is_contiguous() ? cols : x.stride(0), sums, sums_kind);
 }
 csw_fp8_matrix matrix_of(const at::Tensor& codes, const at::Tensor& scales, bool transposed) {
   return {ptr(codes), ptr(scales), (size_t)codes.size(0), (size_t)codes.size(1), (size_t)padded(codes.size(1)), transposed};
@@ -214,14 +216,14 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = types[2] >= 0 && ctx->needs_input_grad(2);
       const at::Tensor rows = grads[0].dim() == 2 ? grads[0] : grads[0].flatten(0, -2);
       const at::Tensor dy = lies_in_rows(rows) ? rows : rows.contiguous();
-      const Quantized g = quantized(dy, type_code(dy.scalar_type()), want_b);
+      const Quantized g = quantized(dy, type_code(dy.scalar_type()), want_b, want_b ? (at::ScalarType)types[2] : at::kFloat);
       const csw_fp8_matrix along = matrix_of(g.codes, g.scales, false), across = matrix_of(g.codes, g.scales, true);
       if (want_x)
         r[0] = product(along, matrix_of(saved[2], saved[3], false), nullptr, dy, (at::ScalarType)types[0], shape);
       if (want_w)
         r[1] = product(across, matrix_of(saved[0], saved[1], false), nullptr, dy, (at::ScalarType)types[1],
                        {dy.size(1), saved[0].size(1)});
-      if (want_b) r[2] = g.sums.to((at::ScalarType)types[2]);
+      if (want_b) r[2] = g.sums;
     }
     if (again) {  // a gradient of these gradients is an error, where one is asked for
       for (at::Tensor& t : r)

@@ -434,11 +434,11 @@ csw_status csw_attention_backward(const csw_attention_shape* shape, const csw_at
  * apart, a multiple of 16 and not less than cols rounded up to 8; the codes lie on 16 bytes.  What lies between a row's last
  * code and the next row is not used (up to 7 bytes of it are written). */
 /* d_x: rows of cols values, x_stride values apart (cols at least).  Where d_sums is given it receives the sum of each column
- * in float32, by way of a workspace of csw_fp8_quantize_workspace bytes (none for up to 128 rows). */
+ * in sums_type, added up in float32 by way of a workspace of csw_fp8_quantize_workspace bytes (none for up to 128 rows). */
 csw_status csw_fp8_quantize_workspace(size_t rows, size_t cols, size_t* bytes);
 csw_status csw_fp8_quantize(const void* d_x, int type, size_t rows, size_t cols, size_t x_stride, void* d_codes,
-                            size_t code_stride, void* d_scales, float* d_sums, void* d_workspace, size_t workspace_bytes,
-                            csw_stream_t stream);
+                            size_t code_stride, void* d_scales, void* d_sums, int sums_type, void* d_workspace,
+                            size_t workspace_bytes, csw_stream_t stream);
 /* The values that codes and scales stand for, rounded to the type, row behind row. */
 csw_status csw_fp8_dequantize(const void* d_codes, size_t code_stride, const void* d_scales, size_t rows, size_t cols,
                               void* d_out, int type, csw_stream_t stream);

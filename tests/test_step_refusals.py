@@ -27,11 +27,13 @@ def mem():
 def test_quantize_arguments(L, mem):
     x, codes, scales, sums, ws = (mem + 8192 * i for i in range(5))
 
-    def quantize(x=x, t=F32, rows=200, cols=5, stride=5, codes=codes, ld=16, scales=scales, sums=None, ws=ws, size=1 << 12):
-        return L.csw_fp8_quantize(x, t, rows, cols, stride, codes, ld, scales, sums, ws, size, None)
+    def quantize(x=x, t=F32, rows=200, cols=5, stride=5, codes=codes, ld=16, scales=scales, sums=None, st=F32, ws=ws,
+                 size=1 << 12):
+        return L.csw_fp8_quantize(x, t, rows, cols, stride, codes, ld, scales, sums, st, ws, size, None)
 
     for bad in (dict(t=3), dict(x=None), dict(x=x + 2), dict(stride=4), dict(codes=None), dict(codes=codes + 8), dict(ld=8),
-                dict(ld=24), dict(cols=17, stride=17), dict(scales=None), dict(sums=sums + 2), dict(sums=sums, ws=None),
+                dict(ld=24), dict(cols=17, stride=17), dict(scales=None), dict(sums=sums + 2), dict(sums=sums, st=3),
+                dict(sums=sums + 1, st=BF16), dict(sums=sums, ws=None),
                 dict(sums=sums, ws=ws + 2), dict(rows=1 << 31), dict(cols=1 << 31, stride=1 << 31, ld=1 << 31),
                 dict(ld=(1 << 39) + 16), dict(stride=1 << 42),
                 dict(rows=(1 << 31) - 1, cols=(1 << 31) - 1, stride=1 << 31, ld=1 << 31)):
