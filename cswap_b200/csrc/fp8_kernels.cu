@@ -868,15 +868,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
               if (lane == 0) store_matrix_tile(&out_map, smem_at(chunk), (int)(col + at), (int)row);
             } else {  // rows that begin anywhere: a row of the chunk at a time, a value a lane
               __syncwarp();
-              T* out = static_cast<T*>(p.out) + (uint64_t)row * p.n + col + at;
-              const int rows = (int)min(p.m - row, 32u), wide = (int)min(p.n - col - at, (uint32_t)kWide);
+              T* to = static_cast<T*>(p.out) + (uint64_t)row * p.n + col + at + lane;
+              const int rows = (int)min(p.m - row, 32u), wide = (int)min(p.n - col - at, (uint32_t)kWide) - lane;
+              const uintptr_t mine = reinterpret_cast<uintptr_t>(chunk) + lane * sizeof(T);
+#pragma unroll 1
+              for (int i = 0; i < rows; i += 8) {
 #pragma unroll
-              for (int j = 0; j < kWide; j += 32) {
-                const int c = j + lane, unit = c / kEachOf<T>, in = c % kEachOf<T> * sizeof(T);
-#pragma unroll 8
-                for (int i = 0; i < 32; ++i) {
-                  const T v = *reinterpret_cast<const T*>(chunk + i * 128 + (unit ^ (i & 7)) * 16 + in);
-                  if (i < rows && c < wide) out[(uint64_t)i * p.n + c] = v;
+                for (int k = 0; k < 8; ++k, to += p.n) {
+#pragma unroll
+                  for (int j = 0; j < kWide; j += 32) {
+                    const T v = *reinterpret_cast<const T*>((mine ^ (k * 16) ^ (j * sizeof(T))) + (i + k) * 128);
+                    if (i + k < rows && j < wide) to[j] = v;
+                  }
                 }
               }
             }
@@ -961,7 +964,7 @@ Way way_for(const Product& p) {
   }
   if (p.steps && !p.exchanged && sms >= 2.0f) {
     const uint64_t tiles = (uint64_t)((p.m + kPairTile - 1) / kPairTile) * ((p.n + kPairTile - 1) / kPairTile);
-    consider(0, 1, 6.0f + rounds(tiles, std::floor(sms / 2)) * (p.steps * 0.3f + (p.packs ? 0.7f : 3.0f)));
+    consider(0, 1, 6.0f + rounds(tiles, std::floor(sms / 2)) * (p.steps * 0.3f + (p.packs ? 0.7f : 2.3f)));
   }
   return best;
 }
