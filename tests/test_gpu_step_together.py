@@ -187,6 +187,37 @@ def test_a_captured_training_step(cs, bits):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("which", ["x", "weight", "bias"])
+def test_a_captured_layer_whose_leaf_has_a_live_graph(cs, which):
+    """A leaf whose gradient belongs to a live graph of another stream, behind a view, too, is refused in a capture; without that
+    graph the layer is captured, and its replay gives the gradient that the eager layer gave."""
+    sets = {"x": normal(64, 40, seed=1), "weight": normal(64, 24, seed=2), "bias": normal(24, seed=3)}
+    leaf = sets[which].requires_grad_(True)
+    call = lambda: cs.fp8_linear(sets["x"].t(), sets["weight"].t(), sets["bias"].view(24))
+    dy = normal(40, 24, seed=4)
+    alive = call()
+    ones = torch.ones(4, device="cuda")
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    raised = None
+    with torch.cuda.stream(side):
+        g.capture_begin()
+        try:
+            call()
+        except RuntimeError as err:
+            raised = str(err)
+        finally:
+            keep = ones + 1  # the capture itself goes on
+            g.capture_end()
+    assert raised is not None and "live graph" in raised and keep.shape == (4,)
+    grad, = torch.autograd.grad(alive, leaf, dy)
+    del alive
+    with torch.cuda.graph(g2 := torch.cuda.CUDAGraph()):
+        again, = torch.autograd.grad(call(), leaf, dy)
+    g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, grad)
+
+
 @pytest.mark.parametrize("m,n,k", [(77, 96, 200), (1, 4096, 4096), (2048, 2048, 512)])
 def test_between_kernels_that_rewrite_the_inputs(cs, m, n, k):
     """A kernel that writes x right before the call and one that overwrites it right behind: the results of the call alone."""
