@@ -18,6 +18,16 @@ int64_t blocks_of(int64_t n) { return n / 128 + (n % 128 != 0); }
 int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
 
 // ---- matrices in 8-bit floating point ------------------------------------------------------------------------------
+// Whether codes lie as the kernels read them: rows `stride` bytes apart, which begin on 16 bytes and have their padding to
+// a multiple of 16 behind them, the last one, too.
+bool lies_padded(const at::Tensor& c, int64_t* stride) {
+  const int64_t rows = c.size(0), cols = c.size(1);
+  *stride = rows > 1 ? c.stride(0) : padded(cols);
+  if (rows == 0 || cols == 0) return true;
+  const int64_t held = (int64_t)c.storage().nbytes() - c.storage_offset();
+  return (cols == 1 || c.stride(1) == 1) && *stride % 16 == 0 && *stride >= cols && held >= rows * *stride &&
+         reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0;
+}
 // codes and scales as fp8_quantize gives them
 bool matrix_of(PyObject* codes, PyObject* scales, const char* name, const char* scales_name, const at::Tensor** t,
                csw_fp8_matrix* m) {
@@ -28,13 +38,9 @@ bool matrix_of(PyObject* codes, PyObject* scales, const char* name, const char* 
   if (c->scalar_type() != at::kFloat8_e4m3fn || c->dim() != 2)
     return value_error("%s must be a matrix of float8_e4m3fn codes", name);
   const int64_t rows = c->size(0), cols = c->size(1);
-  int64_t stride = rows > 1 ? c->stride(0) : padded(cols);
-  if (rows > 0 && cols > 0) {
-    const size_t held = c->storage().nbytes() - (size_t)c->storage_offset();
-    if ((cols > 1 && c->stride(1) != 1) || stride % 16 || stride < cols || held < (size_t)(rows * stride) ||
-        reinterpret_cast<uintptr_t>(c->const_data_ptr()) % 16)
-      return value_error("%s must have rows that begin on 16 bytes and are padded to a multiple of them", name);
-  }
+  int64_t stride;
+  if (!lies_padded(*c, &stride))
+    return value_error("%s must have rows that begin on 16 bytes and are padded to a multiple of them", name);
   if (!same_device(*s, *c, scales_name)) return false;
   if (s->scalar_type() != at::kFloat8_e8m0fnu || s->dim() != 2 || s->size(0) != blocks_of(rows) || s->size(1) != blocks_of(cols))
     return value_error("%s must be float8_e8m0fnu, one for each block of 128 x 128 codes", scales_name);
@@ -94,8 +100,28 @@ Quantized quantized(const at::Tensor& x, int type, bool sums, at::ScalarType sum
   const int64_t cols = x.size(-1);
   return quantized(x, type, rows, cols, x.is_contiguous() ? cols : x.stride(0), sums, sums_kind);
 }
+// of codes that lie padded
 csw_fp8_matrix matrix_of(const at::Tensor& codes, const at::Tensor& scales, bool transposed) {
-  return {ptr(codes), ptr(scales), (size_t)codes.size(0), (size_t)codes.size(1), (size_t)padded(codes.size(1)), transposed};
+  int64_t stride;
+  lies_padded(codes, &stride);
+  return {ptr(codes), ptr(scales), (size_t)codes.size(0), (size_t)codes.size(1), (size_t)stride, transposed};
+}
+// A matrix that autograd has kept, as the kernels read it.  It has been through the program's saved-tensor hooks: a copy that
+// went through the host's memory lies densely, its rows without their padding, which is put back here.
+void as_kept(at::Tensor* codes, at::Tensor* scales, int64_t rows, int64_t cols, const at::Device& on) {
+  auto is = [&](const at::Tensor& t, at::ScalarType kind, int64_t r, int64_t c) {
+    return t.defined() && t.device() == on && t.layout() == at::kStrided && t.scalar_type() == kind && t.dim() == 2 && t.size(0) == r &&
+           t.size(1) == c;
+  };
+  TORCH_CHECK(is(*codes, at::kFloat8_e4m3fn, rows, cols) && is(*scales, at::kFloat8_e8m0fnu, blocks_of(rows), blocks_of(cols)),
+              "fp8_linear: a saved-tensor hook gave back a tensor of another type, shape or device than the one it was given");
+  int64_t stride;
+  if (!lies_padded(*codes, &stride)) {
+    const at::Tensor room = fresh(*codes, {rows, padded(cols)}, at::kByte).narrow(1, 0, cols);
+    room.copy_(codes->view(at::kByte));
+    *codes = room.view(at::kFloat8_e4m3fn);
+  }
+  if (!scales->is_contiguous()) *scales = scales->view(at::kByte).contiguous().view(at::kFloat8_e8m0fnu);
 }
 at::Tensor product(const csw_fp8_matrix& a, const csw_fp8_matrix& b, const at::Tensor* bias, const at::Tensor& like,
                    at::ScalarType kind, at::IntArrayRef sizes) {
@@ -211,18 +237,22 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     if (!grads[0].defined()) return r;
     {
       at::NoGradGuard none;
-      const auto saved = ctx->get_saved_variables();
+      auto saved = ctx->get_saved_variables();
       const auto shape = ctx->saved_data["shape"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
       const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = types[2] >= 0 && ctx->needs_input_grad(2);
       const at::Tensor rows = grads[0].dim() == 2 ? grads[0] : grads[0].flatten(0, -2);
       const at::Tensor dy = lies_in_rows(rows) ? rows : rows.contiguous();
       const Quantized g = quantized(dy, type_code(dy.scalar_type()), want_b, want_b ? (at::ScalarType)types[2] : at::kFloat);
       const csw_fp8_matrix along = matrix_of(g.codes, g.scales, false), across = matrix_of(g.codes, g.scales, true);
-      if (want_x)
+      const int64_t cols = shape.back();
+      if (want_x) {
+        as_kept(&saved[2], &saved[3], dy.size(1), cols, dy.device());
         r[0] = product(along, matrix_of(saved[2], saved[3], false), nullptr, dy, (at::ScalarType)types[0], shape);
-      if (want_w)
-        r[1] = product(across, matrix_of(saved[0], saved[1], false), nullptr, dy, (at::ScalarType)types[1],
-                       {dy.size(1), saved[0].size(1)});
+      }
+      if (want_w) {
+        as_kept(&saved[0], &saved[1], dy.size(0), cols, dy.device());
+        r[1] = product(across, matrix_of(saved[0], saved[1], false), nullptr, dy, (at::ScalarType)types[1], {dy.size(1), cols});
+      }
       if (want_b) r[2] = g.sums;
     }
     if (again) {  // a gradient of these gradients is an error, where one is asked for
