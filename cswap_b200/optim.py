@@ -125,7 +125,7 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None):
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         if capturing:
-            fresh = any(p.grad is not None and not self.state[p] or self.capturable and "device_step" not in group
+            fresh = any(p.grad is not None and not (self.state.get(p) and "device_step" in group)
                         for group in self.param_groups for p in group["params"])
             if fresh or not self.capturable:
                 raise RuntimeError("a step is captured with capturable=True, and after one that is not")

@@ -1,0 +1,94 @@
+"""What the optimizer class does on the host, without a GPU: its kernels are replaced by plain operations that note what they were
+given, a capture by a stream that says it is capturing."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Kernels:
+    """Stands in for the entry points: notes each launch's step and rate, and makes the step."""
+
+    def __init__(self):
+        self.steps, self.fail = [], None
+
+    def step(self, params, grads, step, lr, betas, eps, weight_decay, norm, max_norm, moments):
+        if self.fail is not None and self.fail in [id(p) for p in params]:
+            raise ValueError("refused")
+        t, rate = int(step), float(lr)
+        self.steps.append((t, rate, len(params)))
+        c = 1.0 if norm is None else min(1.0, max_norm / (float(norm) + 1e-6))
+        for p, g, (m, v) in zip(params, grads, moments):
+            m.mul_(betas[0]).add_(g * c, alpha=1 - betas[0])
+            v.mul_(betas[1]).add_((g * c).square(), alpha=1 - betas[1])
+            p.mul_(1 - rate * weight_decay)
+            p.sub_(rate / (1 - betas[0] ** t) * m / (v.sqrt() / math.sqrt(1 - betas[1] ** t) + eps))
+
+    def adamw_step(self, params, grads, ms, vs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, norm=None,
+                   max_norm=1.0, copies=None):
+        self.step(params, grads, step, lr, betas, eps, weight_decay, norm, max_norm, list(zip(ms, vs)))
+
+    def adamw8_step(self, params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, norm=None,
+                    max_norm=1.0, copies=None, seed=0):
+        for s in states:
+            s[0].add_(1)
+        zeros = [(torch.zeros_like(p), torch.zeros_like(p)) for p in params]
+        self.step(params, grads, step, lr, betas, eps, weight_decay, norm, max_norm, zeros)
+
+
+@pytest.fixture
+def kernels(monkeypatch):
+    from cswap_b200 import optim
+    k = Kernels()
+    monkeypatch.setattr(optim, "adamw_step", k.adamw_step)
+    monkeypatch.setattr(optim, "adamw8_step", k.adamw8_step)
+    monkeypatch.setattr(optim, "gradient_norm", lambda ts: torch.stack([t.norm() for t in ts]).norm())
+    return k
+
+
+@pytest.fixture
+def capture(monkeypatch):
+    """A switch: whether the current stream says that it is capturing."""
+    on = [False]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: on[0])
+
+    def switch(value):
+        on[0] = value
+    return switch
+
+
+def AdamW(*args, **kw):
+    import cswap_b200
+    return cswap_b200.AdamW(*args, **kw)
+
+
+def parameters(n=3, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(4 + i, generator=gen)) for i in range(n)]
+
+
+def set_gradients(params, t):
+    for i, p in enumerate(params):
+        p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * t + i))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_without_gradients_does_not_keep_a_step_from_being_captured(kernels, capture, bits):
+    params, frozen = parameters(2), parameters(2, seed=1)
+    opt = AdamW([dict(params=frozen), dict(params=params)], bits=bits, capturable=True)
+    set_gradients(params, 1)
+    capture(True)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()  # none has been made yet
+    capture(False)
+    opt.step()
+    capture(True)
+    opt.step()
+    assert [s[0] for s in kernels.steps] == [1, 2]
+    set_gradients(frozen, 1)  # and now it has gradients, but no state
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    capture(False)
+    assert all(not opt.state.get(p) for p in frozen)
