@@ -133,7 +133,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work: List[tuple] = []  # of one group and one number of steps
+        work: List[tuple] = []  # of one group and one number of steps so far
         every: List[torch.Tensor] = []
         for at, group in enumerate(self.param_groups):
             by_step: dict = {}
@@ -146,33 +146,38 @@ class AdamW(torch.optim.Optimizer):
                 if not (g.is_contiguous() and p.is_contiguous()) and g.stride() != p.stride():
                     g = torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
                 state = self._state_of(p)
-                state["step"] += 1
                 every.append(g)
                 by_step.setdefault(0 if self.capturable else state["step"], []).append((p, g, state))
             if self.capturable and by_step:
                 if "device_step" not in group:
                     device = next(iter(by_step[0]))[0].device
-                    taken = max(state["step"] for _, _, state in by_step[0]) - 1
+                    taken = max(state["step"] for _, _, state in by_step[0])
                     group["device_step"] = torch.full((1,), taken, dtype=torch.int64, device=device)
                     group["device_lr"] = torch.empty(1, dtype=torch.float32, device=device)
                     group["told_lr"] = None
                 if not capturing and group["told_lr"] != group["lr"]:
                     group["device_lr"].fill_(group["lr"])
                     group["told_lr"] = group["lr"]
-                group["device_step"].add_(1)
-            work += [(at, group, step, members) for step, members in by_step.items()]
+            work += [(at, group, taken, members) for taken, members in by_step.items()]
         if not every:
             return loss
         clip = dict(norm=gradient_norm(every), max_norm=self.max_norm) if self.max_norm is not None else {}
-        for at, group, step, members in work:
+        for at, group, taken, members in work:
             params, grads, states = ([m[i] for m in members] for i in range(3))
             rest = dict(betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], **clip)
-            step, lr = (group["device_step"], group["device_lr"]) if self.capturable else (step, group["lr"])
-            if self.bits == 8:
-                held = [(s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"]) for s in states]
-                adamw8_step(params, grads, held, step, lr, seed=(self.seed + at * 0x632be5ab) & 0xffffffff, **rest)
-            else:
-                adamw_step(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step, lr, **rest)
+            step, lr = (group["device_step"].add_(1), group["device_lr"]) if self.capturable else (taken + 1, group["lr"])
+            try:
+                if self.bits == 8:
+                    held = [(s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"]) for s in states]
+                    adamw8_step(params, grads, held, step, lr, seed=(self.seed + at * 0x632be5ab) & 0xffffffff, **rest)
+                else:
+                    adamw_step(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step, lr, **rest)
+            except Exception:  # a call that is refused is no step
+                if self.capturable:
+                    group["device_step"].sub_(1)
+                raise
+            for state in states:
+                state["step"] += 1
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:

@@ -92,3 +92,58 @@ def test_a_group_without_gradients_does_not_keep_a_step_from_being_captured(kern
         opt.step()
     capture(False)
     assert all(not opt.state.get(p) for p in frozen)
+
+
+def steps_of(opt, params):
+    return [opt.state[p].get("step") for p in params]
+
+
+def test_a_step_that_is_refused_is_not_counted(kernels):
+    """Two groups, the second one refused: the first one's step has been made and counts, the other's does not."""
+    first, second = parameters(2), parameters(2, seed=1)
+    opt = AdamW([dict(params=first), dict(params=second)])
+    for t in (1, 2):
+        set_gradients(first + second, t)
+        opt.step()
+    kernels.fail = id(second[0])
+    before = [p.detach().clone() for p in second]
+    with pytest.raises(ValueError, match="refused"):
+        opt.step()
+    assert steps_of(opt, first) == [3, 3] and steps_of(opt, second) == [2, 2]
+    assert all(torch.equal(p, b) for p, b in zip(second, before))
+    kernels.fail = None
+    kernels.steps.clear()
+    opt.step()
+    assert [s[0] for s in kernels.steps] == [4, 3]
+
+
+def test_a_step_that_is_refused_is_not_counted_on_the_device(kernels, capture):
+    first, second = parameters(2), parameters(2, seed=1)
+    opt = AdamW([dict(params=first), dict(params=second)], capturable=True)
+    set_gradients(first + second, 1)
+    kernels.fail = id(second[0])
+    for _ in range(2):  # also of a group that has made no step yet
+        with pytest.raises(ValueError, match="refused"):
+            opt.step()
+    assert steps_of(opt, first) == [2, 2] and steps_of(opt, second) == [0, 0]
+    kernels.fail = None
+    kernels.steps.clear()
+    opt.step()
+    assert [s[0] for s in kernels.steps] == [3, 1]
+
+
+def test_a_norm_that_is_refused_counts_no_step(kernels, monkeypatch):
+    from cswap_b200 import optim
+    params = parameters(2)
+    opt = AdamW(params, max_norm=1.0)
+    set_gradients(params, 1)
+    good = optim.gradient_norm
+
+    def bad(tensors):
+        raise ValueError("refused")
+    monkeypatch.setattr(optim, "gradient_norm", bad)
+    with pytest.raises(ValueError, match="refused"):
+        opt.step()
+    monkeypatch.setattr(optim, "gradient_norm", good)
+    opt.step()
+    assert [s[0] for s in kernels.steps] == [1] and steps_of(opt, params) == [1, 1]
