@@ -176,9 +176,19 @@ class AdamW(torch.optim.Optimizer):
                 if self.capturable:
                     group["device_step"].sub_(1)
                 raise
-            for state in states:
+            for state in states if not capturing else ():
                 state["step"] += 1
         return loss
+
+    def state_dict(self) -> dict:
+        """As torch's.  Steps that replays have made are counted on the device alone: they are asked for here."""
+        for group in self.param_groups:
+            if "device_step" in group:
+                taken = int(group["device_step"])
+                for p in group["params"]:
+                    if self.state.get(p):
+                        self.state[p]["step"] = taken
+        return super().state_dict()
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, which casts a state to its parameter's type: here codes stay codes, averages float32."""

@@ -1,0 +1,102 @@
+"""Checkpoints and copies of the optimizer: what goes on from them makes the steps that the original makes."""
+import io
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+both = pytest.mark.parametrize("bits", [32, 8])
+
+
+@pytest.fixture(scope="module")
+def cs():
+    import cswap_b200
+    assert torch.cuda.is_available()
+    cswap_b200.lib()
+    return cswap_b200
+
+
+def normal(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def parameters():
+    return [torch.nn.Parameter(normal(*s, seed=i)) for i, s in enumerate([(40, 30), (40,), (300,), (1,)])]
+
+
+def groups(params):
+    return [dict(params=params[:2], lr=1e-2), dict(params=params[2:], weight_decay=0.1)]
+
+
+def set_gradients(params, t):
+    for i, p in enumerate(params):
+        g = normal(*p.shape, seed=100 * t + i)
+        if p.grad is None:
+            p.grad = g
+        else:
+            p.grad.copy_(g)
+
+
+def captured(opt):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return graph
+
+
+def through_a_file(state, where):
+    f = io.BytesIO()
+    torch.save(state, f)
+    f.seek(0)
+    return torch.load(f, map_location=where)
+
+
+def same(opt, other, params, again):
+    assert all(torch.equal(p, q) for p, q in zip(params, again))
+    for p, q in zip(params, again):
+        for name, value in opt.state[p].items():
+            held = other.state[q][name]
+            assert torch.equal(value, held) and value.device == held.device if isinstance(value, torch.Tensor) else value == held
+
+
+@both
+@pytest.mark.parametrize("capturable", [False, True])
+def test_replays_count_in_a_checkpoint(cs, bits, capturable):
+    """Ten replays between a checkpoint and the step before them: the next step is the twelfth, also of an optimizer that counts
+    on the host (whose scalars are the host's: a parameter may be off by their last bits)."""
+    params = parameters()
+    opt = cs.AdamW(groups(params), bits=bits, max_norm=1.0, capturable=True, seed=5)
+    set_gradients(params, 1)
+    opt.step()
+    graph = captured(opt)
+    for t in range(2, 12):
+        set_gradients(params, t)
+        graph.replay()
+    state = opt.state_dict()
+    assert [s["step"] for s in state["state"].values()] == [11] * 4
+    again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = cs.AdamW(groups(again), bits=bits, max_norm=1.0, capturable=capturable, seed=5)
+    other.load_state_dict(through_a_file(state, "cuda"))
+    for ps, o in ((params, opt), (again, other)):
+        set_gradients(ps, 12)
+        o.step()
+    if capturable:
+        same(opt, other, params, again)
+        return
+    for p, q in zip(params, again):
+        assert float((p - q).abs().max()) <= 2.0 ** -22 * (float(p.abs().max()) + 0.032)
+        for name, value in opt.state[p].items():
+            assert not isinstance(value, torch.Tensor) or torch.equal(value, other.state[q][name])
+
+
+@both
+def test_a_capture_makes_no_step(cs, bits):
+    params = parameters()
+    opt = cs.AdamW(params, bits=bits, capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    graph = captured(opt)
+    assert [opt.state[p]["step"] for p in params] == [1] * 4
+    graph.replay()
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [2] * 4

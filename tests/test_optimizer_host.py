@@ -147,3 +147,55 @@ def test_a_norm_that_is_refused_counts_no_step(kernels, monkeypatch):
     monkeypatch.setattr(optim, "gradient_norm", good)
     opt.step()
     assert [s[0] for s in kernels.steps] == [1] and steps_of(opt, params) == [1, 1]
+
+
+def replay(opt, times):
+    """What replays of a captured step do to the counts on the device."""
+    for group in opt.param_groups:
+        if "device_step" in group:
+            group["device_step"].add_(times)
+
+
+def saved(opt):
+    """A checkpoint as a program loads it: through a file, into the host's memory."""
+    import io
+    f = io.BytesIO()
+    torch.save(opt.state_dict(), f)
+    f.seek(0)
+    return torch.load(f, map_location="cpu")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [True, False])
+def test_replayed_steps_are_saved(kernels, capture, bits, capturable):
+    """Steps that replays made count in a checkpoint, wherever it goes on."""
+    params = parameters(2)
+    opt = AdamW([dict(params=params[:1]), dict(params=params[1:])], bits=bits, capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    capture(True)
+    opt.step()  # on the device a capture counts nothing, but this stream only says that it captures: step 2
+    capture(False)
+    replay(opt, 98)
+    state = opt.state_dict()
+    assert [s["step"] for s in state["state"].values()] == [100, 100]
+    again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = AdamW([dict(params=again[:1]), dict(params=again[1:])], bits=bits, capturable=capturable)
+    other.load_state_dict(saved(opt))
+    kernels.steps.clear()
+    for ps, o in ((params, opt), (again, other)):
+        set_gradients(ps, 2)
+        o.step()
+    assert [s[0] for s in kernels.steps] == [101] * 4
+    assert all(torch.equal(p, q) for p, q in zip(params, again))
+
+
+def test_a_step_is_counted_where_it_runs(kernels, capture):
+    """Capturing a step makes none."""
+    params = parameters(2)
+    opt = AdamW(params, capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    capture(True)
+    opt.step()
+    assert steps_of(opt, params) == [1, 1]
