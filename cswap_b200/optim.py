@@ -81,6 +81,10 @@ def adamw8_unpack(states: Sequence[State8], exp_avgs: Sequence[torch.Tensor], ex
     _ext().adamw8_convert(states, exp_avgs, exp_avg_sqs, False)
 
 
+# what a group with capturable has besides, of which the first two lie on the device
+_DEVICE_KEYS = ("device_step", "device_lr", "told_lr")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW on adamw_step, or with `bits` 8 on adamw8_step, a launch for each group of parameters.
 
@@ -112,6 +116,14 @@ class AdamW(torch.optim.Optimizer):
                 for name in ("exp_avg", "exp_avg_sq"):
                     state[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         return state
+
+    def _count_on_device(self, group: dict) -> None:
+        """The group's number of steps and its rate, where its parameters are."""
+        held = [(p, self.state[p]) for p in group["params"] if self.state.get(p)]
+        device = held[0][0].device
+        group["device_step"] = torch.full((1,), max(s["step"] for _, s in held), dtype=torch.int64, device=device)
+        group["device_lr"] = torch.empty(1, dtype=torch.float32, device=device).fill_(group["lr"])
+        group["told_lr"] = group["lr"]
 
     def set_lr(self, lr: float) -> None:
         """The learning rate of all groups, also of steps that have been captured."""
@@ -150,11 +162,7 @@ class AdamW(torch.optim.Optimizer):
                 by_step.setdefault(0 if self.capturable else state["step"], []).append((p, g, state))
             if self.capturable and by_step:
                 if "device_step" not in group:
-                    device = next(iter(by_step[0]))[0].device
-                    taken = max(state["step"] for _, _, state in by_step[0])
-                    group["device_step"] = torch.full((1,), taken, dtype=torch.int64, device=device)
-                    group["device_lr"] = torch.empty(1, dtype=torch.float32, device=device)
-                    group["told_lr"] = None
+                    self._count_on_device(group)
                 if not capturing and group["told_lr"] != group["lr"]:
                     group["device_lr"].fill_(group["lr"])
                     group["told_lr"] = group["lr"]
@@ -181,17 +189,25 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def state_dict(self) -> dict:
-        """As torch's.  Steps that replays have made are counted on the device alone: they are asked for here."""
+        """As torch's.  Steps that replays have made are counted on the device alone: they are asked for here, and what lies on
+        the device besides the averages stays out."""
         for group in self.param_groups:
             if "device_step" in group:
-                taken = int(group["device_step"])
-                for p in group["params"]:
-                    if self.state.get(p):
-                        self.state[p]["step"] = taken
-        return super().state_dict()
+                self._set_steps(group, int(group["device_step"]))
+        state = super().state_dict()
+        for group in state["param_groups"]:
+            for key in _DEVICE_KEYS:
+                group.pop(key, None)
+        return state
+
+    def _set_steps(self, group: dict, taken: int) -> None:
+        for p in group["params"]:
+            if self.state.get(p):
+                self.state[p]["step"] = taken
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, which casts a state to its parameter's type: here codes stay codes, averages float32."""
+        """As torch's, which casts a state to its parameter's type: here codes stay codes, averages float32.  A step that was
+        captured before belongs to the state before, and is to be captured again."""
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
@@ -199,3 +215,9 @@ class AdamW(torch.optim.Optimizer):
             for name, value in state_dict["state"].get(i, {}).items():
                 if isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device, copy=True)
+        for group in self.param_groups:
+            taken, *_ = [group.pop(key, None) for key in _DEVICE_KEYS]
+            if taken is not None:  # a checkpoint whose groups hold the device's count, which is the one that is right
+                self._set_steps(group, int(taken))
+            if self.capturable and any(self.state.get(p) for p in group["params"]):
+                self._count_on_device(group)

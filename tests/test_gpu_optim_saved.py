@@ -52,6 +52,16 @@ def through_a_file(state, where):
     return torch.load(f, map_location=where)
 
 
+# A step by scalars of the device and one by scalars of the host, which differ in their last bits: float32's size, root and decay of
+# the step by 2^-23 each, a rate that is float32 on the device by 2^-24 of the size; with the roundings that follow, less than
+# 2^-21 of the parameter and of the move, which is 3.2 lr = 0.032 at most.
+APART = 2.0 ** -21
+
+
+def near(p, q, steps):
+    assert float((p - q).abs().max()) <= steps * APART * (float(p.abs().max()) + 0.032)
+
+
 def same(opt, other, params, again):
     assert all(torch.equal(p, q) for p, q in zip(params, again))
     for p, q in zip(params, again):
@@ -64,7 +74,7 @@ def same(opt, other, params, again):
 @pytest.mark.parametrize("capturable", [False, True])
 def test_replays_count_in_a_checkpoint(cs, bits, capturable):
     """Ten replays between a checkpoint and the step before them: the next step is the twelfth, also of an optimizer that counts
-    on the host (whose scalars are the host's: a parameter may be off by their last bits)."""
+    on the host."""
     params = parameters()
     opt = cs.AdamW(groups(params), bits=bits, max_norm=1.0, capturable=True, seed=5)
     set_gradients(params, 1)
@@ -85,7 +95,7 @@ def test_replays_count_in_a_checkpoint(cs, bits, capturable):
         same(opt, other, params, again)
         return
     for p, q in zip(params, again):
-        assert float((p - q).abs().max()) <= 2.0 ** -22 * (float(p.abs().max()) + 0.032)
+        near(p, q, 1)
         for name, value in opt.state[p].items():
             assert not isinstance(value, torch.Tensor) or torch.equal(value, other.state[q][name])
 
@@ -100,3 +110,47 @@ def test_a_capture_makes_no_step(cs, bits):
     assert [opt.state[p]["step"] for p in params] == [1] * 4
     graph.replay()
     assert [s["step"] for s in opt.state_dict()["state"].values()] == [2] * 4
+
+
+@both
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_a_capturable_optimizer_goes_on_from_the_host_s_memory(cs, bits, where):
+    """Captured right after loading, and replayed: the steps of the original, bit by bit."""
+    params = parameters()
+    opt = cs.AdamW(groups(params), bits=bits, max_norm=1.0, capturable=True, seed=5)
+    for t in (1, 2, 3):
+        set_gradients(params, t)
+        opt.step()
+    state = through_a_file(opt.state_dict(), where)
+    again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = cs.AdamW(groups(again), lr=1.0, bits=bits, max_norm=1.0, capturable=True, seed=5)
+    other.load_state_dict(state)
+    set_gradients(again, 4)
+    graph = captured(other)
+    for t in (4, 5):
+        set_gradients(params, t)
+        opt.step()
+        set_gradients(again, t)
+        graph.replay()
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [s["step"] for s in other.state_dict()["state"].values()] == [5] * 4
+    same(opt, other, params, again)
+
+
+@both
+def test_a_checkpoint_of_an_optimizer_that_is_not_capturable(cs, bits):
+    params = parameters()
+    opt = cs.AdamW(groups(params), bits=bits, seed=5)
+    for t in (1, 2):
+        set_gradients(params, t)
+        opt.step()
+    again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = cs.AdamW(groups(again), bits=bits, capturable=True, seed=5)
+    other.load_state_dict(through_a_file(opt.state_dict(), "cpu"))
+    for t in (3, 4):
+        for ps, o in ((params, opt), (again, other)):
+            set_gradients(ps, t)
+            o.step()
+    for p, q in zip(params, again):
+        near(p, q, 2)
+        for name, value in opt.state[p].items():
+            assert not isinstance(value, torch.Tensor) or torch.equal(value, other.state[q][name])

@@ -199,3 +199,46 @@ def test_a_step_is_counted_where_it_runs(kernels, capture):
     capture(True)
     opt.step()
     assert steps_of(opt, params) == [1, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_holds_nothing_that_lies_on_the_device_in_its_groups(kernels, capture, bits):
+    """What is counted on the device is made anew where the parameters are, so that a step may be captured right away."""
+    params = parameters(2)
+    opt = AdamW(params, lr=0.5, bits=bits, capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    replay(opt, 6)
+    state = saved(opt)
+    assert all(not isinstance(v, torch.Tensor) for g in state["param_groups"] for v in g.values())
+    assert "device_step" in opt.param_groups[0]  # the optimizer itself goes on as it was
+    again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = AdamW(again, lr=0.1, bits=bits, capturable=True)
+    other.load_state_dict(state)
+    set_gradients(again, 2)
+    capture(True)
+    kernels.steps.clear()
+    other.step()
+    assert [s[:2] for s in kernels.steps] == [(8, 0.5)]
+
+
+def test_a_checkpoint_with_the_device_s_numbers_in_its_groups(kernels, capture):
+    """As they were saved before: its count is the one that counts, and the checkpoint stays as it is."""
+    params = parameters(2)
+    opt = AdamW(params, lr=0.5, capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    state = saved(opt)
+    group = state["param_groups"][0]
+    group["device_step"], group["device_lr"], group["told_lr"] = torch.tensor([41]), torch.tensor([0.5]), 0.5
+    for capturable in (True, False):
+        again = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        other = AdamW(again, capturable=capturable)
+        other.load_state_dict(state)
+        set_gradients(again, 2)
+        kernels.steps.clear()
+        other.step()
+        assert [s[:2] for s in kernels.steps] == [(42, 0.5)]
+        assert capturable or "device_step" not in other.param_groups[0]
+    assert int(group["device_step"]) == 41 and "told_lr" in group
+    assert [s["step"] for s in state["state"].values()] == [1, 1]
