@@ -106,6 +106,10 @@ class AdamW(torch.optim.Optimizer):
         self.bits, self.max_norm, self.seed, self.capturable = bits, max_norm, seed, capturable
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self) -> dict:
+        """What copies and pickles have: torch's keeps the groups, their state and the defaults alone."""
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in ("bits", "max_norm", "seed", "capturable")}}
+
     def _state_of(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if not state:

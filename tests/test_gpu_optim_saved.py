@@ -154,3 +154,49 @@ def test_a_checkpoint_of_an_optimizer_that_is_not_capturable(cs, bits):
         near(p, q, 2)
         for name, value in opt.state[p].items():
             assert not isinstance(value, torch.Tensor) or torch.equal(value, other.state[q][name])
+
+
+@both
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_copy_makes_the_same_steps(cs, bits, capturable):
+    import copy
+    params = parameters()
+    opt = cs.AdamW(groups(params), bits=bits, max_norm=1.0, capturable=capturable, seed=9)
+    set_gradients(params, 1)
+    opt.step()
+    other = copy.deepcopy(opt)
+    again = [p for g in other.param_groups for p in g["params"]]
+    for ps, o in ((params, opt), (again, other)):
+        set_gradients(ps, 2)
+        o.step()
+    same(opt, other, params, again)
+
+
+def test_a_step_that_is_refused_is_not_counted(cs):
+    """Averages of another type stand for what a call refuses."""
+    for capturable in (False, True):
+        params = parameters()
+        opt = cs.AdamW(params, capturable=capturable)
+        set_gradients(params, 1)
+        opt.step()
+        good = opt.state[params[0]]["exp_avg"]
+        opt.state[params[0]]["exp_avg"] = good.half()
+        before = [p.detach().clone() for p in params]
+        with pytest.raises(ValueError, match="float32"):
+            opt.step()
+        assert all(torch.equal(p, b) for p, b in zip(params, before))
+        opt.state[params[0]]["exp_avg"] = good
+        set_gradients(params, 2)
+        opt.step()
+        assert [s["step"] for s in opt.state_dict()["state"].values()] == [2] * 4
+
+
+def test_a_frozen_group_beside_a_captured_step(cs):
+    params, frozen = parameters(), parameters()
+    opt = cs.AdamW([dict(params=frozen), dict(params=params)], capturable=True)
+    set_gradients(params, 1)
+    opt.step()
+    graph = captured(opt)
+    graph.replay()
+    assert [opt.state_dict()["state"][i]["step"] for i in range(4, 8)] == [2] * 4
+    assert all(torch.equal(p, q) for p, q in zip(frozen, parameters()))

@@ -242,3 +242,24 @@ def test_a_checkpoint_with_the_device_s_numbers_in_its_groups(kernels, capture):
         assert capturable or "device_step" not in other.param_groups[0]
     assert int(group["device_step"]) == 41 and "told_lr" in group
     assert [s["step"] for s in state["state"].values()] == [1, 1]
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_copy_steps_as_the_original(kernels, how, bits, capturable):
+    import copy
+    import pickle
+    params = parameters(2)
+    opt = AdamW(params, lr=0.1, bits=bits, max_norm=0.5, seed=7, capturable=capturable)
+    set_gradients(params, 1)
+    opt.step()
+    other = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    assert (other.bits, other.max_norm, other.seed, other.capturable) == (bits, 0.5, 7, capturable)
+    again = other.param_groups[0]["params"]
+    assert not any(p is q for p, q in zip(params, again))
+    kernels.steps.clear()
+    for ps, o in ((params, opt), (again, other)):
+        set_gradients(ps, 2)
+        o.step()
+    assert [s[0] for s in kernels.steps] == [2, 2] and all(torch.equal(p, q) for p, q in zip(params, again))
