@@ -4,6 +4,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
 #include <cmath>
@@ -338,18 +339,18 @@ PyObject* fp8_linear_held(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- the optimizer's step ------------------------------------------------------------------------------------------
-// The tensors of a list or tuple; what they are checked for is their caller's.
+// The tensors of a list, a tuple or anything else that can be gone through, once: it lives until the launch, since what it was
+// made of may hold its tensors no longer.  What they are checked for is their caller's.
 struct List {
-  PyObject* fast = nullptr;
+  THPObjectPtr fast;
   Py_ssize_t size = 0;
-  bool of(PyObject* o, const char* name) {
+  bool of(PyObject* o) {
     fast = PySequence_Fast(o, "a list of tensors is wanted");
     if (!fast) return false;
-    size = PySequence_Fast_GET_SIZE(fast);
+    size = PySequence_Fast_GET_SIZE(fast.get());
     return true;
   }
-  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
-  ~List() { Py_XDECREF(fast); }
+  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast.get(), i); }
 };
 bool same_size(const List& l, Py_ssize_t n, const char* name) {
   return l.size == n || value_error("%s must have an entry for each parameter", name);
@@ -404,9 +405,10 @@ bool bytes_of(const at::Tensor& t, const at::Tensor& on, int64_t n, const char* 
   if (t.scalar_type() != at::kByte || t.numel() != n) return value_error("%s has another type or size than its parameter asks for", name);
   return require_flat(t, name);
 }
-bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, size_t role) {
-  List l;
-  if (!l.of(o, "states")) return false;
+bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, size_t role, std::vector<List>* kept) {
+  kept->emplace_back();
+  List& l = kept->back();
+  if (!l.of(o)) return false;
   if (l.size != 4) return value_error("a state is (exp_avg, exp_avg_sq, their scales)");
   void** const to[4] = {&t->exp_avg, &t->exp_avg_sq, &t->exp_avg_scale, &t->exp_avg_sq_scale};
   const int64_t n = on.numel();
@@ -479,13 +481,13 @@ bool options_of(PyObject* const* a, const at::Tensor* on, csw_adamw_options* o) 
   return true;
 }
 
-// params, grads and copies of a call; the first parameter in *on
-bool tensors_of(const List& params, PyObject* grads, PyObject* copies, std::vector<csw_adamw_tensor>* to, Written* written,
-                const at::Tensor** on) {
-  List g, c;
-  if (!g.of(grads, "grads") || !same_size(g, params.size, "grads")) return false;
+// params, grads and copies (an empty list where there are none) of a call; the first parameter in *on
+bool tensors_of(const List& params, PyObject* grads, PyObject* copies, List* grads_list, List* copies_list,
+                std::vector<csw_adamw_tensor>* to, Written* written, const at::Tensor** on) {
+  List &g = *grads_list, &c = *copies_list;
+  if (!g.of(grads) || !same_size(g, params.size, "grads")) return false;
   const bool with_copies = copies != Py_None;
-  if (with_copies && (!c.of(copies, "copies") || !same_size(c, params.size, "copies"))) return false;
+  if (with_copies && (!c.of(copies) || !same_size(c, params.size, "copies"))) return false;
   to->resize(params.size);
   *on = nullptr;
   for (Py_ssize_t i = 0; i < params.size; ++i) {
@@ -509,13 +511,10 @@ bool tensors_of(const List& params, PyObject* grads, PyObject* copies, std::vect
   }
   return true;
 }
-void all_changed(const List& params, PyObject* copies) {
+void all_changed(const List& params, const List& copies) {
   for (Py_ssize_t i = 0; i < params.size; ++i) changed(THPVariable_Unpack(params[i]));
-  if (copies == Py_None) return;
-  List c;
-  if (!c.of(copies, "copies")) return;
-  for (Py_ssize_t i = 0; i < c.size; ++i)
-    if (THPVariable_Check(c[i])) changed(THPVariable_Unpack(c[i]));
+  for (Py_ssize_t i = 0; i < copies.size; ++i)
+    if (THPVariable_Check(copies[i])) changed(THPVariable_Unpack(copies[i]));
 }
 
 bool step_of(const std::vector<csw_adamw_tensor>& tensors, const csw_adamw_options& o, const at::Tensor* on) {
@@ -526,14 +525,14 @@ bool step_of(const std::vector<csw_adamw_tensor>& tensors, const csw_adamw_optio
 // adamw_step(params, grads, exp_avgs, exp_avg_sqs, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm) -> None
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    List params, m, v;
+    List params, g, c, m, v;
     std::vector<csw_adamw_tensor> tensors;
     Written written(4);
     const at::Tensor *on, *t;
     csw_adamw_options o{};
     o.bits = 32;
-    if (!arg_count(n, 13) || !params.of(a[0], "params") || !tensors_of(params, a[1], a[4], &tensors, &written, &on) ||
-        !m.of(a[2], "exp_avgs") || !v.of(a[3], "exp_avg_sqs") || !same_size(m, params.size, "exp_avgs") ||
+    if (!arg_count(n, 13) || !params.of(a[0]) || !tensors_of(params, a[1], a[4], &g, &c, &tensors, &written, &on) ||
+        !m.of(a[2]) || !v.of(a[3]) || !same_size(m, params.size, "exp_avgs") ||
         !same_size(v, params.size, "exp_avg_sqs") || !options_of(a + 5, on, &o))
       return nullptr;
     for (Py_ssize_t i = 0; i < params.size; ++i) {
@@ -546,7 +545,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       written.add(3, *t);
     }
     if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
-    all_changed(params, a[4]);
+    all_changed(params, c);
     for (Py_ssize_t i = 0; i < params.size; ++i) changed(THPVariable_Unpack(m[i])), changed(THPVariable_Unpack(v[i]));
     Py_RETURN_NONE;
   });
@@ -555,14 +554,15 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // adamw8_step(params, grads, states, copies, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed) -> None
 PyObject* adamw8_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    List params, states;
+    List params, g, c, states;
+    std::vector<List> kept;
     std::vector<csw_adamw_tensor> tensors;
     Written written(6);
     const at::Tensor* on;
     csw_adamw_options o{};
     o.bits = 8;
-    if (!arg_count(n, 13) || !params.of(a[0], "params") || !tensors_of(params, a[1], a[3], &tensors, &written, &on) ||
-        !states.of(a[2], "states") || !same_size(states, params.size, "states") || !options_of(a + 4, on, &o))
+    if (!arg_count(n, 13) || !params.of(a[0]) || !tensors_of(params, a[1], a[3], &g, &c, &tensors, &written, &on) ||
+        !states.of(a[2]) || !same_size(states, params.size, "states") || !options_of(a + 4, on, &o))
       return nullptr;
     const unsigned long long seed = PyLong_AsUnsignedLongLong(a[12]);
     if (PyErr_Occurred()) return nullptr;
@@ -572,9 +572,9 @@ PyObject* adamw8_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     o.seed = (uint32_t)seed;
     for (Py_ssize_t i = 0; i < params.size; ++i)
-      if (!eight_of(states[i], THPVariable_Unpack(params[i]), &tensors[i], &written, 2)) return nullptr;
+      if (!eight_of(states[i], THPVariable_Unpack(params[i]), &tensors[i], &written, 2, &kept)) return nullptr;
     if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
-    all_changed(params, a[3]);
+    all_changed(params, c);
     Py_RETURN_NONE;
   });
 }
@@ -583,7 +583,8 @@ PyObject* adamw8_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     List states, m, v;
-    if (!arg_count(n, 4) || !states.of(a[0], "states") || !m.of(a[1], "exp_avgs") || !v.of(a[2], "exp_avg_sqs") ||
+    std::vector<List> kept;
+    if (!arg_count(n, 4) || !states.of(a[0]) || !m.of(a[1]) || !v.of(a[2]) ||
         !same_size(m, states.size, "exp_avgs") || !same_size(v, states.size, "exp_avg_sqs"))
       return nullptr;
     const int pack = PyObject_IsTrue(a[3]);
@@ -601,7 +602,8 @@ PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
           !floats_of(m[i], *first, "exp_avg", &first) || !floats_of(v[i], *first, "exp_avg_sq", &second))
         return nullptr;
       if (!on) on = first;
-      if (!same_device(*first, *on, "exp_avg") || !eight_of(states[i], *first, &t, pack ? &written : nullptr, 0)) return nullptr;
+      if (!same_device(*first, *on, "exp_avg") || !eight_of(states[i], *first, &t, pack ? &written : nullptr, 0, &kept))
+        return nullptr;
       t.param = ptr(*first), t.copy = ptr(*second), t.numel = (size_t)first->numel();
       if (!pack) {
         written.add(0, *first), written.add(1, *second);
@@ -621,7 +623,7 @@ PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* gradient_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     List grads;
-    if (!arg_count(n, 1) || !grads.of(a[0], "tensors")) return nullptr;
+    if (!arg_count(n, 1) || !grads.of(a[0])) return nullptr;
     if (grads.size == 0) {
       value_error("a norm needs a tensor at least");
       return nullptr;
