@@ -356,18 +356,26 @@ bool same_size(const List& l, Py_ssize_t n, const char* name) {
   return l.size == n || value_error("%s must have an entry for each parameter", name);
 }
 
-// What is written by a call, apart: a range for each tensor, by its role.
+// What is written by a call, apart: a range for each tensor, by its role.  And what is read, which may lie where nothing is
+// written, or be the very tensor that its own entry of the lists writes: a value is read by the thread that writes it, before.
 struct Written {
-  using Range = std::pair<const char*, const char*>;
+  struct Range {
+    const char *begin, *end;
+    size_t entry;
+    bool operator<(const Range& o) const { return begin < o.begin; }
+  };
   std::vector<std::vector<Range>> roles;
+  std::vector<Range> read;
   explicit Written(size_t n) : roles(n) {}
-  void add(size_t role, const at::Tensor& t) {
+  static void push(std::vector<Range>* to, const at::Tensor& t, size_t entry) {
     const char* p = static_cast<const char*>(t.const_data_ptr());
-    if (t.numel()) roles[role].push_back({p, p + t.nbytes()});
+    if (t.numel()) to->push_back({p, p + t.nbytes(), entry});
   }
+  void add(size_t role, const at::Tensor& t, size_t entry) { push(&roles[role], t, entry); }
+  void add_read(const at::Tensor& t, size_t entry) { push(&read, t, entry); }
   static bool ascend(const std::vector<Range>& r) {
     for (size_t i = 1; i < r.size(); ++i)
-      if (r[i].first < r[i - 1].second) return false;
+      if (r[i].begin < r[i - 1].end) return false;
     return true;
   }
   // Most programs' tensors of one role ascend in memory, apart from those of the others: no need to sort them then.
@@ -376,13 +384,25 @@ struct Written {
     bool plain = true;
     for (const auto& r : roles) {
       plain = plain && ascend(r);
-      if (!r.empty()) hulls.push_back({r.front().first, r.back().second});
+      if (!r.empty()) hulls.push_back({r.front().begin, r.back().end, 0});
+    }
+    if (!read.empty()) {
+      Range hull = read[0];
+      for (const Range& r : read) hull.begin = std::min(hull.begin, r.begin), hull.end = std::max(hull.end, r.end);
+      hulls.push_back(hull);
     }
     std::sort(hulls.begin(), hulls.end());
     if (plain && ascend(hulls)) return true;
     for (const auto& r : roles) all.insert(all.end(), r.begin(), r.end());
     std::sort(all.begin(), all.end());
-    return ascend(all) || value_error("the tensors that the step writes overlap");
+    if (!ascend(all)) return value_error("the tensors that the step writes overlap");
+    for (const Range& r : read) {
+      auto w = std::partition_point(all.begin(), all.end(), [&](const Range& o) { return o.end <= r.begin; });
+      for (; w != all.end() && w->begin < r.end; ++w)
+        if (w->begin != r.begin || w->end != r.end || w->entry != r.entry)
+          return value_error("a tensor that the step reads overlaps one that it writes");
+    }
+    return true;
   }
 };
 void changed(const at::Tensor& t) {
@@ -405,7 +425,9 @@ bool bytes_of(const at::Tensor& t, const at::Tensor& on, int64_t n, const char* 
   if (t.scalar_type() != at::kByte || t.numel() != n) return value_error("%s has another type or size than its parameter asks for", name);
   return require_flat(t, name);
 }
-bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, size_t role, std::vector<List>* kept) {
+// a state, whose tensors are written in four roles from `role` on, or read
+bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, bool write, size_t role, size_t entry,
+              std::vector<List>* kept) {
   kept->emplace_back();
   List& l = kept->back();
   if (!l.of(o)) return false;
@@ -416,9 +438,11 @@ bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* w
     const at::Tensor* s = as_tensor(l[i], "a state");
     if (!s || !bytes_of(*s, on, i < 2 ? n : blocks_of(n), "a state")) return false;
     *to[i] = ptr(*s);
-    if (written) {
-      written->add(role + i, *s);
+    if (write) {
+      written->add(role + i, *s, entry);
       changed(*s);
+    } else {
+      written->add_read(*s, entry);
     }
   }
   return true;
@@ -501,12 +525,13 @@ bool tensors_of(const List& params, PyObject* grads, PyObject* copies, List* gra
     if (!*on) *on = p;
     if (!same_device(*p, **on, "a parameter")) return false;
     t.param = ptr(*p), t.grad = ptr(*d), t.numel = (size_t)p->numel();
-    written->add(0, *p);
+    written->add(0, *p, i);
+    written->add_read(*d, i);
     if (with_copies && c[i] != Py_None) {
       const at::Tensor* k = as_tensor(c[i], "a copy");
       if (!k || !require_values(*k, "a copy", &t.copy_type) || !lies_like(*k, *p, "a copy")) return false;
       t.copy = ptr(*k);
-      written->add(1, *k);
+      written->add(1, *k, i);
     }
   }
   return true;
@@ -539,10 +564,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const at::Tensor& p = THPVariable_Unpack(params[i]);
       if (!floats_of(m[i], p, "exp_avg", &t)) return nullptr;
       tensors[i].exp_avg = ptr(*t);
-      written.add(2, *t);
+      written.add(2, *t, i);
       if (!floats_of(v[i], p, "exp_avg_sq", &t)) return nullptr;
       tensors[i].exp_avg_sq = ptr(*t);
-      written.add(3, *t);
+      written.add(3, *t, i);
     }
     if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
     all_changed(params, c);
@@ -572,7 +597,7 @@ PyObject* adamw8_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     o.seed = (uint32_t)seed;
     for (Py_ssize_t i = 0; i < params.size; ++i)
-      if (!eight_of(states[i], THPVariable_Unpack(params[i]), &tensors[i], &written, 2, &kept)) return nullptr;
+      if (!eight_of(states[i], THPVariable_Unpack(params[i]), &tensors[i], &written, true, 2, i, &kept)) return nullptr;
     if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
     all_changed(params, c);
     Py_RETURN_NONE;
@@ -602,11 +627,13 @@ PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
           !floats_of(m[i], *first, "exp_avg", &first) || !floats_of(v[i], *first, "exp_avg_sq", &second))
         return nullptr;
       if (!on) on = first;
-      if (!same_device(*first, *on, "exp_avg") || !eight_of(states[i], *first, &t, pack ? &written : nullptr, 0, &kept))
+      if (!same_device(*first, *on, "exp_avg") || !eight_of(states[i], *first, &t, &written, pack, 0, i, &kept))
         return nullptr;
       t.param = ptr(*first), t.copy = ptr(*second), t.numel = (size_t)first->numel();
-      if (!pack) {
-        written.add(0, *first), written.add(1, *second);
+      if (pack) {
+        written.add_read(*first, i), written.add_read(*second, i);
+      } else {
+        written.add(0, *first, i), written.add(1, *second, i);
         changed(*first), changed(*second);
       }
     }

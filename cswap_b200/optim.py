@@ -7,7 +7,8 @@
 * ``AdamW``: a torch.optim.Optimizer on them.
 
 Parameters, gradients and 16-bit copies of the parameters are float32, float16 or bfloat16, each tensor of its own type.
-Tensors lie densely, in the same order in memory for a parameter and what belongs to it, and no two that are written overlap.
+Tensors lie densely, in the same order in memory for a parameter and what belongs to it.  No two that are written overlap, and no
+gradient overlaps one that is, unless it is the very tensor that is written for its parameter.
 Averages are float32 operations, rounded one by one; the same call gives the same bits.  There is no CPU implementation.
 """
 from __future__ import annotations

@@ -49,3 +49,40 @@ def test_what_can_be_gone_through_once(cs, bits):
     assert all(R.bits_equal(a, b) for a, b in zip(ps, want)) and all(R.bits_equal(a, b) for a, b in zip(others, copies))
     assert [t._version - v for t, v in zip(others, versions)] == [1] * 3
     assert float(cs.gradient_norm(g.clone() for g in gs)) == float(cs.gradient_norm(gs))
+
+
+@both
+def test_gradients_where_something_is_written(cs, bits):
+    """A gradient beside, or in the very place of, what its own entry writes; one that lies half there is refused, and so is one in
+    the place of another entry's."""
+    whole = normal(4000, seed=1)
+    want, gs = whole[:1000].clone(), whole[1000:2000].clone()
+    state = lambda n: ([cs.adamw8_state(torch.empty(n, device="cuda"))],) if bits == 8 else ([torch.zeros(n, device="cuda")], [torch.zeros(n, device="cuda")])
+    step(cs, bits, [want], [gs], state(1000))
+    p, g = whole[:1000], whole[1000:2000]
+    step(cs, bits, [p], [g], state(1000), copies=[g])  # the copy goes where the gradient was
+    assert R.bits_equal(p, want) and R.bits_equal(g, want)
+    old = whole.clone()
+    for bad in (whole[500:1500], whole[999:1999], whole[1:1001]):
+        with pytest.raises(ValueError, match="overlap"):
+            step(cs, bits, [p], [bad], state(1000))
+    q = whole[2000:3000]
+    for gs in ([whole[3000:], q], [q, whole[3000:]]):  # in place, and of the other entry
+        call = lambda: step(cs, bits, [p, q], gs, tuple(a + b for a, b in zip(state(1000), state(1000))))
+        if gs[0] is q:
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+            continue
+        call()
+    assert R.bits_equal(old[1000:2000], whole[1000:2000]) and R.bits_equal(old[3000:], whole[3000:])
+    shared = normal(1000, seed=7)  # a gradient of two parameters
+    step(cs, bits, [p, q], [shared, shared], tuple(a + b for a, b in zip(state(1000), state(1000))))
+
+
+def test_averages_where_their_codes_are(cs):
+    room = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    m, v = room[:2000].view(torch.float32), normal(500).abs()
+    state = tuple(room[at:at + n] for at, n in ((1900, 500), (2400, 500), (2900, 4), (2904, 4)))
+    for call in (cs.adamw8_pack, cs.adamw8_unpack):
+        with pytest.raises(ValueError, match="overlap"):
+            call([state], [m], [v])
