@@ -86,3 +86,25 @@ def test_averages_where_their_codes_are(cs):
     for call in (cs.adamw8_pack, cs.adamw8_unpack):
         with pytest.raises(ValueError, match="overlap"):
             call([state], [m], [v])
+
+
+@pytest.mark.parametrize("count", [51, 52, 53, 105, 433])
+@both
+def test_a_list_is_its_parts(cs, bits, count):
+    """Lists around what the kernels' parameters of one launch hold: in 32 bits what the step of each tensor on its own gives."""
+    sizes = [(5 * i + 3) % 200 for i in range(count)]
+    ps, gs, state = made(cs, bits, sizes)
+    alone = [p.clone() for p in ps]
+    step(cs, bits, ps, gs, state, lr=0.1)
+    if bits == 8:  # their random bits go by the place in the lists, their parameters do not: the first step's averages are exact
+        held = [(cs.adamw8_state(p),) for p in alone]
+    else:
+        held = [(torch.zeros_like(p), torch.zeros_like(p)) for p in alone]
+    for p, q, g, s in zip(ps, alone, gs, held):
+        step(cs, bits, [q], [g], tuple([t] for t in s), lr=0.1)
+        assert R.bits_equal(p, q)
+    if bits == 32:
+        for l, own in zip(state, zip(*held)):
+            assert all(R.bits_equal(a, b) for a, b in zip(l, own))
+    want = torch.cat([g.double() for g in gs]).norm()
+    assert abs(float(cs.gradient_norm(gs)) - float(want)) <= float(want) * 2.0 ** -23
