@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <memory>
 #include <utility>
 #include <vector>
 
@@ -364,39 +365,54 @@ struct Written {
     size_t entry;
     bool operator<(const Range& o) const { return begin < o.begin; }
   };
-  std::vector<std::vector<Range>> roles;
-  std::vector<Range> read;
-  explicit Written(size_t n) : roles(n) {}
-  static void push(std::vector<Range>* to, const at::Tensor& t, size_t entry) {
-    const char* p = static_cast<const char*>(t.const_data_ptr());
-    if (t.numel()) to->push_back({p, p + t.nbytes(), entry});
+  static constexpr size_t kMost = 7;  // roles, what is read among them
+  struct Role {
+    Range* first;
+    size_t size;
+  };
+  std::unique_ptr<Range[]> space;
+  Role roles[kMost];
+  size_t count;  // of those that are written; the one behind them is read
+  explicit Written(size_t written) : count(written) {}
+  // for lists of so many entries, each of which reads `reads` tensors
+  void room_for(size_t entries, size_t reads) {
+    space.reset(new Range[(count + reads) * entries]);
+    for (size_t i = 0; i <= count; ++i) roles[i] = {space.get() + i * entries, 0};
   }
-  void add(size_t role, const at::Tensor& t, size_t entry) { push(&roles[role], t, entry); }
-  void add_read(const at::Tensor& t, size_t entry) { push(&read, t, entry); }
-  static bool ascend(const std::vector<Range>& r) {
-    for (size_t i = 1; i < r.size(); ++i)
+  void add(size_t role, const void* p, size_t bytes, size_t entry) {
+    const char* begin = static_cast<const char*>(p);
+    if (bytes) roles[role].first[roles[role].size++] = {begin, begin + bytes, entry};
+  }
+  void add_read(const void* p, size_t bytes, size_t entry) { add(count, p, bytes, entry); }
+  static bool ascend(const Range* r, size_t n) {
+    for (size_t i = 1; i < n; ++i)
       if (r[i].begin < r[i - 1].end) return false;
     return true;
   }
   // Most programs' tensors of one role ascend in memory, apart from those of the others: no need to sort them then.
   bool apart() {
-    std::vector<Range> hulls, all;
+    Range hulls[kMost];
+    size_t n = 0;
     bool plain = true;
-    for (const auto& r : roles) {
-      plain = plain && ascend(r);
-      if (!r.empty()) hulls.push_back({r.front().begin, r.back().end, 0});
+    for (size_t i = 0; i < count; ++i) {
+      const Role& r = roles[i];
+      plain = plain && ascend(r.first, r.size);
+      if (r.size) hulls[n++] = {r.first[0].begin, r.first[r.size - 1].end, 0};
     }
-    if (!read.empty()) {
-      Range hull = read[0];
-      for (const Range& r : read) hull.begin = std::min(hull.begin, r.begin), hull.end = std::max(hull.end, r.end);
-      hulls.push_back(hull);
+    const Role& read = roles[count];
+    if (read.size) {
+      Range& hull = hulls[n++] = read.first[0];
+      for (size_t i = 1; i < read.size; ++i)
+        hull.begin = std::min(hull.begin, read.first[i].begin), hull.end = std::max(hull.end, read.first[i].end);
     }
-    std::sort(hulls.begin(), hulls.end());
-    if (plain && ascend(hulls)) return true;
-    for (const auto& r : roles) all.insert(all.end(), r.begin(), r.end());
+    std::sort(hulls, hulls + n);
+    if (plain && ascend(hulls, n)) return true;
+    std::vector<Range> all;
+    for (size_t i = 0; i < count; ++i) all.insert(all.end(), roles[i].first, roles[i].first + roles[i].size);
     std::sort(all.begin(), all.end());
-    if (!ascend(all)) return value_error("the tensors that the step writes overlap");
-    for (const Range& r : read) {
+    if (!ascend(all.data(), all.size())) return value_error("the tensors that the step writes overlap");
+    for (size_t i = 0; i < read.size; ++i) {
+      const Range& r = read.first[i];
       auto w = std::partition_point(all.begin(), all.end(), [&](const Range& o) { return o.end <= r.begin; });
       for (; w != all.end() && w->begin < r.end; ++w)
         if (w->begin != r.begin || w->end != r.end || w->entry != r.entry)
@@ -428,8 +444,7 @@ bool bytes_of(const at::Tensor& t, const at::Tensor& on, int64_t n, const char* 
 // a state, whose tensors are written in four roles from `role` on, or read
 bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* written, bool write, size_t role, size_t entry,
               std::vector<List>* kept) {
-  kept->emplace_back();
-  List& l = kept->back();
+  List l;
   if (!l.of(o)) return false;
   if (l.size != 4) return value_error("a state is (exp_avg, exp_avg_sq, their scales)");
   void** const to[4] = {&t->exp_avg, &t->exp_avg_sq, &t->exp_avg_scale, &t->exp_avg_sq_scale};
@@ -438,13 +453,15 @@ bool eight_of(PyObject* o, const at::Tensor& on, csw_adamw_tensor* t, Written* w
     const at::Tensor* s = as_tensor(l[i], "a state");
     if (!s || !bytes_of(*s, on, i < 2 ? n : blocks_of(n), "a state")) return false;
     *to[i] = ptr(*s);
+    const size_t bytes = i < 2 ? n : blocks_of(n);
     if (write) {
-      written->add(role + i, *s, entry);
+      written->add(role + i, *to[i], bytes, entry);
       changed(*s);
     } else {
-      written->add_read(*s, entry);
+      written->add_read(*to[i], bytes, entry);
     }
   }
+  if (l.fast.get() != o) kept->push_back(std::move(l));
   return true;
 }
 bool floats_of(PyObject* o, const at::Tensor& as, const char* name, const at::Tensor** t) {
@@ -513,10 +530,10 @@ bool tensors_of(const List& params, PyObject* grads, PyObject* copies, List* gra
   const bool with_copies = copies != Py_None;
   if (with_copies && (!c.of(copies) || !same_size(c, params.size, "copies"))) return false;
   to->resize(params.size);
+  written->room_for(params.size, 1);
   *on = nullptr;
   for (Py_ssize_t i = 0; i < params.size; ++i) {
     csw_adamw_tensor& t = (*to)[i];
-    t = {};
     const at::Tensor* p = as_tensor(params[i], "a parameter");
     const at::Tensor* d = p ? as_tensor(g[i], "a gradient") : nullptr;
     if (!d || !require_values(*p, "a parameter", &t.param_type) || !require_dense(*p, "a parameter") ||
@@ -525,13 +542,13 @@ bool tensors_of(const List& params, PyObject* grads, PyObject* copies, List* gra
     if (!*on) *on = p;
     if (!same_device(*p, **on, "a parameter")) return false;
     t.param = ptr(*p), t.grad = ptr(*d), t.numel = (size_t)p->numel();
-    written->add(0, *p, i);
-    written->add_read(*d, i);
+    written->add(0, t.param, t.numel * p->element_size(), i);
+    written->add_read(t.grad, t.numel * d->element_size(), i);
     if (with_copies && c[i] != Py_None) {
       const at::Tensor* k = as_tensor(c[i], "a copy");
       if (!k || !require_values(*k, "a copy", &t.copy_type) || !lies_like(*k, *p, "a copy")) return false;
       t.copy = ptr(*k);
-      written->add(1, *k, i);
+      written->add(1, t.copy, t.numel * k->element_size(), i);
     }
   }
   return true;
@@ -564,10 +581,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const at::Tensor& p = THPVariable_Unpack(params[i]);
       if (!floats_of(m[i], p, "exp_avg", &t)) return nullptr;
       tensors[i].exp_avg = ptr(*t);
-      written.add(2, *t, i);
+      written.add(2, tensors[i].exp_avg, 4 * tensors[i].numel, i);
       if (!floats_of(v[i], p, "exp_avg_sq", &t)) return nullptr;
       tensors[i].exp_avg_sq = ptr(*t);
-      written.add(3, *t, i);
+      written.add(3, tensors[i].exp_avg_sq, 4 * tensors[i].numel, i);
     }
     if (!written.apart() || !step_of(tensors, o, on)) return nullptr;
     all_changed(params, c);
@@ -616,10 +633,10 @@ PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (pack < 0) return nullptr;
     std::vector<csw_adamw_tensor> tensors(states.size);
     Written written(4);
+    written.room_for(states.size, 4);
     const at::Tensor* on = nullptr;
     for (Py_ssize_t i = 0; i < states.size; ++i) {
       csw_adamw_tensor& t = tensors[i];
-      t = {};
       const at::Tensor* first = as_tensor(m[i], "exp_avg");
       const at::Tensor* second;
       int type;
@@ -631,9 +648,9 @@ PyObject* adamw8_convert(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return nullptr;
       t.param = ptr(*first), t.copy = ptr(*second), t.numel = (size_t)first->numel();
       if (pack) {
-        written.add_read(*first, i), written.add_read(*second, i);
+        written.add_read(t.param, 4 * t.numel, i), written.add_read(t.copy, 4 * t.numel, i);
       } else {
-        written.add(0, *first, i), written.add(1, *second, i);
+        written.add(0, t.param, 4 * t.numel, i), written.add(1, t.copy, 4 * t.numel, i);
         changed(*first), changed(*second);
       }
     }
@@ -659,7 +676,6 @@ PyObject* gradient_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* on = nullptr;
     for (Py_ssize_t i = 0; i < grads.size; ++i) {
       csw_adamw_tensor& t = tensors[i];
-      t = {};
       const at::Tensor* g = as_tensor(grads[i], "a gradient");
       if (!g || !require_values(*g, "a gradient", &t.grad_type) || !require_dense(*g, "a gradient")) return nullptr;
       if (!on) on = g;
