@@ -23,8 +23,10 @@ statistics a second time; pass a closure over F.batch_norm without them).  A
 tensor whose producer was not given stays on the device.  Policy 8, the
 framework's own, keeps the tensor (float32, as all that the engine tracks) on the device as an 8-bit checkpoint
 (`ops.q8_compress`, 1.03 bytes a value) and takes the values it holds for
-backward: no link time, a quarter of the memory.  `policy_` 3 and 4
-select the vDNN and SuperNeurons baselines as in Execution.h:70,243,248.
+backward: no link time, a quarter of the memory.  What a layer of fp8.py keeps is
+no float32 activation but codes, a quarter of it already: every policy passes it
+by, and they stay on the device (`skipped_unsaved` counts the inputs that nothing
+else keeps).  `policy_` 3 and 4 select the vDNN and SuperNeurons baselines as in Execution.h:70,243,248.
 
 The reference swaps the storage's DataPtr under the autograd graph and relies
 on a modified engine to bring it back.  On stock PyTorch the same effect is
