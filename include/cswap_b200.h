@@ -406,10 +406,11 @@ typedef struct {
 } csw_attention_operand;
 /* The kernels' warps wait for one another's copies and products, each time for two seconds or so at the most.  Where that
  * runs out, which takes a fault of the device, what the CTA in question had to compute is NaN, in the results and in the
- * gradients that follow from them, and the next call of csw_attention_forward or csw_attention_backward on that device,
- * of csw_fp8_matmul, or csw_device_status, returns CSW_ERR_TIMEOUT, once; that call launches nothing.
- * csw_attention_wait_limit sets the time for the calls of this process (csw_fp8_matmul's, too) from now on, in clocks of an SM (2^32 to begin with).  A negative one lets the waits run
- * out after -clocks, since the copies they are for are not begun: what a program does then can be tried out with it. */
+ * gradients that follow from them, and the next call of csw_attention_forward, csw_attention_backward, csw_fp8_matmul or
+ * csw_fp8_linear on that device, or csw_device_status, returns CSW_ERR_TIMEOUT, once; that call launches nothing.
+ * csw_attention_wait_limit sets the time for the calls of this process (those two products', too) from now on, in clocks of an SM
+ * (2^32 to begin with).  A negative one lets the waits run out after -clocks, since the copies they are for are not begun: what a
+ * program does then can be tried out with it. */
 csw_status csw_attention_wait_limit(int64_t clocks);
 /* d_lse: batch x heads x q_len float32, the natural logarithm of each row's sum of exp(scale q.k). */
 csw_status csw_attention_forward(const csw_attention_shape* shape, const csw_attention_operand* q,
@@ -450,8 +451,8 @@ typedef struct {
   int transposed;
 } csw_fp8_matrix;
 /* out = a b + bias, with a taken as m x k, b as k x n, out m x n row behind row; the bias (n values of bias_type) may be NULL.
- * Products are exact and summed in float32 by the tensor cores; the sum is rounded to the type once.  m and n are at most 2^31 - 129, k at
- * most 2^31 - 1.  out overlaps no operand.  The same call gives the same bits every time.  Waits are bounded as those of attention (section 7). */
+ * Products are exact and summed in float32 by the tensor cores, which cut off what an addend has below the sum's last bit; the sum is
+ * rounded to the type once.  m and n are at most 2^31 - 129, k at most 2^31 - 1.  out overlaps no operand.  The same call gives the same bits every time.  Waits are bounded as those of attention (section 7). */
 csw_status csw_fp8_matmul(const csw_fp8_matrix* a, const csw_fp8_matrix* b, const void* d_bias, int bias_type, void* d_out,
                           int type, csw_stream_t stream);
 
