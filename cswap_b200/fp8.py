@@ -59,8 +59,8 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Quantized], bias: Op
 
     x is [..., in], weight [out, in], bias [out], each of its own type; their gradients have it, too.  x is kept as codes, and
     the weight's are for the input's gradient; both go through the program's saved-tensor hooks, which may give back tensors of
-    the same type, shape and device that lie otherwise.  Execution's policies, which are for float32 tensors, leave them alone.  A weight that does not change may be given as fp8_quantize(weight), and takes no
-    gradient then (nor do x and the bias)."""
+    the same type, shape and device that lie otherwise.  Execution's policies, which are for float32 tensors, leave them alone.
+    A weight that does not change may be given as fp8_quantize(weight), and takes no gradient then (nor do x and the bias)."""
     if isinstance(weight, torch.Tensor):
         return _ext().fp8_linear(x, weight, bias)
     codes, scales = weight

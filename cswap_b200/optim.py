@@ -93,7 +93,8 @@ class AdamW(torch.optim.Optimizer):
     in 8 bits.  A step takes the number of steps that a parameter has been through from its state; with `capturable` it is
     counted on the device, once for all of a group, and the learning rate lies there too, so that a captured step may be
     replayed: `set_lr` changes it for replays, a scheduler's change of the groups arrives with the next step that is not
-    captured."""
+    captured.  `state_dict` has the number of steps that the device has counted; what goes on from it may count either way.
+    A group of which some call is refused has made no step, the groups before it have."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, bits: int = 32, max_norm: Optional[float] = None, seed: int = 0,

@@ -123,7 +123,7 @@ class BertEncoder(nn.Module):
     """`lean`: attention that keeps its output and one number a row besides its operands (in bfloat16, its probabilities
     without dropout, of which a warning tells where `dropout` is not 0), a feed-forward part that keeps its activation in 8
     bits, norms that take the residual's sum with them.  `fp8`: the layers' products take operands in 8 bits, and keep them
-    as that; lean or not.  The parameters are the same, so that a state of one kind loads into the other."""
+    as that; lean or not.  (It quantizes its weights in every pass, in evaluation, too: they are the parameters as they are.)  The parameters are the same, so that a state of one kind loads into the other."""
 
     def __init__(self, vocab: int = 30522, hidden: int = 768, layers: int = 12, heads: int = 12, ffn: int = 3072,
                  max_seq: int = 512, dropout: float = 0.1, lean: bool = False, fp8: bool = False):
