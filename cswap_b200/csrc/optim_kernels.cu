@@ -68,6 +68,7 @@ struct Table {
   int count;
   uint32_t place;  // of the first tensor in the call
 };
+
 struct Step {
   float b1, rest1, b2, rest2, eps;
   float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
