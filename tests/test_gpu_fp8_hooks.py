@@ -93,3 +93,19 @@ def test_another_tensor_is_refused(cs, other, which):
     with pytest.raises(RuntimeError, match="saved-tensor hook"):
         torch.autograd.grad(y.sum(), (x, w))
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(cs.fp8_linear(x, w).sum(), (x, w)))
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_layer_that_is_computed_again(cs, reentrant):
+    """torch's checkpoints, which keep the input alone and run the layers a second time in backward."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, v, w = normal(70, 50, seed=1).requires_grad_(True), normal(130, 50, seed=2).requires_grad_(True), normal(30, 130, seed=3).requires_grad_(True)
+    dy = normal(70, 30, seed=4)
+    two = lambda t: cs.fp8_linear(cs.gelu(cs.fp8_linear(t, v)), w)
+    want = torch.autograd.grad(two(x), (x, v, w), dy)
+    for t in (x, v, w):
+        t.grad = None
+    checkpoint(two, x, use_reentrant=reentrant).backward(dy)
+    for t, g in zip((x, v, w), want):
+        assert R.bits_equal(t.grad, g)

@@ -59,6 +59,7 @@ APART = 2.0 ** -21
 
 
 def near(p, q, steps):
+    p, q = p.detach(), q.detach()
     assert float((p - q).abs().max()) <= steps * APART * (float(p.abs().max()) + 0.032)
 
 
@@ -200,3 +201,25 @@ def test_a_frozen_group_beside_a_captured_step(cs):
     graph.replay()
     assert [opt.state_dict()["state"][i]["step"] for i in range(4, 8)] == [2] * 4
     assert all(torch.equal(p, q) for p, q in zip(frozen, parameters()))
+
+
+@both
+def test_gradients_that_lie_in_another_order(cs, bits):
+    """A parameter in one order in memory and its gradient in another, in a captured step too: the class puts them in order."""
+    shape = (8, 6, 5, 4)
+    first = torch.nn.Parameter(normal(*shape, seed=1))
+    last = torch.nn.Parameter(normal(*shape, seed=1).to(memory_format=torch.channels_last))
+    opts = [cs.AdamW([p], bits=32 if p is first else bits, capturable=True, seed=1) for p in (first, last)]
+    plain = torch.nn.Parameter(normal(*shape, seed=1).to(memory_format=torch.channels_last))
+    opts.append(cs.AdamW([plain], bits=bits, capturable=True, seed=1))
+    g = normal(*shape, seed=2)
+    first.grad, last.grad = g.to(memory_format=torch.channels_last), g.clone()
+    plain.grad = g.to(memory_format=torch.channels_last)
+    for o in opts:
+        o.step()
+    graph = captured(opts[1])
+    graph.replay()
+    opts[0].step()
+    opts[2].step()
+    assert last.stride() == plain.stride() != first.stride()
+    assert torch.equal(last, plain) and (bits == 8 or torch.equal(last, first))
